@@ -97,6 +97,18 @@ _SIGS = {
     "gs_move_rows": (_i, [_i64, _c, _i64, _c, _i64, _i, C.POINTER(RowField), _i, _c]),
     "gs_ply_unpack": (_i, [_i64, _c, C.c_int32, C.c_int32, C.POINTER(PlyTensor), C.POINTER(C.c_int32), _c]),
     "gs_ply_pack": (_i, [_i64, C.c_int32, C.POINTER(PlyTensor), C.POINTER(C.c_int32), C.c_int32, _c, _c]),
+    "gs_layer_norm_forward": (_i, [_i, _i, _i64, _i, _c, _i64, _c, _c, _f, _c, _c, _c, _c]),
+    "gs_layer_norm_workspace_bytes": (_sz, [_i, _i64, _i]),
+    "gs_layer_norm_backward": (_i, [_i, _i, _i64, _i, _c, _i64, _c, _c, _c, _c, _i64, _c, _c, _c, _c, _c]),
+    "gs_attention_workspace_bytes": (_sz, [_i] * 8),
+    "gs_attention_forward": (_i, [_i] * 7 + [_c, C.POINTER(_i64)] * 3 + [_f, _i, _c, _c, _c, C.POINTER(_i64), _c, _c,
+                                                                         _c, _c]),
+    "gs_attention_backward": (_i, [_i] * 7 + [_c, C.POINTER(_i64)] * 3 + [_f, _i, _c, _c, _c, C.POINTER(_i64), _c, _c]
+                              + [_c, C.POINTER(_i64)] * 4 + [_c, _c]),
+    "gs_orthogonalise_workspace_bytes": (_sz, [_i, _i, _i]),
+    "gs_orthogonalise": (_i, [_i, _i, _i, _i, _c, _i, _c, _c, _c]),
+    "gs_momentum_update": (_i, [_i, _i, _i64, C.POINTER(_c), C.POINTER(_c), _f, _i, _c, _c]),
+    "gs_momentum_apply": (_i, [_i, _i, _i64, C.POINTER(_c), _f, _f, _c, _c]),
     "gs_diag_math": (_i, [_i, _i, _c, _c, _c]),
     "gs_timing_enable": (_i, [_i]),
     "gs_timing_reset": (_i, []),
@@ -162,6 +174,23 @@ def ptr(t):
 def stream_of(device=None):
     import torch
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def dtype_code(dtype):
+    """The C ABI's element type of a torch dtype (GS_F32, GS_BF16, GS_F16)."""
+    import torch
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+
+
+def require_tensor(t, name, device=None):
+    """t is a float32, bfloat16 or float16 HIP device tensor (on `device`)."""
+    import torch
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a HIP device tensor (blitzgs_amd has no CPU path)")
+    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} must be on {device}, got {t.device}")
 
 
 def timing_enable(on=True, stages_only=False):

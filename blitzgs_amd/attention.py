@@ -1,0 +1,117 @@
+"""attention: scaled dot-product attention with a backward that recomputes the
+probabilities.
+
+    o = softmax(scale q k^T) v, per head, over the keys that a query sees
+
+q and o are (B, Hq, Tq, D), k and v (B, Hkv, Tk, D); Hq is a multiple of Hkv,
+and query head h reads key head h // (Hq // Hkv).  float32, bfloat16 or
+float16, one type for all; D from 1 to 128.  Any strides are taken as they are
+as long as the last dimension is contiguous, so projections of shape (B, T, H, D)
+and slices of a fused projection are passed as transposed views.
+
+Query i of batch b sees key j when j < key_lengths[b] and, with causal,
+j <= i + query_start[b].  By default the last query sees the last of Tk keys.
+A query that sees no key gives zeros and no gradient, and keys from
+key_lengths on are never read.
+
+Scores, softmax and all sums are fp32; probabilities are rounded to the
+tensors' type for the product with v.  Nothing of size Tq x Tk is stored: a call
+that needs gradients keeps q, k, v, o, one number per query, and in the 16-bit
+types a second part of o.  Equal inputs give equal bits.
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+
+MAX_HEAD_DIM = 128
+
+
+def _strides(t):
+    return (C.c_int64 * 3)(*t.stride()[:3])
+
+
+def _last_contiguous(t):
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _token_major(like):
+    """An empty (B, H, T, D) tensor that lies as (B, T, H, D), ready for the next projection."""
+    B, H, T, D = like.shape
+    return torch.empty((B, T, H, D), device=like.device, dtype=like.dtype).transpose(1, 2)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, causal, key_lengths, query_start, scale):
+        needs = any(ctx.needs_input_grad[:3])
+        q, k, v = (_last_contiguous(t.detach()) for t in (q, k, v))
+        B, Hq, Tq, D = q.shape
+        Hkv, Tk = k.shape[1:3]
+        lib, sizes = _lib.load(), (_lib.dtype_code(q.dtype), B, Hq, Hkv, Tq, Tk, D)
+        o = _token_major(q)
+        lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32) if needs else None
+        # what the rounding of o leaves, for the backward's sum(do o)
+        rest = _token_major(q) if needs and q.dtype != torch.float32 else None
+        ws = torch.empty(lib.gs_attention_workspace_bytes(*sizes, 0), device=q.device, dtype=torch.uint8)
+        with torch.cuda.device(q.device):
+            _lib.check(lib.gs_attention_forward(
+                *sizes, _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), scale,
+                int(causal), _lib.ptr(key_lengths), _lib.ptr(query_start), _lib.ptr(o), _strides(o), _lib.ptr(rest),
+                _lib.ptr(lse), _lib.ptr(ws), _lib.stream_of(q.device)), "gs_attention_forward")
+        if needs:
+            ctx.save_for_backward(q, k, v, o, rest, lse, key_lengths, query_start)
+            ctx.sizes, ctx.scale, ctx.causal = sizes, scale, causal
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, rest, lse, key_lengths, query_start = ctx.saved_tensors
+        lib, do = _lib.load(), _last_contiguous(do)
+        dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
+        ws = torch.empty(lib.gs_attention_workspace_bytes(*ctx.sizes, 1), device=q.device, dtype=torch.uint8)
+        with torch.cuda.device(q.device):
+            _lib.check(lib.gs_attention_backward(
+                *ctx.sizes, _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), ctx.scale,
+                int(ctx.causal), _lib.ptr(key_lengths), _lib.ptr(query_start), _lib.ptr(o), _strides(o),
+                _lib.ptr(rest), _lib.ptr(lse), _lib.ptr(do), _strides(do), _lib.ptr(dq), _strides(dq), _lib.ptr(dk),
+                _strides(dk), _lib.ptr(dv), _strides(dv), _lib.ptr(ws), _lib.stream_of(q.device)), "gs_attention_backward")
+        return dq, dk, dv, None, None, None, None
+
+
+def _per_batch(t, name, q):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != q.device or t.dtype != torch.int32 or t.shape != q.shape[:1]:
+        raise RuntimeError(f"{name} must be an int32 tensor of shape ({q.shape[0]},) on {q.device}")
+    return t.contiguous()
+
+
+def attention(q, k, v, causal=False, key_lengths=None, query_start=None, scale=None):
+    """Attention of q over k and v; differentiable in the three.
+
+    key_lengths, query_start: int32 (B,) on q's device, or None.
+    scale: a positive number; None for 1 / sqrt(D)."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _lib.require_tensor(t, name, device=None if name == "q" else q.device)
+        if t.dim() != 4:
+            raise RuntimeError(f"{name} must have dimensions (B, H, T, D), got shape {tuple(t.shape)}")
+        if t.dtype != q.dtype:
+            raise RuntimeError(f"{name} must be {q.dtype} like q, got {t.dtype}")
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise RuntimeError("k and v must have one shape, with q's batch and head dimension; got q "
+                           f"{tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise RuntimeError(f"q's {q.shape[1]} heads must be a multiple of k's {k.shape[1]}")
+    if not 1 <= q.shape[3] <= MAX_HEAD_DIM:
+        raise RuntimeError(f"the head dimension must be in 1 to {MAX_HEAD_DIM}, got {q.shape[3]}")
+    scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise RuntimeError(f"scale must be a positive number, got {scale}")
+    if query_start is not None and not causal:
+        raise RuntimeError("query_start needs causal=True")
+    return _Attention.apply(q, k, v, bool(causal), _per_batch(key_lengths, "key_lengths", q),
+                            _per_batch(query_start, "query_start", q), scale)

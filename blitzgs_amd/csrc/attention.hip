@@ -1,0 +1,927 @@
+// Scaled dot-product attention, forward and backward.
+//
+//   forward    S = scale q k^T, P = softmax over the keys a row sees, o = P v
+//   backward   delta = sum(do o),  dP = do v^T,  dS = P (dP - delta)
+//              dv = P^T do,  dq = scale dS k,  dk = scale dS^T q
+// Query i of batch b sees key j when j < key_lengths[b] and, when causal,
+// j <= i + query_start[b].  A row that sees no key has o = 0 and no gradient.
+//
+// Nothing of size Tq x Tk is stored.  The forward walks the keys once with the
+// running maximum and sum of the softmax and keeps one number per row, the
+// logarithm (to base 2) of its sum of exponentials; the backward recomputes
+// P = exp2(S scale log2(e) - lse) from it.
+//
+// Layout.  Every product keeps one side in a wave's registers as the columns
+// of 16x16 matrix-core tiles and streams the other side through LDS as rows:
+//   forward, dq: columns = queries.  S^T = k q^T leaves a query's scores in the
+//     four lanes of its column, so the softmax is lane arithmetic with two
+//     exchanges per 64 keys, and P^T is at once the right operand of
+//     o^T = v^T P^T (dq^T = k^T dS^T), without a lane exchange.
+//   dk, dv: columns = keys.  S = q k^T, then dv^T = do^T P and dk^T = q^T dS.
+// The backward is two kernels that recompute S and dP each: seven products in
+// place of five, but no gradient is summed by atomics, so the same inputs give
+// the same bits, and no fp32 copy of dq goes through memory.
+//
+// The query heads that share a key head are rows of one matrix: their keys are
+// read once for all of them, and dk and dv are summed over them in registers.
+//
+// Precision.  Scores, softmax statistics and all sums are fp32.  P and dS are
+// rounded to the tensors' type as operands of the second product: it is the
+// matrix core's operand type, and the error is that of rounding v or k.
+// delta is subtracted from numbers of its own size, where a row looks at few
+// keys, so a 16-bit forward also keeps what the rounding of o left, in as many
+// bits again, and delta is formed from both parts.
+#include <algorithm>
+
+#include "gs_host.h"
+#include "gs_matrix.h"
+#include "../../include/blitzgs_amd.h"
+
+namespace {
+
+using gs::f4;
+using gs::Frag;
+using gs::Stage;
+using gs::Tile;
+
+constexpr int BK = 64;   // rows of a streamed tile
+constexpr float NEG_INF = -__builtin_inff();
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Strides {
+    int64_t b, h, t;
+};
+
+struct AttnArgs {
+    const void *q, *k, *v, *o, *dout;
+    void *out0, *out1;          // forward: o; dq: dq; dkv: dk, dv
+    void* rest;                 // what rounding o to its type left, or null
+    float* lse;                 // [B][Hq][Tq], base 2
+    float* delta;               // [B][Hq][Tq]
+    float* part;                // partial results of a split, or null
+    float* part_ml;             // forward: (maximum, sum) of a split's row
+    const int* key_lengths;
+    const int* query_start;
+    Strides qs, ks, vs, os, dos, s0, s1;
+    int B, Hkv, G, Tq, Tk, D;
+    int causal, splits, tiles;  // tiles: column tiles per (batch, key head)
+    float scale, c;             // c = scale log2(e)
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The sum and maximum over the four lanes of a column.
+__device__ __forceinline__ float column_max(float v)
+{
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float column_sum(float v)
+{
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+__device__ __forceinline__ int length_of(const AttnArgs& A, int b)
+{
+    return A.key_lengths == nullptr ? A.Tk : max(0, min(A.Tk, A.key_lengths[b]));
+}
+__device__ __forceinline__ int64_t start_of(const AttnArgs& A, int b)
+{
+    return A.query_start == nullptr ? (int64_t)A.Tk - A.Tq : A.query_start[b];
+}
+// How many keys query i sees of `len`.
+__device__ __forceinline__ int seen_of(const AttnArgs& A, int len, int64_t start, int i)
+{
+    if (!A.causal) return len;
+    const int64_t n = start + i + 1;
+    return n < 0 ? 0 : n < len ? (int)n : len;
+}
+
+// One column tile of the kernels whose columns are queries.
+struct QueryTile {
+    int b, hk, tile, split, bh;
+    int len, seen_max, seen_min;   // keys that some / every row of the tile sees
+    int t0, t1;                    // key tiles of this split
+    int64_t start;
+};
+
+template <int COLS>
+__device__ __forceinline__ QueryTile query_tile(const AttnArgs& A)
+{
+    QueryTile w;
+    const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x);
+    w.split = (int)(item % (uint32_t)A.splits);
+    const uint32_t rest = item / (uint32_t)A.splits;
+    // causal: the last tiles see the most keys and go first
+    w.tile = A.tiles - 1 - (int)(rest % (uint32_t)A.tiles);
+    w.bh = (int)(rest / (uint32_t)A.tiles);
+    w.b = w.bh / A.Hkv;
+    w.hk = w.bh % A.Hkv;
+    w.len = length_of(A, w.b);
+    w.start = start_of(A, w.b);
+    const int R = A.G * A.Tq, r0 = w.tile * COLS, r1 = min(R, r0 + COLS) - 1;
+    const bool one_head = r0 / A.Tq == r1 / A.Tq;
+    w.seen_max = seen_of(A, w.len, w.start, one_head ? r1 % A.Tq : A.Tq - 1);
+    w.seen_min = seen_of(A, w.len, w.start, one_head ? r0 % A.Tq : 0);
+    const int tiles = (w.seen_max + BK - 1) / BK, per = (tiles + A.splits - 1) / A.splits;
+    w.t0 = min(tiles, w.split * per);
+    w.t1 = min(tiles, w.t0 + per);
+    return w;
+}
+
+// A query column of this lane: its head, position and the keys it sees.
+struct Column {
+    int r, h, i, seen;
+    bool valid;
+};
+
+__device__ __forceinline__ Column column(const AttnArgs& A, const QueryTile& w, int r)
+{
+    Column c;
+    const int R = A.G * A.Tq;
+    c.r = r;
+    c.valid = r < R;
+    const int rr = c.valid ? r : 0;
+    c.h = w.hk * A.G + rr / A.Tq;
+    c.i = rr % A.Tq;
+    c.seen = c.valid ? seen_of(A, w.len, w.start, c.i) : w.len;
+    return c;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f4 v, int n)
+{
+    if (n >= 4) {
+        T t[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) t[r] = (T)v[r];
+        __builtin_memcpy(p, t, 4 * sizeof(T));
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (r < n) p[r] = (T)v[r];
+    }
+}
+
+// Four neighbours of o, and what their rounding leaves.
+template <typename T>
+__device__ __forceinline__ void store_o(T* p, T* rest, f4 v, int n)
+{
+    store4(p, v, n);
+    if (rest == nullptr) return;
+    f4 left;
+#pragma unroll
+    for (int r = 0; r < 4; r++) left[r] = v[r] - (float)(T)v[r];
+    store4(rest, left, n);
+}
+
+// ------------------------------------------------------------------- forward
+
+template <typename T, int DP, int NQ>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
+{
+    using L = Tile<T, DP>;
+    constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NQ, WORDS = BK * L::CHUNKS;
+    extern __shared__ uint4 lds[];   // [2][k tile, v tile]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const QueryTile w = query_tile<COLS>(A);
+    const T* kb = (const T*)A.k + w.b * A.ks.b + w.hk * A.ks.h;
+    const T* vb = (const T*)A.v + w.b * A.vs.b + w.hk * A.vs.h;
+
+    Column col[NQ];
+    Frag<T> q[NQ][KC];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        col[n] = column(A, w, w.tile * COLS + (wave * NQ + n) * 16 + i);
+        const T* p = (const T*)A.q + w.b * A.qs.b + col[n].h * A.qs.h + col[n].i * A.qs.t;
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+            q[n][c] = gs::frag_global<T>(p + 32 * c + 8 * g, col[n].valid ? A.D - 32 * c - 8 * g : 0);
+    }
+    f4 o[DT][NQ];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        m[n] = NEG_INF;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d][n] = f4{0, 0, 0, 0};
+    }
+
+    Stage<T, DP, BK> sk, sv;
+    if (w.t0 < w.t1) {
+        sk.load(kb + (int64_t)w.t0 * BK * A.ks.t, A.ks.t, w.len - w.t0 * BK, A.D);
+        sv.load(vb + (int64_t)w.t0 * BK * A.vs.t, A.vs.t, w.len - w.t0 * BK, A.D);
+        sk.store(lds);
+        sv.store(lds + WORDS);
+    }
+    __syncthreads();
+    for (int t = w.t0; t < w.t1; t++) {
+        const uint4* kt = lds + ((t - w.t0) & 1) * 2 * WORDS;
+        const uint4* vt = kt + WORDS;
+        const int k0 = t * BK;
+        if (t + 1 < w.t1) {
+            sk.load(kb + (int64_t)(t + 1) * BK * A.ks.t, A.ks.t, w.len - k0 - BK, A.D);
+            sv.load(vb + (int64_t)(t + 1) * BK * A.vs.t, A.vs.t, w.len - k0 - BK, A.D);
+        }
+        f4 s[4][NQ];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+#pragma unroll
+            for (int n = 0; n < NQ; n++) s[u][n] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const Frag<T> a = L::rows(kt, 16 * u, 32 * c);
+#pragma unroll
+                for (int n = 0; n < NQ; n++) s[u][n] = gs::mma(a, q[n][c], s[u][n]);
+            }
+        }
+        if (k0 + BK > w.seen_min) {
+#pragma unroll
+            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (k0 + 16 * u + 4 * g + r >= col[n].seen) s[u][n][r] = NEG_INF;
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            float top = s[0][n][0];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) top = fmaxf(top, s[u][n][r]);
+            top = fmaxf(m[n], column_max(top) * A.c);
+            const float base = top == NEG_INF ? 0.0f : top;
+            const float shrink = exp2_fast(m[n] - base);
+            m[n] = top;
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    s[u][n][r] = exp2_fast(__builtin_fmaf(s[u][n][r], A.c, -base));
+                    sum += s[u][n][r];
+                }
+            l[n] = __builtin_fmaf(l[n], shrink, sum);
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d][n] *= shrink;
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            Frag<T> p[NQ];
+#pragma unroll
+            for (int n = 0; n < NQ; n++) p[n] = gs::frag_of_tiles<T>(s[2 * kk][n], s[2 * kk + 1][n]);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const Frag<T> a = L::cols(vt, 32 * kk, 16 * d);
+#pragma unroll
+                for (int n = 0; n < NQ; n++) o[d][n] = gs::mma(a, p[n], o[d][n]);
+            }
+        }
+        if (t + 1 < w.t1) {
+            uint4* next = lds + ((t + 1 - w.t0) & 1) * 2 * WORDS;
+            sk.store(next);
+            sv.store(next + WORDS);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const float sum = column_sum(l[n]);
+        if (!col[n].valid) continue;
+        const int64_t row = (int64_t)w.bh * A.G * A.Tq + col[n].r;   // = (b Hq + h) Tq + i
+        if (A.part != nullptr) {
+            const int64_t at = (int64_t)w.split * A.B * A.Hkv * A.G * A.Tq + row;
+            float* p = A.part + at * A.D;
+#pragma unroll
+            for (int d = 0; d < DT; d++) store4(p + 16 * d + 4 * g, o[d][n], A.D - 16 * d - 4 * g);
+            if (g == 0) {
+                A.part_ml[2 * at] = m[n];
+                A.part_ml[2 * at + 1] = sum;
+            }
+            continue;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int64_t out = w.b * A.s0.b + col[n].h * A.s0.h + col[n].i * A.s0.t;
+        T* rest = A.rest == nullptr ? nullptr : (T*)A.rest + out;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const int at = 16 * d + 4 * g;
+            store_o((T*)A.out0 + out + at, rest == nullptr ? nullptr : rest + at, o[d][n] * inv, A.D - at);
+        }
+        if (g == 0 && A.lse != nullptr) A.lse[row] = sum == 0.0f ? -NEG_INF : m[n] + __builtin_log2f(sum);
+    }
+}
+
+// Joins the splits of a row: one wave per row.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs A)
+{
+    const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63;
+    float m = NEG_INF;
+    for (int s = 0; s < A.splits; s++) m = fmaxf(m, A.part_ml[2 * (s * rows + row)]);
+    const float base = m == NEG_INF ? 0.0f : m;
+    float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    for (int s = 0; s < A.splits; s++) {
+        const int64_t at = s * rows + row;
+        const float f = exp2_fast(A.part_ml[2 * at] - base);
+        sum = __builtin_fmaf(A.part_ml[2 * at + 1], f, sum);
+        if (lane < A.D) o0 = __builtin_fmaf(A.part[at * A.D + lane], f, o0);
+        if (lane + 64 < A.D) o1 = __builtin_fmaf(A.part[at * A.D + lane + 64], f, o1);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int Hq = A.Hkv * A.G, i = (int)(row % A.Tq), h = (int)(row / A.Tq % Hq), b = (int)(row / A.Tq / Hq);
+    const int64_t out = b * A.s0.b + h * A.s0.h + i * A.s0.t;
+    T* p = (T*)A.out0 + out;
+    const float x0 = o0 * inv, x1 = o1 * inv;
+    if (lane < A.D) p[lane] = (T)x0;
+    if (lane + 64 < A.D) p[lane + 64] = (T)x1;
+    if (A.rest != nullptr) {
+        T* rest = (T*)A.rest + out;
+        if (lane < A.D) rest[lane] = (T)(x0 - (float)(T)x0);
+        if (lane + 64 < A.D) rest[lane + 64] = (T)(x1 - (float)(T)x1);
+    }
+    if (lane == 0 && A.lse != nullptr) A.lse[row] = sum == 0.0f ? -NEG_INF : m + __builtin_log2f(sum);
+}
+
+// ------------------------------------------------------------------ backward
+
+// dq, and delta for the other kernel.
+template <typename T, int DP, int NQ>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
+{
+    using L = Tile<T, DP>;
+    constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NQ, WORDS = BK * L::CHUNKS;
+    extern __shared__ uint4 lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const QueryTile w = query_tile<COLS>(A);
+    const T* kb = (const T*)A.k + w.b * A.ks.b + w.hk * A.ks.h;
+    const T* vb = (const T*)A.v + w.b * A.vs.b + w.hk * A.vs.h;
+
+    Column col[NQ];
+    Frag<T> q[NQ][KC], go[NQ][KC];
+    float lse[NQ], delta[NQ];
+    f4 acc[DT][NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        col[n] = column(A, w, w.tile * COLS + (wave * NQ + n) * 16 + i);
+        const T* p = (const T*)A.q + w.b * A.qs.b + col[n].h * A.qs.h + col[n].i * A.qs.t;
+        const T* pg = (const T*)A.dout + w.b * A.dos.b + col[n].h * A.dos.h + col[n].i * A.dos.t;
+        const int64_t oat = w.b * A.os.b + col[n].h * A.os.h + col[n].i * A.os.t;
+        const T* po = (const T*)A.o + oat;
+        const T* pr = (const T*)A.rest + oat;
+        float d = 0.0f;
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            const int at = 32 * c + 8 * g, left = col[n].valid ? A.D - at : 0;
+            q[n][c] = gs::frag_global<T>(p + at, left);
+            go[n][c] = gs::frag_global<T>(pg + at, left);
+            const Frag<T> fo = gs::frag_global<T>(po + at, left);
+            const Frag<T> fr = gs::frag_global<T>(pr + at, A.rest == nullptr ? 0 : left);
+            T a[8], b[8], e[8];
+            __builtin_memcpy(a, &go[n][c], 8 * sizeof(T));
+            __builtin_memcpy(b, &fo, 8 * sizeof(T));
+            __builtin_memcpy(e, &fr, 8 * sizeof(T));
+#pragma unroll
+            for (int j = 0; j < 8; j++) d = __builtin_fmaf((float)a[j], (float)b[j] + (float)e[j], d);
+        }
+        delta[n] = column_sum(d);
+        const int64_t row = (int64_t)w.bh * A.G * A.Tq + col[n].r;
+        lse[n] = col[n].valid ? A.lse[row] : -NEG_INF;
+        if (col[n].valid && g == 0 && w.split == 0) A.delta[row] = delta[n];
+#pragma unroll
+        for (int d2 = 0; d2 < DT; d2++) acc[d2][n] = f4{0, 0, 0, 0};
+    }
+
+    Stage<T, DP, BK> sk, sv;
+    if (w.t0 < w.t1) {
+        sk.load(kb + (int64_t)w.t0 * BK * A.ks.t, A.ks.t, w.len - w.t0 * BK, A.D);
+        sv.load(vb + (int64_t)w.t0 * BK * A.vs.t, A.vs.t, w.len - w.t0 * BK, A.D);
+        sk.store(lds);
+        sv.store(lds + WORDS);
+    }
+    __syncthreads();
+    for (int t = w.t0; t < w.t1; t++) {
+        const uint4* kt = lds + ((t - w.t0) & 1) * 2 * WORDS;
+        const uint4* vt = kt + WORDS;
+        const int k0 = t * BK;
+        if (t + 1 < w.t1) {
+            sk.load(kb + (int64_t)(t + 1) * BK * A.ks.t, A.ks.t, w.len - k0 - BK, A.D);
+            sv.load(vb + (int64_t)(t + 1) * BK * A.vs.t, A.vs.t, w.len - k0 - BK, A.D);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            f4 s[2][NQ], dp[2][NQ];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int n = 0; n < NQ; n++) s[u][n] = dp[u][n] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const Frag<T> a = L::rows(kt, 32 * kk + 16 * u, 32 * c), b = L::rows(vt, 32 * kk + 16 * u, 32 * c);
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) {
+                        s[u][n] = gs::mma(a, q[n][c], s[u][n]);
+                        dp[u][n] = gs::mma(b, go[n][c], dp[u][n]);
+                    }
+                }
+            }
+            const bool part = k0 + BK > w.seen_min;
+            Frag<T> ds[NQ];
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float p = exp2_fast(__builtin_fmaf(s[u][n][r], A.c, -lse[n]));
+                        float x = p * (dp[u][n][r] - delta[n]);
+                        if (part && k0 + 32 * kk + 16 * u + 4 * g + r >= col[n].seen) x = 0.0f;
+                        s[u][n][r] = x;
+                    }
+                ds[n] = gs::frag_of_tiles<T>(s[0][n], s[1][n]);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const Frag<T> a = L::cols(kt, 32 * kk, 16 * d);
+#pragma unroll
+                for (int n = 0; n < NQ; n++) acc[d][n] = gs::mma(a, ds[n], acc[d][n]);
+            }
+        }
+        if (t + 1 < w.t1) {
+            uint4* next = lds + ((t + 1 - w.t0) & 1) * 2 * WORDS;
+            sk.store(next);
+            sv.store(next + WORDS);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        if (!col[n].valid) continue;
+        if (A.part != nullptr) {
+            const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
+            float* p = A.part + (w.split * rows + (int64_t)w.bh * A.G * A.Tq + col[n].r) * A.D;
+#pragma unroll
+            for (int d = 0; d < DT; d++) store4(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+        } else {
+            T* p = (T*)A.out0 + w.b * A.s0.b + col[n].h * A.s0.h + col[n].i * A.s0.t;
+#pragma unroll
+            for (int d = 0; d < DT; d++) store4(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+        }
+    }
+}
+
+// dk and dv.  A wave holds 16 NK keys; the block streams the queries of every
+// head that shares them, QT rows at a time.
+template <typename T, int DP, int NK, int QT>
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
+{
+    using L = Tile<T, DP>;
+    constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NK, WORDS = QT * L::CHUNKS, BUF = 2 * WORDS + QT / 2;
+    extern __shared__ uint4 lds[];   // [2][q tile, do tile, lse[QT], delta[QT]]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x);
+    const int split = (int)(item % (uint32_t)A.splits);
+    const uint32_t rest = item / (uint32_t)A.splits;
+    const int tile = (int)(rest % (uint32_t)A.tiles), bh = (int)(rest / (uint32_t)A.tiles);
+    const int b = bh / A.Hkv, hk = bh % A.Hkv, len = length_of(A, b), key0 = tile * COLS;
+    const int64_t start = start_of(A, b);
+
+    Frag<T> k[NK][KC], v[NK][KC];
+    f4 dk[DT][NK], dv[DT][NK];
+    int key[NK];
+#pragma unroll
+    for (int n = 0; n < NK; n++) {
+        key[n] = key0 + (wave * NK + n) * 16 + i;
+        const bool held = key[n] < len;
+        const T* pk = (const T*)A.k + b * A.ks.b + hk * A.ks.h + (int64_t)(held ? key[n] : 0) * A.ks.t;
+        const T* pv = (const T*)A.v + b * A.vs.b + hk * A.vs.h + (int64_t)(held ? key[n] : 0) * A.vs.t;
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            const int at = 32 * c + 8 * g, left = held ? A.D - at : 0;
+            k[n][c] = gs::frag_global<T>(pk + at, left);
+            v[n][c] = gs::frag_global<T>(pv + at, left);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++) dk[d][n] = dv[d][n] = f4{0, 0, 0, 0};
+    }
+
+    // the first query tile that sees the block's first key
+    const int64_t first = A.causal ? (int64_t)key0 - start : 0;
+    const int tiles = (A.Tq + QT - 1) / QT;
+    const int from = key0 >= len ? tiles : first <= 0 ? 0 : first >= A.Tq ? tiles : (int)first / QT;
+    const int per_head = tiles - from, total = per_head * A.G, per = (total + A.splits - 1) / A.splits;
+    const int e0 = min(total, split * per), e1 = min(total, e0 + per);
+
+    Stage<T, DP, QT> sq, sg;
+    float stat = 0.0f;   // threads 0 .. QT - 1: lse, QT .. 2 QT - 1: delta
+    auto fetch = [&](int e) {
+        const int h = hk * A.G + e / per_head, q0 = (from + e % per_head) * QT, n = A.Tq - q0;
+        sq.load((const T*)A.q + b * A.qs.b + h * A.qs.h + (int64_t)q0 * A.qs.t, A.qs.t, n, A.D);
+        sg.load((const T*)A.dout + b * A.dos.b + h * A.dos.h + (int64_t)q0 * A.dos.t, A.dos.t, n, A.D);
+        if (threadIdx.x < 2 * QT) {
+            const int r = threadIdx.x % QT;
+            const int64_t row = ((int64_t)b * A.Hkv * A.G + h) * A.Tq + q0 + r;
+            if (threadIdx.x < QT) stat = r < n ? A.lse[row] : -NEG_INF;
+            else stat = r < n ? A.delta[row] : 0.0f;
+        }
+    };
+    auto put = [&](uint4* to) {
+        sq.store(to);
+        sg.store(to + WORDS);
+        if (threadIdx.x < 2 * QT) ((float*)(to + 2 * WORDS))[threadIdx.x] = stat;
+    };
+    if (e0 < e1) {
+        fetch(e0);
+        put(lds);
+    }
+    __syncthreads();
+    for (int e = e0; e < e1; e++) {
+        const uint4* qt = lds + ((e - e0) & 1) * BUF;
+        const uint4* gt = qt + WORDS;
+        const float* st = (const float*)(gt + WORDS);
+        const int q0 = (from + e % per_head) * QT;
+        if (e + 1 < e1) fetch(e + 1);
+        const bool part = A.causal && start + q0 < (int64_t)key0 + COLS - 1;
+#pragma unroll
+        for (int kk = 0; kk < QT / 32; kk++) {
+            f4 s[2][NK], dp[2][NK];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int n = 0; n < NK; n++) s[u][n] = dp[u][n] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const Frag<T> a = L::rows(qt, 32 * kk + 16 * u, 32 * c), d = L::rows(gt, 32 * kk + 16 * u, 32 * c);
+#pragma unroll
+                    for (int n = 0; n < NK; n++) {
+                        s[u][n] = gs::mma(a, k[n][c], s[u][n]);
+                        dp[u][n] = gs::mma(d, v[n][c], dp[u][n]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int r0 = 32 * kk + 16 * u + 4 * g;
+                const f4 lse = *(const f4*)(st + r0), delta = *(const f4*)(st + QT + r0);
+#pragma unroll
+                for (int n = 0; n < NK; n++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        float p = exp2_fast(__builtin_fmaf(s[u][n][r], A.c, -lse[r]));
+                        float x = p * (dp[u][n][r] - delta[r]);
+                        if (part && key[n] > start + q0 + r0 + r) p = x = 0.0f;
+                        s[u][n][r] = p;
+                        dp[u][n][r] = x;
+                    }
+            }
+            Frag<T> fp[NK], fs[NK];
+#pragma unroll
+            for (int n = 0; n < NK; n++) {
+                fp[n] = gs::frag_of_tiles<T>(s[0][n], s[1][n]);
+                fs[n] = gs::frag_of_tiles<T>(dp[0][n], dp[1][n]);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const Frag<T> a = L::cols(gt, 32 * kk, 16 * d), c = L::cols(qt, 32 * kk, 16 * d);
+#pragma unroll
+                for (int n = 0; n < NK; n++) {
+                    dv[d][n] = gs::mma(a, fp[n], dv[d][n]);
+                    dk[d][n] = gs::mma(c, fs[n], dk[d][n]);
+                }
+            }
+        }
+        if (e + 1 < e1) put(lds + ((e + 1 - e0) & 1) * BUF);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NK; n++) {
+        if (key[n] >= A.Tk) continue;
+        const bool held = key[n] < len;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const int at = 16 * d + 4 * g, left = A.D - at;
+            const f4 xk = held ? dk[d][n] * A.scale : f4{0, 0, 0, 0}, xv = held ? dv[d][n] : f4{0, 0, 0, 0};
+            if (A.part != nullptr) {
+                const int64_t rows = (int64_t)A.B * A.Hkv * A.Tk, row = (int64_t)bh * A.Tk + key[n];
+                store4(A.part + (2 * split * rows + row) * A.D + at, xk, left);
+                store4(A.part + ((2 * split + 1) * rows + row) * A.D + at, xv, left);
+            } else {
+                store4((T*)A.out0 + b * A.s0.b + hk * A.s0.h + (int64_t)key[n] * A.s0.t + at, xk, left);
+                store4((T*)A.out1 + b * A.s1.b + hk * A.s1.h + (int64_t)key[n] * A.s1.t + at, xv, left);
+            }
+        }
+    }
+}
+
+// Adds the splits' partial gradients: [splits][per][rows = B H Tn][D] to each of
+// `per` tensors.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__ part, int splits, int per, int64_t rows,
+                                                       int H, int Tn, int D, T* out0, T* out1, Strides s0, Strides s1)
+{
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= rows * D) return;
+    const int64_t row = id / D;
+    const int d = (int)(id - row * D), t = (int)(row % Tn), h = (int)(row / Tn % H), b = (int)(row / Tn / H);
+    const int which = blockIdx.y;
+    float s = 0.0f;
+    for (int k = 0; k < splits; k++) s += part[((int64_t)k * per + which) * rows * D + id];
+    const Strides st = which == 0 ? s0 : s1;
+    (which == 0 ? out0 : out1)[b * st.b + h * st.h + t * st.t + d] = (T)s;
+}
+
+// ------------------------------------------------------------------ launching
+
+// Workgroups that keep the chip's 256 CUs busy at two per CU, with a second
+// round to even out their ends.
+constexpr int ENOUGH = 1024;
+
+int padded(int D) { return (D + 31) / 32 * 32; }
+
+// Splits of a walk of `steps` tiles when there are `blocks` column tiles: as
+// many as fill the chip, none shorter than four tiles.
+int splits_of(int64_t blocks, int steps)
+{
+    if (blocks >= ENOUGH / 2 || steps < 8) return 1;
+    const int64_t want = (ENOUGH + blocks - 1) / blocks;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));
+}
+
+// How the three walks of one problem are cut.
+struct Plan {
+    int nq, nk, tiles_q, tiles_k, splits_f, splits_q, splits_k, qt;
+    size_t fwd_bytes, bwd_bytes;
+};
+
+Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D)
+{
+    Plan p{};
+    const int DP = padded(D);
+    const int64_t heads = (int64_t)B * Hkv, rows = (int64_t)G * Tq;
+    // 32 columns per wave halve the LDS reads per product; 16 where the
+    // registers do not hold 32, or where 32 would leave CUs without work
+    const bool wide = !(type == GS_F32 && DP > 64);
+    p.nq = wide && heads * ((rows + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
+    p.nk = wide && DP <= 64 && heads * (((int64_t)Tk + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
+    p.qt = 64;
+    p.tiles_q = (int)((rows + 64 * p.nq - 1) / (64 * p.nq));
+    p.tiles_k = (int)(((int64_t)Tk + 64 * p.nk - 1) / (64 * p.nk));
+    p.splits_f = p.splits_q = splits_of(heads * p.tiles_q, (Tk + BK - 1) / BK);
+    p.splits_k = splits_of(heads * p.tiles_k, (int)std::min<int64_t>((int64_t)G * ((Tq + p.qt - 1) / p.qt), 1 << 20));
+    const size_t all = (size_t)heads * (size_t)rows;
+    p.fwd_bytes = p.splits_f > 1 ? (size_t)p.splits_f * all * (size_t)(D + 2) * 4 : 0;
+    const size_t dq = p.splits_q > 1 ? (size_t)p.splits_q * all * (size_t)D * 4 : 0;
+    const size_t dkv = p.splits_k > 1 ? (size_t)p.splits_k * 2 * (size_t)heads * (size_t)Tk * (size_t)D * 4 : 0;
+    p.bwd_bytes = (all * 4 + 255) / 256 * 256 + std::max(dq, dkv);   // delta, then one walk's partial results
+    return p;
+}
+
+template <typename K>
+int launch(const char* name, K kernel, int64_t blocks, size_t lds, const AttnArgs& A, hipStream_t stream)
+{
+    GS_REQUIRE(blocks < 0x7fffffff, "attention: too many workgroups");
+    if (lds > 65536)
+        GS_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    GS_TIMED(name, stream, hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, stream, A));
+    GS_LAUNCH_CHECK(name);
+    return GS_OK;
+}
+
+template <typename T, int DP, int NQ>
+int forward_one(const AttnArgs& A, hipStream_t stream)
+{
+    const size_t lds = (size_t)4 * BK * Tile<T, DP>::CHUNKS * 16;
+    return launch("attn_fwd_kernel", attn_fwd_kernel<T, DP, NQ>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
+                  stream);
+}
+
+template <typename T, int DP, int NQ>
+int dq_one(const AttnArgs& A, hipStream_t stream)
+{
+    const size_t lds = (size_t)4 * BK * Tile<T, DP>::CHUNKS * 16;
+    return launch("attn_dq_kernel", attn_dq_kernel<T, DP, NQ>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
+                  stream);
+}
+
+template <typename T, int DP, int NK>
+int dkv_one(const AttnArgs& A, hipStream_t stream)
+{
+    constexpr int QT = 64;
+    const size_t lds = (size_t)2 * (2 * QT * Tile<T, DP>::CHUNKS + QT / 2) * 16;
+    return launch("attn_dkv_kernel", attn_dkv_kernel<T, DP, NK, QT>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
+                  stream);
+}
+
+enum Walk { FORWARD, DQ, DKV };
+
+template <Walk W, typename T, int DP>
+int run_width(const AttnArgs& A, int wide, hipStream_t stream)
+{
+    constexpr bool TWO = !(sizeof(T) == 4 && DP > 64);
+    if constexpr (W == FORWARD) {
+        if constexpr (TWO)
+            if (wide == 2) return forward_one<T, DP, 2>(A, stream);
+        return forward_one<T, DP, 1>(A, stream);
+    } else if constexpr (W == DQ) {
+        if constexpr (TWO)
+            if (wide == 2) return dq_one<T, DP, 2>(A, stream);
+        return dq_one<T, DP, 1>(A, stream);
+    } else {
+        if constexpr (DP <= 64)
+            if (wide == 2) return dkv_one<T, DP, 2>(A, stream);
+        return dkv_one<T, DP, 1>(A, stream);
+    }
+}
+
+template <Walk W, typename T>
+int run_type(const AttnArgs& A, int wide, hipStream_t stream)
+{
+    switch (padded(A.D)) {
+        case 32: return run_width<W, T, 32>(A, wide, stream);
+        case 64: return run_width<W, T, 64>(A, wide, stream);
+        case 96: return run_width<W, T, 96>(A, wide, stream);
+        default: return run_width<W, T, 128>(A, wide, stream);
+    }
+}
+
+template <Walk W>
+int run(int type, const AttnArgs& A, int wide, hipStream_t stream)
+{
+    if (type == GS_F32) return run_type<W, float>(A, wide, stream);
+    if (type == GS_BF16) return run_type<W, gs::bf16>(A, wide, stream);
+    return run_type<W, gs::f16>(A, wide, stream);
+}
+
+template <typename T>
+void join(const AttnArgs& A, hipStream_t stream)
+{
+    const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
+    GS_TIMED("attn_join_kernel", stream,
+             hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, A));
+}
+
+template <typename T>
+void add(const AttnArgs& A, int per, int H, int Tn, hipStream_t stream)
+{
+    const int64_t rows = (int64_t)A.B * H * Tn, blocks = (rows * A.D + 255) / 256;
+    GS_TIMED("attn_add_kernel", stream,
+             hipLaunchKernelGGL(attn_add_kernel<T>, dim3((unsigned)blocks, (unsigned)per), dim3(256), 0, stream, A.part,
+                                A.splits, per, rows, H, Tn, A.D, (T*)A.out0, (T*)A.out1, A.s0, A.s1));
+}
+
+Strides strides_of(const int64_t* s) { return {s[0], s[1], s[2]}; }
+
+int check(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, float scale)
+{
+    GS_REQUIRE(gs::dtype_known(type), "attention: unknown element type %d", type);
+    GS_REQUIRE(B >= 0 && Tq >= 0 && Tk >= 0, "attention: sizes must not be negative");
+    GS_REQUIRE(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0,
+               "attention: the number of query heads (%d) must be a multiple of the number of key heads (%d)", Hq, Hkv);
+    GS_REQUIRE(D >= 1 && D <= 128, "attention: the head dimension must be in [1, 128], got %d", D);
+    GS_REQUIRE(scale > 0.0f && scale <= 3.0e38f, "attention: scale must be a positive number");
+    GS_REQUIRE((int64_t)(Hq / Hkv) * Tq < 0x7fffff00ll && Tk < 0x7fffff00,
+               "attention: too many queries or keys for one head");
+    GS_REQUIRE((int64_t)B * Hq * Tq < (1ll << 32) && (int64_t)B * Hkv * Tk < (1ll << 32),
+               "attention: too many rows");
+    return GS_OK;
+}
+
+AttnArgs args_of(int B, int Hq, int Hkv, int Tq, int Tk, int D, float scale, int causal, const int* key_lengths,
+                 const int* query_start)
+{
+    AttnArgs A{};
+    A.B = B;
+    A.Hkv = Hkv;
+    A.G = Hq / Hkv;
+    A.Tq = Tq;
+    A.Tk = Tk;
+    A.D = D;
+    A.scale = scale;
+    A.c = scale * LOG2E;
+    A.causal = causal != 0;
+    A.key_lengths = key_lengths;
+    A.query_start = query_start;
+    return A;
+}
+
+}  // namespace
+
+extern "C" size_t gs_attention_workspace_bytes(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, int backward)
+{
+    if (check(type, B, Hq, Hkv, Tq, Tk, D, 1.0f) != GS_OK) return 0;
+    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D);
+    return std::max<size_t>(256, backward ? p.bwd_bytes : p.fwd_bytes);
+}
+
+extern "C" int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, const void* q,
+                                    const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                    const int64_t* v_strides, float scale, int causal, const int* key_lengths,
+                                    const int* query_start, void* o, const int64_t* o_strides, void* o_rest,
+                                    float* lse, void* workspace, hipStream_t stream)
+{
+    gs::clear_error();
+    if (int rc = check(type, B, Hq, Hkv, Tq, Tk, D, scale)) return rc;
+    if (B == 0 || Tq == 0) return GS_OK;
+    GS_REQUIRE(q && o && q_strides && k_strides && v_strides && o_strides, "attention: q, o and all strides must be given");
+    GS_REQUIRE(Tk == 0 || (k && v), "attention: k and v must be non-null");
+    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D);
+    GS_REQUIRE(p.splits_f == 1 || workspace != nullptr, "attention: this size needs the workspace");
+    AttnArgs A = args_of(B, Hq, Hkv, Tq, Tk, D, scale, causal, key_lengths, query_start);
+    A.q = q;
+    A.k = k;
+    A.v = v;
+    A.out0 = o;
+    A.rest = o_rest;
+    A.lse = lse;
+    A.qs = strides_of(q_strides);
+    A.ks = strides_of(k_strides);
+    A.vs = strides_of(v_strides);
+    A.s0 = strides_of(o_strides);
+    A.splits = p.splits_f;
+    A.tiles = p.tiles_q;
+    if (A.splits > 1) {
+        A.part = (float*)workspace;
+        A.part_ml = A.part + (size_t)A.splits * B * Hq * (size_t)Tq * D;
+    }
+    if (int rc = run<FORWARD>(type, A, p.nq, stream)) return rc;
+    if (A.splits > 1) {
+        if (type == GS_F32) join<float>(A, stream);
+        else if (type == GS_BF16) join<gs::bf16>(A, stream);
+        else join<gs::f16>(A, stream);
+        GS_LAUNCH_CHECK("attn_join_kernel");
+    }
+    return GS_OK;
+}
+
+extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, const void* q,
+                                     const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                     const int64_t* v_strides, float scale, int causal, const int* key_lengths,
+                                     const int* query_start, const void* o, const int64_t* o_strides, const void* o_rest,
+                                     const float* lse, const void* dout, const int64_t* dout_strides, void* dq, const int64_t* dq_strides,
+                                     void* dk, const int64_t* dk_strides, void* dv, const int64_t* dv_strides,
+                                     void* workspace, hipStream_t stream)
+{
+    gs::clear_error();
+    if (int rc = check(type, B, Hq, Hkv, Tq, Tk, D, scale)) return rc;
+    if (B == 0 || (Tq == 0 && Tk == 0)) return GS_OK;
+    GS_REQUIRE(q_strides && k_strides && v_strides && o_strides && dout_strides && dq_strides && dk_strides &&
+                   dv_strides,
+               "attention: all strides must be given");
+    GS_REQUIRE(workspace != nullptr, "attention: the backward needs the workspace");
+    GS_REQUIRE(Tq == 0 || (q && o && lse && dout && dq), "attention: q, o, lse, dout and dq must be non-null");
+    GS_REQUIRE(Tk == 0 || (k && v && dk && dv), "attention: k, v, dk and dv must be non-null");
+    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D);
+    AttnArgs A = args_of(B, Hq, Hkv, Tq, Tk, D, scale, causal, key_lengths, query_start);
+    A.q = q;
+    A.k = k;
+    A.v = v;
+    A.o = o;
+    A.rest = const_cast<void*>(o_rest);
+    A.dout = dout;
+    A.lse = const_cast<float*>(lse);
+    A.delta = (float*)workspace;
+    A.qs = strides_of(q_strides);
+    A.ks = strides_of(k_strides);
+    A.vs = strides_of(v_strides);
+    A.os = strides_of(o_strides);
+    A.dos = strides_of(dout_strides);
+    float* part = (float*)((char*)workspace + ((size_t)B * Hq * (size_t)Tq * 4 + 255) / 256 * 256);
+    auto add_all = [&](int per, int H, int Tn) {
+        if (type == GS_F32) add<float>(A, per, H, Tn, stream);
+        else if (type == GS_BF16) add<gs::bf16>(A, per, H, Tn, stream);
+        else add<gs::f16>(A, per, H, Tn, stream);
+    };
+    if (Tq > 0) {
+        A.out0 = dq;
+        A.s0 = strides_of(dq_strides);
+        A.splits = p.splits_q;
+        A.tiles = p.tiles_q;
+        A.part = A.splits > 1 ? part : nullptr;
+        if (int rc = run<DQ>(type, A, p.nq, stream)) return rc;
+        if (A.splits > 1) {
+            add_all(1, Hq, Tq);
+            GS_LAUNCH_CHECK("attn_add_kernel");
+        }
+    }
+    if (Tk > 0) {
+        A.out0 = dk;
+        A.out1 = dv;
+        A.s0 = strides_of(dk_strides);
+        A.s1 = strides_of(dv_strides);
+        A.splits = p.splits_k;
+        A.tiles = p.tiles_k;
+        A.part = A.splits > 1 ? part : nullptr;
+        if (int rc = run<DKV>(type, A, p.nk, stream)) return rc;
+        if (A.splits > 1) {
+            add_all(2, Hkv, Tk);
+            GS_LAUNCH_CHECK("attn_add_kernel");
+        }
+    }
+    return GS_OK;
+}

@@ -643,6 +643,88 @@ int gs_ply_pack(int64_t P, int32_t n_tensors, const gs_ply_tensor* tensors, cons
 int gs_diag_math(int op, int n, const float* x, float* y, gs_stream_t stream);
 
 /* ------------------------------------------------------------------------ *
+ * Operators of a token network that predicts Gaussians and is trained through
+ * the rasterizer.  They have no counterpart in the reference.  Tensors are of
+ * one element type, GS_F32, GS_BF16 or GS_F16; every sum is fp32.
+ * ------------------------------------------------------------------------ */
+#define GS_F32 0
+#define GS_BF16 1
+#define GS_F16 2
+
+/* Layer normalisation of `rows` rows of `width` (1 to 32768) elements:
+ *   z = (x - mean) / sqrt(var + eps),  y = weight z + bias
+ * x's rows are x_stride elements apart (0: one row for all), contiguous
+ * inside; y, dx are contiguous.  weight and bias (width, either may be NULL)
+ * are of param_type: `type` or GS_F32.  mean and rstd (rows) are written for
+ * the backward, or both NULL.
+ * Backward: dx always; dweight and dbias (width, of param_type) unless NULL,
+ * added up in a fixed order through the workspace of
+ * gs_layer_norm_workspace_bytes (0 bytes: invalid arguments). */
+int gs_layer_norm_forward(int type, int param_type, int64_t rows, int width, const void* x,
+                          int64_t x_stride, const void* weight, const void* bias, float eps, void* y,
+                          float* mean, float* rstd, gs_stream_t stream);
+size_t gs_layer_norm_workspace_bytes(int type, int64_t rows, int width);
+int gs_layer_norm_backward(int type, int param_type, int64_t rows, int width, const void* x,
+                           int64_t x_stride, const void* weight, const float* mean, const float* rstd,
+                           const void* dy, int64_t dy_stride, void* dx, void* dweight, void* dbias,
+                           void* workspace, gs_stream_t stream);
+
+/* Attention: o = softmax(scale q k^T) v per head, q and o (B, Hq, Tq, D), k and
+ * v (B, Hkv, Tk, D), Hq a multiple of Hkv (query head h reads key head
+ * h / (Hq / Hkv)), D from 1 to 128.  Each tensor comes with three strides in
+ * elements, of its batch, head and token dimension; D is contiguous.
+ *   Query i of batch b sees key j when j < key_lengths[b] (device int32 (B),
+ * clamped to [0, Tk]; NULL: Tk) and, if causal, j <= i + query_start[b]
+ * (device int32 (B); NULL: Tk - Tq).  Keys from key_lengths on are not read; a
+ * row that sees no key gives zeros.  Among the keys below the length, values
+ * that a row does not see must be finite.
+ *   lse (B, Hq, Tq) fp32, may be NULL: the base-2 logarithm of each row's sum of
+ * exponentials (+inf for a row that sees no key), which the backward takes.
+ *   o_rest, with o's strides and type, may be NULL: o's value before its
+ * rounding less o.  A backward that is given it forms sum(do o) from both; with
+ * GS_F32 there is nothing to keep.
+ *   The workspace's size (gs_attention_workspace_bytes, 0: invalid arguments)
+ * depends on sizes alone.  Results do not depend on the order of execution. */
+size_t gs_attention_workspace_bytes(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D,
+                                    int backward);
+int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, const void* q,
+                         const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                         const void* v, const int64_t* v_strides, float scale, int causal,
+                         const int* key_lengths, const int* query_start, void* o,
+                         const int64_t* o_strides, void* o_rest, float* lse, void* workspace,
+                         gs_stream_t stream);
+int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, const void* q,
+                          const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          const void* v, const int64_t* v_strides, float scale, int causal,
+                          const int* key_lengths, const int* query_start, const void* o,
+                          const int64_t* o_strides, const void* o_rest, const float* lse,
+                          const void* dout,
+                          const int64_t* dout_strides, void* dq, const int64_t* dq_strides, void* dk,
+                          const int64_t* dk_strides, void* dv, const int64_t* dv_strides,
+                          void* workspace, gs_stream_t stream);
+
+/* The orthogonalised update of `count` matrices (m, n), contiguous: `steps` (1
+ * to 32) steps of A = X X^T, X = a X + (b A + c A A) X with (a, b, c) =
+ * (3.4445, -4.7750, 2.0315) from X = update / (|update|_F + 1e-7), over the
+ * shorter side's rows; products with fp32's accuracy.  out may not overlap
+ * update.  Sides and count up to 65536 and 65535.  workspace: 256-byte aligned,
+ * of gs_orthogonalise_workspace_bytes (0: invalid arguments). */
+size_t gs_orthogonalise_workspace_bytes(int count, int m, int n);
+int gs_orthogonalise(int type, int count, int m, int n, const void* update, int steps, void* out,
+                     void* workspace, gs_stream_t stream);
+
+/* The momentum step around it, for up to 32 tensors of `size` elements; the
+ * pointer arrays are host arrays of device pointers.
+ *   update: momentum = beta momentum + grad, and update[i] (fp32, stacked) =
+ *           nesterov ? grad + beta momentum : momentum
+ *   apply:  param = param keep - lr update[i] */
+int gs_momentum_update(int type, int count, int64_t size, const void* const* grads,
+                       float* const* momenta, float beta, int nesterov, float* update,
+                       gs_stream_t stream);
+int gs_momentum_apply(int type, int count, int64_t size, void* const* params, float keep, float lr,
+                      const float* update, gs_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
  * Per-kernel timing (the counterpart of the reference's MyTimerOnGPU,
  * diff-gaussian-rasterization_r/cuda_rasterizer/timers.cu:11-79).  on = 1:
  * every kernel launch is bracketed by HIP events on its stream, and so are
