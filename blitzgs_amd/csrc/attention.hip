@@ -46,6 +46,7 @@ using gs::Tile;
 
 constexpr int BK = 64;   // rows of a streamed tile
 constexpr float NEG_INF = -__builtin_inff();
+constexpr float SLACK = 8.0f;   // of the softmax's running base, in powers of two
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Strides {
@@ -149,10 +150,12 @@ __device__ __forceinline__ Column column(const AttnArgs& A, const QueryTile& w, 
     return c;
 }
 
-template <typename T>
+// The first n of four neighbours; unless ODD, all of them or none.
+template <bool ODD, typename T>
 __device__ __forceinline__ void store4(T* p, f4 v, int n)
 {
-    if (n >= 4) {
+    if constexpr (!ODD) {
+        if (n <= 0) return;
         T t[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) t[r] = (T)v[r];
@@ -165,26 +168,27 @@ __device__ __forceinline__ void store4(T* p, f4 v, int n)
 }
 
 // Four neighbours of o, and what their rounding leaves.
-template <typename T>
+template <bool ODD, typename T>
 __device__ __forceinline__ void store_o(T* p, T* rest, f4 v, int n)
 {
-    store4(p, v, n);
+    store4<ODD>(p, v, n);
     if (rest == nullptr) return;
     f4 left;
 #pragma unroll
     for (int r = 0; r < 4; r++) left[r] = v[r] - (float)(T)v[r];
-    store4(rest, left, n);
+    store4<ODD>(rest, left, n);
 }
 
 // ------------------------------------------------------------------- forward
 
-template <typename T, int DP, int NQ>
+template <typename T, int DP, int NQ, bool ODD>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NQ, WORDS = BK * L::CHUNKS;
     extern __shared__ uint4 lds[];   // [2][k tile, v tile]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const L tile_of;
     const QueryTile w = query_tile<COLS>(A);
     const T* kb = (const T*)A.k + w.b * A.ks.b + w.hk * A.ks.h;
     const T* vb = (const T*)A.v + w.b * A.vs.b + w.hk * A.vs.h;
@@ -197,7 +201,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
         const T* p = (const T*)A.q + w.b * A.qs.b + col[n].h * A.qs.h + col[n].i * A.qs.t;
 #pragma unroll
         for (int c = 0; c < KC; c++)
-            q[n][c] = gs::frag_global<T>(p + 32 * c + 8 * g, col[n].valid ? A.D - 32 * c - 8 * g : 0);
+            q[n][c] = gs::frag_global<T, ODD>(p + 32 * c + 8 * g, col[n].valid ? A.D - 32 * c - 8 * g : 0);
     }
     f4 o[DT][NQ];
     float m[NQ], l[NQ];
@@ -209,7 +213,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
         for (int d = 0; d < DT; d++) o[d][n] = f4{0, 0, 0, 0};
     }
 
-    Stage<T, DP, BK> sk, sv;
+    Stage<T, DP, BK, ODD> sk, sv;
     if (w.t0 < w.t1) {
         sk.load(kb + (int64_t)w.t0 * BK * A.ks.t, A.ks.t, w.len - w.t0 * BK, A.D);
         sv.load(vb + (int64_t)w.t0 * BK * A.vs.t, A.vs.t, w.len - w.t0 * BK, A.D);
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
             for (int n = 0; n < NQ; n++) s[u][n] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < KC; c++) {
-                const Frag<T> a = L::rows(kt, 16 * u, 32 * c);
+                const Frag<T> a = tile_of.rows(kt, 16 * u, 32 * c);
 #pragma unroll
                 for (int n = 0; n < NQ; n++) s[u][n] = gs::mma(a, q[n][c], s[u][n]);
             }
@@ -253,10 +257,18 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
             for (int u = 0; u < 4; u++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) top = fmaxf(top, s[u][n][r]);
-            top = fmaxf(m[n], column_max(top) * A.c);
-            const float base = top == NEG_INF ? 0.0f : top;
-            const float shrink = exp2_fast(m[n] - base);
-            m[n] = top;
+            top = column_max(top) * A.c;
+            // the base follows the maximum once that is 2^8 above it: sums and
+            // products in between are larger by that much, which costs nothing
+            if (__any(top > m[n] + SLACK)) {
+                const float next = fmaxf(m[n], top);
+                const float shrink = next == NEG_INF ? 1.0f : exp2_fast(m[n] - next);
+                m[n] = next;
+                l[n] *= shrink;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d][n] *= shrink;
+            }
+            const float base = m[n] == NEG_INF ? 0.0f : m[n];
             float sum = 0.0f;
 #pragma unroll
             for (int u = 0; u < 4; u++)
@@ -265,9 +277,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
                     s[u][n][r] = exp2_fast(__builtin_fmaf(s[u][n][r], A.c, -base));
                     sum += s[u][n][r];
                 }
-            l[n] = __builtin_fmaf(l[n], shrink, sum);
-#pragma unroll
-            for (int d = 0; d < DT; d++) o[d][n] *= shrink;
+            l[n] += sum;
         }
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
@@ -276,7 +286,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
             for (int n = 0; n < NQ; n++) p[n] = gs::frag_of_tiles<T>(s[2 * kk][n], s[2 * kk + 1][n]);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const Frag<T> a = L::cols(vt, 32 * kk, 16 * d);
+                const Frag<T> a = tile_of.cols(vt, 32 * kk, 16 * d);
 #pragma unroll
                 for (int n = 0; n < NQ; n++) o[d][n] = gs::mma(a, p[n], o[d][n]);
             }
@@ -297,7 +307,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
             const int64_t at = (int64_t)w.split * A.B * A.Hkv * A.G * A.Tq + row;
             float* p = A.part + at * A.D;
 #pragma unroll
-            for (int d = 0; d < DT; d++) store4(p + 16 * d + 4 * g, o[d][n], A.D - 16 * d - 4 * g);
+            for (int d = 0; d < DT; d++) store4<ODD>(p + 16 * d + 4 * g, o[d][n], A.D - 16 * d - 4 * g);
             if (g == 0) {
                 A.part_ml[2 * at] = m[n];
                 A.part_ml[2 * at + 1] = sum;
@@ -310,7 +320,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             const int at = 16 * d + 4 * g;
-            store_o((T*)A.out0 + out + at, rest == nullptr ? nullptr : rest + at, o[d][n] * inv, A.D - at);
+            store_o<ODD>((T*)A.out0 + out + at, rest == nullptr ? nullptr : rest + at, o[d][n] * inv, A.D - at);
         }
         if (g == 0 && A.lse != nullptr) A.lse[row] = sum == 0.0f ? -NEG_INF : m[n] + __builtin_log2f(sum);
     }
@@ -352,13 +362,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs A)
 // ------------------------------------------------------------------ backward
 
 // dq, and delta for the other kernel.
-template <typename T, int DP, int NQ>
+template <typename T, int DP, int NQ, bool ODD>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NQ, WORDS = BK * L::CHUNKS;
     extern __shared__ uint4 lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const L tile_of;
     const QueryTile w = query_tile<COLS>(A);
     const T* kb = (const T*)A.k + w.b * A.ks.b + w.hk * A.ks.h;
     const T* vb = (const T*)A.v + w.b * A.vs.b + w.hk * A.vs.h;
@@ -379,10 +390,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const int at = 32 * c + 8 * g, left = col[n].valid ? A.D - at : 0;
-            q[n][c] = gs::frag_global<T>(p + at, left);
-            go[n][c] = gs::frag_global<T>(pg + at, left);
-            const Frag<T> fo = gs::frag_global<T>(po + at, left);
-            const Frag<T> fr = gs::frag_global<T>(pr + at, A.rest == nullptr ? 0 : left);
+            q[n][c] = gs::frag_global<T, ODD>(p + at, left);
+            go[n][c] = gs::frag_global<T, ODD>(pg + at, left);
+            const Frag<T> fo = gs::frag_global<T, ODD>(po + at, left);
+            const Frag<T> fr = gs::frag_global<T, ODD>(pr + at, A.rest == nullptr ? 0 : left);
             T a[8], b[8], e[8];
             __builtin_memcpy(a, &go[n][c], 8 * sizeof(T));
             __builtin_memcpy(b, &fo, 8 * sizeof(T));
@@ -398,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
         for (int d2 = 0; d2 < DT; d2++) acc[d2][n] = f4{0, 0, 0, 0};
     }
 
-    Stage<T, DP, BK> sk, sv;
+    Stage<T, DP, BK, ODD> sk, sv;
     if (w.t0 < w.t1) {
         sk.load(kb + (int64_t)w.t0 * BK * A.ks.t, A.ks.t, w.len - w.t0 * BK, A.D);
         sv.load(vb + (int64_t)w.t0 * BK * A.vs.t, A.vs.t, w.len - w.t0 * BK, A.D);
@@ -423,7 +434,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
                 for (int n = 0; n < NQ; n++) s[u][n] = dp[u][n] = f4{0, 0, 0, 0};
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
-                    const Frag<T> a = L::rows(kt, 32 * kk + 16 * u, 32 * c), b = L::rows(vt, 32 * kk + 16 * u, 32 * c);
+                    const Frag<T> a = tile_of.rows(kt, 32 * kk + 16 * u, 32 * c), b = tile_of.rows(vt, 32 * kk + 16 * u, 32 * c);
 #pragma unroll
                     for (int n = 0; n < NQ; n++) {
                         s[u][n] = gs::mma(a, q[n][c], s[u][n]);
@@ -448,7 +459,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
             }
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const Frag<T> a = L::cols(kt, 32 * kk, 16 * d);
+                const Frag<T> a = tile_of.cols(kt, 32 * kk, 16 * d);
 #pragma unroll
                 for (int n = 0; n < NQ; n++) acc[d][n] = gs::mma(a, ds[n], acc[d][n]);
             }
@@ -467,24 +478,25 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
             const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
             float* p = A.part + (w.split * rows + (int64_t)w.bh * A.G * A.Tq + col[n].r) * A.D;
 #pragma unroll
-            for (int d = 0; d < DT; d++) store4(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+            for (int d = 0; d < DT; d++) store4<ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
         } else {
             T* p = (T*)A.out0 + w.b * A.s0.b + col[n].h * A.s0.h + col[n].i * A.s0.t;
 #pragma unroll
-            for (int d = 0; d < DT; d++) store4(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+            for (int d = 0; d < DT; d++) store4<ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
         }
     }
 }
 
 // dk and dv.  A wave holds 16 NK keys; the block streams the queries of every
 // head that shares them, QT rows at a time.
-template <typename T, int DP, int NK, int QT>
+template <typename T, int DP, int NK, int QT, bool ODD>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NK, WORDS = QT * L::CHUNKS, BUF = 2 * WORDS + QT / 2;
     extern __shared__ uint4 lds[];   // [2][q tile, do tile, lse[QT], delta[QT]]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const L tile_of;
     const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x);
     const int split = (int)(item % (uint32_t)A.splits);
     const uint32_t rest = item / (uint32_t)A.splits;
@@ -504,8 +516,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const int at = 32 * c + 8 * g, left = held ? A.D - at : 0;
-            k[n][c] = gs::frag_global<T>(pk + at, left);
-            v[n][c] = gs::frag_global<T>(pv + at, left);
+            k[n][c] = gs::frag_global<T, ODD>(pk + at, left);
+            v[n][c] = gs::frag_global<T, ODD>(pv + at, left);
         }
 #pragma unroll
         for (int d = 0; d < DT; d++) dk[d][n] = dv[d][n] = f4{0, 0, 0, 0};
@@ -518,7 +530,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
     const int per_head = tiles - from, total = per_head * A.G, per = (total + A.splits - 1) / A.splits;
     const int e0 = min(total, split * per), e1 = min(total, e0 + per);
 
-    Stage<T, DP, QT> sq, sg;
+    Stage<T, DP, QT, ODD> sq, sg;
     float stat = 0.0f;   // threads 0 .. QT - 1: lse, QT .. 2 QT - 1: delta
     auto fetch = [&](int e) {
         const int h = hk * A.G + e / per_head, q0 = (from + e % per_head) * QT, n = A.Tq - q0;
@@ -557,7 +569,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
                 for (int n = 0; n < NK; n++) s[u][n] = dp[u][n] = f4{0, 0, 0, 0};
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
-                    const Frag<T> a = L::rows(qt, 32 * kk + 16 * u, 32 * c), d = L::rows(gt, 32 * kk + 16 * u, 32 * c);
+                    const Frag<T> a = tile_of.rows(qt, 32 * kk + 16 * u, 32 * c), d = tile_of.rows(gt, 32 * kk + 16 * u, 32 * c);
 #pragma unroll
                     for (int n = 0; n < NK; n++) {
                         s[u][n] = gs::mma(a, k[n][c], s[u][n]);
@@ -588,7 +600,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
             }
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const Frag<T> a = L::cols(gt, 32 * kk, 16 * d), c = L::cols(qt, 32 * kk, 16 * d);
+                const Frag<T> a = tile_of.cols(gt, 32 * kk, 16 * d), c = tile_of.cols(qt, 32 * kk, 16 * d);
 #pragma unroll
                 for (int n = 0; n < NK; n++) {
                     dv[d][n] = gs::mma(a, fp[n], dv[d][n]);
@@ -609,11 +621,11 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
             const f4 xk = held ? dk[d][n] * A.scale : f4{0, 0, 0, 0}, xv = held ? dv[d][n] : f4{0, 0, 0, 0};
             if (A.part != nullptr) {
                 const int64_t rows = (int64_t)A.B * A.Hkv * A.Tk, row = (int64_t)bh * A.Tk + key[n];
-                store4(A.part + (2 * split * rows + row) * A.D + at, xk, left);
-                store4(A.part + ((2 * split + 1) * rows + row) * A.D + at, xv, left);
+                store4<ODD>(A.part + (2 * split * rows + row) * A.D + at, xk, left);
+                store4<ODD>(A.part + ((2 * split + 1) * rows + row) * A.D + at, xv, left);
             } else {
-                store4((T*)A.out0 + b * A.s0.b + hk * A.s0.h + (int64_t)key[n] * A.s0.t + at, xk, left);
-                store4((T*)A.out1 + b * A.s1.b + hk * A.s1.h + (int64_t)key[n] * A.s1.t + at, xv, left);
+                store4<ODD>((T*)A.out0 + b * A.s0.b + hk * A.s0.h + (int64_t)key[n] * A.s0.t + at, xk, left);
+                store4<ODD>((T*)A.out1 + b * A.s1.b + hk * A.s1.h + (int64_t)key[n] * A.s1.t + at, xv, left);
             }
         }
     }
@@ -653,6 +665,12 @@ int splits_of(int64_t blocks, int steps)
     return (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));
 }
 
+enum Walk { FORWARD, DQ, DKV };
+
+// Whether a wave's registers hold 32 columns, which halve the LDS reads per
+// product, or 16.
+constexpr bool two_columns(Walk w, bool f32, int DP) { return w == DKV ? DP <= 64 : !(f32 && DP > 64); }
+
 // How the three walks of one problem are cut.
 struct Plan {
     int nq, nk, tiles_q, tiles_k, splits_f, splits_q, splits_k, qt;
@@ -664,11 +682,11 @@ Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D)
     Plan p{};
     const int DP = padded(D);
     const int64_t heads = (int64_t)B * Hkv, rows = (int64_t)G * Tq;
-    // 32 columns per wave halve the LDS reads per product; 16 where the
-    // registers do not hold 32, or where 32 would leave CUs without work
-    const bool wide = !(type == GS_F32 && DP > 64);
-    p.nq = wide && heads * ((rows + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
-    p.nk = wide && DP <= 64 && heads * (((int64_t)Tk + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
+    // 16 columns also where 32 would leave CUs without work, and for head
+    // dimensions that end inside 16 bytes
+    const bool whole = D % (16 / gs::dtype_bytes(type)) == 0, f32 = type == GS_F32;
+    p.nq = whole && two_columns(DQ, f32, DP) && heads * ((rows + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
+    p.nk = whole && two_columns(DKV, f32, DP) && heads * (((int64_t)Tk + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
     p.qt = 64;
     p.tiles_q = (int)((rows + 64 * p.nq - 1) / (64 * p.nq));
     p.tiles_k = (int)(((int64_t)Tk + 64 * p.nk - 1) / (64 * p.nk));
@@ -693,50 +711,46 @@ int launch(const char* name, K kernel, int64_t blocks, size_t lds, const AttnArg
     return GS_OK;
 }
 
-template <typename T, int DP, int NQ>
+template <typename T, int DP, int NQ, bool ODD>
 int forward_one(const AttnArgs& A, hipStream_t stream)
 {
     const size_t lds = (size_t)4 * BK * Tile<T, DP>::CHUNKS * 16;
-    return launch("attn_fwd_kernel", attn_fwd_kernel<T, DP, NQ>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
+    return launch("attn_fwd_kernel", attn_fwd_kernel<T, DP, NQ, ODD>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
                   stream);
 }
 
-template <typename T, int DP, int NQ>
+template <typename T, int DP, int NQ, bool ODD>
 int dq_one(const AttnArgs& A, hipStream_t stream)
 {
     const size_t lds = (size_t)4 * BK * Tile<T, DP>::CHUNKS * 16;
-    return launch("attn_dq_kernel", attn_dq_kernel<T, DP, NQ>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
+    return launch("attn_dq_kernel", attn_dq_kernel<T, DP, NQ, ODD>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
                   stream);
 }
 
-template <typename T, int DP, int NK>
+template <typename T, int DP, int NK, bool ODD>
 int dkv_one(const AttnArgs& A, hipStream_t stream)
 {
     constexpr int QT = 64;
     const size_t lds = (size_t)2 * (2 * QT * Tile<T, DP>::CHUNKS + QT / 2) * 16;
-    return launch("attn_dkv_kernel", attn_dkv_kernel<T, DP, NK, QT>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
+    return launch("attn_dkv_kernel", attn_dkv_kernel<T, DP, NK, QT, ODD>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
                   stream);
 }
 
-enum Walk { FORWARD, DQ, DKV };
+template <Walk W, typename T, int DP, int N, bool ODD>
+int run_one(const AttnArgs& A, hipStream_t stream)
+{
+    if constexpr (W == FORWARD) return forward_one<T, DP, N, ODD>(A, stream);
+    else if constexpr (W == DQ) return dq_one<T, DP, N, ODD>(A, stream);
+    else return dkv_one<T, DP, N, ODD>(A, stream);
+}
 
 template <Walk W, typename T, int DP>
 int run_width(const AttnArgs& A, int wide, hipStream_t stream)
 {
-    constexpr bool TWO = !(sizeof(T) == 4 && DP > 64);
-    if constexpr (W == FORWARD) {
-        if constexpr (TWO)
-            if (wide == 2) return forward_one<T, DP, 2>(A, stream);
-        return forward_one<T, DP, 1>(A, stream);
-    } else if constexpr (W == DQ) {
-        if constexpr (TWO)
-            if (wide == 2) return dq_one<T, DP, 2>(A, stream);
-        return dq_one<T, DP, 1>(A, stream);
-    } else {
-        if constexpr (DP <= 64)
-            if (wide == 2) return dkv_one<T, DP, 2>(A, stream);
-        return dkv_one<T, DP, 1>(A, stream);
-    }
+    if (A.D % gs::Vec<T>::N != 0) return run_one<W, T, DP, 1, true>(A, stream);
+    if constexpr (two_columns(W, sizeof(T) == 4, DP))
+        if (wide == 2) return run_one<W, T, DP, 2, false>(A, stream);
+    return run_one<W, T, DP, 1, false>(A, stream);
 }
 
 template <Walk W, typename T>

@@ -15,8 +15,10 @@ inline bool dtype_known(int t) { return t >= 0 && t <= 2; }
 inline int dtype_bytes(int t) { return t == 0 ? 4 : 2; }
 
 // Sixteen bytes of elements, and an access to them at any element's address:
-// rows of odd widths and views with odd strides start at any multiple of the
-// element, which gfx950's global memory instructions take as they are.
+// views with odd strides start at any multiple of the element, which gfx950's
+// global memory instructions take as they are.  Rows whose width is not a whole
+// number of these go through kernels of their own: a partial access beside a
+// whole one in the same loop costs the whole one its single instruction.
 template <typename T>
 struct Vec {
     static constexpr int N = 16 / (int)sizeof(T);
@@ -35,29 +37,6 @@ template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r)
 {
     __builtin_memcpy(p, &r, 16);
-}
-
-// The first n elements (0..N) at p, the others zero.
-template <typename T>
-__device__ __forceinline__ Vec<T> load_part(const T* p, int n)
-{
-    if (n >= Vec<T>::N) return load_vec(p);
-    Vec<T> r;
-#pragma unroll
-    for (int i = 0; i < Vec<T>::N; i++) r.v[i] = i < n ? p[i] : (T)0.0f;
-    return r;
-}
-
-template <typename T>
-__device__ __forceinline__ void store_part(T* p, const Vec<T>& r, int n)
-{
-    if (n >= Vec<T>::N) {
-        store_vec(p, r);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < Vec<T>::N; i++)
-        if (i < n) p[i] = r.v[i];
 }
 
 }  // namespace gs

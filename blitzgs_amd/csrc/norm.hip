@@ -25,33 +25,30 @@
 
 namespace {
 
-using gs::Vec;
-
 constexpr int BLOCK = 256;
 constexpr int MAX_WIDTH = 32768;
 // Partial rows of the column sums: two blocks per CU, enough waves in flight
 // to cover memory latency and few enough partial rows to add up quickly.
 constexpr int MAX_PARTS = 512;
 
-template <typename W>
-__device__ __forceinline__ void load_params(const W* p, int at, int n, float (&out)[8], int count, float none)
+template <int V, typename W>
+__device__ __forceinline__ void load_params(const W* p, int at, float (&out)[V], float none)
 {
+    if (p == nullptr) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) out[i] = none;
-    if (p == nullptr) return;
-    if (n >= count) {
-        W t[8];
-        if (count == 8) __builtin_memcpy(t, p + at, 8 * sizeof(W));
-        else __builtin_memcpy(t, p + at, 4 * sizeof(W));
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < count) out[i] = (float)t[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < n && i < count) out[i] = (float)p[at + i];
+        for (int i = 0; i < V; i++) out[i] = none;
+        return;
     }
+    W t[V];
+    __builtin_memcpy(t, p + at, V * sizeof(W));
+#pragma unroll
+    for (int i = 0; i < V; i++) out[i] = (float)t[i];
 }
+
+template <typename T, int V>
+struct Chunk {
+    T v[V];
+};
 
 // The sum of v over the LPR threads of a row, in every one of them.  Rows of
 // more than a wave meet in LDS (`meet`, one slot per wave; two barriers).
@@ -86,10 +83,10 @@ struct NormArgs {
     float eps;
 };
 
-template <typename T, typename W, int LPR, int NC>
+template <typename T, typename W, int V, int LPR, int NC>
 __global__ __launch_bounds__(LPR > BLOCK ? LPR : BLOCK) void norm_fwd_kernel(NormArgs A)
 {
-    constexpr int V = Vec<T>::N, RPB = LPR > BLOCK ? 1 : BLOCK / LPR;
+    constexpr int RPB = LPR > BLOCK ? 1 : BLOCK / LPR;
     __shared__ float meet[LPR > 64 ? LPR / 64 : 1];
     const int l = threadIdx.x % LPR;
     const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
@@ -101,38 +98,38 @@ __global__ __launch_bounds__(LPR > BLOCK ? LPR : BLOCK) void norm_fwd_kernel(Nor
     float s = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const int at = (c * LPR + l) * V, n = A.width - at;
-        Vec<T> t{};
-        if (n > 0) t = gs::load_part(x + at, n);
+        const int at = (c * LPR + l) * V;
+        Chunk<T, V> t{};
+        if (at < A.width) __builtin_memcpy(&t, x + at, sizeof(t));
 #pragma unroll
         for (int i = 0; i < V; i++) {
             v[c][i] = (float)t.v[i];
-            s += i < n ? v[c][i] : 0.0f;
+            s += v[c][i];
         }
     }
     const float mean = row_sum<LPR>(s, meet) * inv_n;
     float q = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const int n = A.width - (c * LPR + l) * V;
+        const bool in = (c * LPR + l) * V < A.width;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            v[c][i] -= mean;
-            if (i < n) q = __builtin_fmaf(v[c][i], v[c][i], q);
+            v[c][i] = in ? v[c][i] - mean : 0.0f;
+            q = __builtin_fmaf(v[c][i], v[c][i], q);
         }
     }
     const float rstd = 1.0f / __builtin_sqrtf(row_sum<LPR>(q, meet) * inv_n + A.eps);
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const int at = (c * LPR + l) * V, n = A.width - at;
-        if (n <= 0) continue;
-        float w[8], b[8];
-        load_params((const W*)A.w, at, n, w, V, 1.0f);
-        load_params((const W*)A.b, at, n, b, V, 0.0f);
-        Vec<T> t;
+        const int at = (c * LPR + l) * V;
+        if (at >= A.width) continue;
+        float w[V], b[V];
+        load_params<V>((const W*)A.w, at, w, 1.0f);
+        load_params<V>((const W*)A.b, at, b, 0.0f);
+        Chunk<T, V> t;
 #pragma unroll
         for (int i = 0; i < V; i++) t.v[i] = (T)__builtin_fmaf(v[c][i] * rstd, w[i], b[i]);
-        gs::store_part(y + at, t, n);
+        __builtin_memcpy(y + at, &t, sizeof(t));
     }
     if (l == 0 && A.mean != nullptr) {
         A.mean[row] = mean;
@@ -140,10 +137,10 @@ __global__ __launch_bounds__(LPR > BLOCK ? LPR : BLOCK) void norm_fwd_kernel(Nor
     }
 }
 
-template <typename T, typename W, int LPR, int NC>
+template <typename T, typename W, int V, int LPR, int NC>
 __global__ __launch_bounds__(LPR > BLOCK ? LPR : BLOCK) void norm_bwd_kernel(NormArgs A)
 {
-    constexpr int V = Vec<T>::N, THREADS = LPR > BLOCK ? LPR : BLOCK, RPB = THREADS / LPR;
+    constexpr int THREADS = LPR > BLOCK ? LPR : BLOCK, RPB = THREADS / LPR;
     __shared__ float meet[LPR > 64 ? LPR / 64 : 1];
     __shared__ float sums[RPB > 1 ? (RPB - 1) * LPR * V : 1];
     const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR;
@@ -151,14 +148,10 @@ __global__ __launch_bounds__(LPR > BLOCK ? LPR : BLOCK) void norm_bwd_kernel(Nor
     float w[NC][V], dw[NC][V], db[NC][V];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const int at = (c * LPR + l) * V, n = A.width - at;
-        float t[8];
-        load_params((const W*)A.w, at, n > 0 ? n : 0, t, V, A.w == nullptr ? 1.0f : 0.0f);
+        const int at = (c * LPR + l) * V;
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            w[c][i] = t[i];
-            dw[c][i] = db[c][i] = 0.0f;
-        }
+        for (int i = 0; i < V; i++) w[c][i] = dw[c][i] = db[c][i] = 0.0f;
+        if (at < A.width) load_params<V>((const W*)A.w, at, w[c], 1.0f);
     }
     // a row's threads leave the loop together: its barriers are met by whole rows
     for (int64_t row = (int64_t)blockIdx.x * RPB + sub; row < A.rows; row += (int64_t)gridDim.x * RPB) {
@@ -170,18 +163,19 @@ __global__ __launch_bounds__(LPR > BLOCK ? LPR : BLOCK) void norm_bwd_kernel(Nor
         float sh = 0.0f, shz = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            const int at = (c * LPR + l) * V, n = A.width - at;
-            Vec<T> tx{}, tg{};
-            if (n > 0) {
-                tx = gs::load_part(x + at, n);
-                tg = gs::load_part(dy + at, n);
+            const int at = (c * LPR + l) * V;
+            const bool in = at < A.width;
+            Chunk<T, V> tx{}, tg{};
+            if (in) {
+                __builtin_memcpy(&tx, x + at, sizeof(tx));
+                __builtin_memcpy(&tg, dy + at, sizeof(tg));
             }
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const float g = (float)tg.v[i];
-                z[c][i] = i < n ? ((float)tx.v[i] - mean) * rstd : 0.0f;
+                z[c][i] = in ? ((float)tx.v[i] - mean) * rstd : 0.0f;
                 h[c][i] = g * w[c][i];
-                sh += i < n ? h[c][i] : 0.0f;
+                sh += h[c][i];
                 shz = __builtin_fmaf(h[c][i], z[c][i], shz);
                 dw[c][i] = __builtin_fmaf(g, z[c][i], dw[c][i]);
                 db[c][i] += g;
@@ -190,12 +184,12 @@ __global__ __launch_bounds__(LPR > BLOCK ? LPR : BLOCK) void norm_bwd_kernel(Nor
         const float mh = row_sum<LPR>(sh, meet) * inv_n, mhz = row_sum<LPR>(shz, meet) * inv_n;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            const int at = (c * LPR + l) * V, n = A.width - at;
-            if (n <= 0) continue;
-            Vec<T> t;
+            const int at = (c * LPR + l) * V;
+            if (at >= A.width) continue;
+            Chunk<T, V> t;
 #pragma unroll
             for (int i = 0; i < V; i++) t.v[i] = (T)(rstd * (h[c][i] - mh - z[c][i] * mhz));
-            gs::store_part(dx + at, t, n);
+            __builtin_memcpy(dx + at, &t, sizeof(t));
         }
     }
     if (A.parts == nullptr) return;
@@ -214,6 +208,7 @@ __global__ __launch_bounds__(LPR > BLOCK ? LPR : BLOCK) void norm_bwd_kernel(Nor
                 }
                 __syncthreads();
                 if (sub == 0) {
+#pragma unroll 1
                     for (int r = 0; r < RPB - 1; r++) {
 #pragma unroll
                         for (int i = 0; i < V; i++) acc[i] += sums[(r * V + i) * LPR + l];
@@ -253,23 +248,30 @@ __global__ __launch_bounds__(1024) void norm_columns_kernel(const float* __restr
     }
 }
 
-// Threads per row and chunks per thread: the fewest threads that hold the row
-// in one 16-byte chunk each, then a wave with up to 32 elements per lane, then
-// 4 and 16 waves.  More elements per lane would spill the backward's five
+// Elements per access (16 bytes; one where the width is no multiple of that),
+// threads per row and accesses per thread: the fewest threads that hold the
+// row in one access each, then a wave with up to 32 elements per lane, then 4
+// and 16 waves.  More elements per lane would spill the backward's five
 // values per element.
 struct Shape {
-    int lpr, nc;
+    int v, lpr, nc;
 };
 
 Shape shape_of(int width, int vec)
 {
-    const int chunks = (width + vec - 1) / vec, most = 32 / vec;
-    for (int lpr = 8; lpr <= 64; lpr *= 2)
-        if (chunks <= lpr) return {lpr, 1};
-    for (int lpr = 64; lpr <= 1024; lpr *= 4)
-        for (int nc = 2; nc <= most; nc *= 2)
-            if (chunks <= lpr * nc) return {lpr, nc};
-    return {0, 0};
+    const int v = width % vec == 0 ? vec : 1, chunks = width / v;
+    if (v == 1) {
+        for (int lpr = 64; lpr <= 1024; lpr *= 4)
+            for (int nc : {1, 2, 4, 8, 12, 16, 32})
+                if ((lpr == 64 || nc >= 16) && chunks <= lpr * nc) return {v, lpr, nc};
+    } else {
+        for (int lpr = 8; lpr <= 64; lpr *= 2)
+            if (chunks <= lpr) return {v, lpr, 1};
+        for (int lpr = 64; lpr <= 1024; lpr *= 4)
+            for (int nc = 2; nc <= 32 / v; nc *= 2)
+                if (chunks <= lpr * nc) return {v, lpr, nc};
+    }
+    return {};
 }
 
 int rows_per_block(const Shape& s) { return s.lpr >= BLOCK ? 1 : BLOCK / s.lpr; }
@@ -280,40 +282,57 @@ int parts_of(int64_t rows, const Shape& s)
     return (int)(n < MAX_PARTS ? n : MAX_PARTS);
 }
 
-template <typename T, typename W, bool BWD, int LPR, int NC>
+template <typename T, typename W, bool BWD, int V, int LPR, int NC>
 void launch_one(const NormArgs& A, unsigned blocks, hipStream_t stream)
 {
     const dim3 threads(LPR > BLOCK ? LPR : BLOCK);
     if constexpr (BWD)
         GS_TIMED("norm_bwd_kernel", stream,
-                 hipLaunchKernelGGL((norm_bwd_kernel<T, W, LPR, NC>), dim3(blocks), threads, 0, stream, A));
+                 hipLaunchKernelGGL((norm_bwd_kernel<T, W, V, LPR, NC>), dim3(blocks), threads, 0, stream, A));
     else
         GS_TIMED("norm_fwd_kernel", stream,
-                 hipLaunchKernelGGL((norm_fwd_kernel<T, W, LPR, NC>), dim3(blocks), threads, 0, stream, A));
+                 hipLaunchKernelGGL((norm_fwd_kernel<T, W, V, LPR, NC>), dim3(blocks), threads, 0, stream, A));
 }
 
 template <typename T, typename W, bool BWD>
 void launch_shape(const Shape& s, const NormArgs& A, unsigned blocks, hipStream_t stream)
 {
-#define GS_NORM_CASE(L, C) \
-    case L * 16 + C: return launch_one<T, W, BWD, L, C>(A, blocks, stream)
-    switch (s.lpr * 16 + s.nc) {
-        GS_NORM_CASE(8, 1);
-        GS_NORM_CASE(16, 1);
-        GS_NORM_CASE(32, 1);
-        GS_NORM_CASE(64, 1);
-        GS_NORM_CASE(64, 2);
-        GS_NORM_CASE(64, 4);
-        GS_NORM_CASE(256, 2);
-        GS_NORM_CASE(256, 4);
-        GS_NORM_CASE(1024, 2);
-        GS_NORM_CASE(1024, 4);
+    constexpr int V = gs::Vec<T>::N;
+#define GS_NORM_CASE(v, L, C) \
+    case L * 64 + C: return launch_one<T, W, BWD, v, L, C>(A, blocks, stream)
+    if (s.v == 1) {
+        switch (s.lpr * 64 + s.nc) {
+            GS_NORM_CASE(1, 64, 1);
+            GS_NORM_CASE(1, 64, 2);
+            GS_NORM_CASE(1, 64, 4);
+            GS_NORM_CASE(1, 64, 8);
+            GS_NORM_CASE(1, 64, 12);
+            GS_NORM_CASE(1, 64, 16);
+            GS_NORM_CASE(1, 64, 32);
+            GS_NORM_CASE(1, 256, 16);
+            GS_NORM_CASE(1, 256, 32);
+            GS_NORM_CASE(1, 1024, 16);
+            GS_NORM_CASE(1, 1024, 32);
+        }
+        return;
     }
-    if constexpr (sizeof(T) == 4) {
-        switch (s.lpr * 16 + s.nc) {
-            GS_NORM_CASE(64, 8);
-            GS_NORM_CASE(256, 8);
-            GS_NORM_CASE(1024, 8);
+    switch (s.lpr * 64 + s.nc) {
+        GS_NORM_CASE(V, 8, 1);
+        GS_NORM_CASE(V, 16, 1);
+        GS_NORM_CASE(V, 32, 1);
+        GS_NORM_CASE(V, 64, 1);
+        GS_NORM_CASE(V, 64, 2);
+        GS_NORM_CASE(V, 64, 4);
+        GS_NORM_CASE(V, 256, 2);
+        GS_NORM_CASE(V, 256, 4);
+        GS_NORM_CASE(V, 1024, 2);
+        GS_NORM_CASE(V, 1024, 4);
+    }
+    if constexpr (V == 4) {
+        switch (s.lpr * 64 + s.nc) {
+            GS_NORM_CASE(V, 64, 8);
+            GS_NORM_CASE(V, 256, 8);
+            GS_NORM_CASE(V, 1024, 8);
         }
     }
 #undef GS_NORM_CASE

@@ -86,10 +86,15 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(const T* __restrict__ g,
     const int64_t per = ((size + NORM_PARTS - 1) / NORM_PARTS + V - 1) / V * V;
     const int64_t from = per * blockIdx.x, to = from + per < size ? from + per : size;
     float s = 0.0f;
-    for (int64_t i = from + (int64_t)threadIdx.x * V; i < to; i += 256 * V) {
-        const gs::Vec<T> t = gs::load_part(p + i, (int)(to - i < V ? to - i : V));
+    const int64_t whole = to - (to - from) % V;
+    for (int64_t i = from + (int64_t)threadIdx.x * V; i < whole; i += 256 * V) {
+        const gs::Vec<T> t = gs::load_vec(p + i);
 #pragma unroll
         for (int k = 0; k < V; k++) s = __builtin_fmaf((float)t.v[k], (float)t.v[k], s);
+    }
+    if (from < to && whole + threadIdx.x < to) {
+        const float t = (float)p[whole + threadIdx.x];
+        s = __builtin_fmaf(t, t, s);
     }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
@@ -148,6 +153,44 @@ __device__ __forceinline__ Frag<f16> column_frag(const uint4* t, int col)
     return f;
 }
 
+// Both planes of an operand's next S x KT tile (DOWN: KT x S, k down its rows)
+// on their way to LDS, in registers.
+template <int S, bool DOWN>
+struct Pair {
+    static constexpr int CH = S * KT / 8 / 256, W = DOWN ? S / 8 : KT / 8;   // chunks per thread, per row
+    const f16* p;
+    int64_t plane, row, step;
+    uint4 hi[CH], lo[CH];
+
+    __device__ __forceinline__ void at(const Planes& m, const f16* base, int first)
+    {
+        const int r = threadIdx.x / W, c = threadIdx.x % W * 8;
+        p = DOWN ? base + (int64_t)r * m.ld + first + c : base + (int64_t)(first + r) * m.ld + c;
+        plane = m.plane;
+        row = (int64_t)(256 / W) * m.ld;
+        step = DOWN ? (int64_t)KT * m.ld : KT;
+    }
+    __device__ __forceinline__ void load()
+    {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            hi[c] = *(const uint4*)(p + c * row);
+            lo[c] = *(const uint4*)(p + c * row + plane);
+        }
+        p += step;
+    }
+    __device__ __forceinline__ void store(uint4* th, uint4* tl) const
+    {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int r = threadIdx.x / W + c * (256 / W);
+            const int e = DOWN ? Tile<f16, S>::chunk(r, threadIdx.x % W) : Tile<f16, KT>::chunk(r, threadIdx.x % W);
+            th[e] = hi[c];
+            tl[e] = lo[c];
+        }
+    }
+};
+
 // A block computes S x S of the result, four waves a quarter each: columns of
 // its matrix-core tiles are rows of the left operand, rows are columns of the
 // result, so that a lane holds four neighbours of one row of the result.
@@ -155,7 +198,6 @@ template <Kind K, int S, typename T>
 __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
 {
     constexpr int H = S / 2, U = H / 16;
-    constexpr int CH = S * KT / 8 / 256;             // chunks per thread of one operand's plane
     constexpr int WORDS = S * KT / 8;                // of one operand's plane
     __shared__ uint4 lds[2][4][WORDS];               // left hi, lo, right hi, lo
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
@@ -177,48 +219,32 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
     const f16* lp = A.l.p + batch * A.l.stride;
     const f16* rp = A.r.p + batch * A.r.stride;
 
-    uint4 st[4][CH];
-    auto fetch = [&](int k0) {
-#pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int id = threadIdx.x + 256 * c;
-            const f16* p = lp + (int64_t)(m0 + id / 4) * A.l.ld + k0 + id % 4 * 8;
-            st[0][c] = *(const uint4*)p;
-            st[1][c] = *(const uint4*)(p + A.l.plane);
-            if constexpr (K == APPLY) p = rp + (int64_t)(k0 + id / (S / 8)) * A.r.ld + n0 + id % (S / 8) * 8;
-            else p = rp + (int64_t)(n0 + id / 4) * A.r.ld + k0 + id % 4 * 8;
-            st[2][c] = *(const uint4*)p;
-            st[3][c] = *(const uint4*)(p + A.r.plane);
-        }
-    };
-    auto put = [&](int b) {
-#pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int id = threadIdx.x + 256 * c;
-            const int at = Tile<f16, KT>::chunk(id / 4, id % 4);
-            const int rt = K == APPLY ? Tile<f16, S>::chunk(id / (S / 8), id % (S / 8)) : at;
-            lds[b][0][at] = st[0][c];
-            lds[b][1][at] = st[1][c];
-            lds[b][2][rt] = st[2][c];
-            lds[b][3][rt] = st[3][c];
-        }
-    };
+    Pair<S, false> sl;
+    Pair<S, K == APPLY> sr;
+    sl.at(A.l, lp, m0);
+    sr.at(A.r, rp, n0);
+    const Tile<f16, KT> tile;
     const int ml = (wave & 1) * H, nl = (wave >> 1) * H;
     f4 acc[U][U];   // [columns of the result][rows of the result]
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
         for (int v = 0; v < U; v++) acc[u][v] = f4{0, 0, 0, 0};
-    fetch(0);
-    put(0);
+    sl.load();
+    sr.load();
+    sl.store(lds[0][0], lds[0][1]);
+    sr.store(lds[0][2], lds[0][3]);
     __syncthreads();
     for (int k0 = 0, b = 0; k0 < A.k; k0 += KT, b ^= 1) {
-        if (k0 + KT < A.k) fetch(k0 + KT);
+        if (k0 + KT < A.k) {
+            sl.load();
+            sr.load();
+        }
         Frag<f16> lh[U], ll[U];
 #pragma unroll
         for (int v = 0; v < U; v++) {
-            lh[v] = Tile<f16, KT>::rows(lds[b][0], ml + 16 * v, 0);
-            ll[v] = Tile<f16, KT>::rows(lds[b][1], ml + 16 * v, 0);
+            lh[v] = tile.rows(lds[b][0], ml + 16 * v, 0);
+            ll[v] = tile.rows(lds[b][1], ml + 16 * v, 0);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -227,8 +253,8 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
                 rh = column_frag<S>(lds[b][2], nl + 16 * u);
                 rl = column_frag<S>(lds[b][3], nl + 16 * u);
             } else {
-                rh = Tile<f16, KT>::rows(lds[b][2], nl + 16 * u, 0);
-                rl = Tile<f16, KT>::rows(lds[b][3], nl + 16 * u, 0);
+                rh = tile.rows(lds[b][2], nl + 16 * u, 0);
+                rl = tile.rows(lds[b][3], nl + 16 * u, 0);
             }
 #pragma unroll
             for (int v = 0; v < U; v++) {
@@ -237,7 +263,10 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
                 acc[u][v] = gs::mma(rh, lh[v], acc[u][v]);
             }
         }
-        if (k0 + KT < A.k) put(b ^ 1);
+        if (k0 + KT < A.k) {
+            sl.store(lds[b ^ 1][0], lds[b ^ 1][1]);
+            sr.store(lds[b ^ 1][2], lds[b ^ 1][3]);
+        }
         __syncthreads();
     }
     const int k = extra_scale(A.small[batch], A.step);
@@ -341,12 +370,13 @@ int product(int S, const ProductArgs& A, int count, hipStream_t stream)
 {
     const int64_t per = K == APPLY ? (int64_t)A.tiles_m * A.tiles_n : (int64_t)A.tiles_m * (A.tiles_m + 1) / 2;
     GS_REQUIRE(per * count < 0x7fffffff, "orthogonalise: too many tiles for one launch");
+    constexpr const char* name = K == SQUARE ? "orth_square" : K == POLY ? "orth_poly" : "orth_apply";
     const dim3 grid((unsigned)(per * count));
     if (S == 128)
-        GS_TIMED("orth_product_kernel", stream,
+        GS_TIMED(name, stream,
                  hipLaunchKernelGGL((orth_product_kernel<K, 128, T>), grid, dim3(256), 0, stream, A));
     else
-        GS_TIMED("orth_product_kernel", stream,
+        GS_TIMED(name, stream,
                  hipLaunchKernelGGL((orth_product_kernel<K, 64, T>), grid, dim3(256), 0, stream, A));
     GS_LAUNCH_CHECK("orth_product_kernel");
     return GS_OK;
