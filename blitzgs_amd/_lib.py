@@ -100,7 +100,7 @@ _SIGS = {
     "gs_layer_norm_forward": (_i, [_i, _i, _i64, _i, _c, _i64, _c, _c, _f, _c, _c, _c, _c]),
     "gs_layer_norm_workspace_bytes": (_sz, [_i, _i64, _i]),
     "gs_layer_norm_backward": (_i, [_i, _i, _i64, _i, _c, _i64, _c, _c, _c, _c, _i64, _c, _c, _c, _c, _c]),
-    "gs_attention_workspace_bytes": (_sz, [_i] * 8),
+    "gs_attention_workspace_bytes": (_sz, [_i] * 9),
     "gs_attention_forward": (_i, [_i] * 7 + [_c, C.POINTER(_i64)] * 3 + [_f, _i, _c, _c, _c, C.POINTER(_i64), _c, _c,
                                                                          _c, _c]),
     "gs_attention_backward": (_i, [_i] * 7 + [_c, C.POINTER(_i64)] * 3 + [_f, _i, _c, _c, _c, C.POINTER(_i64), _c, _c]

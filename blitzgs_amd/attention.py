@@ -55,7 +55,7 @@ class _Attention(torch.autograd.Function):
         lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32) if needs else None
         # what the rounding of o leaves, for the backward's sum(do o)
         rest = _token_major(q) if needs and q.dtype != torch.float32 else None
-        ws = torch.empty(lib.gs_attention_workspace_bytes(*sizes, 0), device=q.device, dtype=torch.uint8)
+        ws = torch.empty(lib.gs_attention_workspace_bytes(*sizes, int(causal), 0), device=q.device, dtype=torch.uint8)
         with torch.cuda.device(q.device):
             _lib.check(lib.gs_attention_forward(
                 *sizes, _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), scale,
@@ -72,7 +72,7 @@ class _Attention(torch.autograd.Function):
         q, k, v, o, rest, lse, key_lengths, query_start = ctx.saved_tensors
         lib, do = _lib.load(), _last_contiguous(do)
         dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
-        ws = torch.empty(lib.gs_attention_workspace_bytes(*ctx.sizes, 1), device=q.device, dtype=torch.uint8)
+        ws = torch.empty(lib.gs_attention_workspace_bytes(*ctx.sizes, int(ctx.causal), 1), device=q.device, dtype=torch.uint8)
         with torch.cuda.device(q.device):
             _lib.check(lib.gs_attention_backward(
                 *ctx.sizes, _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), ctx.scale,

@@ -41,6 +41,7 @@ namespace {
 
 using gs::f4;
 using gs::Frag;
+using gs::Fill;
 using gs::Stage;
 using gs::Tile;
 
@@ -99,6 +100,27 @@ __device__ __forceinline__ int seen_of(const AttnArgs& A, int len, int64_t start
     return n < 0 ? 0 : n < len ? (int)n : len;
 }
 
+// A workgroup's share: a column tile of one (batch, key head), and a split of
+// its walk.  Each XCD gets a run of neighbours, which stream the same rows
+// through its L2.  Where a causal limit makes a tile's place decide its cost and
+// the runs are not whole heads, one XCD would get the costly half of a head;
+// there the costliest tiles of all heads go first, dealt out in turn.  dk, dv
+// of 4 key heads of 8192 keys: 695 us, in runs 1181, head by head 1030.
+struct Share {
+    int bh, tile, split;
+};
+
+__device__ __forceinline__ Share share_of(const AttnArgs& A, int cost_heads)
+{
+    const uint32_t heads = (uint32_t)(A.B * A.Hkv), tiles = (uint32_t)A.tiles, splits = (uint32_t)A.splits;
+    if (!A.causal || cost_heads % 8 == 0) {
+        const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x), rest = item / splits;
+        return {(int)(rest / tiles), (int)(rest % tiles), (int)(item % splits)};
+    }
+    const uint32_t rest = blockIdx.x / splits;
+    return {(int)(rest % heads), (int)(rest / heads), (int)(blockIdx.x % splits)};
+}
+
 // One column tile of the kernels whose columns are queries.
 struct QueryTile {
     int b, hk, tile, split, bh;
@@ -111,12 +133,10 @@ template <int COLS>
 __device__ __forceinline__ QueryTile query_tile(const AttnArgs& A)
 {
     QueryTile w;
-    const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x);
-    w.split = (int)(item % (uint32_t)A.splits);
-    const uint32_t rest = item / (uint32_t)A.splits;
-    // causal: the last tiles see the most keys and go first
-    w.tile = A.tiles - 1 - (int)(rest % (uint32_t)A.tiles);
-    w.bh = (int)(rest / (uint32_t)A.tiles);
+    const Share share = share_of(A, A.B * A.Hkv * A.G);
+    w.split = share.split;
+    w.tile = A.tiles - 1 - share.tile;   // causal: the last tiles see the most keys
+    w.bh = share.bh;
     w.b = w.bh / A.Hkv;
     w.hk = w.bh % A.Hkv;
     w.len = length_of(A, w.b);
@@ -181,7 +201,7 @@ __device__ __forceinline__ void store_o(T* p, T* rest, f4 v, int n)
 
 // ------------------------------------------------------------------- forward
 
-template <typename T, int DP, int NQ, bool ODD>
+template <typename T, int DP, int NQ, Fill F>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
@@ -201,7 +221,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
         const T* p = (const T*)A.q + w.b * A.qs.b + col[n].h * A.qs.h + col[n].i * A.qs.t;
 #pragma unroll
         for (int c = 0; c < KC; c++)
-            q[n][c] = gs::frag_global<T, ODD>(p + 32 * c + 8 * g, col[n].valid ? A.D - 32 * c - 8 * g : 0);
+            q[n][c] = gs::frag_global<T, F == gs::ODD>(p + 32 * c + 8 * g, col[n].valid ? A.D - 32 * c - 8 * g : 0);
     }
     f4 o[DT][NQ];
     float m[NQ], l[NQ];
@@ -213,22 +233,29 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
         for (int d = 0; d < DT; d++) o[d][n] = f4{0, 0, 0, 0};
     }
 
-    Stage<T, DP, BK, ODD> sk, sv;
+    Stage<T, DP, BK, F> sk, sv;
+    auto fetch = [&](int t) {
+        uint4* to = lds + ((t - w.t0) & 1) * 2 * WORDS;
+        sk.fetch(to, kb + (int64_t)t * BK * A.ks.t, A.ks.t, w.len - t * BK, A.D);
+        sv.fetch(to + WORDS, vb + (int64_t)t * BK * A.vs.t, A.vs.t, w.len - t * BK, A.D);
+    };
+    auto put = [&](int t) {
+        uint4* to = lds + ((t - w.t0) & 1) * 2 * WORDS;
+        sk.put(to);
+        sv.put(to + WORDS);
+    };
     if (w.t0 < w.t1) {
-        sk.load(kb + (int64_t)w.t0 * BK * A.ks.t, A.ks.t, w.len - w.t0 * BK, A.D);
-        sv.load(vb + (int64_t)w.t0 * BK * A.vs.t, A.vs.t, w.len - w.t0 * BK, A.D);
-        sk.store(lds);
-        sv.store(lds + WORDS);
+#pragma unroll
+        for (int k = 0; k < 4; k++) sk.clear(lds + k * WORDS, A.D);
+        fetch(w.t0);
+        put(w.t0);
     }
     __syncthreads();
     for (int t = w.t0; t < w.t1; t++) {
         const uint4* kt = lds + ((t - w.t0) & 1) * 2 * WORDS;
         const uint4* vt = kt + WORDS;
         const int k0 = t * BK;
-        if (t + 1 < w.t1) {
-            sk.load(kb + (int64_t)(t + 1) * BK * A.ks.t, A.ks.t, w.len - k0 - BK, A.D);
-            sv.load(vb + (int64_t)(t + 1) * BK * A.vs.t, A.vs.t, w.len - k0 - BK, A.D);
-        }
+        if (t + 1 < w.t1) fetch(t + 1);
         f4 s[4][NQ];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -291,11 +318,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
                 for (int n = 0; n < NQ; n++) o[d][n] = gs::mma(a, p[n], o[d][n]);
             }
         }
-        if (t + 1 < w.t1) {
-            uint4* next = lds + ((t + 1 - w.t0) & 1) * 2 * WORDS;
-            sk.store(next);
-            sv.store(next + WORDS);
-        }
+        if (t + 1 < w.t1) put(t + 1);
         __syncthreads();
     }
 #pragma unroll
@@ -307,7 +330,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
             const int64_t at = (int64_t)w.split * A.B * A.Hkv * A.G * A.Tq + row;
             float* p = A.part + at * A.D;
 #pragma unroll
-            for (int d = 0; d < DT; d++) store4<ODD>(p + 16 * d + 4 * g, o[d][n], A.D - 16 * d - 4 * g);
+            for (int d = 0; d < DT; d++) store4<F == gs::ODD>(p + 16 * d + 4 * g, o[d][n], A.D - 16 * d - 4 * g);
             if (g == 0) {
                 A.part_ml[2 * at] = m[n];
                 A.part_ml[2 * at + 1] = sum;
@@ -320,7 +343,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             const int at = 16 * d + 4 * g;
-            store_o<ODD>((T*)A.out0 + out + at, rest == nullptr ? nullptr : rest + at, o[d][n] * inv, A.D - at);
+            store_o<F == gs::ODD>((T*)A.out0 + out + at, rest == nullptr ? nullptr : rest + at, o[d][n] * inv, A.D - at);
         }
         if (g == 0 && A.lse != nullptr) A.lse[row] = sum == 0.0f ? -NEG_INF : m[n] + __builtin_log2f(sum);
     }
@@ -362,7 +385,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs A)
 // ------------------------------------------------------------------ backward
 
 // dq, and delta for the other kernel.
-template <typename T, int DP, int NQ, bool ODD>
+template <typename T, int DP, int NQ, Fill F>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
@@ -390,10 +413,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const int at = 32 * c + 8 * g, left = col[n].valid ? A.D - at : 0;
-            q[n][c] = gs::frag_global<T, ODD>(p + at, left);
-            go[n][c] = gs::frag_global<T, ODD>(pg + at, left);
-            const Frag<T> fo = gs::frag_global<T, ODD>(po + at, left);
-            const Frag<T> fr = gs::frag_global<T, ODD>(pr + at, A.rest == nullptr ? 0 : left);
+            q[n][c] = gs::frag_global<T, F == gs::ODD>(p + at, left);
+            go[n][c] = gs::frag_global<T, F == gs::ODD>(pg + at, left);
+            const Frag<T> fo = gs::frag_global<T, F == gs::ODD>(po + at, left);
+            const Frag<T> fr = gs::frag_global<T, F == gs::ODD>(pr + at, A.rest == nullptr ? 0 : left);
             T a[8], b[8], e[8];
             __builtin_memcpy(a, &go[n][c], 8 * sizeof(T));
             __builtin_memcpy(b, &fo, 8 * sizeof(T));
@@ -409,29 +432,39 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
         for (int d2 = 0; d2 < DT; d2++) acc[d2][n] = f4{0, 0, 0, 0};
     }
 
-    Stage<T, DP, BK, ODD> sk, sv;
+    Stage<T, DP, BK, F> sk, sv;
+    auto fetch = [&](int t) {
+        uint4* to = lds + ((t - w.t0) & 1) * 2 * WORDS;
+        sk.fetch(to, kb + (int64_t)t * BK * A.ks.t, A.ks.t, w.len - t * BK, A.D);
+        sv.fetch(to + WORDS, vb + (int64_t)t * BK * A.vs.t, A.vs.t, w.len - t * BK, A.D);
+    };
+    auto put = [&](int t) {
+        uint4* to = lds + ((t - w.t0) & 1) * 2 * WORDS;
+        sk.put(to);
+        sv.put(to + WORDS);
+    };
     if (w.t0 < w.t1) {
-        sk.load(kb + (int64_t)w.t0 * BK * A.ks.t, A.ks.t, w.len - w.t0 * BK, A.D);
-        sv.load(vb + (int64_t)w.t0 * BK * A.vs.t, A.vs.t, w.len - w.t0 * BK, A.D);
-        sk.store(lds);
-        sv.store(lds + WORDS);
+#pragma unroll
+        for (int k = 0; k < 4; k++) sk.clear(lds + k * WORDS, A.D);
+        fetch(w.t0);
+        put(w.t0);
     }
     __syncthreads();
     for (int t = w.t0; t < w.t1; t++) {
         const uint4* kt = lds + ((t - w.t0) & 1) * 2 * WORDS;
         const uint4* vt = kt + WORDS;
         const int k0 = t * BK;
-        if (t + 1 < w.t1) {
-            sk.load(kb + (int64_t)(t + 1) * BK * A.ks.t, A.ks.t, w.len - k0 - BK, A.D);
-            sv.load(vb + (int64_t)(t + 1) * BK * A.vs.t, A.vs.t, w.len - k0 - BK, A.D);
-        }
+        if (t + 1 < w.t1) fetch(t + 1);
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
             f4 s[2][NQ], dp[2][NQ];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
 #pragma unroll
-                for (int n = 0; n < NQ; n++) s[u][n] = dp[u][n] = f4{0, 0, 0, 0};
+                for (int n = 0; n < NQ; n++) {
+                    s[u][n] = f4{0, 0, 0, 0};
+                    dp[u][n] = f4{-delta[n], -delta[n], -delta[n], -delta[n]};   // the sums start at -delta
+                }
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
                     const Frag<T> a = tile_of.rows(kt, 32 * kk + 16 * u, 32 * c), b = tile_of.rows(vt, 32 * kk + 16 * u, 32 * c);
@@ -442,7 +475,15 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
                     }
                 }
             }
-            const bool part = k0 + BK > w.seen_min;
+            if (k0 + BK > w.seen_min) {
+#pragma unroll
+                for (int n = 0; n < NQ; n++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (k0 + 32 * kk + 16 * u + 4 * g + r >= col[n].seen) s[u][n][r] = NEG_INF;
+            }
             Frag<T> ds[NQ];
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
@@ -451,9 +492,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const float p = exp2_fast(__builtin_fmaf(s[u][n][r], A.c, -lse[n]));
-                        float x = p * (dp[u][n][r] - delta[n]);
-                        if (part && k0 + 32 * kk + 16 * u + 4 * g + r >= col[n].seen) x = 0.0f;
-                        s[u][n][r] = x;
+                        s[u][n][r] = p * dp[u][n][r];
                     }
                 ds[n] = gs::frag_of_tiles<T>(s[0][n], s[1][n]);
             }
@@ -464,11 +503,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
                 for (int n = 0; n < NQ; n++) acc[d][n] = gs::mma(a, ds[n], acc[d][n]);
             }
         }
-        if (t + 1 < w.t1) {
-            uint4* next = lds + ((t + 1 - w.t0) & 1) * 2 * WORDS;
-            sk.store(next);
-            sv.store(next + WORDS);
-        }
+        if (t + 1 < w.t1) put(t + 1);
         __syncthreads();
     }
 #pragma unroll
@@ -478,29 +513,27 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
             const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
             float* p = A.part + (w.split * rows + (int64_t)w.bh * A.G * A.Tq + col[n].r) * A.D;
 #pragma unroll
-            for (int d = 0; d < DT; d++) store4<ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+            for (int d = 0; d < DT; d++) store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
         } else {
             T* p = (T*)A.out0 + w.b * A.s0.b + col[n].h * A.s0.h + col[n].i * A.s0.t;
 #pragma unroll
-            for (int d = 0; d < DT; d++) store4<ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+            for (int d = 0; d < DT; d++) store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
         }
     }
 }
 
 // dk and dv.  A wave holds 16 NK keys; the block streams the queries of every
 // head that shares them, QT rows at a time.
-template <typename T, int DP, int NK, int QT, bool ODD>
+template <typename T, int DP, int NK, int QT, Fill F>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NK, WORDS = QT * L::CHUNKS, BUF = 2 * WORDS + QT / 2;
-    extern __shared__ uint4 lds[];   // [2][q tile, do tile, lse[QT], delta[QT]]
+    extern __shared__ uint4 lds[];   // [2][q tile, do tile, lse[QT], -delta[QT]]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const L tile_of;
-    const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x);
-    const int split = (int)(item % (uint32_t)A.splits);
-    const uint32_t rest = item / (uint32_t)A.splits;
-    const int tile = (int)(rest % (uint32_t)A.tiles), bh = (int)(rest / (uint32_t)A.tiles);
+    const Share share = share_of(A, A.B * A.Hkv);
+    const int split = share.split, tile = share.tile, bh = share.bh;   // causal: the first keys are seen most
     const int b = bh / A.Hkv, hk = bh % A.Hkv, len = length_of(A, b), key0 = tile * COLS;
     const int64_t start = start_of(A, b);
 
@@ -516,8 +549,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const int at = 32 * c + 8 * g, left = held ? A.D - at : 0;
-            k[n][c] = gs::frag_global<T, ODD>(pk + at, left);
-            v[n][c] = gs::frag_global<T, ODD>(pv + at, left);
+            k[n][c] = gs::frag_global<T, F == gs::ODD>(pk + at, left);
+            v[n][c] = gs::frag_global<T, F == gs::ODD>(pv + at, left);
         }
 #pragma unroll
         for (int d = 0; d < DT; d++) dk[d][n] = dv[d][n] = f4{0, 0, 0, 0};
@@ -530,26 +563,28 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
     const int per_head = tiles - from, total = per_head * A.G, per = (total + A.splits - 1) / A.splits;
     const int e0 = min(total, split * per), e1 = min(total, e0 + per);
 
-    Stage<T, DP, QT, ODD> sq, sg;
-    float stat = 0.0f;   // threads 0 .. QT - 1: lse, QT .. 2 QT - 1: delta
-    auto fetch = [&](int e) {
+    Stage<T, DP, QT, F> sq, sg;
+    float stat = 0.0f;   // threads 0 .. QT - 1: lse, QT .. 2 QT - 1: -delta
+    auto fetch = [&](int e, uint4* to) {
         const int h = hk * A.G + e / per_head, q0 = (from + e % per_head) * QT, n = A.Tq - q0;
-        sq.load((const T*)A.q + b * A.qs.b + h * A.qs.h + (int64_t)q0 * A.qs.t, A.qs.t, n, A.D);
-        sg.load((const T*)A.dout + b * A.dos.b + h * A.dos.h + (int64_t)q0 * A.dos.t, A.dos.t, n, A.D);
+        sq.fetch(to, (const T*)A.q + b * A.qs.b + h * A.qs.h + (int64_t)q0 * A.qs.t, A.qs.t, n, A.D);
+        sg.fetch(to + WORDS, (const T*)A.dout + b * A.dos.b + h * A.dos.h + (int64_t)q0 * A.dos.t, A.dos.t, n, A.D);
         if (threadIdx.x < 2 * QT) {
             const int r = threadIdx.x % QT;
             const int64_t row = ((int64_t)b * A.Hkv * A.G + h) * A.Tq + q0 + r;
             if (threadIdx.x < QT) stat = r < n ? A.lse[row] : -NEG_INF;
-            else stat = r < n ? A.delta[row] : 0.0f;
+            else stat = r < n ? -A.delta[row] : 0.0f;
         }
     };
     auto put = [&](uint4* to) {
-        sq.store(to);
-        sg.store(to + WORDS);
+        sq.put(to);
+        sg.put(to + WORDS);
         if (threadIdx.x < 2 * QT) ((float*)(to + 2 * WORDS))[threadIdx.x] = stat;
     };
     if (e0 < e1) {
-        fetch(e0);
+#pragma unroll
+        for (int k = 0; k < 4; k++) sq.clear(lds + k / 2 * BUF + k % 2 * WORDS, A.D);
+        fetch(e0, lds);
         put(lds);
     }
     __syncthreads();
@@ -558,15 +593,21 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
         const uint4* gt = qt + WORDS;
         const float* st = (const float*)(gt + WORDS);
         const int q0 = (from + e % per_head) * QT;
-        if (e + 1 < e1) fetch(e + 1);
+        if (e + 1 < e1) fetch(e + 1, lds + ((e + 1 - e0) & 1) * BUF);
+        // row r of the tile sees key `key` when r >= sees + key - key0
         const bool part = A.causal && start + q0 < (int64_t)key0 + COLS - 1;
+        const int sees = part ? (int)(key0 - start - q0) : 0;   // between -COLS and QT
 #pragma unroll
         for (int kk = 0; kk < QT / 32; kk++) {
             f4 s[2][NK], dp[2][NK];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
+                const f4 delta = *(const f4*)(st + QT + 32 * kk + 16 * u + 4 * g);
 #pragma unroll
-                for (int n = 0; n < NK; n++) s[u][n] = dp[u][n] = f4{0, 0, 0, 0};
+                for (int n = 0; n < NK; n++) {
+                    s[u][n] = f4{0, 0, 0, 0};
+                    dp[u][n] = delta;   // the sums start at -delta
+                }
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
                     const Frag<T> a = tile_of.rows(qt, 32 * kk + 16 * u, 32 * c), d = tile_of.rows(gt, 32 * kk + 16 * u, 32 * c);
@@ -577,19 +618,26 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
                     }
                 }
             }
+            if (part) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int n = 0; n < NK; n++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (32 * kk + 16 * u + 4 * g + r < sees + key[n] - key0) s[u][n][r] = NEG_INF;
+            }
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int r0 = 32 * kk + 16 * u + 4 * g;
-                const f4 lse = *(const f4*)(st + r0), delta = *(const f4*)(st + QT + r0);
+                const f4 lse = *(const f4*)(st + r0);
 #pragma unroll
                 for (int n = 0; n < NK; n++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        float p = exp2_fast(__builtin_fmaf(s[u][n][r], A.c, -lse[r]));
-                        float x = p * (dp[u][n][r] - delta[r]);
-                        if (part && key[n] > start + q0 + r0 + r) p = x = 0.0f;
+                        const float p = exp2_fast(__builtin_fmaf(s[u][n][r], A.c, -lse[r]));
                         s[u][n][r] = p;
-                        dp[u][n][r] = x;
+                        dp[u][n][r] = p * dp[u][n][r];
                     }
             }
             Frag<T> fp[NK], fs[NK];
@@ -621,11 +669,11 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
             const f4 xk = held ? dk[d][n] * A.scale : f4{0, 0, 0, 0}, xv = held ? dv[d][n] : f4{0, 0, 0, 0};
             if (A.part != nullptr) {
                 const int64_t rows = (int64_t)A.B * A.Hkv * A.Tk, row = (int64_t)bh * A.Tk + key[n];
-                store4<ODD>(A.part + (2 * split * rows + row) * A.D + at, xk, left);
-                store4<ODD>(A.part + ((2 * split + 1) * rows + row) * A.D + at, xv, left);
+                store4<F == gs::ODD>(A.part + (2 * split * rows + row) * A.D + at, xk, left);
+                store4<F == gs::ODD>(A.part + ((2 * split + 1) * rows + row) * A.D + at, xv, left);
             } else {
-                store4<ODD>((T*)A.out0 + b * A.s0.b + hk * A.s0.h + (int64_t)key[n] * A.s0.t + at, xk, left);
-                store4<ODD>((T*)A.out1 + b * A.s1.b + hk * A.s1.h + (int64_t)key[n] * A.s1.t + at, xv, left);
+                store4<F == gs::ODD>((T*)A.out0 + b * A.s0.b + hk * A.s0.h + (int64_t)key[n] * A.s0.t + at, xk, left);
+                store4<F == gs::ODD>((T*)A.out1 + b * A.s1.b + hk * A.s1.h + (int64_t)key[n] * A.s1.t + at, xv, left);
             }
         }
     }
@@ -657,10 +705,11 @@ constexpr int ENOUGH = 1024;
 int padded(int D) { return (D + 31) / 32 * 32; }
 
 // Splits of a walk of `steps` tiles when there are `blocks` column tiles: as
-// many as fill the chip, none shorter than four tiles.
-int splits_of(int64_t blocks, int steps)
+// many as fill the chip (tiles of unequal cost: twice over), none shorter than
+// four tiles.
+int splits_of(int64_t blocks, int steps, bool unequal)
 {
-    if (blocks >= ENOUGH / 2 || steps < 8) return 1;
+    if (blocks >= (unequal ? ENOUGH : ENOUGH / 2) || steps < 8) return 1;
     const int64_t want = (ENOUGH + blocks - 1) / blocks;
     return (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));
 }
@@ -669,15 +718,15 @@ enum Walk { FORWARD, DQ, DKV };
 
 // Whether a wave's registers hold 32 columns, which halve the LDS reads per
 // product, or 16.
-constexpr bool two_columns(Walk w, bool f32, int DP) { return w == DKV ? DP <= 64 : !(f32 && DP > 64); }
+constexpr bool two_columns(Walk w, bool f32, int DP) { return w == DKV ? DP <= (f32 ? 32 : 64) : !(f32 && DP > 64); }
 
 // How the three walks of one problem are cut.
 struct Plan {
-    int nq, nk, tiles_q, tiles_k, splits_f, splits_q, splits_k, qt;
+    int nq, nk, splits_f, splits_q, splits_k, qt;
     size_t fwd_bytes, bwd_bytes;
 };
 
-Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D)
+Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D, bool causal)
 {
     Plan p{};
     const int DP = padded(D);
@@ -688,10 +737,9 @@ Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D)
     p.nq = whole && two_columns(DQ, f32, DP) && heads * ((rows + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
     p.nk = whole && two_columns(DKV, f32, DP) && heads * (((int64_t)Tk + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
     p.qt = 64;
-    p.tiles_q = (int)((rows + 64 * p.nq - 1) / (64 * p.nq));
-    p.tiles_k = (int)(((int64_t)Tk + 64 * p.nk - 1) / (64 * p.nk));
-    p.splits_f = p.splits_q = splits_of(heads * p.tiles_q, (Tk + BK - 1) / BK);
-    p.splits_k = splits_of(heads * p.tiles_k, (int)std::min<int64_t>((int64_t)G * ((Tq + p.qt - 1) / p.qt), 1 << 20));
+    const int64_t tiles_q = (rows + 64 * p.nq - 1) / (64 * p.nq), tiles_k = ((int64_t)Tk + 64 * p.nk - 1) / (64 * p.nk);
+    p.splits_f = p.splits_q = splits_of(heads * tiles_q, (Tk + BK - 1) / BK, causal);
+    p.splits_k = splits_of(heads * tiles_k, (int)std::min<int64_t>((int64_t)G * ((Tq + p.qt - 1) / p.qt), 1 << 20), causal);
     const size_t all = (size_t)heads * (size_t)rows;
     p.fwd_bytes = p.splits_f > 1 ? (size_t)p.splits_f * all * (size_t)(D + 2) * 4 : 0;
     const size_t dq = p.splits_q > 1 ? (size_t)p.splits_q * all * (size_t)D * 4 : 0;
@@ -711,46 +759,60 @@ int launch(const char* name, K kernel, int64_t blocks, size_t lds, const AttnArg
     return GS_OK;
 }
 
-template <typename T, int DP, int NQ, bool ODD>
+template <typename T, int DP, int NQ, Fill F>
 int forward_one(const AttnArgs& A, hipStream_t stream)
 {
     const size_t lds = (size_t)4 * BK * Tile<T, DP>::CHUNKS * 16;
-    return launch("attn_fwd_kernel", attn_fwd_kernel<T, DP, NQ, ODD>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
+    return launch("attn_fwd_kernel", attn_fwd_kernel<T, DP, NQ, F>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
                   stream);
 }
 
-template <typename T, int DP, int NQ, bool ODD>
+template <typename T, int DP, int NQ, Fill F>
 int dq_one(const AttnArgs& A, hipStream_t stream)
 {
     const size_t lds = (size_t)4 * BK * Tile<T, DP>::CHUNKS * 16;
-    return launch("attn_dq_kernel", attn_dq_kernel<T, DP, NQ, ODD>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
+    return launch("attn_dq_kernel", attn_dq_kernel<T, DP, NQ, F>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
                   stream);
 }
 
-template <typename T, int DP, int NK, bool ODD>
+template <typename T, int DP, int NK, Fill F>
 int dkv_one(const AttnArgs& A, hipStream_t stream)
 {
     constexpr int QT = 64;
     const size_t lds = (size_t)2 * (2 * QT * Tile<T, DP>::CHUNKS + QT / 2) * 16;
-    return launch("attn_dkv_kernel", attn_dkv_kernel<T, DP, NK, QT, ODD>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
+    return launch("attn_dkv_kernel", attn_dkv_kernel<T, DP, NK, QT, F>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
                   stream);
 }
 
-template <Walk W, typename T, int DP, int N, bool ODD>
-int run_one(const AttnArgs& A, hipStream_t stream)
+template <Walk W, typename T, int DP, int N, Fill F>
+int run_one(AttnArgs A, hipStream_t stream)
 {
-    if constexpr (W == FORWARD) return forward_one<T, DP, N, ODD>(A, stream);
-    else if constexpr (W == DQ) return dq_one<T, DP, N, ODD>(A, stream);
-    else return dkv_one<T, DP, N, ODD>(A, stream);
+    const int64_t columns = W == DKV ? A.Tk : (int64_t)A.G * A.Tq;
+    A.tiles = (int)((columns + 64 * N - 1) / (64 * N));
+    if constexpr (W == FORWARD) return forward_one<T, DP, N, F>(A, stream);
+    else if constexpr (W == DQ) return dq_one<T, DP, N, F>(A, stream);
+    else return dkv_one<T, DP, N, F>(A, stream);
+}
+
+// Whether a walk's streamed rows may be loaded straight to LDS: all but views at
+// odd addresses, for which 16 columns per wave are enough.
+bool direct(const void* p, const Strides& s, int elem)
+{
+    const int64_t v = 16 / elem;
+    return ((uintptr_t)p & 15) == 0 && s.b % v == 0 && s.h % v == 0 && s.t % v == 0 && s.t >= 0 &&
+           s.t * elem * BK < (1ll << 31);
 }
 
 template <Walk W, typename T, int DP>
 int run_width(const AttnArgs& A, int wide, hipStream_t stream)
 {
-    if (A.D % gs::Vec<T>::N != 0) return run_one<W, T, DP, 1, true>(A, stream);
+    if (A.D % gs::Vec<T>::N != 0) return run_one<W, T, DP, 1, gs::ODD>(A, stream);
+    const bool aligned = W == DKV ? direct(A.q, A.qs, sizeof(T)) && direct(A.dout, A.dos, sizeof(T))
+                                  : direct(A.k, A.ks, sizeof(T)) && direct(A.v, A.vs, sizeof(T));
+    if (!aligned) return run_one<W, T, DP, 1, gs::WHOLE>(A, stream);
     if constexpr (two_columns(W, sizeof(T) == 4, DP))
-        if (wide == 2) return run_one<W, T, DP, 2, false>(A, stream);
-    return run_one<W, T, DP, 1, false>(A, stream);
+        if (wide == 2) return run_one<W, T, DP, 2, gs::DIRECT>(A, stream);
+    return run_one<W, T, DP, 1, gs::DIRECT>(A, stream);
 }
 
 template <Walk W, typename T>
@@ -826,10 +888,11 @@ AttnArgs args_of(int B, int Hq, int Hkv, int Tq, int Tk, int D, float scale, int
 
 }  // namespace
 
-extern "C" size_t gs_attention_workspace_bytes(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, int backward)
+extern "C" size_t gs_attention_workspace_bytes(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, int causal,
+                                               int backward)
 {
     if (check(type, B, Hq, Hkv, Tq, Tk, D, 1.0f) != GS_OK) return 0;
-    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D);
+    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal != 0);
     return std::max<size_t>(256, backward ? p.bwd_bytes : p.fwd_bytes);
 }
 
@@ -844,7 +907,7 @@ extern "C" int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, in
     if (B == 0 || Tq == 0) return GS_OK;
     GS_REQUIRE(q && o && q_strides && k_strides && v_strides && o_strides, "attention: q, o and all strides must be given");
     GS_REQUIRE(Tk == 0 || (k && v), "attention: k and v must be non-null");
-    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D);
+    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal != 0);
     GS_REQUIRE(p.splits_f == 1 || workspace != nullptr, "attention: this size needs the workspace");
     AttnArgs A = args_of(B, Hq, Hkv, Tq, Tk, D, scale, causal, key_lengths, query_start);
     A.q = q;
@@ -858,7 +921,6 @@ extern "C" int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, in
     A.vs = strides_of(v_strides);
     A.s0 = strides_of(o_strides);
     A.splits = p.splits_f;
-    A.tiles = p.tiles_q;
     if (A.splits > 1) {
         A.part = (float*)workspace;
         A.part_ml = A.part + (size_t)A.splits * B * Hq * (size_t)Tq * D;
@@ -890,7 +952,7 @@ extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, i
     GS_REQUIRE(workspace != nullptr, "attention: the backward needs the workspace");
     GS_REQUIRE(Tq == 0 || (q && o && lse && dout && dq), "attention: q, o, lse, dout and dq must be non-null");
     GS_REQUIRE(Tk == 0 || (k && v && dk && dv), "attention: k, v, dk and dv must be non-null");
-    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D);
+    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal != 0);
     AttnArgs A = args_of(B, Hq, Hkv, Tq, Tk, D, scale, causal, key_lengths, query_start);
     A.q = q;
     A.k = k;
@@ -915,8 +977,7 @@ extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, i
         A.out0 = dq;
         A.s0 = strides_of(dq_strides);
         A.splits = p.splits_q;
-        A.tiles = p.tiles_q;
-        A.part = A.splits > 1 ? part : nullptr;
+            A.part = A.splits > 1 ? part : nullptr;
         if (int rc = run<DQ>(type, A, p.nq, stream)) return rc;
         if (A.splits > 1) {
             add_all(1, Hq, Tq);
@@ -929,7 +990,6 @@ extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, i
         A.s0 = strides_of(dk_strides);
         A.s1 = strides_of(dv_strides);
         A.splits = p.splits_k;
-        A.tiles = p.tiles_k;
         A.part = A.splits > 1 ? part : nullptr;
         if (int rc = run<DKV>(type, A, p.nk, stream)) return rc;
         if (A.splits > 1) {

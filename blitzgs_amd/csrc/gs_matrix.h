@@ -56,28 +56,27 @@ __device__ __forceinline__ Frag<T> frag_of_tiles(f4 a, f4 b)
         f.lo = a;
         f.hi = b;
     } else {
-        T t[8];
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            t[r] = (T)a[r];
-            t[4 + r] = (T)b[r];
-        }
+        // in pairs, which the conversion instruction takes
+        typedef T t2 __attribute__((ext_vector_type(2)));
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        const t2 t[4] = {__builtin_convertvector(f2{a[0], a[1]}, t2), __builtin_convertvector(f2{a[2], a[3]}, t2),
+                         __builtin_convertvector(f2{b[0], b[1]}, t2), __builtin_convertvector(f2{b[2], b[3]}, t2)};
         f.v = __builtin_bit_cast(s8, t);
     }
     return f;
 }
 
 // The first n (at most 8) elements at p, the others zero, as an operand whose
-// k(g, j) is 8 g + j.  Unless ODD, n is a whole number of 16-byte pieces or
+// k(g, j) is 8 g + j.  Unless BY_ELEMENT, n is a whole number of 16-byte pieces or
 // not positive.
-template <typename T, bool ODD>
+template <typename T, bool BY_ELEMENT>
 __device__ __forceinline__ Frag<T> frag_global(const T* p, int n)
 {
     constexpr int V = Vec<T>::N;
     Vec<T> v[8 / V] = {};
 #pragma unroll
     for (int h = 0; h < 8 / V; h++) {
-        if constexpr (ODD) {
+        if constexpr (BY_ELEMENT) {
 #pragma unroll
             for (int e = 0; e < V; e++)
                 if (h * V + e < n) v[h].v[e] = p[h * V + e];
@@ -96,22 +95,29 @@ __device__ __forceinline__ Frag<T> frag_global(const T* p, int n)
 }
 
 // A tile of rows of DP elements in LDS.  A row's 16-byte chunks are permuted by
-// an XOR of the row's low bits, so that the two ways it is read meet every
-// bank equally: 16 rows at one chunk (row operands), and four neighbouring
-// rows at two chunks (column operands).  The XOR repeats every 8 rows and
-// every 8 (or 4) chunks, so a lane's addresses are a few numbers, kept in
-// registers, plus constants that fit the LDS instructions' offsets.
+// an XOR of the row's low bits, so that both ways it is read meet all 64 banks
+// equally.  A 16-byte read is served 16 lanes at a time, of which 8 read one
+// chunk of rows 0-3 and 12-15 and 8 the next chunk of rows 4-11 (or the other
+// way round); the transposing read 32 at a time, two chunks of 8 rows.  With
+// chunk c of row r at c ^ x(r) each takes 16 different places of 256 bytes for
+//   rows of 256 bytes   x = 2 (r % 8)       of 128 bytes   x = r & 6
+//   of 64 or 192 bytes  x = 2 (r / 4 % 2)
+// (an XOR of ((r & 3) << 1 | (r >> 2) & 1), which meets 8 lanes' banks equally,
+// cost half as many LDS cycles again).  The lane-dependent part of an address
+// is one of a few numbers kept in registers; the rest fits the instruction's
+// offset.
 template <typename T, int DP>
 struct Tile {
     static constexpr int CHUNKS = DP * (int)sizeof(T) / 16;
-    static constexpr bool EIGHT = CHUNKS % 8 == 0;
+    // chunks that the XOR ranges over, and how many bases rows() and cols() need
+    static constexpr int SPAN = CHUNKS % 16 == 0 ? 16 : CHUNKS % 8 == 0 ? 8 : 4;
+    static constexpr int RB = sizeof(T) == 4 ? 2 * SPAN / 8 : SPAN / 4, CB = sizeof(T) == 4 ? SPAN : SPAN / 2;
 
-    int row_at[2], col_at[sizeof(T) == 4 ? 8 : 4];
+    int row_at[RB], col_at[CB];
 
     __device__ static __forceinline__ int chunk(int row, int c)
     {
-        if constexpr (EIGHT) return row * CHUNKS + (c ^ (((row & 3) << 1) | ((row >> 2) & 1)));
-        else return row * CHUNKS + (c ^ ((row & 2) | ((row >> 2) & 1)));
+        return row * CHUNKS + (c ^ (SPAN == 16 ? 2 * (row & 7) : SPAN == 8 ? row & 6 : (row >> 1) & 2));
     }
 
     __device__ __forceinline__ Tile()
@@ -119,31 +125,28 @@ struct Tile {
         const int i = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int e = 0; e < 2; e++) row_at[e] = chunk(i, 2 * g + e);
+            for (int b = 0; b < RB; b++) row_at[b] = chunk(i, 8 * (b >> 1) + 2 * g + (b & 1));
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int d = 0; d < 2; d++) col_at[2 * r + d] = chunk(4 * g + r, 4 * d + i / 4) * 4 + i % 4;
+            for (int b = 0; b < CB; b++) col_at[b] = chunk(4 * g + (b & 3), 4 * (b >> 2) + i / 4) * 4 + i % 4;
         } else {
 #pragma unroll
-            for (int e = 0; e < 2; e++) row_at[e] = chunk(i, EIGHT ? 4 * e + g : g);
+            for (int b = 0; b < RB; b++) row_at[b] = chunk(i, 4 * b + g);
 #pragma unroll
-            for (int d = 0; d < 4; d++)
-                col_at[d] = 2 * chunk(4 * g + i / 4, EIGHT || d < 2 ? 2 * d + (i % 4) / 2 : 0) + i % 2;
+            for (int b = 0; b < CB; b++) col_at[b] = 2 * chunk(4 * g + i / 4, 2 * b + (i % 4) / 2) + i % 2;
         }
     }
 
     // Rows row + i, k(g, j) = k0 + 8 g + j; row a multiple of 16, k0 of 32.
     __device__ __forceinline__ Frag<T> rows(const uint4* t, int row, int k0) const
     {
-        const int c = k0 / 32;
+        constexpr int STEP = 2 * (int)sizeof(T);   // chunks of 32 k
+        const int c = k0 / 32 * STEP, b = c % SPAN / STEP, at = row * CHUNKS + c / SPAN * SPAN;
         Frag<T> f;
         if constexpr (sizeof(T) == 4) {
-            f.lo = __builtin_bit_cast(f4, t[row_at[0] + row * CHUNKS + 8 * c]);
-            f.hi = __builtin_bit_cast(f4, t[row_at[1] + row * CHUNKS + 8 * c]);
+            f.lo = __builtin_bit_cast(f4, t[row_at[2 * b] + at]);
+            f.hi = __builtin_bit_cast(f4, t[row_at[2 * b + 1] + at]);
         } else {
-            f.v = __builtin_bit_cast(
-                s8, t[EIGHT ? row_at[c & 1] + row * CHUNKS + 8 * (c >> 1) : row_at[0] + row * CHUNKS + 4 * c]);
+            f.v = __builtin_bit_cast(s8, t[row_at[b] + at]);
         }
         return f;
     }
@@ -154,43 +157,68 @@ struct Tile {
     // fetch 4 rows of 16 elements.
     __device__ __forceinline__ Frag<T> cols(const uint4* t, int row, int col) const
     {
-        const int d = col / 16;
+        constexpr int STEP = (int)sizeof(T);       // chunks of 16 columns
+        const int c = col / 16 * STEP, b = c % SPAN / STEP, at = row * CHUNKS + c / SPAN * SPAN;
         Frag<T> f;
         if constexpr (sizeof(T) == 4) {
             const float* e = (const float*)t;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                f.lo[r] = e[col_at[2 * r + (d & 1)] + (row * CHUNKS + 8 * (d >> 1)) * 4];
-                f.hi[r] = e[col_at[2 * r + (d & 1)] + ((row + 16) * CHUNKS + 8 * (d >> 1)) * 4];
+                f.lo[r] = e[col_at[4 * b + r] + 4 * at];
+                f.hi[r] = e[col_at[4 * b + r] + 4 * (at + 16 * CHUNKS)];
             }
         } else {
             typedef __attribute__((address_space(3))) s4 lds_s4;
-            const int at = EIGHT ? col_at[d & 3] + 16 * (d >> 2) : col_at[d & 1] + 8 * (d >> 1);
-            const s4* e = (const s4*)t;
-            const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(e + at + 2 * row * CHUNKS));
-            const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(e + at + 2 * (row + 16) * CHUNKS));
-            f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+            const s4* e = (const s4*)t + col_at[b] + 2 * at;
+            const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)e);
+            const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(e + 2 * 16 * CHUNKS));
+            f.v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
         }
         return f;
     }
 };
 
-// ROWS x DP elements on their way from global memory to a Tile: each of the
-// block's 256 threads carries CPT chunks in registers.
-template <typename T, int DP, int ROWS, bool ODD>
+// How a tile's rows come to LDS.
+//   DIRECT  by loads that write LDS themselves: no registers, no LDS stores.
+//           Rows are 16-byte aligned, D is a whole number of 16 bytes, and a
+//           tile spans less than 2^31 bytes.  Rows beyond the last hold the
+//           last one again; clear() has to have zeroed the elements from D on.
+//   WHOLE   through registers, 16 bytes at a time, from any address; rows and
+//           elements beyond the last are zero
+//   ODD     through registers, element by element: D is no multiple of 16 bytes
+enum Fill { DIRECT, WHOLE, ODD };
+
+template <typename T, int DP, int ROWS, Fill F>
 struct Stage {
     static constexpr int CHUNKS = Tile<T, DP>::CHUNKS, CPT = ROWS * CHUNKS / 256, V = Vec<T>::N;
     static_assert(ROWS * CHUNKS % 256 == 0, "a whole number of chunks per thread");
     Vec<T> r[CPT];
 
-    // Rows 0 .. n_rows - 1 at p (the rest zero), `stride` elements apart, of D elements.
-    __device__ __forceinline__ void load(const T* p, int64_t stride, int n_rows, int D)
+    // Begins to fetch rows 0 .. n_rows - 1 (n_rows >= 1) at p, `stride` elements
+    // apart, of D elements, for the tile t.
+    __device__ __forceinline__ void fetch(uint4* t, const T* p, int64_t stride, int n_rows, int D)
     {
+        if constexpr (F == DIRECT) {
+            const int s = (int)stride;
+            typedef const __attribute__((address_space(1))) void* global_ptr;
+            typedef __attribute__((address_space(3))) void* lds_ptr;
+#pragma unroll
+            for (int k = 0; k < CPT; k++) {
+                // place `id` of the tile holds chunk `at` of its row
+                const int id = threadIdx.x + 256 * k, row = id / CHUNKS;
+                const int at = Tile<T, DP>::chunk(row, id % CHUNKS) - row * CHUNKS;
+                const int from = n_rows >= ROWS ? row : min(row, n_rows - 1);
+                uint4* to = t + 256 * k + (threadIdx.x & ~63u);   // + 16 bytes per lane
+                if (at * V < D)
+                    __builtin_amdgcn_global_load_lds((global_ptr)(p + (from * s + at * V)), (lds_ptr)to, 16, 0, 0);
+            }
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < CPT; k++) {
             const int id = threadIdx.x + 256 * k, row = id / CHUNKS, at = id % CHUNKS * V;
             r[k] = {};
-            if constexpr (ODD) {
+            if constexpr (F == ODD) {
 #pragma unroll
                 for (int e = 0; e < V; e++)
                     if (row < n_rows && at + e < D) r[k].v[e] = p[row * stride + at + e];
@@ -199,8 +227,21 @@ struct Stage {
             }
         }
     }
-    __device__ __forceinline__ void store(uint4* t) const
+    // DIRECT: before the first fetch, for each tile that will be fetched.
+    __device__ __forceinline__ static void clear(uint4* t, int D)
     {
+        if constexpr (F != DIRECT) return;
+        if (D == DP) return;
+#pragma unroll
+        for (int k = 0; k < CPT; k++) {
+            const int id = threadIdx.x + 256 * k, row = id / CHUNKS;
+            if ((Tile<T, DP>::chunk(row, id % CHUNKS) - row * CHUNKS) * V >= D) t[id] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    // Ends it; a barrier comes before the tile is read.
+    __device__ __forceinline__ void put(uint4* t) const
+    {
+        if constexpr (F == DIRECT) return;
 #pragma unroll
         for (int k = 0; k < CPT; k++) {
             const int id = threadIdx.x + 256 * k;

@@ -138,23 +138,10 @@ __global__ __launch_bounds__(256) void orth_split_kernel(const T* __restrict__ g
 
 enum Kind { SQUARE, POLY, APPLY };   // A = X X^T;  B = a I + b A + c A A;  X = B X
 
-// The operand rows of eight k of columns col + i of a tile with k down its rows.
-template <int DP>
-__device__ __forceinline__ Frag<f16> column_frag(const uint4* t, int col)
-{
-    const int i = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-    const int r = 8 * g + i / 4, c = col / 8 + (i % 4) / 2, half = i % 2;
-    typedef __attribute__((address_space(3))) gs::s4 lds_s4;
-    const gs::s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)((gs::s4*)(t + Tile<f16, DP>::chunk(r, c)) + half));
-    const gs::s4 b =
-        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)((gs::s4*)(t + Tile<f16, DP>::chunk(r + 4, c)) + half));
-    Frag<f16> f;
-    f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    return f;
-}
-
 // Both planes of an operand's next S x KT tile (DOWN: KT x S, k down its rows)
-// on their way to LDS, in registers.
+// on their way to LDS, in registers.  DOWN's rows go to LDS in the order in
+// which Tile::cols takes them as k = 8 g + j, each half of its columns as a
+// tile of its own.
 template <int S, bool DOWN>
 struct Pair {
     static constexpr int CH = S * KT / 8 / 256, W = DOWN ? S / 8 : KT / 8;   // chunks per thread, per row
@@ -184,7 +171,9 @@ struct Pair {
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int r = threadIdx.x / W + c * (256 / W);
-            const int e = DOWN ? Tile<f16, S>::chunk(r, threadIdx.x % W) : Tile<f16, KT>::chunk(r, threadIdx.x % W);
+            const int to = 4 * (r / 8) + r % 4 + 16 * (r / 4 % 2);
+            constexpr int HW = W / 2;
+            const int e = DOWN ? threadIdx.x % W / HW * KT * HW + Tile<f16, S / 2>::chunk(to, threadIdx.x % HW) : Tile<f16, KT>::chunk(r, threadIdx.x % W);
             th[e] = hi[c];
             tl[e] = lo[c];
         }
@@ -224,6 +213,7 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
     sl.at(A.l, lp, m0);
     sr.at(A.r, rp, n0);
     const Tile<f16, KT> tile;
+    const Tile<f16, H> down;
     const int ml = (wave & 1) * H, nl = (wave >> 1) * H;
     f4 acc[U][U];   // [columns of the result][rows of the result]
 #pragma unroll
@@ -243,18 +233,18 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
         Frag<f16> lh[U], ll[U];
 #pragma unroll
         for (int v = 0; v < U; v++) {
-            lh[v] = tile.rows(lds[b][0], ml + 16 * v, 0);
-            ll[v] = tile.rows(lds[b][1], ml + 16 * v, 0);
+            lh[v] = tile.rows(lds[b][0] + ml * KT / 8, 16 * v, 0);
+            ll[v] = tile.rows(lds[b][1] + ml * KT / 8, 16 * v, 0);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             Frag<f16> rh, rl;
             if constexpr (K == APPLY) {
-                rh = column_frag<S>(lds[b][2], nl + 16 * u);
-                rl = column_frag<S>(lds[b][3], nl + 16 * u);
+                rh = down.cols(lds[b][2] + nl * KT / 8, 0, 16 * u);
+                rl = down.cols(lds[b][3] + nl * KT / 8, 0, 16 * u);
             } else {
-                rh = tile.rows(lds[b][2], nl + 16 * u, 0);
-                rl = tile.rows(lds[b][3], nl + 16 * u, 0);
+                rh = tile.rows(lds[b][2] + nl * KT / 8, 16 * u, 0);
+                rl = tile.rows(lds[b][3] + nl * KT / 8, 16 * u, 0);
             }
 #pragma unroll
             for (int v = 0; v < U; v++) {

@@ -686,7 +686,7 @@ int gs_layer_norm_backward(int type, int param_type, int64_t rows, int width, co
  *   The workspace's size (gs_attention_workspace_bytes, 0: invalid arguments)
  * depends on sizes alone.  Results do not depend on the order of execution. */
 size_t gs_attention_workspace_bytes(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D,
-                                    int backward);
+                                    int causal, int backward);
 int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, const void* q,
                          const int64_t* q_strides, const void* k, const int64_t* k_strides,
                          const void* v, const int64_t* v_strides, float scale, int causal,
