@@ -43,42 +43,51 @@ def _token_major(like):
     return torch.empty((B, T, H, D), device=like.device, dtype=like.dtype).transpose(1, 2)
 
 
+def _workspace(sizes, causal, key_lengths, backward, device):
+    unequal = int(causal or key_lengths is not None)
+    return _lib.workspace(_lib.load().gs_attention_workspace_bytes(*sizes, unequal, backward), device)
+
+
+def _forward(q, k, v, causal, key_lengths, query_start, scale, grads):
+    """o and, for a backward, (sizes, what rounding o left, lse)."""
+    B, Hq, Tq, D = q.shape
+    Hkv, Tk = k.shape[1:3]
+    sizes = _lib.dtype_code(q.dtype), B, Hq, Hkv, Tq, Tk, D
+    o = _token_major(q)
+    lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32) if grads else None
+    rest = _token_major(q) if grads and q.dtype != torch.float32 else None
+    ws = _workspace(sizes, causal, key_lengths, 0, q.device)
+    with _lib.on_device(q.device):
+        _lib.check(_lib.load().gs_attention_forward(
+            *sizes, _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), scale, int(causal),
+            _lib.ptr(key_lengths), _lib.ptr(query_start), _lib.ptr(o), _strides(o), _lib.ptr(rest), _lib.ptr(lse),
+            _lib.ptr(ws), _lib.stream_of(q.device)), "gs_attention_forward")
+    return o, (sizes, rest, lse)
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, causal, key_lengths, query_start, scale):
-        needs = any(ctx.needs_input_grad[:3])
         q, k, v = (_last_contiguous(t.detach()) for t in (q, k, v))
-        B, Hq, Tq, D = q.shape
-        Hkv, Tk = k.shape[1:3]
-        lib, sizes = _lib.load(), (_lib.dtype_code(q.dtype), B, Hq, Hkv, Tq, Tk, D)
-        o = _token_major(q)
-        lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32) if needs else None
-        # what the rounding of o leaves, for the backward's sum(do o)
-        rest = _token_major(q) if needs and q.dtype != torch.float32 else None
-        ws = torch.empty(lib.gs_attention_workspace_bytes(*sizes, int(causal), 0), device=q.device, dtype=torch.uint8)
-        with torch.cuda.device(q.device):
-            _lib.check(lib.gs_attention_forward(
-                *sizes, _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), scale,
-                int(causal), _lib.ptr(key_lengths), _lib.ptr(query_start), _lib.ptr(o), _strides(o), _lib.ptr(rest),
-                _lib.ptr(lse), _lib.ptr(ws), _lib.stream_of(q.device)), "gs_attention_forward")
-        if needs:
-            ctx.save_for_backward(q, k, v, o, rest, lse, key_lengths, query_start)
-            ctx.sizes, ctx.scale, ctx.causal = sizes, scale, causal
+        o, (ctx.sizes, rest, lse) = _forward(q, k, v, causal, key_lengths, query_start, scale, True)
+        ctx.save_for_backward(q, k, v, o, rest, lse, key_lengths, query_start)
+        ctx.scale, ctx.causal = scale, causal
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, o, rest, lse, key_lengths, query_start = ctx.saved_tensors
-        lib, do = _lib.load(), _last_contiguous(do)
+        do = _last_contiguous(do)
         dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
-        ws = torch.empty(lib.gs_attention_workspace_bytes(*ctx.sizes, int(ctx.causal), 1), device=q.device, dtype=torch.uint8)
-        with torch.cuda.device(q.device):
-            _lib.check(lib.gs_attention_backward(
+        ws = _workspace(ctx.sizes, ctx.causal, key_lengths, 1, q.device)
+        with _lib.on_device(q.device):
+            _lib.check(_lib.load().gs_attention_backward(
                 *ctx.sizes, _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), ctx.scale,
                 int(ctx.causal), _lib.ptr(key_lengths), _lib.ptr(query_start), _lib.ptr(o), _strides(o),
                 _lib.ptr(rest), _lib.ptr(lse), _lib.ptr(do), _strides(do), _lib.ptr(dq), _strides(dq), _lib.ptr(dk),
-                _strides(dk), _lib.ptr(dv), _strides(dv), _lib.ptr(ws), _lib.stream_of(q.device)), "gs_attention_backward")
+                _strides(dk), _lib.ptr(dv), _strides(dv), _lib.ptr(ws), _lib.stream_of(q.device)),
+                "gs_attention_backward")
         return dq, dk, dv, None, None, None, None
 
 
@@ -113,5 +122,7 @@ def attention(q, k, v, causal=False, key_lengths=None, query_start=None, scale=N
         raise RuntimeError(f"scale must be a positive number, got {scale}")
     if query_start is not None and not causal:
         raise RuntimeError("query_start needs causal=True")
-    return _Attention.apply(q, k, v, bool(causal), _per_batch(key_lengths, "key_lengths", q),
-                            _per_batch(query_start, "query_start", q), scale)
+    how = bool(causal), _per_batch(key_lengths, "key_lengths", q), _per_batch(query_start, "query_start", q), scale
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(q, k, v, *how)
+    return _forward(*(_last_contiguous(t) for t in (q, k, v)), *how, False)[0]

@@ -101,11 +101,12 @@ __device__ __forceinline__ int seen_of(const AttnArgs& A, int len, int64_t start
 }
 
 // A workgroup's share: a column tile of one (batch, key head), and a split of
-// its walk.  Each XCD gets a run of neighbours, which stream the same rows
-// through its L2.  Where a causal limit makes a tile's place decide its cost and
-// the runs are not whole heads, one XCD would get the costly half of a head;
-// there the costliest tiles of all heads go first, dealt out in turn.  dk, dv
-// of 4 key heads of 8192 keys: 695 us, in runs 1181, head by head 1030.
+// its walk.  Where all tiles cost the same, each XCD gets a run of neighbours,
+// which stream the same rows through its L2.  With a causal limit that holds for
+// runs of whole heads only, else one XCD gets the costly half of a head; with
+// key lengths it holds for none.  There the costliest tiles of all heads go
+// first, dealt out in turn.  dk, dv of 4 key heads of 8192 keys, causal: 695 us,
+// in runs 1181; 8 batches of up to 32768 keys, one query: 112 us, in runs 145.
 struct Share {
     int bh, tile, split;
 };
@@ -113,7 +114,7 @@ struct Share {
 __device__ __forceinline__ Share share_of(const AttnArgs& A, int cost_heads)
 {
     const uint32_t heads = (uint32_t)(A.B * A.Hkv), tiles = (uint32_t)A.tiles, splits = (uint32_t)A.splits;
-    if (!A.causal || cost_heads % 8 == 0) {
+    if (A.key_lengths == nullptr && (!A.causal || cost_heads % 8 == 0)) {
         const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x), rest = item / splits;
         return {(int)(rest / tiles), (int)(rest % tiles), (int)(item % splits)};
     }
@@ -343,43 +344,49 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             const int at = 16 * d + 4 * g;
-            store_o<F == gs::ODD>((T*)A.out0 + out + at, rest == nullptr ? nullptr : rest + at, o[d][n] * inv, A.D - at);
+            store_o<F == gs::ODD>((T*)A.out0 + out + at, rest == nullptr ? nullptr : rest + at, o[d][n] * inv,
+                                  A.D - at);
         }
         if (g == 0 && A.lse != nullptr) A.lse[row] = sum == 0.0f ? -NEG_INF : m[n] + __builtin_log2f(sum);
     }
 }
 
-// Joins the splits of a row: one wave per row.
+// Joins the splits of a row: one workgroup per row, a wave every fourth split.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs A)
 {
-    const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const int lane = threadIdx.x & 63;
+    __shared__ float sums[4][130];
+    const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq, row = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float m = NEG_INF;
-    for (int s = 0; s < A.splits; s++) m = fmaxf(m, A.part_ml[2 * (s * rows + row)]);
+    for (int s = lane; s < A.splits; s += 64) m = fmaxf(m, A.part_ml[2 * (s * rows + row)]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
     const float base = m == NEG_INF ? 0.0f : m;
     float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int s = 0; s < A.splits; s++) {
+#pragma unroll 4
+    for (int s = wave; s < A.splits; s += 4) {
         const int64_t at = s * rows + row;
         const float f = exp2_fast(A.part_ml[2 * at] - base);
         sum = __builtin_fmaf(A.part_ml[2 * at + 1], f, sum);
         if (lane < A.D) o0 = __builtin_fmaf(A.part[at * A.D + lane], f, o0);
         if (lane + 64 < A.D) o1 = __builtin_fmaf(A.part[at * A.D + lane + 64], f, o1);
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    sums[wave][lane] = o0;
+    sums[wave][64 + lane] = o1;
+    if (lane == 0) sums[wave][128] = sum;
+    __syncthreads();
+    const int d = threadIdx.x;
+    sum = (sums[0][128] + sums[1][128]) + (sums[2][128] + sums[3][128]);
     const int Hq = A.Hkv * A.G, i = (int)(row % A.Tq), h = (int)(row / A.Tq % Hq), b = (int)(row / A.Tq / Hq);
     const int64_t out = b * A.s0.b + h * A.s0.h + i * A.s0.t;
-    T* p = (T*)A.out0 + out;
-    const float x0 = o0 * inv, x1 = o1 * inv;
-    if (lane < A.D) p[lane] = (T)x0;
-    if (lane + 64 < A.D) p[lane + 64] = (T)x1;
-    if (A.rest != nullptr) {
-        T* rest = (T*)A.rest + out;
-        if (lane < A.D) rest[lane] = (T)(x0 - (float)(T)x0);
-        if (lane + 64 < A.D) rest[lane + 64] = (T)(x1 - (float)(T)x1);
+    if (d < A.D) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float x = ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) * inv;
+        ((T*)A.out0)[out + d] = (T)x;
+        if (A.rest != nullptr) ((T*)A.rest)[out + d] = (T)(x - (float)(T)x);
     }
-    if (lane == 0 && A.lse != nullptr) A.lse[row] = sum == 0.0f ? -NEG_INF : m + __builtin_log2f(sum);
+    if (d == 0 && A.lse != nullptr) A.lse[row] = sum == 0.0f ? -NEG_INF : m + __builtin_log2f(sum);
 }
 
 // ------------------------------------------------------------------ backward
@@ -467,7 +474,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
                 }
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
-                    const Frag<T> a = tile_of.rows(kt, 32 * kk + 16 * u, 32 * c), b = tile_of.rows(vt, 32 * kk + 16 * u, 32 * c);
+                    const Frag<T> a = tile_of.rows(kt, 32 * kk + 16 * u, 32 * c);
+                    const Frag<T> b = tile_of.rows(vt, 32 * kk + 16 * u, 32 * c);
 #pragma unroll
                     for (int n = 0; n < NQ; n++) {
                         s[u][n] = gs::mma(a, q[n][c], s[u][n]);
@@ -513,11 +521,13 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
             const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
             float* p = A.part + (w.split * rows + (int64_t)w.bh * A.G * A.Tq + col[n].r) * A.D;
 #pragma unroll
-            for (int d = 0; d < DT; d++) store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+            for (int d = 0; d < DT; d++)
+                store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
         } else {
             T* p = (T*)A.out0 + w.b * A.s0.b + col[n].h * A.s0.h + col[n].i * A.s0.t;
 #pragma unroll
-            for (int d = 0; d < DT; d++) store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+            for (int d = 0; d < DT; d++)
+                store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
         }
     }
 }
@@ -610,7 +620,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
                 }
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
-                    const Frag<T> a = tile_of.rows(qt, 32 * kk + 16 * u, 32 * c), d = tile_of.rows(gt, 32 * kk + 16 * u, 32 * c);
+                    const Frag<T> a = tile_of.rows(qt, 32 * kk + 16 * u, 32 * c);
+                    const Frag<T> d = tile_of.rows(gt, 32 * kk + 16 * u, 32 * c);
 #pragma unroll
                     for (int n = 0; n < NK; n++) {
                         s[u][n] = gs::mma(a, k[n][c], s[u][n]);
@@ -682,8 +693,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
 // Adds the splits' partial gradients: [splits][per][rows = B H Tn][D] to each of
 // `per` tensors.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__ part, int splits, int per, int64_t rows,
-                                                       int H, int Tn, int D, T* out0, T* out1, Strides s0, Strides s1)
+__global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__ part, int splits, int per,
+                                                       int64_t rows, int H, int Tn, int D, T* out0, T* out1, Strides s0, Strides s1)
 {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= rows * D) return;
@@ -691,6 +702,7 @@ __global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__
     const int d = (int)(id - row * D), t = (int)(row % Tn), h = (int)(row / Tn % H), b = (int)(row / Tn / H);
     const int which = blockIdx.y;
     float s = 0.0f;
+#pragma unroll 8
     for (int k = 0; k < splits; k++) s += part[((int64_t)k * per + which) * rows * D + id];
     const Strides st = which == 0 ? s0 : s1;
     (which == 0 ? out0 : out1)[b * st.b + h * st.h + t * st.t + d] = (T)s;
@@ -706,12 +718,16 @@ int padded(int D) { return (D + 31) / 32 * 32; }
 
 // Splits of a walk of `steps` tiles when there are `blocks` column tiles: as
 // many as fill the chip (tiles of unequal cost: twice over), none shorter than
-// four tiles.
+// four tiles.  With a tile per CU already, a split has to save more than the
+// partial results cost: none shorter than 16 (370 tiles of 17 steps: 23 us in
+// four splits and 35 us to join them, against 36 us whole).
 int splits_of(int64_t blocks, int steps, bool unequal)
 {
-    if (blocks >= (unequal ? ENOUGH : ENOUGH / 2) || steps < 8) return 1;
-    const int64_t want = (ENOUGH + blocks - 1) / blocks;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));
+    const int64_t enough = unequal ? 2 * ENOUGH : ENOUGH;
+    const int least = blocks < ENOUGH / 4 ? 4 : 16;
+    if (blocks >= enough / 2 || steps < 2 * least) return 1;
+    const int64_t want = (enough + blocks - 1) / blocks;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / least));
 }
 
 enum Walk { FORWARD, DQ, DKV };
@@ -726,7 +742,7 @@ struct Plan {
     size_t fwd_bytes, bwd_bytes;
 };
 
-Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D, bool causal)
+Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D, bool unequal)
 {
     Plan p{};
     const int DP = padded(D);
@@ -738,8 +754,9 @@ Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D, bool causal
     p.nk = whole && two_columns(DKV, f32, DP) && heads * (((int64_t)Tk + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
     p.qt = 64;
     const int64_t tiles_q = (rows + 64 * p.nq - 1) / (64 * p.nq), tiles_k = ((int64_t)Tk + 64 * p.nk - 1) / (64 * p.nk);
-    p.splits_f = p.splits_q = splits_of(heads * tiles_q, (Tk + BK - 1) / BK, causal);
-    p.splits_k = splits_of(heads * tiles_k, (int)std::min<int64_t>((int64_t)G * ((Tq + p.qt - 1) / p.qt), 1 << 20), causal);
+    p.splits_f = p.splits_q = splits_of(heads * tiles_q, (Tk + BK - 1) / BK, unequal);
+    p.splits_k =
+        splits_of(heads * tiles_k, (int)std::min<int64_t>((int64_t)G * ((Tq + p.qt - 1) / p.qt), 1 << 20), unequal);
     const size_t all = (size_t)heads * (size_t)rows;
     p.fwd_bytes = p.splits_f > 1 ? (size_t)p.splits_f * all * (size_t)(D + 2) * 4 : 0;
     const size_t dq = p.splits_q > 1 ? (size_t)p.splits_q * all * (size_t)D * 4 : 0;
@@ -780,8 +797,8 @@ int dkv_one(const AttnArgs& A, hipStream_t stream)
 {
     constexpr int QT = 64;
     const size_t lds = (size_t)2 * (2 * QT * Tile<T, DP>::CHUNKS + QT / 2) * 16;
-    return launch("attn_dkv_kernel", attn_dkv_kernel<T, DP, NK, QT, F>, (int64_t)A.B * A.Hkv * A.tiles * A.splits, lds, A,
-                  stream);
+    return launch("attn_dkv_kernel", attn_dkv_kernel<T, DP, NK, QT, F>, (int64_t)A.B * A.Hkv * A.tiles * A.splits,
+                  lds, A, stream);
 }
 
 template <Walk W, typename T, int DP, int N, Fill F>
@@ -839,7 +856,7 @@ void join(const AttnArgs& A, hipStream_t stream)
 {
     const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
     GS_TIMED("attn_join_kernel", stream,
-             hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, A));
+             hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, stream, A));
 }
 
 template <typename T>
@@ -888,12 +905,12 @@ AttnArgs args_of(int B, int Hq, int Hkv, int Tq, int Tk, int D, float scale, int
 
 }  // namespace
 
-extern "C" size_t gs_attention_workspace_bytes(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, int causal,
+extern "C" size_t gs_attention_workspace_bytes(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, int unequal,
                                                int backward)
 {
     if (check(type, B, Hq, Hkv, Tq, Tk, D, 1.0f) != GS_OK) return 0;
-    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal != 0);
-    return std::max<size_t>(256, backward ? p.bwd_bytes : p.fwd_bytes);
+    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, unequal != 0);
+    return backward ? p.bwd_bytes : p.fwd_bytes;
 }
 
 extern "C" int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, const void* q,
@@ -907,7 +924,7 @@ extern "C" int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, in
     if (B == 0 || Tq == 0) return GS_OK;
     GS_REQUIRE(q && o && q_strides && k_strides && v_strides && o_strides, "attention: q, o and all strides must be given");
     GS_REQUIRE(Tk == 0 || (k && v), "attention: k and v must be non-null");
-    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal != 0);
+    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal || key_lengths);
     GS_REQUIRE(p.splits_f == 1 || workspace != nullptr, "attention: this size needs the workspace");
     AttnArgs A = args_of(B, Hq, Hkv, Tq, Tk, D, scale, causal, key_lengths, query_start);
     A.q = q;
@@ -949,10 +966,10 @@ extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, i
     GS_REQUIRE(q_strides && k_strides && v_strides && o_strides && dout_strides && dq_strides && dk_strides &&
                    dv_strides,
                "attention: all strides must be given");
-    GS_REQUIRE(workspace != nullptr, "attention: the backward needs the workspace");
     GS_REQUIRE(Tq == 0 || (q && o && lse && dout && dq), "attention: q, o, lse, dout and dq must be non-null");
     GS_REQUIRE(Tk == 0 || (k && v && dk && dv), "attention: k, v, dk and dv must be non-null");
-    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal != 0);
+    const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal || key_lengths);
+    GS_REQUIRE(p.bwd_bytes == 0 || workspace != nullptr, "attention: the backward needs the workspace");
     AttnArgs A = args_of(B, Hq, Hkv, Tq, Tk, D, scale, causal, key_lengths, query_start);
     A.q = q;
     A.k = k;

@@ -234,8 +234,10 @@ __global__ __launch_bounds__(1024) void norm_columns_kernel(const float* __restr
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = blockIdx.x * 64 + lane;
     float s = 0.0f;
-    if (col < 2 * width)
+    if (col < 2 * width) {
+#pragma unroll 8
         for (int p = wave; p < n_parts; p += 16) s += parts[(size_t)p * 2 * width + col];
+    }
     sums[wave][lane] = s;
     __syncthreads();
     if (wave != 0 || col >= 2 * width) return;

@@ -138,44 +138,43 @@ __global__ __launch_bounds__(256) void orth_split_kernel(const T* __restrict__ g
 
 enum Kind { SQUARE, POLY, APPLY };   // A = X X^T;  B = a I + b A + c A A;  X = B X
 
-// Both planes of an operand's next S x KT tile (DOWN: KT x S, k down its rows)
-// on their way to LDS, in registers.  DOWN's rows go to LDS in the order in
-// which Tile::cols takes them as k = 8 g + j, each half of its columns as a
-// tile of its own.
+// Both planes of an operand's next S x KT tile (DOWN: KT x S, k down its rows),
+// loaded straight to LDS.  DOWN's rows lie in the order in which Tile::cols
+// takes them as k = 8 g + j, each half of its columns as a tile of its own.
 template <int S, bool DOWN>
 struct Pair {
-    static constexpr int CH = S * KT / 8 / 256, W = DOWN ? S / 8 : KT / 8;   // chunks per thread, per row
-    const f16* p;
-    int64_t plane, row, step;
-    uint4 hi[CH], lo[CH];
+    static constexpr int CH = S * KT / 8 / 256;                  // chunks per thread and plane
+    static constexpr int W = DOWN ? S / 16 : KT / 8;             // chunks per row of a tile
+    using L = Tile<f16, 8 * W>;
+    const f16* p[CH];
+    int64_t plane, step;
 
     __device__ __forceinline__ void at(const Planes& m, const f16* base, int first)
     {
-        const int r = threadIdx.x / W, c = threadIdx.x % W * 8;
-        p = DOWN ? base + (int64_t)r * m.ld + first + c : base + (int64_t)(first + r) * m.ld + c;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            // place `id` of the tile holds this chunk of this row
+            const int id = threadIdx.x + 256 * c, row = id / W % (DOWN ? KT : S), col = L::chunk(row, id % W) - row * W;
+            if constexpr (DOWN) {
+                const int k = 8 * (row % 16 / 4) + 4 * (row / 16) + row % 4, half = id / (KT * W);
+                p[c] = base + (int64_t)k * m.ld + first + half * (S / 2) + col * 8;
+            } else {
+                p[c] = base + (int64_t)(first + row) * m.ld + col * 8;
+            }
+        }
         plane = m.plane;
-        row = (int64_t)(256 / W) * m.ld;
         step = DOWN ? (int64_t)KT * m.ld : KT;
     }
-    __device__ __forceinline__ void load()
+    __device__ __forceinline__ void fetch(uint4* hi, uint4* lo)
     {
+        typedef const __attribute__((address_space(1))) void* global_ptr;
+        typedef __attribute__((address_space(3))) void* lds_ptr;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            hi[c] = *(const uint4*)(p + c * row);
-            lo[c] = *(const uint4*)(p + c * row + plane);
-        }
-        p += step;
-    }
-    __device__ __forceinline__ void store(uint4* th, uint4* tl) const
-    {
-#pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int r = threadIdx.x / W + c * (256 / W);
-            const int to = 4 * (r / 8) + r % 4 + 16 * (r / 4 % 2);
-            constexpr int HW = W / 2;
-            const int e = DOWN ? threadIdx.x % W / HW * KT * HW + Tile<f16, S / 2>::chunk(to, threadIdx.x % HW) : Tile<f16, KT>::chunk(r, threadIdx.x % W);
-            th[e] = hi[c];
-            tl[e] = lo[c];
+            const int to = 256 * c + (threadIdx.x & ~63u);   // + 16 bytes per lane
+            __builtin_amdgcn_global_load_lds((global_ptr)p[c], (lds_ptr)(hi + to), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((global_ptr)(p[c] + plane), (lds_ptr)(lo + to), 16, 0, 0);
+            p[c] += step;
         }
     }
 };
@@ -220,15 +219,13 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
     for (int u = 0; u < U; u++)
 #pragma unroll
         for (int v = 0; v < U; v++) acc[u][v] = f4{0, 0, 0, 0};
-    sl.load();
-    sr.load();
-    sl.store(lds[0][0], lds[0][1]);
-    sr.store(lds[0][2], lds[0][3]);
+    sl.fetch(lds[0][0], lds[0][1]);
+    sr.fetch(lds[0][2], lds[0][3]);
     __syncthreads();
     for (int k0 = 0, b = 0; k0 < A.k; k0 += KT, b ^= 1) {
         if (k0 + KT < A.k) {
-            sl.load();
-            sr.load();
+            sl.fetch(lds[b ^ 1][0], lds[b ^ 1][1]);
+            sr.fetch(lds[b ^ 1][2], lds[b ^ 1][3]);
         }
         Frag<f16> lh[U], ll[U];
 #pragma unroll
@@ -252,10 +249,6 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
                 acc[u][v] = gs::mma(rh, ll[v], acc[u][v]);
                 acc[u][v] = gs::mma(rh, lh[v], acc[u][v]);
             }
-        }
-        if (k0 + KT < A.k) {
-            sl.store(lds[b ^ 1][0], lds[b ^ 1][1]);
-            sr.store(lds[b ^ 1][2], lds[b ^ 1][3]);
         }
         __syncthreads();
     }

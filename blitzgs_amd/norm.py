@@ -29,26 +29,29 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _forward(x, weight, bias, eps, grads):
+    """y and, for a backward, (the parameters' type, mean, rstd)."""
+    rows = _rows(x)
+    n, width = rows.shape
+    w = None if weight is None else weight.contiguous()
+    b = None if bias is None else bias.contiguous()
+    params = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    mean, rstd = torch.empty((2, n), device=x.device, dtype=torch.float32) if grads else (None, None)
+    with _lib.on_device(x.device):
+        _lib.check(_lib.load().gs_layer_norm_forward(
+            _lib.dtype_code(x.dtype), _lib.dtype_code(params), n, width, _lib.ptr(rows), _row_stride(rows),
+            _lib.ptr(w), _lib.ptr(b), eps, _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd), _lib.stream_of(x.device)),
+            "gs_layer_norm_forward")
+    return y, (params, mean, rstd)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        rows = _rows(x.detach())
-        n, width = rows.shape
-        needs = any(ctx.needs_input_grad[:3])
-        w = None if weight is None else weight.detach().contiguous()
-        b = None if bias is None else bias.detach().contiguous()
-        params = next((p.dtype for p in (w, b) if p is not None), x.dtype)
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        mean, rstd = (torch.empty(n, device=x.device, dtype=torch.float32) if needs else None for _ in range(2))
-        with torch.cuda.device(x.device):
-            _lib.check(_lib.load().gs_layer_norm_forward(
-                _lib.dtype_code(x.dtype), _lib.dtype_code(params), n, width, _lib.ptr(rows), _row_stride(rows),
-                _lib.ptr(w), _lib.ptr(b), eps, _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd), _lib.stream_of(x.device)),
-                "gs_layer_norm_forward")
-        if needs:
-            ctx.save_for_backward(x, weight, mean, rstd)
-            ctx.params = params
-            ctx.columns = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
+        y, (ctx.params, mean, rstd) = _forward(x.detach(), weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.columns = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
         return y
 
     @staticmethod
@@ -61,10 +64,8 @@ class _LayerNorm(torch.autograd.Function):
         dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
         dw, db = (torch.empty(width, device=x.device, dtype=ctx.params) if c else None for c in ctx.columns)
         lib, code = _lib.load(), _lib.dtype_code(x.dtype)
-        ws = None
-        if any(ctx.columns):
-            ws = torch.empty(lib.gs_layer_norm_workspace_bytes(code, n, width), device=x.device, dtype=torch.uint8)
-        with torch.cuda.device(x.device):
+        ws = _lib.workspace(lib.gs_layer_norm_workspace_bytes(code, n, width), x.device) if any(ctx.columns) else None
+        with _lib.on_device(x.device):
             _lib.check(lib.gs_layer_norm_backward(
                 code, _lib.dtype_code(ctx.params), n, width, _lib.ptr(rows), _row_stride(rows), _lib.ptr(w),
                 _lib.ptr(mean), _lib.ptr(rstd), _lib.ptr(drows), _row_stride(drows), _lib.ptr(dx), _lib.ptr(dw),
@@ -89,4 +90,6 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise RuntimeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
     if not 0.0 <= eps < float("inf"):
         raise RuntimeError(f"eps must be a finite number of at least 0, got {eps}")
-    return _LayerNorm.apply(x, weight, bias, float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _forward(x, weight, bias, float(eps), False)[0]

@@ -25,8 +25,8 @@ def _orthogonalise(stack, steps):
     count, m, n = stack.shape
     lib = _lib.load()
     out = torch.empty_like(stack)
-    ws = torch.empty(lib.gs_orthogonalise_workspace_bytes(count, m, n), device=stack.device, dtype=torch.uint8)
-    with torch.cuda.device(stack.device):
+    ws = _lib.workspace(lib.gs_orthogonalise_workspace_bytes(count, m, n), stack.device)
+    with _lib.on_device(stack.device):
         _lib.check(lib.gs_orthogonalise(_lib.dtype_code(stack.dtype), count, m, n, _lib.ptr(stack), steps,
                                         _lib.ptr(out), _lib.ptr(ws), _lib.stream_of(stack.device)), "gs_orthogonalise")
     return out
@@ -88,7 +88,7 @@ class OrthogonalMomentum(torch.optim.Optimizer):
                 alike.setdefault((p.device, p.dtype, tuple(p.shape)), []).append(p)
             for (device, dtype, shape), params in alike.items():
                 for i in range(0, len(params), _MAX_PER_CALL):
-                    with torch.cuda.device(device):
+                    with _lib.on_device(device):
                         self._update(group, params[i:i + _MAX_PER_CALL], device, dtype, shape)
         return loss
 

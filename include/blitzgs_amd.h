@@ -683,10 +683,11 @@ int gs_layer_norm_backward(int type, int param_type, int64_t rows, int width, co
  *   o_rest, with o's strides and type, may be NULL: o's value before its
  * rounding less o.  A backward that is given it forms sum(do o) from both; with
  * GS_F32 there is nothing to keep.
- *   The workspace's size (gs_attention_workspace_bytes, 0: invalid arguments)
- * depends on sizes alone.  Results do not depend on the order of execution. */
+ *   The workspace's size (gs_attention_workspace_bytes; 0: none is needed, or
+ * the arguments are invalid) depends on the sizes and on `unequal`: whether the call is causal or is given
+ * key_lengths.  Results do not depend on the order of execution. */
 size_t gs_attention_workspace_bytes(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D,
-                                    int causal, int backward);
+                                    int unequal, int backward);
 int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, const void* q,
                          const int64_t* q_strides, const void* k, const int64_t* k_strides,
                          const void* v, const int64_t* v_strides, float scale, int causal,
