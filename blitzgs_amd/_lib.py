@@ -176,38 +176,6 @@ def stream_of(device=None):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
-
-
-def dtype_code(dtype):
-    """The C ABI's element type of a torch dtype (GS_F32, GS_BF16, GS_F16)."""
-    return _DTYPES[str(dtype)]
-
-
-def require_tensor(t, name, device=None):
-    """t is a float32, bfloat16 or float16 HIP device tensor (on `device`)."""
-    import torch
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise RuntimeError(f"{name} must be a HIP device tensor (blitzgs_amd has no CPU path)")
-    if str(t.dtype) not in _DTYPES:
-        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if device is not None and t.device != device:
-        raise RuntimeError(f"{name} must be on {device}, got {t.device}")
-
-
-def on_device(device):
-    """A context in which `device` is the current one: launches go to the current device."""
-    import contextlib
-    import torch
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def workspace(nbytes, device):
-    """A byte buffer of a *_bytes query's size; None where nothing is needed."""
-    import torch
-    return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
-
-
 def timing_enable(on=True, stages_only=False):
     """on: time every kernel launch and the stages (stages_only: the stages
     alone, without per-kernel events in the way); off: nothing."""

@@ -24,7 +24,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _tensors as _t
 
 MAX_HEAD_DIM = 128
 
@@ -45,23 +45,23 @@ def _token_major(like):
 
 def _workspace(sizes, causal, key_lengths, backward, device):
     unequal = int(causal or key_lengths is not None)
-    return _lib.workspace(_lib.load().gs_attention_workspace_bytes(*sizes, unequal, backward), device)
+    return _t.workspace(_t.load().gs_attention_workspace_bytes(*sizes, unequal, backward), device)
 
 
 def _forward(q, k, v, causal, key_lengths, query_start, scale, grads):
     """o and, for a backward, (sizes, what rounding o left, lse)."""
     B, Hq, Tq, D = q.shape
     Hkv, Tk = k.shape[1:3]
-    sizes = _lib.dtype_code(q.dtype), B, Hq, Hkv, Tq, Tk, D
+    sizes = _t.DTYPE_CODES[q.dtype], B, Hq, Hkv, Tq, Tk, D
     o = _token_major(q)
     lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32) if grads else None
     rest = _token_major(q) if grads and q.dtype != torch.float32 else None
     ws = _workspace(sizes, causal, key_lengths, 0, q.device)
-    with _lib.on_device(q.device):
-        _lib.check(_lib.load().gs_attention_forward(
-            *sizes, _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), scale, int(causal),
-            _lib.ptr(key_lengths), _lib.ptr(query_start), _lib.ptr(o), _strides(o), _lib.ptr(rest), _lib.ptr(lse),
-            _lib.ptr(ws), _lib.stream_of(q.device)), "gs_attention_forward")
+    with _t.on_device(q.device):
+        _t.check(_t.load().gs_attention_forward(
+            *sizes, _t.ptr(q), _strides(q), _t.ptr(k), _strides(k), _t.ptr(v), _strides(v), scale, int(causal),
+            _t.ptr(key_lengths), _t.ptr(query_start), _t.ptr(o), _strides(o), _t.ptr(rest), _t.ptr(lse),
+            _t.ptr(ws), _t.stream(q.device)), "gs_attention_forward")
     return o, (sizes, rest, lse)
 
 
@@ -81,12 +81,12 @@ class _Attention(torch.autograd.Function):
         do = _last_contiguous(do)
         dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
         ws = _workspace(ctx.sizes, ctx.causal, key_lengths, 1, q.device)
-        with _lib.on_device(q.device):
-            _lib.check(_lib.load().gs_attention_backward(
-                *ctx.sizes, _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), ctx.scale,
-                int(ctx.causal), _lib.ptr(key_lengths), _lib.ptr(query_start), _lib.ptr(o), _strides(o),
-                _lib.ptr(rest), _lib.ptr(lse), _lib.ptr(do), _strides(do), _lib.ptr(dq), _strides(dq), _lib.ptr(dk),
-                _strides(dk), _lib.ptr(dv), _strides(dv), _lib.ptr(ws), _lib.stream_of(q.device)),
+        with _t.on_device(q.device):
+            _t.check(_t.load().gs_attention_backward(
+                *ctx.sizes, _t.ptr(q), _strides(q), _t.ptr(k), _strides(k), _t.ptr(v), _strides(v), ctx.scale,
+                int(ctx.causal), _t.ptr(key_lengths), _t.ptr(query_start), _t.ptr(o), _strides(o),
+                _t.ptr(rest), _t.ptr(lse), _t.ptr(do), _strides(do), _t.ptr(dq), _strides(dq), _t.ptr(dk),
+                _strides(dk), _t.ptr(dv), _strides(dv), _t.ptr(ws), _t.stream(q.device)),
                 "gs_attention_backward")
         return dq, dk, dv, None, None, None, None
 
@@ -105,7 +105,7 @@ def attention(q, k, v, causal=False, key_lengths=None, query_start=None, scale=N
     key_lengths, query_start: int32 (B,) on q's device, or None.
     scale: a positive number; None for 1 / sqrt(D)."""
     for name, t in (("q", q), ("k", k), ("v", v)):
-        _lib.require_tensor(t, name, device=None if name == "q" else q.device)
+        _t.require_tensor(t, name, device=None if name == "q" else q.device)
         if t.dim() != 4:
             raise RuntimeError(f"{name} must have dimensions (B, H, T, D), got shape {tuple(t.shape)}")
         if t.dtype != q.dtype:
@@ -123,6 +123,6 @@ def attention(q, k, v, causal=False, key_lengths=None, query_start=None, scale=N
     if query_start is not None and not causal:
         raise RuntimeError("query_start needs causal=True")
     how = bool(causal), _per_batch(key_lengths, "key_lengths", q), _per_batch(query_start, "query_start", q), scale
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _t.wants_grad(q, k, v):
         return _Attention.apply(q, k, v, *how)
     return _forward(*(_last_contiguous(t) for t in (q, k, v)), *how, False)[0]

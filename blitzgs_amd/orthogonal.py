@@ -16,19 +16,19 @@ import ctypes as C
 
 import torch
 
-from . import _lib
+from . import _tensors as _t
 
 _MAX_PER_CALL = 32      # tensors per gs_momentum_* call
 
 
 def _orthogonalise(stack, steps):
     count, m, n = stack.shape
-    lib = _lib.load()
+    lib = _t.load()
     out = torch.empty_like(stack)
-    ws = _lib.workspace(lib.gs_orthogonalise_workspace_bytes(count, m, n), stack.device)
-    with _lib.on_device(stack.device):
-        _lib.check(lib.gs_orthogonalise(_lib.dtype_code(stack.dtype), count, m, n, _lib.ptr(stack), steps,
-                                        _lib.ptr(out), _lib.ptr(ws), _lib.stream_of(stack.device)), "gs_orthogonalise")
+    ws = _t.workspace(lib.gs_orthogonalise_workspace_bytes(count, m, n), stack.device)
+    with _t.on_device(stack.device):
+        _t.check(lib.gs_orthogonalise(_t.DTYPE_CODES[stack.dtype], count, m, n, _t.ptr(stack), steps,
+                                        _t.ptr(out), _t.ptr(ws), _t.stream(stack.device)), "gs_orthogonalise")
     return out
 
 
@@ -38,7 +38,7 @@ def orthogonalise(update, steps=5):
 
     All matrices of one call go through the device together.  Not
     differentiable.  steps: 1 to 32."""
-    _lib.require_tensor(update, "update")
+    _t.require_tensor(update, "update")
     if update.dim() < 2 or max(update.shape[-2:]) > 65536:
         raise RuntimeError(f"update must hold matrices with sides of up to 65536, got shape {tuple(update.shape)}")
     if not isinstance(steps, int) or not 1 <= steps <= 32:
@@ -80,7 +80,7 @@ class OrthogonalMomentum(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.grad is None or p.numel() == 0:
                     continue
-                _lib.require_tensor(p, "param")
+                _t.require_tensor(p, "param")
                 if p.dim() != 2:
                     raise RuntimeError(f"OrthogonalMomentum takes matrices, got shape {tuple(p.shape)}")
                 if not p.is_contiguous() or p.grad.dtype != p.dtype or p.grad.is_sparse:
@@ -88,24 +88,24 @@ class OrthogonalMomentum(torch.optim.Optimizer):
                 alike.setdefault((p.device, p.dtype, tuple(p.shape)), []).append(p)
             for (device, dtype, shape), params in alike.items():
                 for i in range(0, len(params), _MAX_PER_CALL):
-                    with _lib.on_device(device):
+                    with _t.on_device(device):
                         self._update(group, params[i:i + _MAX_PER_CALL], device, dtype, shape)
         return loss
 
     def _update(self, group, params, device, dtype, shape):
-        lib, code, n = _lib.load(), _lib.dtype_code(dtype), len(params)
-        stream, size = _lib.stream_of(device), shape[0] * shape[1]
+        lib, code, n = _t.load(), _t.DTYPE_CODES[dtype], len(params)
+        stream, size = _t.stream(device), shape[0] * shape[1]
         for p in params:
             if "momentum_buffer" not in self.state[p]:
                 self.state[p]["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
         grads = [p.grad.contiguous() for p in params]
         pointers = lambda ts: (C.c_void_p * n)(*(t.data_ptr() for t in ts))  # noqa: E731
         update = torch.empty((n, *shape), device=device, dtype=torch.float32)
-        _lib.check(lib.gs_momentum_update(code, n, size, pointers(grads),
+        _t.check(lib.gs_momentum_update(code, n, size, pointers(grads),
                                           pointers([self.state[p]["momentum_buffer"] for p in params]),
-                                          group["momentum"], int(group["nesterov"]), _lib.ptr(update), stream),
+                                          group["momentum"], int(group["nesterov"]), _t.ptr(update), stream),
                    "gs_momentum_update")
         update = _orthogonalise(update, group["steps"])
         scale = max(1.0, shape[0] / shape[1]) ** 0.5
-        _lib.check(lib.gs_momentum_apply(code, n, size, pointers(params), 1.0 - group["lr"] * group["weight_decay"],
-                                         group["lr"] * scale, _lib.ptr(update), stream), "gs_momentum_apply")
+        _t.check(lib.gs_momentum_apply(code, n, size, pointers(params), 1.0 - group["lr"] * group["weight_decay"],
+                                         group["lr"] * scale, _t.ptr(update), stream), "gs_momentum_apply")
