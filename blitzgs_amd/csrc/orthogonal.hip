@@ -75,6 +75,30 @@ __device__ __forceinline__ void split(float x, f16& hi, f16& lo)
     lo = (f16)(x - (float)hi);
 }
 
+// What takes G to the planes of X at the start, and -log2 |X| there.
+__device__ __forceinline__ float start_scale(float norm, float& small)
+{
+    const float len = norm / (norm + NORM_FLOOR);
+    // squares that underflow: the norm is unknown but below 2^-60
+    small = len > 0.0f ? fminf(-__builtin_log2f(len), 40.0f) : norm == 0.0f ? 20.0f : 0.0f;
+    return __builtin_ldexpf(SX, extra_scale(small, 0)) / (norm + NORM_FLOOR);
+}
+
+// c[v] + a b[v] for operands in two planes; lo lo is below the planes' last bit.
+// One plane's products of all v before the next: neighbours do not wait for
+// each other's sums.
+template <int N>
+__device__ __forceinline__ void three(const Frag<f16>& ah, const Frag<f16>& al, const Frag<f16> (&bh)[N],
+                                      const Frag<f16> (&bl)[N], f4 (&c)[N])
+{
+#pragma unroll
+    for (int v = 0; v < N; v++) c[v] = gs::mma(al, bh[v], c[v]);
+#pragma unroll
+    for (int v = 0; v < N; v++) c[v] = gs::mma(ah, bl[v], c[v]);
+#pragma unroll
+    for (int v = 0; v < N; v++) c[v] = gs::mma(ah, bh[v], c[v]);
+}
+
 // ------------------------------------------------------------- the normalised X
 
 template <typename T>
@@ -113,10 +137,8 @@ __global__ __launch_bounds__(256) void orth_split_kernel(const T* __restrict__ g
     const T* p = g + (int64_t)blockIdx.z * rows * cols;
     float s = 0.0f;
     for (int k = 0; k < NORM_PARTS; k++) s += parts[blockIdx.z * NORM_PARTS + k];
-    const float norm = __builtin_sqrtf(s), len = norm / (norm + NORM_FLOOR);
-    // squares that underflow: the norm is unknown but below 2^-60
-    const float sm = len > 0.0f ? fminf(-__builtin_log2f(len), 40.0f) : norm == 0.0f ? 20.0f : 0.0f;
-    const float scale = __builtin_ldexpf(SX, extra_scale(sm, 0)) / (norm + NORM_FLOOR);
+    float sm;
+    const float scale = start_scale(__builtin_sqrtf(s), sm);
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) small[blockIdx.z] = sm;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int y0 = blockIdx.y * 64, x0 = blockIdx.x * 64;   // of the tile in X
@@ -243,12 +265,7 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
                 rh = tile.rows(lds[b][2] + nl * KT / 8, 16 * u, 0);
                 rl = tile.rows(lds[b][3] + nl * KT / 8, 16 * u, 0);
             }
-#pragma unroll
-            for (int v = 0; v < U; v++) {
-                acc[u][v] = gs::mma(rl, lh[v], acc[u][v]);
-                acc[u][v] = gs::mma(rh, ll[v], acc[u][v]);
-                acc[u][v] = gs::mma(rh, lh[v], acc[u][v]);
-            }
+            three(rh, rl, lh, ll, acc[u]);
         }
         __syncthreads();
     }
@@ -304,6 +321,235 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
                 }
             }
         }
+    }
+}
+
+// ---------------------------------------------------- a small matrix in one CU
+
+// The whole iteration of one matrix whose planes of X and A fit in LDS: X as
+// panels of 32 columns, A in the same form, B in A's place.  The launches of the
+// products above cost more than the work of such a matrix (250 x 96: 93 us in
+// 17 launches).  Eight waves share the 32 x 32 blocks of each product; results
+// wait in registers until every wave has read their operands.
+constexpr int SMALL_THREADS = 512, SMALL_WAVES = SMALL_THREADS / 64;
+constexpr int SMALL_BLOCKS = 5;           // of X per wave
+constexpr int SMALL_LDS = 156 * 1024;
+
+// Four neighbours of a row, from column `col` (a multiple of 4), of panels at p.
+template <int PANEL>
+__device__ __forceinline__ f16* quad(uint4* p, int row, int col)
+{
+    return (f16*)(p + col / 32 * PANEL + Tile<f16, 32>::chunk(row, col % 32 / 8)) + col % 8;
+}
+
+// Block e of the lower triangle, row by row.
+__device__ __forceinline__ void corner(int e, int& bm, int& bn)
+{
+    bm = 0;
+    while ((bm + 1) * (bm + 2) / 2 <= e) bm++;
+    bn = e - bm * (bm + 1) / 2;
+}
+
+// acc = the 32 x 32 block (bm, bn) of Y Y^T, Y's planes in `depth` panels.
+template <int PANEL>
+__device__ __forceinline__ void square_block(const Tile<f16, 32>& tile, const uint4* hi, const uint4* lo, int depth, int bm,
+                                             int bn, f4 (&acc)[2][2])
+{
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int v = 0; v < 2; v++) acc[u][v] = f4{0, 0, 0, 0};
+    for (int p = 0; p < depth; p++, hi += PANEL, lo += PANEL) {
+        Frag<f16> lh[2], ll[2];
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+            lh[v] = tile.rows(hi + bm * 128, 16 * v, 0);
+            ll[v] = tile.rows(lo + bm * 128, 16 * v, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const Frag<f16> rh = tile.rows(hi + bn * 128, 16 * u, 0), rl = tile.rows(lo + bn * 128, 16 * u, 0);
+            three(rh, rl, lh, ll, acc[u]);
+        }
+    }
+}
+
+// Both planes of four neighbours (row, col ..) of a symmetric matrix, and where
+// `both` of (col .., row) too; from and to are a column's place.
+template <int PANEL>
+__device__ __forceinline__ void store_symmetric(uint4* ph, uint4* pl, int row, int col, int row_to, int col_to, bool both,
+                                                f4 x)
+{
+    f16 hi[4], lo[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) split(x[r], hi[r], lo[r]);
+    __builtin_memcpy(quad<PANEL>(ph, row, col_to), hi, 8);
+    __builtin_memcpy(quad<PANEL>(pl, row, col_to), lo, 8);
+    if (!both) return;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        quad<PANEL>(ph, col + r, row_to & ~3)[row_to & 3] = hi[r];
+        quad<PANEL>(pl, col + r, row_to & ~3)[row_to & 3] = lo[r];
+    }
+}
+
+// Where B's column c lies, so that rows() reads it in the order of X's cols().
+__device__ __forceinline__ int place(int c) { return c / 32 * 32 + c % 16 / 4 * 8 + c % 32 / 16 * 4 + c % 4; }
+
+template <typename T, int MP>
+__global__ __launch_bounds__(SMALL_THREADS) void orth_small_kernel(const T* __restrict__ update, T* __restrict__ result,
+                                                                   int m, int n, int tall, int np, int steps)
+{
+    constexpr int MB = MP / 32, PANEL = MP * 4, SQ = MB * (MB + 1) / 2, PER = (SQ + SMALL_WAVES - 1) / SMALL_WAVES;
+    extern __shared__ uint4 lds[];
+    const int panels = np / 32, blocks = MB * panels, size = m * n;
+    uint4 *xh = lds, *xl = xh + panels * PANEL, *ah = xl + panels * PANEL, *al = ah + MB * PANEL;
+    const Tile<f16, 32> tile;
+    const int lane = threadIdx.x & 63;
+    int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    const T* src = update + (int64_t)blockIdx.x * size;
+    T* dst = result + (int64_t)blockIdx.x * size;
+
+    float s = 0.0f;
+#pragma unroll 8
+    for (int e = threadIdx.x; e < size; e += SMALL_THREADS) s = __builtin_fmaf((float)src[e], (float)src[e], s);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
+    float* sums = (float*)ah;
+    if (lane == 0) sums[wave] = s;
+    for (int e = threadIdx.x; e < 2 * panels * PANEL; e += SMALL_THREADS) xh[e] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < SMALL_WAVES; w++) s += sums[w];
+    float small;
+    const float scale = start_scale(__builtin_sqrtf(s), small);
+    // a wave takes rows of G, a lane every 64th element of one
+#pragma unroll 2
+    for (int r = wave; r < m; r += SMALL_WAVES)
+#pragma unroll 4
+        for (int c = lane; c < n; c += 64) {
+            const int row = tall ? c : r, col = tall ? r : c;
+            f16 hi, lo;
+            split((float)src[r * n + c] * scale, hi, lo);
+            quad<PANEL>(xh, row, col & ~3)[col & 3] = hi;
+            quad<PANEL>(xl, row, col & ~3)[col & 3] = lo;
+        }
+    __syncthreads();
+    for (int step = 0; step < steps; step++) {
+        // the blocks' addresses are formed anew in each step: kept, they would not fit the registers
+        asm volatile("" : "+s"(wave), "+v"(i), "+v"(g));
+        const int k = extra_scale(small, step);
+        const bool last = step + 1 == steps;
+        f4 acc[PER][2][2];
+        // A = X X^T
+#pragma unroll
+        for (int q = 0; q < PER; q++) {
+            int bm, bn;
+            corner(wave + q * SMALL_WAVES, bm, bn);
+            if (bm >= MB) continue;
+            square_block<PANEL>(tile, xh, xl, panels, bm, bn, acc[q]);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int v = 0; v < 2; v++) {
+                    const int row = 32 * bm + 16 * v + i, col = 32 * bn + 16 * u + 4 * g;
+                    store_symmetric<PANEL>(ah, al, row, col, row, col, bm != bn, acc[q][u][v] * (SA / (SX * SX)));
+                }
+        }
+        __syncthreads();
+        // B = a I + b A + c A A
+        const float cc = __builtin_ldexpf(QC / SA, -4 * k), cb = __builtin_ldexpf(QB, -2 * k);
+#pragma unroll
+        for (int q = 0; q < PER; q++) {
+            int bm, bn;
+            corner(wave + q * SMALL_WAVES, bm, bn);
+            if (bm >= MB) continue;
+            square_block<PANEL>(tile, ah, al, MB, bm, bn, acc[q]);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int v = 0; v < 2; v++) {
+                    const int row = 32 * bm + 16 * v + i, col = 32 * bn + 16 * u + 4 * g;
+                    f16 hi[4], lo[4];
+                    __builtin_memcpy(hi, quad<PANEL>(ah, row, col), 8);
+                    __builtin_memcpy(lo, quad<PANEL>(al, row, col), 8);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float x = __builtin_fmaf(cb, (float)hi[r] + (float)lo[r], acc[q][u][v][r] * cc);
+                        acc[q][u][v][r] = row == col + r ? x + QA * SA : x;
+                    }
+                }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < PER; q++) {
+            int bm, bn;
+            corner(wave + q * SMALL_WAVES, bm, bn);
+            if (bm >= MB) continue;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int v = 0; v < 2; v++) {
+                    const int row = 32 * bm + 16 * v + i, col = 32 * bn + 16 * u + 4 * g;
+                    store_symmetric<PANEL>(ah, al, row, col, place(row), place(col), bm != bn, acc[q][u][v]);
+                }
+        }
+        __syncthreads();
+        // X = B X
+        f4 xs[SMALL_BLOCKS][2][2];
+#pragma unroll
+        for (int q = 0; q < SMALL_BLOCKS; q++) {
+            const int e = wave + q * SMALL_WAVES, bm = e % MB, bn = e / MB;
+            if (e >= blocks) continue;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int v = 0; v < 2; v++) xs[q][u][v] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < MB; p++) {
+                Frag<f16> lh[2], ll[2];
+#pragma unroll
+                for (int v = 0; v < 2; v++) {
+                    lh[v] = tile.rows(ah + p * PANEL + bm * 128, 16 * v, 0);
+                    ll[v] = tile.rows(al + p * PANEL + bm * 128, 16 * v, 0);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const Frag<f16> rh = tile.cols(xh + bn * PANEL, 32 * p, 16 * u);
+                    const Frag<f16> rl = tile.cols(xl + bn * PANEL, 32 * p, 16 * u);
+                    three(rh, rl, lh, ll, xs[q][u]);
+                }
+            }
+        }
+        __syncthreads();
+        const float out_scale = last ? __builtin_ldexpf(1.0f / (SA * SX), -k)
+                                     : __builtin_ldexpf(1.0f / SA, extra_scale(small, step + 1) - k);
+#pragma unroll
+        for (int q = 0; q < SMALL_BLOCKS; q++) {
+            const int e = wave + q * SMALL_WAVES, bm = e % MB, bn = e / MB;
+            if (e >= blocks) continue;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int v = 0; v < 2; v++) {
+                    const int row = 32 * bm + 16 * v + i, col = 32 * bn + 16 * u + 4 * g;
+                    const f4 x = xs[q][u][v] * out_scale;
+                    if (last) {
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (row < (tall ? n : m) && col + r < (tall ? m : n))
+                                dst[tall ? (col + r) * n + row : row * n + col + r] = (T)x[r];
+                        continue;
+                    }
+                    f16 hi[4], lo[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) split(x[r], hi[r], lo[r]);
+                    __builtin_memcpy(quad<PANEL>(xh, row, col), hi, 8);
+                    __builtin_memcpy(quad<PANEL>(xl, row, col), lo, 8);
+                }
+        }
+        __syncthreads();
     }
 }
 
@@ -365,9 +611,37 @@ int product(int S, const ProductArgs& A, int count, hipStream_t stream)
     return GS_OK;
 }
 
+// The padded short side of a matrix that one workgroup takes, 0 if none does.
+int small_side(int m, int n)
+{
+    const int64_t s = up(m < n ? m : n, 32), l = up(m < n ? n : m, 32);
+    if (s > 128 || s * (l + s) * 4 > SMALL_LDS || s / 32 * (l / 32) > SMALL_BLOCKS * SMALL_WAVES) return 0;
+    return (int)s;
+}
+
+template <typename T, int MP>
+int orthogonalise_small(int count, int m, int n, const T* g, int steps, T* out, hipStream_t stream)
+{
+    const int np = (int)up(m < n ? n : m, 32), lds = MP * (np + MP) * 4;
+    if (lds > 65536)
+        GS_HIP(hipFuncSetAttribute((const void*)orth_small_kernel<T, MP>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   SMALL_LDS));
+    GS_TIMED("orth_small_kernel", stream,
+             hipLaunchKernelGGL((orth_small_kernel<T, MP>), dim3((unsigned)count), dim3(SMALL_THREADS), lds, stream, g,
+                                out, m, n, (int)(m > n), np, steps));
+    GS_LAUNCH_CHECK("orth_small_kernel");
+    return GS_OK;
+}
+
 template <typename T>
 int orthogonalise(int count, int m, int n, const T* g, int steps, T* out, void* workspace, hipStream_t stream)
 {
+    switch (small_side(m, n)) {
+        case 32: return orthogonalise_small<T, 32>(count, m, n, g, steps, out, stream);
+        case 64: return orthogonalise_small<T, 64>(count, m, n, g, steps, out, stream);
+        case 96: return orthogonalise_small<T, 96>(count, m, n, g, steps, out, stream);
+        case 128: return orthogonalise_small<T, 128>(count, m, n, g, steps, out, stream);
+    }
     const Layout L = layout_of(count, m, n);
     const int tall = m > n, S = tile_of(count, m < n ? m : n, m < n ? n : m);
     float* parts = (float*)workspace;
@@ -462,8 +736,8 @@ __global__ __launch_bounds__(256) void apply_kernel(MomentumBatch B, int64_t siz
 extern "C" size_t gs_orthogonalise_workspace_bytes(int count, int m, int n)
 {
     if (check(GS_F32, count, m, n) != GS_OK) return 0;
-    const Layout L = layout_of(count, m, n);
-    return L.bytes < 256 ? 256 : (size_t)L.bytes;
+    if (count == 0 || m == 0 || n == 0 || small_side(m, n) != 0) return 0;
+    return (size_t)layout_of(count, m, n).bytes;
 }
 
 extern "C" int gs_orthogonalise(int type, int count, int m, int n, const void* update, int steps, void* out,
@@ -473,7 +747,8 @@ extern "C" int gs_orthogonalise(int type, int count, int m, int n, const void* u
     if (int rc = check(type, count, m, n)) return rc;
     GS_REQUIRE(steps >= 1 && steps <= 32, "orthogonalise: steps must be in [1, 32], got %d", steps);
     if (count == 0 || m == 0 || n == 0) return GS_OK;
-    GS_REQUIRE(update && out && workspace, "orthogonalise: update, out and workspace must be non-null");
+    GS_REQUIRE(update && out, "orthogonalise: update and out must be non-null");
+    GS_REQUIRE(workspace || small_side(m, n) != 0, "orthogonalise: this size needs the workspace");
     GS_REQUIRE(((uintptr_t)workspace & 255) == 0, "orthogonalise: the workspace must be 256-byte aligned");
     if (type == GS_F32) return orthogonalise(count, m, n, (const float*)update, steps, (float*)out, workspace, stream);
     if (type == GS_BF16)

@@ -709,7 +709,8 @@ int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int 
  * (3.4445, -4.7750, 2.0315) from X = update / (|update|_F + 1e-7), over the
  * shorter side's rows; products with fp32's accuracy.  out may not overlap
  * update.  Sides and count up to 65536 and 65535.  workspace: 256-byte aligned,
- * of gs_orthogonalise_workspace_bytes (0: invalid arguments). */
+ * of gs_orthogonalise_workspace_bytes (0: none is needed, or the arguments are
+ * invalid). */
 size_t gs_orthogonalise_workspace_bytes(int count, int m, int n);
 int gs_orthogonalise(int type, int count, int m, int n, const void* update, int steps, void* out,
                      void* workspace, gs_stream_t stream);
