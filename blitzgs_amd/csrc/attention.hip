@@ -200,6 +200,10 @@ __device__ __forceinline__ void store_o(T* p, T* rest, f4 v, int n)
     store4<ODD>(rest, left, n);
 }
 
+// The tile that is read and the one that is being loaded come to a step as two
+// restricted pointers: only so does the compiler know that the loads need not
+// have arrived before the reads.
+
 // ------------------------------------------------------------------- forward
 
 template <typename T, int DP, int NQ, Fill F>
@@ -235,28 +239,25 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
     }
 
     Stage<T, DP, BK, F> sk, sv;
-    auto fetch = [&](int t) {
-        uint4* to = lds + ((t - w.t0) & 1) * 2 * WORDS;
+    auto fetch = [&](int t, uint4* to) __attribute__((always_inline)) {
         sk.fetch(to, kb + (int64_t)t * BK * A.ks.t, A.ks.t, w.len - t * BK, A.D);
         sv.fetch(to + WORDS, vb + (int64_t)t * BK * A.vs.t, A.vs.t, w.len - t * BK, A.D);
     };
-    auto put = [&](int t) {
-        uint4* to = lds + ((t - w.t0) & 1) * 2 * WORDS;
+    auto put = [&](uint4* to) {
         sk.put(to);
         sv.put(to + WORDS);
     };
     if (w.t0 < w.t1) {
 #pragma unroll
         for (int k = 0; k < 4; k++) sk.clear(lds + k * WORDS, A.D);
-        fetch(w.t0);
-        put(w.t0);
+        fetch(w.t0, lds);
+        put(lds);
     }
     __syncthreads();
-    for (int t = w.t0; t < w.t1; t++) {
-        const uint4* kt = lds + ((t - w.t0) & 1) * 2 * WORDS;
+    auto step = [&](int t, const uint4* __restrict__ kt, uint4* __restrict__ next) __attribute__((always_inline)) {
         const uint4* vt = kt + WORDS;
         const int k0 = t * BK;
-        if (t + 1 < w.t1) fetch(t + 1);
+        if (t + 1 < w.t1) fetch(t + 1, next);
         f4 s[4][NQ];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -319,9 +320,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
                 for (int n = 0; n < NQ; n++) o[d][n] = gs::mma(a, p[n], o[d][n]);
             }
         }
-        if (t + 1 < w.t1) put(t + 1);
+        if (t + 1 < w.t1) put(next);
         __syncthreads();
-    }
+    };
+    for (int t = w.t0; t < w.t1; t++)
+        step(t, lds + ((t - w.t0) & 1) * 2 * WORDS, lds + ((t + 1 - w.t0) & 1) * 2 * WORDS);
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const float sum = column_sum(l[n]);
@@ -440,28 +443,25 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
     }
 
     Stage<T, DP, BK, F> sk, sv;
-    auto fetch = [&](int t) {
-        uint4* to = lds + ((t - w.t0) & 1) * 2 * WORDS;
+    auto fetch = [&](int t, uint4* to) __attribute__((always_inline)) {
         sk.fetch(to, kb + (int64_t)t * BK * A.ks.t, A.ks.t, w.len - t * BK, A.D);
         sv.fetch(to + WORDS, vb + (int64_t)t * BK * A.vs.t, A.vs.t, w.len - t * BK, A.D);
     };
-    auto put = [&](int t) {
-        uint4* to = lds + ((t - w.t0) & 1) * 2 * WORDS;
+    auto put = [&](uint4* to) {
         sk.put(to);
         sv.put(to + WORDS);
     };
     if (w.t0 < w.t1) {
 #pragma unroll
         for (int k = 0; k < 4; k++) sk.clear(lds + k * WORDS, A.D);
-        fetch(w.t0);
-        put(w.t0);
+        fetch(w.t0, lds);
+        put(lds);
     }
     __syncthreads();
-    for (int t = w.t0; t < w.t1; t++) {
-        const uint4* kt = lds + ((t - w.t0) & 1) * 2 * WORDS;
+    auto step = [&](int t, const uint4* __restrict__ kt, uint4* __restrict__ next) __attribute__((always_inline)) {
         const uint4* vt = kt + WORDS;
         const int k0 = t * BK;
-        if (t + 1 < w.t1) fetch(t + 1);
+        if (t + 1 < w.t1) fetch(t + 1, next);
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
             f4 s[2][NQ], dp[2][NQ];
@@ -511,9 +511,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
                 for (int n = 0; n < NQ; n++) acc[d][n] = gs::mma(a, ds[n], acc[d][n]);
             }
         }
-        if (t + 1 < w.t1) put(t + 1);
+        if (t + 1 < w.t1) put(next);
         __syncthreads();
-    }
+    };
+    for (int t = w.t0; t < w.t1; t++)
+        step(t, lds + ((t - w.t0) & 1) * 2 * WORDS, lds + ((t + 1 - w.t0) & 1) * 2 * WORDS);
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         if (!col[n].valid) continue;
@@ -574,22 +576,27 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
     const int e0 = min(total, split * per), e1 = min(total, e0 + per);
 
     Stage<T, DP, QT, F> sq, sg;
-    float stat = 0.0f;   // threads 0 .. QT - 1: lse, QT .. 2 QT - 1: -delta
-    auto fetch = [&](int e, uint4* to) {
+    // threads 0 .. QT - 1: lse, QT .. 2 QT - 1: delta, as loaded; put() finishes them,
+    // so that nothing waits for them, and the tiles' loads before them, until then
+    float stat = 0.0f;
+    bool real = false;
+    const bool is_lse = threadIdx.x < QT;
+    auto fetch = [&](int e, uint4* to) __attribute__((always_inline)) {
         const int h = hk * A.G + e / per_head, q0 = (from + e % per_head) * QT, n = A.Tq - q0;
         sq.fetch(to, (const T*)A.q + b * A.qs.b + h * A.qs.h + (int64_t)q0 * A.qs.t, A.qs.t, n, A.D);
         sg.fetch(to + WORDS, (const T*)A.dout + b * A.dos.b + h * A.dos.h + (int64_t)q0 * A.dos.t, A.dos.t, n, A.D);
         if (threadIdx.x < 2 * QT) {
             const int r = threadIdx.x % QT;
-            const int64_t row = ((int64_t)b * A.Hkv * A.G + h) * A.Tq + q0 + r;
-            if (threadIdx.x < QT) stat = r < n ? A.lse[row] : -NEG_INF;
-            else stat = r < n ? -A.delta[row] : 0.0f;
+            const int64_t row = ((int64_t)b * A.Hkv * A.G + h) * A.Tq + q0 + min(r, n - 1);
+            real = r < n;
+            stat = *((is_lse ? A.lse : A.delta) + row);
         }
     };
     auto put = [&](uint4* to) {
         sq.put(to);
         sg.put(to + WORDS);
-        if (threadIdx.x < 2 * QT) ((float*)(to + 2 * WORDS))[threadIdx.x] = stat;
+        if (threadIdx.x < 2 * QT)
+            ((float*)(to + 2 * WORDS))[threadIdx.x] = is_lse ? (real ? stat : -NEG_INF) : real ? -stat : 0.0f;
     };
     if (e0 < e1) {
 #pragma unroll
@@ -598,12 +605,11 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
         put(lds);
     }
     __syncthreads();
-    for (int e = e0; e < e1; e++) {
-        const uint4* qt = lds + ((e - e0) & 1) * BUF;
+    auto step = [&](int e, const uint4* __restrict__ qt, uint4* __restrict__ next) __attribute__((always_inline)) {
         const uint4* gt = qt + WORDS;
         const float* st = (const float*)(gt + WORDS);
         const int q0 = (from + e % per_head) * QT;
-        if (e + 1 < e1) fetch(e + 1, lds + ((e + 1 - e0) & 1) * BUF);
+        if (e + 1 < e1) fetch(e + 1, next);
         // row r of the tile sees key `key` when r >= sees + key - key0
         const bool part = A.causal && start + q0 < (int64_t)key0 + COLS - 1;
         const int sees = part ? (int)(key0 - start - q0) : 0;   // between -COLS and QT
@@ -667,9 +673,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
                 }
             }
         }
-        if (e + 1 < e1) put(lds + ((e + 1 - e0) & 1) * BUF);
+        if (e + 1 < e1) put(next);
         __syncthreads();
-    }
+    };
+    for (int e = e0; e < e1; e++) step(e, lds + ((e - e0) & 1) * BUF, lds + ((e + 1 - e0) & 1) * BUF);
 #pragma unroll
     for (int n = 0; n < NK; n++) {
         if (key[n] >= A.Tk) continue;
