@@ -204,12 +204,12 @@ struct Pair {
 // A block computes S x S of the result, four waves a quarter each: columns of
 // its matrix-core tiles are rows of the left operand, rows are columns of the
 // result, so that a lane holds four neighbours of one row of the result.
-template <Kind K, int S, typename T>
-__global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
+template <Kind K, int S, int STAGES, typename T>
+__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void orth_product_kernel(ProductArgs A)
 {
     constexpr int H = S / 2, U = H / 16;
     constexpr int WORDS = S * KT / 8;                // of one operand's plane
-    __shared__ uint4 lds[2][4][WORDS];               // left hi, lo, right hi, lo
+    extern __shared__ uint4 lds[];                   // [STAGES][left hi, lo, right hi, lo]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const uint32_t per = K == APPLY ? (uint32_t)A.tiles_m * A.tiles_n : (uint32_t)A.tiles_m * (A.tiles_m + 1) / 2;
     const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x);
@@ -241,87 +241,129 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
     for (int u = 0; u < U; u++)
 #pragma unroll
         for (int v = 0; v < U; v++) acc[u][v] = f4{0, 0, 0, 0};
-    sl.fetch(lds[0][0], lds[0][1]);
-    sr.fetch(lds[0][2], lds[0][3]);
-    __syncthreads();
-    for (int k0 = 0, b = 0; k0 < A.k; k0 += KT, b ^= 1) {
-        if (k0 + KT < A.k) {
-            sl.fetch(lds[b ^ 1][0], lds[b ^ 1][1]);
-            sr.fetch(lds[b ^ 1][2], lds[b ^ 1][3]);
-        }
+    // the loads of STAGES - 1 tiles are in flight; `waiting` of them may still
+    // be when the oldest is read
+    constexpr int LOADS = 4 * (S * KT / 8 / 256), waiting = LOADS * (STAGES - 2);
+    const int tiles = A.k / KT;
+    auto fetch = [&](uint4* to) __attribute__((always_inline)) {
+        sl.fetch(to, to + WORDS);
+        sr.fetch(to + 2 * WORDS, to + 3 * WORDS);
+    };
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; t++)
+        if (t < tiles) fetch(lds + t * 4 * WORDS);
+    // two restricted pointers tell the compiler that the loads need not have
+    // arrived before the reads
+    auto step = [&](int t, const uint4* __restrict__ at, uint4* __restrict__ next) __attribute__((always_inline)) {
+        // tile t is there for all waves, and all waves are done with tile t - 1
+        if (t + STAGES - 2 < tiles) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(waiting) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (t + STAGES - 1 < tiles) fetch(next);
         Frag<f16> lh[U], ll[U];
 #pragma unroll
         for (int v = 0; v < U; v++) {
-            lh[v] = tile.rows(lds[b][0] + ml * KT / 8, 16 * v, 0);
-            ll[v] = tile.rows(lds[b][1] + ml * KT / 8, 16 * v, 0);
+            lh[v] = tile.rows(at + ml * KT / 8, 16 * v, 0);
+            ll[v] = tile.rows(at + WORDS + ml * KT / 8, 16 * v, 0);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             Frag<f16> rh, rl;
             if constexpr (K == APPLY) {
-                rh = down.cols(lds[b][2] + nl * KT / 8, 0, 16 * u);
-                rl = down.cols(lds[b][3] + nl * KT / 8, 0, 16 * u);
+                rh = down.cols(at + 2 * WORDS + nl * KT / 8, 0, 16 * u);
+                rl = down.cols(at + 3 * WORDS + nl * KT / 8, 0, 16 * u);
             } else {
-                rh = tile.rows(lds[b][2] + nl * KT / 8, 16 * u, 0);
-                rl = tile.rows(lds[b][3] + nl * KT / 8, 16 * u, 0);
+                rh = tile.rows(at + 2 * WORDS + nl * KT / 8, 16 * u, 0);
+                rl = tile.rows(at + 3 * WORDS + nl * KT / 8, 16 * u, 0);
             }
             three(rh, rl, lh, ll, acc[u]);
         }
-        __syncthreads();
-    }
+    };
+    for (int t = 0; t < tiles; t++)
+        step(t, lds + t % STAGES * 4 * WORDS, lds + (t + STAGES - 1) % STAGES * 4 * WORDS);
     const int k = extra_scale(A.small[batch], A.step);
     float scale = A.scale;
     if constexpr (K == POLY) scale = __builtin_ldexpf(scale, -4 * k);
     if constexpr (K == APPLY)
         scale = __builtin_ldexpf(scale, A.final_out != nullptr ? -k : extra_scale(A.small[batch], A.step + 1) - k);
     const float add_scale = __builtin_ldexpf(QB, -2 * k);
-    f16* out = A.out.p + batch * A.out.stride;
-    const f16* add = A.add.p + batch * A.add.stride;
+    if constexpr (K == APPLY) {
+        if (A.final_out != nullptr) {
+            T* f = (T*)A.final_out + (int64_t)batch * A.rows * A.cols;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
+            for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int v = 0; v < U; v++) {
-            const int row = m0 + ml + 16 * v + i, col = n0 + nl + 16 * u + 4 * g;
-            f4 x = acc[u][v] * scale;
-            if constexpr (K == APPLY) {
-                if (A.final_out != nullptr) {
-                    T* f = (T*)A.final_out + (int64_t)batch * A.rows * A.cols;
+                for (int v = 0; v < U; v++) {
+                    const int row = m0 + ml + 16 * v + i, col = n0 + nl + 16 * u + 4 * g;
 #pragma unroll
                     for (int r = 0; r < 4; r++)
                         if (row < A.rows && col + r < A.cols)
-                            f[A.tall ? (int64_t)(col + r) * A.rows + row : (int64_t)row * A.cols + col + r] = (T)x[r];
-                    continue;
+                            f[A.tall ? (int64_t)(col + r) * A.rows + row : (int64_t)row * A.cols + col + r] =
+                                (T)(acc[u][v][r] * scale);
                 }
-            }
+            return;
+        }
+    }
+    const f16* add = A.add.p + batch * A.add.stride;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int v = 0; v < U; v++) {
+            acc[u][v] *= scale;
             if constexpr (K == POLY) {
+                const int row = m0 + ml + 16 * v + i, col = n0 + nl + 16 * u + 4 * g;
                 f16 hi[4], lo[4];
                 const f16* p = add + (int64_t)row * A.add.ld + col;
                 __builtin_memcpy(hi, p, 8);
                 __builtin_memcpy(lo, p + A.add.plane, 8);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    x[r] = __builtin_fmaf(add_scale, (float)hi[r] + (float)lo[r], x[r]);
-                    if (row == col + r && row < A.rows) x[r] += QA * SA;
-                }
-            }
-            f16 hi[4], lo[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) split(x[r], hi[r], lo[r]);
-            f16* p = out + (int64_t)row * A.out.ld + col;
-            __builtin_memcpy(p, hi, 8);
-            __builtin_memcpy(p + A.out.plane, lo, 8);
-            if constexpr (K != APPLY) {
-                if (tm != tn) {
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        f16* q = out + (int64_t)(col + r) * A.out.ld + row;
-                        q[0] = hi[r];
-                        q[A.out.plane] = lo[r];
-                    }
+                    acc[u][v][r] = __builtin_fmaf(add_scale, (float)hi[r] + (float)lo[r], acc[u][v][r]);
+                    if (row == col + r && row < A.rows) acc[u][v][r] += QA * SA;
                 }
             }
         }
-    }
+    // Both planes of the block go through LDS and leave as whole rows of 2 S bytes
+    // (from the lanes' registers they would leave in pieces of 8 bytes, and the
+    // transposed block's of 2: 5 us more per launch).
+    f16* out = A.out.p + batch * A.out.stride;
+    constexpr int CH = S / 8, LO = S * S;
+    f16* eh = (f16*)lds;
+    auto at = [](int row, int col) { return row * S + ((col / 8) ^ (row & (CH - 1) & 15)) * 8 + col % 8; };
+    auto leave = [&](int row0, int col0) {
+        __syncthreads();
+#pragma unroll 4
+        for (int id = threadIdx.x; id < S * CH; id += 256) {
+            const int row = id / CH, col = id % CH * 8;
+            f16* p = out + (int64_t)(row0 + row) * A.out.ld + col0 + col;
+            *(uint4*)p = *(const uint4*)(eh + at(row, col));
+            *(uint4*)(p + A.out.plane) = *(const uint4*)(eh + LO + at(row, col));
+        }
+    };
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int v = 0; v < U; v++) {
+            f16 hi[4], lo[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) split(acc[u][v][r], hi[r], lo[r]);
+            f16* p = eh + at(ml + 16 * v + i, nl + 16 * u + 4 * g);
+            __builtin_memcpy(p, hi, 8);
+            __builtin_memcpy(p + LO, lo, 8);
+        }
+    leave(m0, n0);
+    if (K == APPLY || tm == tn) return;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int v = 0; v < U; v++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                f16* p = eh + at(nl + 16 * u + 4 * g + r, ml + 16 * v + i);
+                split(acc[u][v][r], p[0], p[LO]);
+            }
+    leave(n0, m0);
 }
 
 // ---------------------------------------------------- a small matrix in one CU
@@ -594,21 +636,27 @@ int check(int type, int count, int m, int n)
     return GS_OK;
 }
 
+template <Kind K, int S, int STAGES, typename T>
+int launch(const char* name, const ProductArgs& A, int64_t blocks, hipStream_t stream)
+{
+    constexpr int lds = STAGES * 4 * S * KT * 2;
+    const auto kernel = orth_product_kernel<K, S, STAGES, T>;
+    if (lds > 65536)
+        GS_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    GS_TIMED(name, stream, hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, stream, A));
+    GS_LAUNCH_CHECK(name);
+    return GS_OK;
+}
+
 template <Kind K, typename T>
 int product(int S, const ProductArgs& A, int count, hipStream_t stream)
 {
     const int64_t per = K == APPLY ? (int64_t)A.tiles_m * A.tiles_n : (int64_t)A.tiles_m * (A.tiles_m + 1) / 2;
     GS_REQUIRE(per * count < 0x7fffffff, "orthogonalise: too many tiles for one launch");
     constexpr const char* name = K == SQUARE ? "orth_square" : K == POLY ? "orth_poly" : "orth_apply";
-    const dim3 grid((unsigned)(per * count));
-    if (S == 128)
-        GS_TIMED(name, stream,
-                 hipLaunchKernelGGL((orth_product_kernel<K, 128, T>), grid, dim3(256), 0, stream, A));
-    else
-        GS_TIMED(name, stream,
-                 hipLaunchKernelGGL((orth_product_kernel<K, 64, T>), grid, dim3(256), 0, stream, A));
-    GS_LAUNCH_CHECK("orth_product_kernel");
-    return GS_OK;
+    if (S == 64) return launch<K, 64, 2, T>(name, A, per * count, stream);
+    if (per * count <= 256) return launch<K, 128, 4, T>(name, A, per * count, stream);
+    return launch<K, 128, 2, T>(name, A, per * count, stream);
 }
 
 // The padded short side of a matrix that one workgroup takes, 0 if none does.
