@@ -723,16 +723,16 @@ constexpr int ENOUGH = 1024;
 
 int padded(int D) { return (D + 31) / 32 * 32; }
 
-// Splits of a walk of `steps` tiles when there are `blocks` column tiles: as
-// many as fill the chip (tiles of unequal cost: twice over), none shorter than
-// four tiles.  With a tile per CU already, a split has to save more than the
-// partial results cost: none shorter than 16 (370 tiles of 17 steps: 23 us in
-// four splits and 35 us to join them, against 36 us whole).
-int splits_of(int64_t blocks, int steps, bool unequal)
+// Splits of a walk of `steps` tiles when there are `blocks` column tiles: up to
+// `enough` workgroups.  A split's partial results cost as much as `least` steps,
+// which is as short as one gets.  With a tile per CU already, a split has to
+// save more: none shorter than 16 (370 tiles of 17 steps: 23 us in four splits
+// and 35 us to join them, against 27 us whole), and none at all at two per CU
+// unless the walks' costs differ.
+int splits_of(int64_t blocks, int steps, int least, int64_t enough, bool unequal)
 {
-    const int64_t enough = unequal ? 2 * ENOUGH : ENOUGH;
-    const int least = blocks < ENOUGH / 4 ? 4 : 16;
-    if (blocks >= enough / 2 || steps < 2 * least) return 1;
+    if (blocks >= ENOUGH / 4) least = 16;
+    if (blocks >= (unequal ? ENOUGH : ENOUGH / 2) || steps < 2 * least) return 1;
     const int64_t want = (enough + blocks - 1) / blocks;
     return (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / least));
 }
@@ -761,9 +761,9 @@ Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D, bool unequa
     p.nk = whole && two_columns(DKV, f32, DP) && heads * (((int64_t)Tk + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
     p.qt = 64;
     const int64_t tiles_q = (rows + 64 * p.nq - 1) / (64 * p.nq), tiles_k = ((int64_t)Tk + 64 * p.nk - 1) / (64 * p.nk);
-    p.splits_f = p.splits_q = splits_of(heads * tiles_q, (Tk + BK - 1) / BK, unequal);
-    p.splits_k =
-        splits_of(heads * tiles_k, (int)std::min<int64_t>((int64_t)G * ((Tq + p.qt - 1) / p.qt), 1 << 20), unequal);
+    p.splits_f = p.splits_q = splits_of(heads * tiles_q, (Tk + BK - 1) / BK, 4, unequal ? 2 * ENOUGH : ENOUGH, unequal);
+    const int64_t steps_k = (int64_t)G * ((Tq + p.qt - 1) / p.qt);
+    p.splits_k = splits_of(heads * tiles_k, (int)std::min<int64_t>(steps_k, 1 << 20), 8, ENOUGH, unequal);
     const size_t all = (size_t)heads * (size_t)rows;
     p.fwd_bytes = p.splits_f > 1 ? (size_t)p.splits_f * all * (size_t)(D + 2) * 4 : 0;
     const size_t dq = p.splits_q > 1 ? (size_t)p.splits_q * all * (size_t)D * 4 : 0;

@@ -111,6 +111,7 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(const T* __restrict__ g,
     const int64_t from = per * blockIdx.x, to = from + per < size ? from + per : size;
     float s = 0.0f;
     const int64_t whole = to - (to - from) % V;
+#pragma unroll 4
     for (int64_t i = from + (int64_t)threadIdx.x * V; i < whole; i += 256 * V) {
         const gs::Vec<T> t = gs::load_vec(p + i);
 #pragma unroll
@@ -204,12 +205,12 @@ struct Pair {
 // A block computes S x S of the result, four waves a quarter each: columns of
 // its matrix-core tiles are rows of the left operand, rows are columns of the
 // result, so that a lane holds four neighbours of one row of the result.
-template <Kind K, int S, int STAGES, typename T>
-__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void orth_product_kernel(ProductArgs A)
+template <Kind K, int S, typename T>
+__global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
 {
     constexpr int H = S / 2, U = H / 16;
     constexpr int WORDS = S * KT / 8;                // of one operand's plane
-    extern __shared__ uint4 lds[];                   // [STAGES][left hi, lo, right hi, lo]
+    __shared__ uint4 lds[2 * 4 * WORDS];             // [2][left hi, lo, right hi, lo]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const uint32_t per = K == APPLY ? (uint32_t)A.tiles_m * A.tiles_n : (uint32_t)A.tiles_m * (A.tiles_m + 1) / 2;
     const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x);
@@ -241,24 +242,17 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void orth_product_kernel(
     for (int u = 0; u < U; u++)
 #pragma unroll
         for (int v = 0; v < U; v++) acc[u][v] = f4{0, 0, 0, 0};
-    // the loads of STAGES - 1 tiles are in flight; `waiting` of them may still
-    // be when the oldest is read
-    constexpr int LOADS = 4 * (S * KT / 8 / 256), waiting = LOADS * (STAGES - 2);
     const int tiles = A.k / KT;
     auto fetch = [&](uint4* to) __attribute__((always_inline)) {
         sl.fetch(to, to + WORDS);
         sr.fetch(to + 2 * WORDS, to + 3 * WORDS);
     };
-#pragma unroll
-    for (int t = 0; t < STAGES - 1; t++)
-        if (t < tiles) fetch(lds + t * 4 * WORDS);
+    fetch(lds);
     // two restricted pointers tell the compiler that the loads need not have
     // arrived before the reads
     auto step = [&](int t, const uint4* __restrict__ at, uint4* __restrict__ next) __attribute__((always_inline)) {
-        // tile t is there for all waves, and all waves are done with tile t - 1
-        if (t + STAGES - 2 < tiles) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(waiting) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + STAGES - 1 < tiles) fetch(next);
+        __syncthreads();   // tile t is there for all waves, and all are done with tile t - 1
+        if (t + 1 < tiles) fetch(next);
         Frag<f16> lh[U], ll[U];
 #pragma unroll
         for (int v = 0; v < U; v++) {
@@ -279,27 +273,41 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void orth_product_kernel(
         }
     };
     for (int t = 0; t < tiles; t++)
-        step(t, lds + t % STAGES * 4 * WORDS, lds + (t + STAGES - 1) % STAGES * 4 * WORDS);
+        step(t, lds + t % 2 * 4 * WORDS, lds + (t + 1) % 2 * 4 * WORDS);
     const int k = extra_scale(A.small[batch], A.step);
     float scale = A.scale;
     if constexpr (K == POLY) scale = __builtin_ldexpf(scale, -4 * k);
     if constexpr (K == APPLY)
         scale = __builtin_ldexpf(scale, A.final_out != nullptr ? -k : extra_scale(A.small[batch], A.step + 1) - k);
     const float add_scale = __builtin_ldexpf(QB, -2 * k);
+    // What leaves goes through LDS and leaves as whole rows of the block (from the
+    // lanes' registers it would leave in pieces of 8 bytes, and a transposed
+    // block's of 2: 5 us more per launch).
+    __syncthreads();
     if constexpr (K == APPLY) {
         if (A.final_out != nullptr) {
             T* f = (T*)A.final_out + (int64_t)batch * A.rows * A.cols;
+            float* e = (float*)lds;
+            auto at = [](int y, int x) { return y * S + (((x / 4) ^ (y & 15)) * 4) + x % 4; };
+            const int y0 = A.tall ? n0 : m0, x0 = A.tall ? m0 : n0, height = A.tall ? A.cols : A.rows,
+                      width = A.tall ? A.rows : A.cols;
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int v = 0; v < U; v++) {
-                    const int row = m0 + ml + 16 * v + i, col = n0 + nl + 16 * u + 4 * g;
+                    const int row = ml + 16 * v + i, col = nl + 16 * u + 4 * g;
+                    if (A.tall) {
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (row < A.rows && col + r < A.cols)
-                            f[A.tall ? (int64_t)(col + r) * A.rows + row : (int64_t)row * A.cols + col + r] =
-                                (T)(acc[u][v][r] * scale);
+                        for (int r = 0; r < 4; r++) e[at(col + r, row)] = acc[u][v][r] * scale;
+                    } else {
+                        *(f4*)(e + at(row, col)) = acc[u][v] * scale;
+                    }
                 }
+            __syncthreads();
+            for (int id = threadIdx.x; id < S * S; id += 256) {
+                const int y = id / S, x = id % S;
+                if (y0 + y < height && x0 + x < width) f[(int64_t)(y0 + y) * width + x0 + x] = (T)e[at(y, x)];
+            }
             return;
         }
     }
@@ -322,9 +330,6 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void orth_product_kernel(
                 }
             }
         }
-    // Both planes of the block go through LDS and leave as whole rows of 2 S bytes
-    // (from the lanes' registers they would leave in pieces of 8 bytes, and the
-    // transposed block's of 2: 5 us more per launch).
     f16* out = A.out.p + batch * A.out.stride;
     constexpr int CH = S / 8, LO = S * S;
     f16* eh = (f16*)lds;
@@ -339,7 +344,6 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void orth_product_kernel(
             *(uint4*)(p + A.out.plane) = *(const uint4*)(eh + LO + at(row, col));
         }
     };
-    __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
@@ -636,27 +640,18 @@ int check(int type, int count, int m, int n)
     return GS_OK;
 }
 
-template <Kind K, int S, int STAGES, typename T>
-int launch(const char* name, const ProductArgs& A, int64_t blocks, hipStream_t stream)
-{
-    constexpr int lds = STAGES * 4 * S * KT * 2;
-    const auto kernel = orth_product_kernel<K, S, STAGES, T>;
-    if (lds > 65536)
-        GS_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    GS_TIMED(name, stream, hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, stream, A));
-    GS_LAUNCH_CHECK(name);
-    return GS_OK;
-}
-
 template <Kind K, typename T>
 int product(int S, const ProductArgs& A, int count, hipStream_t stream)
 {
     const int64_t per = K == APPLY ? (int64_t)A.tiles_m * A.tiles_n : (int64_t)A.tiles_m * (A.tiles_m + 1) / 2;
     GS_REQUIRE(per * count < 0x7fffffff, "orthogonalise: too many tiles for one launch");
     constexpr const char* name = K == SQUARE ? "orth_square" : K == POLY ? "orth_poly" : "orth_apply";
-    if (S == 64) return launch<K, 64, 2, T>(name, A, per * count, stream);
-    if (per * count <= 256) return launch<K, 128, 4, T>(name, A, per * count, stream);
-    return launch<K, 128, 2, T>(name, A, per * count, stream);
+    const dim3 grid((unsigned)(per * count));
+    if (S == 128)
+        GS_TIMED(name, stream, hipLaunchKernelGGL((orth_product_kernel<K, 128, T>), grid, dim3(256), 0, stream, A));
+    else GS_TIMED(name, stream, hipLaunchKernelGGL((orth_product_kernel<K, 64, T>), grid, dim3(256), 0, stream, A));
+    GS_LAUNCH_CHECK(name);
+    return GS_OK;
 }
 
 // The padded short side of a matrix that one workgroup takes, 0 if none does.
