@@ -16,6 +16,12 @@ mirror the reference's operator API:
   blitzgs_amd.plyio      : trained-scene PLY save / load (records <-> tensors on the GPU)
   blitzgs_amd.checkpoint : the training checkpoint tuple, file naming and resume
                            at another world size
+and, for a network in front of the rasterizer that predicts Gaussians (float32,
+bfloat16, float16):
+  blitzgs_amd.norm       : layer_norm
+  blitzgs_amd.attention  : attention (shared heads, causal limit, key lengths)
+  blitzgs_amd.orthogonal : orthogonalise, OrthogonalMomentum (weight matrices' optimiser)
+  blitzgs_amd.examples.train_predictor trains such a network with them
 Drop-in packages with the reference's module names live in blitzgs_amd/dropin.
 """
 __version__ = "0.1.0"

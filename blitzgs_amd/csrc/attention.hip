@@ -701,7 +701,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
 // `per` tensors.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__ part, int splits, int per,
-                                                       int64_t rows, int H, int Tn, int D, T* out0, T* out1, Strides s0, Strides s1)
+                                                       int64_t rows, int H, int Tn, int D, T* out0, T* out1,
+                                                       Strides s0, Strides s1)
 {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= rows * D) return;
@@ -929,7 +930,8 @@ extern "C" int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, in
     gs::clear_error();
     if (int rc = check(type, B, Hq, Hkv, Tq, Tk, D, scale)) return rc;
     if (B == 0 || Tq == 0) return GS_OK;
-    GS_REQUIRE(q && o && q_strides && k_strides && v_strides && o_strides, "attention: q, o and all strides must be given");
+    GS_REQUIRE(q && o && q_strides && k_strides && v_strides && o_strides,
+               "attention: q, o and all strides must be given");
     GS_REQUIRE(Tk == 0 || (k && v), "attention: k and v must be non-null");
     const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal || key_lengths);
     GS_REQUIRE(p.splits_f == 1 || workspace != nullptr, "attention: this size needs the workspace");
@@ -962,9 +964,9 @@ extern "C" int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, in
 extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, const void* q,
                                      const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                                      const int64_t* v_strides, float scale, int causal, const int* key_lengths,
-                                     const int* query_start, const void* o, const int64_t* o_strides, const void* o_rest,
-                                     const float* lse, const void* dout, const int64_t* dout_strides, void* dq, const int64_t* dq_strides,
-                                     void* dk, const int64_t* dk_strides, void* dv, const int64_t* dv_strides,
+                                     const int* query_start, const void* o, const int64_t* o_strides,
+                                     const void* o_rest, const float* lse, const void* dout,
+                                     const int64_t* dout_strides, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv, const int64_t* dv_strides,
                                      void* workspace, hipStream_t stream)
 {
     gs::clear_error();

@@ -102,7 +102,8 @@ __device__ __forceinline__ void three(const Frag<f16>& ah, const Frag<f16>& al, 
 // ------------------------------------------------------------- the normalised X
 
 template <typename T>
-__global__ __launch_bounds__(256) void orth_norm_kernel(const T* __restrict__ g, int64_t size, float* __restrict__ parts)
+__global__ __launch_bounds__(256) void orth_norm_kernel(const T* __restrict__ g, int64_t size,
+                                                        float* __restrict__ parts)
 {
     __shared__ float sums[4];
     const T* p = g + (int64_t)blockIdx.y * size;
@@ -145,7 +146,8 @@ __global__ __launch_bounds__(256) void orth_split_kernel(const T* __restrict__ g
     const int y0 = blockIdx.y * 64, x0 = blockIdx.x * 64;   // of the tile in X
     const int gy = tall ? x0 : y0, gx = tall ? y0 : x0;     // in G
     for (int k = wave; k < 64; k += 4)
-        tile[k][lane] = gy + k < rows && gx + lane < cols ? (float)p[(int64_t)(gy + k) * cols + gx + lane] * scale : 0.0f;
+        tile[k][lane] =
+            gy + k < rows && gx + lane < cols ? (float)p[(int64_t)(gy + k) * cols + gx + lane] * scale : 0.0f;
     __syncthreads();
     f16* out = x.p + blockIdx.z * x.stride;
     for (int k = wave; k < 64; k += 4) {
@@ -398,8 +400,8 @@ __device__ __forceinline__ void corner(int e, int& bm, int& bn)
 
 // acc = the 32 x 32 block (bm, bn) of Y Y^T, Y's planes in `depth` panels.
 template <int PANEL>
-__device__ __forceinline__ void square_block(const Tile<f16, 32>& tile, const uint4* hi, const uint4* lo, int depth, int bm,
-                                             int bn, f4 (&acc)[2][2])
+__device__ __forceinline__ void square_block(const Tile<f16, 32>& tile, const uint4* hi, const uint4* lo, int depth,
+                                             int bm, int bn, f4 (&acc)[2][2])
 {
 #pragma unroll
     for (int u = 0; u < 2; u++)
@@ -423,8 +425,8 @@ __device__ __forceinline__ void square_block(const Tile<f16, 32>& tile, const ui
 // Both planes of four neighbours (row, col ..) of a symmetric matrix, and where
 // `both` of (col .., row) too; from and to are a column's place.
 template <int PANEL>
-__device__ __forceinline__ void store_symmetric(uint4* ph, uint4* pl, int row, int col, int row_to, int col_to, bool both,
-                                                f4 x)
+__device__ __forceinline__ void store_symmetric(uint4* ph, uint4* pl, int row, int col, int row_to, int col_to,
+                                                bool both, f4 x)
 {
     f16 hi[4], lo[4];
 #pragma unroll
