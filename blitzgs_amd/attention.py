@@ -79,14 +79,17 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, do):
         q, k, v, o, rest, lse, key_lengths, query_start = ctx.saved_tensors
         do = _last_contiguous(do)
-        dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
+        dq, dk, dv = _token_major(q), None, None
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dk, dv = _token_major(k), _token_major(v)
+        beside = _strides(k if dk is None else dk)   # dk's and dv's strides
         ws = _workspace(ctx.sizes, ctx.causal, key_lengths, 1, q.device)
         with _t.on_device(q.device):
             _t.check(_t.load().gs_attention_backward(
                 *ctx.sizes, _t.ptr(q), _strides(q), _t.ptr(k), _strides(k), _t.ptr(v), _strides(v), ctx.scale,
                 int(ctx.causal), _t.ptr(key_lengths), _t.ptr(query_start), _t.ptr(o), _strides(o),
                 _t.ptr(rest), _t.ptr(lse), _t.ptr(do), _strides(do), _t.ptr(dq), _strides(dq), _t.ptr(dk),
-                _strides(dk), _t.ptr(dv), _strides(dv), _t.ptr(ws), _t.stream(q.device)),
+                beside, _t.ptr(dv), beside, _t.ptr(ws), _t.stream(q.device)),
                 "gs_attention_backward")
         return dq, dk, dv, None, None, None, None
 

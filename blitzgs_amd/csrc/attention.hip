@@ -776,7 +776,7 @@ Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D, bool unequa
 template <typename K>
 int launch(const char* name, K kernel, int64_t blocks, size_t lds, const AttnArgs& A, hipStream_t stream)
 {
-    GS_REQUIRE(blocks < 0x7fffffff, "attention: too many workgroups");
+    GS_REQUIRE(blocks < (1 << 24), "attention: too many workgroups for one launch");
     if (lds > 65536)
         GS_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     GS_TIMED(name, stream, hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, stream, A));
@@ -966,7 +966,8 @@ extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, i
                                      const int64_t* v_strides, float scale, int causal, const int* key_lengths,
                                      const int* query_start, const void* o, const int64_t* o_strides,
                                      const void* o_rest, const float* lse, const void* dout,
-                                     const int64_t* dout_strides, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv, const int64_t* dv_strides,
+                                     const int64_t* dout_strides, void* dq, const int64_t* dq_strides, void* dk,
+                                     const int64_t* dk_strides, void* dv, const int64_t* dv_strides,
                                      void* workspace, hipStream_t stream)
 {
     gs::clear_error();
@@ -976,7 +977,8 @@ extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, i
                    dv_strides,
                "attention: all strides must be given");
     GS_REQUIRE(Tq == 0 || (q && o && lse && dout && dq), "attention: q, o, lse, dout and dq must be non-null");
-    GS_REQUIRE(Tk == 0 || (k && v && dk && dv), "attention: k, v, dk and dv must be non-null");
+    GS_REQUIRE(Tk == 0 || (k && v), "attention: k and v must be non-null");
+    GS_REQUIRE((dk == nullptr) == (dv == nullptr), "attention: dk and dv come together");
     const Plan p = plan_of(type, B, Hkv, Hq / Hkv, Tq, Tk, D, causal || key_lengths);
     GS_REQUIRE(p.bwd_bytes == 0 || workspace != nullptr, "attention: the backward needs the workspace");
     AttnArgs A = args_of(B, Hq, Hkv, Tq, Tk, D, scale, causal, key_lengths, query_start);
@@ -1010,7 +1012,7 @@ extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, i
             GS_LAUNCH_CHECK("attn_add_kernel");
         }
     }
-    if (Tk > 0) {
+    if (Tk > 0 && dk != nullptr) {
         A.out0 = dk;
         A.out1 = dv;
         A.s0 = strides_of(dk_strides);

@@ -30,6 +30,7 @@ constexpr int MAX_WIDTH = 32768;
 // Partial rows of the column sums: two blocks per CU, enough waves in flight
 // to cover memory latency and few enough partial rows to add up quickly.
 constexpr int MAX_PARTS = 512;
+constexpr int MAX_BLOCKS = 1 << 20;   // of the forward: more rows are walked with that stride
 
 template <int V, typename W>
 __device__ __forceinline__ void load_params(const W* p, int at, float (&out)[V], float none)
@@ -89,51 +90,52 @@ __global__ __launch_bounds__(LPR > BLOCK ? LPR : BLOCK) void norm_fwd_kernel(Nor
     constexpr int RPB = LPR > BLOCK ? 1 : BLOCK / LPR;
     __shared__ float meet[LPR > 64 ? LPR / 64 : 1];
     const int l = threadIdx.x % LPR;
-    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
-    if (row >= A.rows) return;   // whole rows: with LPR > 64 the block has one row
-    const T* x = (const T*)A.x + row * A.xs;
-    T* y = (T*)A.y + row * A.width;
     const float inv_n = 1.0f / (float)A.width;
-    float v[NC][V];
-    float s = 0.0f;
+    // whole rows leave the loop together: with LPR > 64 the block has one row
+    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR; row < A.rows; row += (int64_t)gridDim.x * RPB) {
+        const T* x = (const T*)A.x + row * A.xs;
+        T* y = (T*)A.y + row * A.width;
+        float v[NC][V];
+        float s = 0.0f;
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const int at = (c * LPR + l) * V;
-        Chunk<T, V> t{};
-        if (at < A.width) __builtin_memcpy(&t, x + at, sizeof(t));
+        for (int c = 0; c < NC; c++) {
+            const int at = (c * LPR + l) * V;
+            Chunk<T, V> t{};
+            if (at < A.width) __builtin_memcpy(&t, x + at, sizeof(t));
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            v[c][i] = (float)t.v[i];
-            s += v[c][i];
+            for (int i = 0; i < V; i++) {
+                v[c][i] = (float)t.v[i];
+                s += v[c][i];
+            }
         }
-    }
-    const float mean = row_sum<LPR>(s, meet) * inv_n;
-    float q = 0.0f;
+        const float mean = row_sum<LPR>(s, meet) * inv_n;
+        float q = 0.0f;
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const bool in = (c * LPR + l) * V < A.width;
+        for (int c = 0; c < NC; c++) {
+            const bool in = (c * LPR + l) * V < A.width;
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            v[c][i] = in ? v[c][i] - mean : 0.0f;
-            q = __builtin_fmaf(v[c][i], v[c][i], q);
+            for (int i = 0; i < V; i++) {
+                v[c][i] = in ? v[c][i] - mean : 0.0f;
+                q = __builtin_fmaf(v[c][i], v[c][i], q);
+            }
         }
-    }
-    const float rstd = 1.0f / __builtin_sqrtf(row_sum<LPR>(q, meet) * inv_n + A.eps);
+        const float rstd = 1.0f / __builtin_sqrtf(row_sum<LPR>(q, meet) * inv_n + A.eps);
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const int at = (c * LPR + l) * V;
-        if (at >= A.width) continue;
-        float w[V], b[V];
-        load_params<V>((const W*)A.w, at, w, 1.0f);
-        load_params<V>((const W*)A.b, at, b, 0.0f);
-        Chunk<T, V> t;
+        for (int c = 0; c < NC; c++) {
+            const int at = (c * LPR + l) * V;
+            if (at >= A.width) continue;
+            float w[V], b[V];
+            load_params<V>((const W*)A.w, at, w, 1.0f);
+            load_params<V>((const W*)A.b, at, b, 0.0f);
+            Chunk<T, V> t;
 #pragma unroll
-        for (int i = 0; i < V; i++) t.v[i] = (T)__builtin_fmaf(v[c][i] * rstd, w[i], b[i]);
-        __builtin_memcpy(y + at, &t, sizeof(t));
-    }
-    if (l == 0 && A.mean != nullptr) {
-        A.mean[row] = mean;
-        A.rstd[row] = rstd;
+            for (int i = 0; i < V; i++) t.v[i] = (T)__builtin_fmaf(v[c][i] * rstd, w[i], b[i]);
+            __builtin_memcpy(y + at, &t, sizeof(t));
+        }
+        if (l == 0 && A.mean != nullptr) {
+            A.mean[row] = mean;
+            A.rstd[row] = rstd;
+        }
     }
 }
 
@@ -389,7 +391,8 @@ extern "C" int gs_layer_norm_forward(int type, int param_type, int64_t rows, int
     A.xs = x_stride;
     A.width = width;
     A.eps = eps;
-    launch<false>(type, param_type, s, A, gs_div_up((size_t)rows, (size_t)rows_per_block(s)), stream);
+    const int64_t blocks = (rows + rows_per_block(s) - 1) / rows_per_block(s);
+    launch<false>(type, param_type, s, A, (unsigned)(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS), stream);
     GS_LAUNCH_CHECK("norm_fwd_kernel");
     return GS_OK;
 }

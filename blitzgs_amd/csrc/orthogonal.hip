@@ -24,6 +24,9 @@
 // A and A A are symmetric: their tiles on and below the diagonal are computed
 // and stored twice.  The planes are padded to whole tiles with zeros, so the
 // products have no edge cases.
+#include <algorithm>
+#include <utility>
+
 #include "gs_host.h"
 #include "gs_matrix.h"
 #include "../../include/blitzgs_amd.h"
@@ -60,6 +63,8 @@ struct ProductArgs {
     const float* small;         // -log2 |X| of each matrix at the start
     int step;
     float scale;
+    int splits;                 // of the sums' depth
+    float* part;                // [tile][split][S x S], in the order of the lanes' registers
 };
 
 // X's planes hold X SX 2^k, and A's A SA 4^k, where 2^k |X| <= 1 at this step.
@@ -190,6 +195,11 @@ struct Pair {
         plane = m.plane;
         step = DOWN ? (int64_t)KT * m.ld : KT;
     }
+    __device__ __forceinline__ void skip(int tiles)
+    {
+#pragma unroll
+        for (int c = 0; c < CH; c++) p[c] += tiles * step;
+    }
     __device__ __forceinline__ void fetch(uint4* hi, uint4* lo)
     {
         typedef const __attribute__((address_space(1))) void* global_ptr;
@@ -206,8 +216,10 @@ struct Pair {
 
 // A block computes S x S of the result, four waves a quarter each: columns of
 // its matrix-core tiles are rows of the left operand, rows are columns of the
-// result, so that a lane holds four neighbours of one row of the result.
-template <Kind K, int S, typename T>
+// result, so that a lane holds four neighbours of one row of the result.  With
+// splits > 1 a block sums a part of the depth and leaves it in memory as it lies
+// in its registers; GATHER then adds a tile's parts in order and finishes it.
+template <Kind K, int S, bool GATHER, typename T>
 __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
 {
     constexpr int H = S / 2, U = H / 16;
@@ -215,7 +227,8 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
     __shared__ uint4 lds[2 * 4 * WORDS];             // [2][left hi, lo, right hi, lo]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const uint32_t per = K == APPLY ? (uint32_t)A.tiles_m * A.tiles_n : (uint32_t)A.tiles_m * (A.tiles_m + 1) / 2;
-    const uint32_t item = gs::xcd_item(blockIdx.x, gridDim.x);
+    const uint32_t place = gs::xcd_item(blockIdx.x, gridDim.x), splits = GATHER ? 1u : (uint32_t)A.splits;
+    const uint32_t item = place / splits;
     const int batch = (int)(item / per);
     int tm, tn;
     if constexpr (K == APPLY) {
@@ -232,10 +245,6 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
     const f16* lp = A.l.p + batch * A.l.stride;
     const f16* rp = A.r.p + batch * A.r.stride;
 
-    Pair<S, false> sl;
-    Pair<S, K == APPLY> sr;
-    sl.at(A.l, lp, m0);
-    sr.at(A.r, rp, n0);
     const Tile<f16, KT> tile;
     const Tile<f16, H> down;
     const int ml = (wave & 1) * H, nl = (wave >> 1) * H;
@@ -244,38 +253,62 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(ProductArgs A)
     for (int u = 0; u < U; u++)
 #pragma unroll
         for (int v = 0; v < U; v++) acc[u][v] = f4{0, 0, 0, 0};
-    const int tiles = A.k / KT;
-    auto fetch = [&](uint4* to) __attribute__((always_inline)) {
-        sl.fetch(to, to + WORDS);
-        sr.fetch(to + 2 * WORDS, to + 3 * WORDS);
-    };
-    fetch(lds);
-    // two restricted pointers tell the compiler that the loads need not have
-    // arrived before the reads
-    auto step = [&](int t, const uint4* __restrict__ at, uint4* __restrict__ next) __attribute__((always_inline)) {
-        __syncthreads();   // tile t is there for all waves, and all are done with tile t - 1
-        if (t + 1 < tiles) fetch(next);
-        Frag<f16> lh[U], ll[U];
+    f4* part = (f4*)A.part + (int64_t)item * A.splits * (U * U * 256) + threadIdx.x;
+    if constexpr (GATHER) {
+        for (int p = 0; p < A.splits; p++, part += U * U * 256)
 #pragma unroll
-        for (int v = 0; v < U; v++) {
-            lh[v] = tile.rows(at + ml * KT / 8, 16 * v, 0);
-            ll[v] = tile.rows(at + WORDS + ml * KT / 8, 16 * v, 0);
-        }
+            for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            Frag<f16> rh, rl;
-            if constexpr (K == APPLY) {
-                rh = down.cols(at + 2 * WORDS + nl * KT / 8, 0, 16 * u);
-                rl = down.cols(at + 3 * WORDS + nl * KT / 8, 0, 16 * u);
-            } else {
-                rh = tile.rows(at + 2 * WORDS + nl * KT / 8, 16 * u, 0);
-                rl = tile.rows(at + 3 * WORDS + nl * KT / 8, 16 * u, 0);
+                for (int v = 0; v < U; v++) acc[u][v] += part[(u * U + v) * 256];
+    } else {
+        const int all = A.k / KT, split = (int)(place % splits), begin = all * split / A.splits,
+                  tiles = all * (split + 1) / A.splits - begin;
+        Pair<S, false> sl;
+        Pair<S, K == APPLY> sr;
+        sl.at(A.l, lp, m0);
+        sr.at(A.r, rp, n0);
+        sl.skip(begin);
+        sr.skip(begin);
+        auto fetch = [&](uint4* to) __attribute__((always_inline)) {
+            sl.fetch(to, to + WORDS);
+            sr.fetch(to + 2 * WORDS, to + 3 * WORDS);
+        };
+        fetch(lds);
+        // two restricted pointers tell the compiler that the loads need not have
+        // arrived before the reads
+        auto step = [&](int t, const uint4* __restrict__ at, uint4* __restrict__ next) __attribute__((always_inline)) {
+            __syncthreads();   // tile t is there for all waves, and all are done with tile t - 1
+            if (t + 1 < tiles) fetch(next);
+            Frag<f16> lh[U], ll[U];
+#pragma unroll
+            for (int v = 0; v < U; v++) {
+                lh[v] = tile.rows(at + ml * KT / 8, 16 * v, 0);
+                ll[v] = tile.rows(at + WORDS + ml * KT / 8, 16 * v, 0);
             }
-            three(rh, rl, lh, ll, acc[u]);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                Frag<f16> rh, rl;
+                if constexpr (K == APPLY) {
+                    rh = down.cols(at + 2 * WORDS + nl * KT / 8, 0, 16 * u);
+                    rl = down.cols(at + 3 * WORDS + nl * KT / 8, 0, 16 * u);
+                } else {
+                    rh = tile.rows(at + 2 * WORDS + nl * KT / 8, 16 * u, 0);
+                    rl = tile.rows(at + 3 * WORDS + nl * KT / 8, 16 * u, 0);
+                }
+                three(rh, rl, lh, ll, acc[u]);
+            }
+        };
+        for (int t = 0; t < tiles; t++)
+            step(t, lds + t % 2 * 4 * WORDS, lds + (t + 1) % 2 * 4 * WORDS);
+        if (A.splits > 1) {
+            part += (int64_t)split * (U * U * 256);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int v = 0; v < U; v++) part[(u * U + v) * 256] = acc[u][v];
+            return;
         }
-    };
-    for (int t = 0; t < tiles; t++)
-        step(t, lds + t % 2 * 4 * WORDS, lds + (t + 1) % 2 * 4 * WORDS);
+    }
     const int k = extra_scale(A.small[batch], A.step);
     float scale = A.scale;
     if constexpr (K == POLY) scale = __builtin_ldexpf(scale, -4 * k);
@@ -605,7 +638,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void orth_small_kernel(const T* __re
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// The workspace: partial sums and the matrices' sizes, then the planes of X (twice), A and B.
+// The workspace: partial sums and the matrices' sizes, the planes of X (twice), A
+// and B, and the split products' parts.
 struct Layout {
     int m, n;               // padded sides, m the shorter
     int64_t parts, x, sq;   // bytes of each piece
@@ -620,6 +654,17 @@ int tile_of(int count, int64_t m, int64_t n)
     return (int64_t)count * (pm / 128) * (pn / 128) >= 256 ? 128 : 64;
 }
 
+// Splits of a product's depth where its tiles leave half of the CUs without work:
+// up to two workgroups per CU, none shorter than 16 staged tiles.  One 1024 x 4096
+// matrix (36 tiles of X X^T) 818 -> 520 us; with 144 tiles the parts cost more
+// than they save (four 1024 x 1024: 484 us whole, 527 split).
+int splits_of(int64_t tiles, int depth)
+{
+    if (tiles >= 128) return 1;
+    const int64_t want = (512 + tiles - 1) / tiles, most = depth / KT / 16;
+    return (int)(most < 1 ? 1 : want < most ? want : most);
+}
+
 Layout layout_of(int count, int m, int n)
 {
     Layout L{};
@@ -629,7 +674,13 @@ Layout layout_of(int count, int m, int n)
     L.parts = up((int64_t)count * (NORM_PARTS + 1) * 4, 256);
     L.x = up((int64_t)count * L.m * L.n * 4, 256);
     L.sq = up((int64_t)count * L.m * L.m * 4, 256);
-    L.bytes = L.parts + 2 * L.x + 2 * L.sq;
+    const int64_t tm = L.m / t, tn = L.n / t, sq = count * (tm * (tm + 1) / 2), full = count * tm * tn;
+    int64_t most = 0;
+    for (const auto& [tiles, depth] : {std::pair<int64_t, int>{sq, L.n}, {sq, L.m}, {full, L.m}}) {
+        const int splits = splits_of(tiles, depth);
+        if (splits > 1 && tiles * splits > most) most = tiles * splits;
+    }
+    L.bytes = L.parts + 2 * L.x + 2 * L.sq + most * t * t * 4;
     return L;
 }
 
@@ -646,13 +697,27 @@ template <Kind K, typename T>
 int product(int S, const ProductArgs& A, int count, hipStream_t stream)
 {
     const int64_t per = K == APPLY ? (int64_t)A.tiles_m * A.tiles_n : (int64_t)A.tiles_m * (A.tiles_m + 1) / 2;
-    GS_REQUIRE(per * count < 0x7fffffff, "orthogonalise: too many tiles for one launch");
+    GS_REQUIRE(per * count < (1 << 24), "orthogonalise: too many tiles for one launch");
     constexpr const char* name = K == SQUARE ? "orth_square" : K == POLY ? "orth_poly" : "orth_apply";
-    const dim3 grid((unsigned)(per * count));
+    ProductArgs P = A;
+    P.splits = splits_of(per * count, A.k);
+    const dim3 grid((unsigned)(per * count * P.splits));
     if (S == 128)
-        GS_TIMED(name, stream, hipLaunchKernelGGL((orth_product_kernel<K, 128, T>), grid, dim3(256), 0, stream, A));
-    else GS_TIMED(name, stream, hipLaunchKernelGGL((orth_product_kernel<K, 64, T>), grid, dim3(256), 0, stream, A));
+        GS_TIMED(name, stream,
+                 hipLaunchKernelGGL((orth_product_kernel<K, 128, false, T>), grid, dim3(256), 0, stream, P));
+    else
+        GS_TIMED(name, stream,
+                 hipLaunchKernelGGL((orth_product_kernel<K, 64, false, T>), grid, dim3(256), 0, stream, P));
     GS_LAUNCH_CHECK(name);
+    if (P.splits == 1) return GS_OK;
+    const dim3 tiles((unsigned)(per * count));
+    if (S == 128)
+        GS_TIMED("orth_gather", stream,
+                 hipLaunchKernelGGL((orth_product_kernel<K, 128, true, T>), tiles, dim3(256), 0, stream, P));
+    else
+        GS_TIMED("orth_gather", stream,
+                 hipLaunchKernelGGL((orth_product_kernel<K, 64, true, T>), tiles, dim3(256), 0, stream, P));
+    GS_LAUNCH_CHECK("orth_gather");
     return GS_OK;
 }
 
@@ -709,6 +774,7 @@ int orthogonalise(int count, int m, int n, const T* g, int steps, T* out, void* 
     A.rows = tall ? n : m;
     A.tall = tall;
     A.small = small;
+    A.part = (float*)(at + 2 * L.x + 2 * L.sq);
     A.tiles_m = L.m / S;
     for (int s = 0; s < steps; s++) {
         const bool last = s + 1 == steps;
@@ -756,13 +822,13 @@ template <typename T>
 __global__ __launch_bounds__(256) void momentum_kernel(MomentumBatch B, int64_t size, float beta, int nesterov,
                                                        float* __restrict__ update)
 {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= size) return;
-    const float g = (float)((const T*)B.grad[blockIdx.y])[e];
-    float* mp = B.momentum[blockIdx.y] + e;
-    const float m = __builtin_fmaf(beta, *mp, g);
-    *mp = m;
-    update[blockIdx.y * size + e] = nesterov ? __builtin_fmaf(beta, m, g) : m;
+    const T* grad = (const T*)B.grad[blockIdx.y];
+    float *momentum = B.momentum[blockIdx.y], *out = update + blockIdx.y * size;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < size; e += (int64_t)gridDim.x * 256) {
+        const float g = (float)grad[e], m = __builtin_fmaf(beta, momentum[e], g);
+        momentum[e] = m;
+        out[e] = nesterov ? __builtin_fmaf(beta, m, g) : m;
+    }
 }
 
 // p = p keep - lr update
@@ -770,10 +836,15 @@ template <typename T>
 __global__ __launch_bounds__(256) void apply_kernel(MomentumBatch B, int64_t size, float keep, float lr,
                                                     const float* __restrict__ update)
 {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= size) return;
-    T* p = (T*)B.param[blockIdx.y] + e;
-    *p = (T)__builtin_fmaf(-lr, update[blockIdx.y * size + e], (float)*p * keep);
+    T* param = (T*)B.param[blockIdx.y];
+    const float* u = update + blockIdx.y * size;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < size; e += (int64_t)gridDim.x * 256)
+        param[e] = (T)__builtin_fmaf(-lr, u[e], (float)param[e] * keep);
+}
+
+dim3 grid_of(int64_t size, int count)
+{
+    return dim3((unsigned)std::min<int64_t>((size + 255) / 256, 16384), (unsigned)count);
 }
 
 }  // namespace
@@ -816,7 +887,7 @@ extern "C" int gs_momentum_update(int type, int count, int64_t size, const void*
         B.grad[i] = grads[i];
         B.momentum[i] = momenta[i];
     }
-    const dim3 grid(gs_div_up((size_t)size, 256), (unsigned)count);
+    const dim3 grid = grid_of(size, count);
     if (type == GS_F32)
         hipLaunchKernelGGL(momentum_kernel<float>, grid, dim3(256), 0, stream, B, size, beta, nesterov, update);
     else if (type == GS_BF16)
@@ -840,7 +911,7 @@ extern "C" int gs_momentum_apply(int type, int count, int64_t size, void* const*
         GS_REQUIRE(params[i], "momentum: null tensor %d", i);
         B.param[i] = params[i];
     }
-    const dim3 grid(gs_div_up((size_t)size, 256), (unsigned)count);
+    const dim3 grid = grid_of(size, count);
     if (type == GS_F32) hipLaunchKernelGGL(apply_kernel<float>, grid, dim3(256), 0, stream, B, size, keep, lr, update);
     else if (type == GS_BF16)
         hipLaunchKernelGGL(apply_kernel<gs::bf16>, grid, dim3(256), 0, stream, B, size, keep, lr, update);

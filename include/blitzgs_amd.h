@@ -683,6 +683,7 @@ int gs_layer_norm_backward(int type, int param_type, int64_t rows, int width, co
  *   o_rest, with o's strides and type, may be NULL: o's value before its
  * rounding less o.  A backward that is given it forms sum(do o) from both; with
  * GS_F32 there is nothing to keep.
+ *   The backward writes dq, and dk and dv unless both are NULL.
  *   The workspace's size (gs_attention_workspace_bytes; 0: none is needed, or
  * the arguments are invalid) depends on the sizes and on `unequal`: whether the call is causal or is given
  * key_lengths.  Results do not depend on the order of execution. */

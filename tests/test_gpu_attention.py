@@ -204,6 +204,18 @@ def test_gradient_against_differences(gpu):
         assert abs((f(*up) - f(*down)) / (2 * h) - along) <= 1e-2 * (1 + abs(along)), name
 
 
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (0, 2)])
+def test_some_gradients_only(gpu, wanted):
+    # a frozen context, or frozen queries: the gradients asked for are the same bits
+    from blitzgs_amd.attention import attention
+    q, k, v, do = _inputs(torch.bfloat16, 2, 4, 2, 60, 90, 64)
+    full = _run(q, k, v, do)
+    leaves = [x.detach().requires_grad_(i in wanted) for i, x in enumerate((q, k, v))]
+    got = torch.autograd.grad(attention(*leaves), [leaves[i] for i in wanted], do)
+    for i, g in zip(wanted, got):
+        assert torch.equal(g, full[("dq", "dk", "dv")[i]])
+
+
 def test_equal_bits_and_another_stream(gpu):
     q, k, v, do = _inputs(torch.bfloat16, 2, 8, 2, 500, 700, 64)
     how = dict(causal=True, key_lengths=_int(700, 333))

@@ -38,6 +38,13 @@ def test_large_tiles(gpu, t):
     _check(_rand((40, 190, 400), t, 2))
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shape", [(130, 2100), (2, 1500, 140), (200, 1100)])
+def test_long_sums_of_few_tiles(gpu, t, shape):
+    # the depth of X X^T is cut into parts
+    _check(_rand(shape, t, 7))
+
+
 @pytest.mark.parametrize("steps", [1, 2, 5, 8])
 def test_steps(gpu, steps):
     _check(_rand((2, 60, 90), torch.float32, steps), steps)

@@ -75,7 +75,7 @@ def test_attention(lib):
                                          NZ, NZ, s, NZ, s, dk, s, NZ, s, ws, None)
     _refused(lib, bwd(ws=None), b"workspace")
     _refused(lib, bwd(o=None), b"non-null")
-    _refused(lib, bwd(dk=None), b"non-null")
+    _refused(lib, bwd(dk=None), b"together")
     assert lib.gs_attention_workspace_bytes(BF16, 1, 2, 1, 4, 4, 0, 0, 0) == 0
     # one query over many keys is split and needs room for partial results
     assert lib.gs_attention_workspace_bytes(BF16, 1, 1, 1, 1, 100000, 64, 0, 0) >= 2 * 66 * 4
