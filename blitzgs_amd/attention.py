@@ -40,57 +40,55 @@ def _last_contiguous(t):
 def _token_major(like):
     """An empty (B, H, T, D) tensor that lies as (B, T, H, D), ready for the next projection."""
     B, H, T, D = like.shape
-    return torch.empty((B, T, H, D), device=like.device, dtype=like.dtype).transpose(1, 2)
-
-
-def _workspace(sizes, causal, key_lengths, backward, device):
-    unequal = int(causal or key_lengths is not None)
-    return _t.workspace(_t.load().gs_attention_workspace_bytes(*sizes, unequal, backward), device)
+    return torch.empty_strided((B, H, T, D), (T * H * D, D, H * D, 1), device=like.device, dtype=like.dtype)
 
 
 def _forward(q, k, v, causal, key_lengths, query_start, scale, grads):
-    """o and, for a backward, (sizes, what rounding o left, lse)."""
+    """o and, for a backward, what rounding o left, lse, and what the backward is called with."""
     B, Hq, Tq, D = q.shape
     Hkv, Tk = k.shape[1:3]
-    sizes = _t.DTYPE_CODES[q.dtype], B, Hq, Hkv, Tq, Tk, D
+    lib, sizes = _t.load(), (_t.DTYPE_CODES[q.dtype], B, Hq, Hkv, Tq, Tk, D)
+    unequal = int(causal or key_lengths is not None)
     o = _token_major(q)
     lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32) if grads else None
     rest = _token_major(q) if grads and q.dtype != torch.float32 else None
-    ws = _workspace(sizes, causal, key_lengths, 0, q.device)
+    ws = _t.workspace(lib.gs_attention_workspace_bytes(*sizes, unequal, 0), q.device)
+    strides = _strides(q), _strides(k), _strides(v), _strides(o)
     with _t.on_device(q.device):
-        _t.check(_t.load().gs_attention_forward(
-            *sizes, _t.ptr(q), _strides(q), _t.ptr(k), _strides(k), _t.ptr(v), _strides(v), scale, int(causal),
-            _t.ptr(key_lengths), _t.ptr(query_start), _t.ptr(o), _strides(o), _t.ptr(rest), _t.ptr(lse),
+        _t.check(lib.gs_attention_forward(
+            *sizes, q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(), strides[2], scale, int(causal),
+            _t.ptr(key_lengths), _t.ptr(query_start), o.data_ptr(), strides[3], _t.ptr(rest), _t.ptr(lse),
             _t.ptr(ws), _t.stream(q.device)), "gs_attention_forward")
-    return o, (sizes, rest, lse)
+    return o, rest, lse, (sizes, strides, unequal, scale, int(causal))
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, causal, key_lengths, query_start, scale):
         q, k, v = (_last_contiguous(t.detach()) for t in (q, k, v))
-        o, (ctx.sizes, rest, lse) = _forward(q, k, v, causal, key_lengths, query_start, scale, True)
+        o, rest, lse, ctx.how = _forward(q, k, v, causal, key_lengths, query_start, scale, True)
         ctx.save_for_backward(q, k, v, o, rest, lse, key_lengths, query_start)
-        ctx.scale, ctx.causal = scale, causal
+        ctx.ws_bytes = _t.load().gs_attention_workspace_bytes(*ctx.how[0], ctx.how[2], 1)
         return o
 
+    # The autograd engine calls this from a thread of its own, on the forward's
+    # device and stream: what does not need the gradient is prepared by forward.
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, o, rest, lse, key_lengths, query_start = ctx.saved_tensors
+        sizes, (qs, ks, vs, os), _, scale, causal = ctx.how
         do = _last_contiguous(do)
-        dq, dk, dv = _token_major(q), None, None
+        dq, dk, dv, beside = _token_major(q), None, None, ks
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dk, dv = _token_major(k), _token_major(v)
-        beside = _strides(k if dk is None else dk)   # dk's and dv's strides
-        ws = _workspace(ctx.sizes, ctx.causal, key_lengths, 1, q.device)
-        with _t.on_device(q.device):
-            _t.check(_t.load().gs_attention_backward(
-                *ctx.sizes, _t.ptr(q), _strides(q), _t.ptr(k), _strides(k), _t.ptr(v), _strides(v), ctx.scale,
-                int(ctx.causal), _t.ptr(key_lengths), _t.ptr(query_start), _t.ptr(o), _strides(o),
-                _t.ptr(rest), _t.ptr(lse), _t.ptr(do), _strides(do), _t.ptr(dq), _strides(dq), _t.ptr(dk),
-                beside, _t.ptr(dv), beside, _t.ptr(ws), _t.stream(q.device)),
-                "gs_attention_backward")
+            beside = _strides(dk)
+        ws = _t.workspace(ctx.ws_bytes, q.device)
+        _t.check(_t.load().gs_attention_backward(
+            *sizes, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, scale, causal, _t.ptr(key_lengths),
+            _t.ptr(query_start), o.data_ptr(), os, _t.ptr(rest), lse.data_ptr(), do.data_ptr(), _strides(do),
+            dq.data_ptr(), os, _t.ptr(dk), beside, _t.ptr(dv), beside, _t.ptr(ws), _t.stream(q.device)),
+            "gs_attention_backward")
         return dq, dk, dv, None, None, None, None
 
 

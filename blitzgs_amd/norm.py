@@ -27,56 +27,50 @@ def _rows(t, width):
     return t, n, apart if n > 1 else width
 
 
-def _stats(stats, n):
-    if stats is None:
-        return None, None
-    return stats.data_ptr(), stats.data_ptr() + 4 * n
-
-
 def _forward(x, weight, bias, eps, grads):
-    """y and, for a backward, the parameters' type and each row's mean and 1 / deviation."""
+    """y and, for a backward, each row's mean and 1 / deviation and what the backward is called with."""
     width = x.shape[-1]
     rows, n, apart = _rows(x, width)
-    w = None if weight is None else weight.contiguous()
-    b = None if bias is None else bias.contiguous()
     params = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+    code, param_code = _t.DTYPE_CODES[x.dtype], _t.DTYPE_CODES[params]
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     stats = torch.empty((2, n), device=x.device, dtype=torch.float32) if grads else None
-    mean, rstd = _stats(stats, n)
+    mean = stats.data_ptr() if grads else None
     with _t.on_device(x.device):
         _t.check(_t.load().gs_layer_norm_forward(
-            _t.DTYPE_CODES[x.dtype], _t.DTYPE_CODES[params], n, width, _t.ptr(rows), apart,
-            _t.ptr(w), _t.ptr(b), eps, _t.ptr(y), mean, rstd, _t.stream(x.device)),
-            "gs_layer_norm_forward")
-    return y, params, stats
+            code, param_code, n, width, rows.data_ptr(), apart, _t.ptr(weight), _t.ptr(bias), eps, y.data_ptr(), mean,
+            mean + 4 * n if grads else None, _t.stream(x.device)), "gs_layer_norm_forward")
+    return y, stats, (code, param_code, n, width, params)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, ctx.params, stats = _forward(x, weight, bias, eps, True)
+        y, stats, ctx.how = _forward(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.columns = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
+        ctx.wants = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
+        code, _, n, width, _ = ctx.how
+        ctx.ws_bytes = _t.load().gs_layer_norm_workspace_bytes(code, n, width) if any(ctx.wants) else 0
         return y
 
+    # The autograd engine calls this from a thread of its own, on the forward's
+    # device and stream: what does not need the gradient is prepared by forward.
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
-        width = x.shape[-1]
-        rows, n, apart = _rows(x, width)
+        code, param_code, n, width, params = ctx.how
+        device = x.device
+        rows, _, apart = _rows(x, width)
         drows, _, dapart = _rows(dy, width)
-        mean, rstd = _stats(stats, n)
-        w = None if weight is None else weight.contiguous()
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        dw, db = (torch.empty(width, device=x.device, dtype=ctx.params) if c else None for c in ctx.columns)
-        lib, code = _t.load(), _t.DTYPE_CODES[x.dtype]
-        ws = _t.workspace(lib.gs_layer_norm_workspace_bytes(code, n, width), x.device) if any(ctx.columns) else None
-        with _t.on_device(x.device):
-            _t.check(lib.gs_layer_norm_backward(
-                code, _t.DTYPE_CODES[ctx.params], n, width, _t.ptr(rows), apart, _t.ptr(w),
-                mean, rstd, _t.ptr(drows), dapart, _t.ptr(dx), _t.ptr(dw), _t.ptr(db),
-                _t.ptr(ws), _t.stream(x.device)), "gs_layer_norm_backward")
+        dx = torch.empty(x.shape, device=device, dtype=x.dtype)
+        dw = torch.empty(width, device=device, dtype=params) if ctx.wants[0] else None
+        db = torch.empty(width, device=device, dtype=params) if ctx.wants[1] else None
+        ws = _t.workspace(ctx.ws_bytes, device)
+        mean = stats.data_ptr()
+        _t.check(_t.load().gs_layer_norm_backward(
+            code, param_code, n, width, rows.data_ptr(), apart, _t.ptr(weight), mean, mean + 4 * n, drows.data_ptr(),
+            dapart, dx.data_ptr(), _t.ptr(dw), _t.ptr(db), _t.ptr(ws), _t.stream(device)), "gs_layer_norm_backward")
         return dx, dw, db, None
 
 
@@ -97,6 +91,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise RuntimeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
     if not 0.0 <= eps < float("inf"):
         raise RuntimeError(f"eps must be a finite number of at least 0, got {eps}")
+    weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
     if _t.wants_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _forward(x, weight, bias, float(eps), False)[0]
