@@ -698,22 +698,28 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
 }
 
 // Adds the splits' partial gradients: [splits][per][rows = B H Tn][D] to each of
-// `per` tensors.
+// `per` tensors; a wave per row, its splits in order.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__ part, int splits, int per,
                                                        int64_t rows, int H, int Tn, int D, T* out0, T* out1,
                                                        Strides s0, Strides s1)
 {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= rows * D) return;
-    const int64_t row = id / D;
-    const int d = (int)(id - row * D), t = (int)(row % Tn), h = (int)(row / Tn % H), b = (int)(row / Tn / H);
-    const int which = blockIdx.y;
-    float s = 0.0f;
-#pragma unroll 8
-    for (int k = 0; k < splits; k++) s += part[((int64_t)k * per + which) * rows * D + id];
+    const int lane = threadIdx.x & 63, which = blockIdx.y;
     const Strides st = which == 0 ? s0 : s1;
-    (which == 0 ? out0 : out1)[b * st.b + h * st.h + t * st.t + d] = (T)s;
+    T* out = which == 0 ? out0 : out1;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
+        float x0 = 0.0f, x1 = 0.0f;
+        const float* p = part + (which * rows + row) * D;
+#pragma unroll 8
+        for (int k = 0; k < splits; k++, p += per * rows * D) {
+            if (lane < D) x0 += p[lane];
+            if (lane + 64 < D) x1 += p[lane + 64];
+        }
+        const uint32_t r = (uint32_t)row, t = r % (uint32_t)Tn, bh = r / (uint32_t)Tn, h = bh % H, b = bh / H;
+        T* to = out + b * st.b + h * st.h + t * st.t;
+        if (lane < D) to[lane] = (T)x0;
+        if (lane + 64 < D) to[lane + 64] = (T)x1;
+    }
 }
 
 // ------------------------------------------------------------------ launching
@@ -870,7 +876,7 @@ void join(const AttnArgs& A, hipStream_t stream)
 template <typename T>
 void add(const AttnArgs& A, int per, int H, int Tn, hipStream_t stream)
 {
-    const int64_t rows = (int64_t)A.B * H * Tn, blocks = (rows * A.D + 255) / 256;
+    const int64_t rows = (int64_t)A.B * H * Tn, blocks = std::min<int64_t>((rows + 3) / 4, 1 << 20);
     GS_TIMED("attn_add_kernel", stream,
              hipLaunchKernelGGL(attn_add_kernel<T>, dim3((unsigned)blocks, (unsigned)per), dim3(256), 0, stream, A.part,
                                 A.splits, per, rows, H, Tn, A.D, (T*)A.out0, (T*)A.out1, A.s0, A.s1));
