@@ -361,20 +361,29 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs A)
     __shared__ float sums[4][130];
     const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq, row = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float* ml = A.part_ml + 2 * row;   // a split's maximum and sum, 2 rows apart
     float m = NEG_INF;
-    for (int s = lane; s < A.splits; s += 64) m = fmaxf(m, A.part_ml[2 * (s * rows + row)]);
+    for (int s = lane; s < A.splits; s += 64) m = fmaxf(m, ml[2 * s * rows]);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
     const float base = m == NEG_INF ? 0.0f : m;
+    // splits wave, wave + 4, ...: lane k keeps the factor of the k-th of 64
     float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-#pragma unroll 4
-    for (int s = wave; s < A.splits; s += 4) {
-        const int64_t at = s * rows + row;
-        const float f = exp2_fast(A.part_ml[2 * at] - base);
-        sum = __builtin_fmaf(A.part_ml[2 * at + 1], f, sum);
-        if (lane < A.D) o0 = __builtin_fmaf(A.part[at * A.D + lane], f, o0);
-        if (lane + 64 < A.D) o1 = __builtin_fmaf(A.part[at * A.D + lane + 64], f, o1);
+    for (int s0 = wave; s0 < A.splits; s0 += 256) {
+        const int s = s0 + 4 * lane, n = min(64, (A.splits - s0 + 3) / 4);
+        const float f = lane < n ? exp2_fast(ml[2 * s * rows] - base) : 0.0f;
+        sum = __builtin_fmaf(lane < n ? ml[2 * s * rows + 1] : 0.0f, f, sum);
+        const float* p = A.part + (s0 * rows + row) * A.D;
+#pragma unroll 8
+        for (int k = 0; k < n; k++) {
+            const float fk = __shfl(f, k, 64);
+            if (lane < A.D) o0 = __builtin_fmaf(p[lane], fk, o0);
+            if (lane + 64 < A.D) o1 = __builtin_fmaf(p[lane + 64], fk, o1);
+            p += 4 * rows * A.D;
+        }
     }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
     sums[wave][lane] = o0;
     sums[wave][64 + lane] = o1;
     if (lane == 0) sums[wave][128] = sum;
