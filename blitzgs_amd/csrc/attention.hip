@@ -62,6 +62,11 @@ constexpr float NEG_INF = -__builtin_inff();
 constexpr float SLACK = 8.0f;   // of the softmax's running base, in powers of two
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Workgroups per CU that the registers are shared out for; the tiles of wide fp32
+// heads leave room for one in LDS.
+template <typename T, int DP>
+constexpr int PER_CU = sizeof(T) == 4 && DP > 64 ? 1 : 2;
+
 struct Strides {
     int64_t b, h, t;
 };
@@ -219,7 +224,7 @@ __device__ __forceinline__ void store_o(T* p, T* rest, f4 v, int n)
 // ------------------------------------------------------------------- forward
 
 template <typename T, int DP, int NQ, Fill F>
-__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
+__global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_fwd_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NQ, WORDS = BK * L::CHUNKS;
@@ -366,23 +371,26 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs A)
     }
 }
 
-// Joins the splits of a row: one workgroup per row, a wave every fourth split.
-template <typename T>
+// Joins the splits of a row, W waves a row: wave w takes splits w, w + W, ...
+// One wave where the rows alone fill the chip, else the workgroup's four.
+template <typename T, int W>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs A)
 {
-    __shared__ float sums[4][130];
-    const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq, row = blockIdx.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float sums[W][130];
+    const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
+    const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
+    const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= rows) return;
     const float* ml = A.part_ml + 2 * row;   // a split's maximum and sum, 2 rows apart
     float m = NEG_INF;
     for (int s = lane; s < A.splits; s += 64) m = fmaxf(m, ml[2 * s * rows]);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
     const float base = m == NEG_INF ? 0.0f : m;
-    // splits wave, wave + 4, ...: lane k keeps the factor of the k-th of 64
+    // of 64 of the wave's splits lane k keeps the k-th's factor
     float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int s0 = wave; s0 < A.splits; s0 += 256) {
-        const int s = s0 + 4 * lane, n = min(64, (A.splits - s0 + 3) / 4);
+    for (int s0 = wave; s0 < A.splits; s0 += 64 * W) {
+        const int s = s0 + W * lane, n = min(64, (A.splits - s0 + W - 1) / W);
         const float f = lane < n ? exp2_fast(ml[2 * s * rows] - base) : 0.0f;
         sum = __builtin_fmaf(lane < n ? ml[2 * s * rows + 1] : 0.0f, f, sum);
         const float* p = A.part + (s0 * rows + row) * A.D;
@@ -391,33 +399,45 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs A)
             const float fk = __shfl(f, k, 64);
             if (lane < A.D) o0 = __builtin_fmaf(p[lane], fk, o0);
             if (lane + 64 < A.D) o1 = __builtin_fmaf(p[lane + 64], fk, o1);
-            p += 4 * rows * A.D;
+            p += W * rows * A.D;
         }
     }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
-    sums[wave][lane] = o0;
-    sums[wave][64 + lane] = o1;
-    if (lane == 0) sums[wave][128] = sum;
-    __syncthreads();
-    const int d = threadIdx.x;
-    sum = (sums[0][128] + sums[1][128]) + (sums[2][128] + sums[3][128]);
-    const int Hq = A.Hkv * A.G, i = (int)(row % A.Tq), h = (int)(row / A.Tq % Hq), b = (int)(row / A.Tq / Hq);
-    const int64_t out = b * A.s0.b + h * A.s0.h + i * A.s0.t;
-    if (d < A.D) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const float x = ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) * inv;
-        ((T*)A.out0)[out + d] = (T)x;
-        if (A.rest != nullptr) ((T*)A.rest)[out + d] = (T)(x - (float)(T)x);
+    if constexpr (W > 1) {
+        sums[wave][lane] = o0;
+        sums[wave][64 + lane] = o1;
+        if (lane == 0) sums[wave][128] = sum;
+        __syncthreads();
+        if (wave != 0) return;
+        o0 = o1 = sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            o0 += sums[w][lane];
+            o1 += sums[w][64 + lane];
+            sum += sums[w][128];
+        }
     }
-    if (d == 0 && A.lse != nullptr) A.lse[row] = sum == 0.0f ? -NEG_INF : m + __builtin_log2f(sum);
+    const uint32_t r = (uint32_t)row, i = r % (uint32_t)A.Tq, bh = r / (uint32_t)A.Tq, Hq = A.Hkv * A.G;
+    const int64_t out = bh / Hq * A.s0.b + bh % Hq * A.s0.h + i * A.s0.t;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, x0 = o0 * inv, x1 = o1 * inv;
+    T *o = (T*)A.out0 + out, *rest = (T*)A.rest + out;
+    if (lane < A.D) {
+        o[lane] = (T)x0;
+        if (A.rest != nullptr) rest[lane] = (T)(x0 - (float)(T)x0);
+    }
+    if (lane + 64 < A.D) {
+        o[lane + 64] = (T)x1;
+        if (A.rest != nullptr) rest[lane + 64] = (T)(x1 - (float)(T)x1);
+    }
+    if (lane == 0 && A.lse != nullptr) A.lse[row] = sum == 0.0f ? -NEG_INF : m + __builtin_log2f(sum);
 }
 
 // ------------------------------------------------------------------ backward
 
 // dq, and delta for the other kernel.
 template <typename T, int DP, int NQ, Fill F>
-__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
+__global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dq_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NQ, WORDS = BK * L::CHUNKS;
@@ -558,7 +578,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs A)
 // dk and dv.  A wave holds 16 NK keys; the block streams the queries of every
 // head that shares them, QT rows at a time.
 template <typename T, int DP, int NK, int QT, Fill F>
-__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs A)
+__global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NK, WORDS = QT * L::CHUNKS, BUF = 2 * WORDS + QT / 2;
@@ -753,14 +773,16 @@ int padded(int D) { return (D + 31) / 32 * 32; }
 
 // Splits of a walk of `steps` tiles when there are `blocks` column tiles: up to
 // `enough` workgroups.  A split's partial results cost as much as `least` steps,
-// which is as short as one gets.  With a tile per CU already, a split has to
-// save more: none shorter than 16 (370 tiles of 17 steps: 23 us in four splits
-// and 35 us to join them, against 27 us whole), and none at all at two per CU
-// unless the walks' costs differ.
+// which is as short as one gets.  With a tile per CU already, only long walks of
+// unequal cost are split, none shorter than 32 (256 tiles of 32 steps: 37 us in
+// two splits and 41 us to join them; whole, in 512 half as wide tiles, 41 us).
 int splits_of(int64_t blocks, int steps, int least, int64_t enough, bool unequal)
 {
-    if (blocks >= ENOUGH / 4) least = 16;
-    if (blocks >= (unequal ? ENOUGH : ENOUGH / 2) || steps < 2 * least) return 1;
+    if (blocks >= ENOUGH / 4) {
+        if (!unequal || blocks >= ENOUGH) return 1;
+        least = 32;
+    }
+    if (steps < 2 * least) return 1;
     const int64_t want = (enough + blocks - 1) / blocks;
     return (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / least));
 }
@@ -782,11 +804,11 @@ Plan plan_of(int type, int B, int Hkv, int G, int Tq, int Tk, int D, bool unequa
     Plan p{};
     const int DP = padded(D);
     const int64_t heads = (int64_t)B * Hkv, rows = (int64_t)G * Tq;
-    // 16 columns also where 32 would leave CUs without work, and for head
-    // dimensions that end inside 16 bytes
+    // 16 columns also where 32 would leave less than two workgroups per CU, and for
+    // head dimensions that end inside 16 bytes
     const bool whole = D % (16 / gs::dtype_bytes(type)) == 0, f32 = type == GS_F32;
-    p.nq = whole && two_columns(DQ, f32, DP) && heads * ((rows + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
-    p.nk = whole && two_columns(DKV, f32, DP) && heads * (((int64_t)Tk + 127) / 128) >= ENOUGH / 4 ? 2 : 1;
+    p.nq = whole && two_columns(DQ, f32, DP) && heads * ((rows + 127) / 128) >= ENOUGH / 2 ? 2 : 1;
+    p.nk = whole && two_columns(DKV, f32, DP) && heads * (((int64_t)Tk + 127) / 128) >= ENOUGH / 2 ? 2 : 1;
     p.qt = 64;
     const int64_t tiles_q = (rows + 64 * p.nq - 1) / (64 * p.nq), tiles_k = ((int64_t)Tk + 64 * p.nk - 1) / (64 * p.nk);
     p.splits_f = p.splits_q = splits_of(heads * tiles_q, (Tk + BK - 1) / BK, 4, unequal ? 2 * ENOUGH : ENOUGH, unequal);
@@ -890,8 +912,13 @@ template <typename T>
 void join(const AttnArgs& A, hipStream_t stream)
 {
     const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
-    GS_TIMED("attn_join_kernel", stream,
-             hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, stream, A));
+    if (rows >= 4096)
+        GS_TIMED("attn_join_kernel", stream,
+                 hipLaunchKernelGGL((attn_join_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream,
+                                    A));
+    else
+        GS_TIMED("attn_join_kernel", stream,
+                 hipLaunchKernelGGL((attn_join_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, stream, A));
 }
 
 template <typename T>
