@@ -372,9 +372,10 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_fwd_kernel(AttnArgs
 }
 
 // Joins the splits of a row, W waves a row: wave w takes splits w, w + W, ...
-// One wave where the rows alone fill the chip, else the workgroup's four.
+// One wave where the rows alone fill the chip, 16 where few rows leave them the
+// latency of many splits (8 rows of 128 splits: 14 us with four waves), else four.
 template <typename T, int W>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs A)
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void attn_join_kernel(AttnArgs A)
 {
     __shared__ float sums[W][130];
     const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
@@ -916,6 +917,9 @@ void join(const AttnArgs& A, hipStream_t stream)
         GS_TIMED("attn_join_kernel", stream,
                  hipLaunchKernelGGL((attn_join_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream,
                                     A));
+    else if (rows < 512 && A.splits > 16)
+        GS_TIMED("attn_join_kernel", stream,
+                 hipLaunchKernelGGL((attn_join_kernel<T, 16>), dim3((unsigned)rows), dim3(1024), 0, stream, A));
     else
         GS_TIMED("attn_join_kernel", stream,
                  hipLaunchKernelGGL((attn_join_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, stream, A));
