@@ -38,10 +38,10 @@
 // maximum and half a conversion, 65 % of its cycles, beside 33 % matrix work.  The
 // others are near the matrix core's practical rate, dk, dv behind for want of
 // registers: 16 keys a wave at D = 128, two waves per SIMD.
-//   2 x 16 heads, 4096 x 4096, D 64     forward 209 us (658 TFLOP/s), dq 222 (929
-//                                       with its recomputation), dk dv 325 (846)
-//   16 heads on 4, 8192 causal, D 128   329 us (836), 395 (1044), 716 (768)
-//   8 x 32 heads on 8, one query, up to 32768 keys, D 128   105 + 11 us to join
+//   2 x 16 heads, 4096 x 4096, D 64     forward 201 us (683 TFLOP/s), dq 215 (959
+//                                       with its recomputation), dk dv 312 (881)
+//   16 heads on 4, 8192 causal, D 128   325 us (846), 390 (1056), 703 (782)
+//   8 x 32 heads on 8, one query, up to 32768 keys, D 128   106 + 6 us to join
 //                                       the splits (537 MB, 4.8 TB/s in all)
 #include <algorithm>
 

@@ -20,8 +20,8 @@
 // same bits.  All sums and statistics are fp32 whatever the tensors' type;
 // each output is rounded to its type once.
 //
-// 65536 x 1024 bfloat16, fp32 parameters: forward 52 us (268 MB, 5.1 TB/s),
-// backward 85 us (403 MB, 4.8 TB/s) and 4 us for the partial rows; a large copy
+// 65536 x 1024 bfloat16, fp32 parameters: forward 54 us (268 MB, 4.9 TB/s),
+// backward 85 us (403 MB, 4.7 TB/s) and 4 us for the partial rows; a large copy
 // reaches 5.15 TB/s.
 #include "gs_host.h"
 #include "gs_types.h"

@@ -25,8 +25,8 @@
 // and stored twice.  The planes are padded to whole tiles with zeros, so the
 // products have no edge cases.
 //
-// Eight 1024 x 4096 fp32 matrices: 2.05 ms, per step X X^T 151 us, B 52 us, B X
-// 197 us (1045 TFLOP/s of float16 products; a large library product reaches 1190
+// Eight 1024 x 4096 fp32 matrices: 2.03 ms, per step X X^T 150 us, B 52 us, B X
+// 194 us (1060 TFLOP/s of float16 products; a large library product reaches 1190
 // on the card).  The symmetric products' 288 tiles leave a second place on most
 // CUs empty: 64-wide tiles were slower (191 us), parts of the depth no faster.
 #include <algorithm>
