@@ -12,7 +12,9 @@ and slices of a fused projection are passed as transposed views.
 Query i of batch b sees key j when j < key_lengths[b] and, with causal,
 j <= i + query_start[b].  By default the last query sees the last of Tk keys.
 A query that sees no key gives zeros and no gradient, and keys from
-key_lengths on are never read.
+key_lengths on are never read, nor are those that no query sees.  A NaN or an
+infinity reaches the queries that see its key and, in the backward, the keys that
+its query sees, and no others.
 
 Scores, softmax and all sums are fp32; probabilities are rounded to the
 tensors' type for the product with v.  Nothing of size Tq x Tk is stored: a call

@@ -38,12 +38,13 @@
 // maximum and half a conversion, 65 % of its cycles, beside 33 % matrix work.  The
 // others are near the matrix core's practical rate, dk, dv behind for want of
 // registers: 16 keys a wave at D = 128, two waves per SIMD.
-//   2 x 16 heads, 4096 x 4096, D 64     forward 201 us (683 TFLOP/s), dq 215 (959
-//                                       with its recomputation), dk dv 312 (881)
-//   16 heads on 4, 8192 causal, D 128   325 us (846), 390 (1056), 703 (782)
-//   8 x 32 heads on 8, one query, up to 32768 keys, D 128   106 + 6 us to join
-//                                       the splits (537 MB, 4.8 TB/s in all)
+//   2 x 16 heads, 4096 x 4096, D 64     forward 210 us (654 TFLOP/s), dq 215 (959
+//                                       with its recomputation), dk dv 320 (859)
+//   16 heads on 4, 8192 causal, D 128   330 us (833), 396 (1041), 719 (765)
+//   8 x 32 heads on 8, one query, up to 32768 keys, D 128   111 + 7 us to join
+//                                       the splits (537 MB, 4.6 TB/s in all)
 #include <algorithm>
+#include <type_traits>
 
 #include "gs_host.h"
 #include "gs_matrix.h"
@@ -184,7 +185,7 @@ __device__ __forceinline__ Column column(const AttnArgs& A, const QueryTile& w, 
     const int rr = c.valid ? r : 0;
     c.h = w.hk * A.G + rr / A.Tq;
     c.i = rr % A.Tq;
-    c.seen = c.valid ? seen_of(A, w.len, w.start, c.i) : w.len;
+    c.seen = c.valid ? seen_of(A, w.len, w.start, c.i) : w.seen_max;
     return c;
 }
 
@@ -217,6 +218,24 @@ __device__ __forceinline__ void store_o(T* p, T* rest, f4 v, int n)
     store4<ODD>(rest, left, n);
 }
 
+// A weight of zero does not keep a NaN or an infinity of a tile's row from the
+// columns that do not see the row.  So in the tiles that a mask cuts, put() makes
+// such elements zero, and the columns that do see them get them after the walk,
+// from memory.  With that work beside the product instead, under a branch that is
+// never taken, its registers spilled; with a barrier of its own at the beginning of
+// a step the 577 x 1025 forward took 34 us in place of 31.
+
+// Adds to x those of the first n of four neighbours that are not finite.
+template <typename T>
+__device__ __forceinline__ void add_rest(f4& x, const T* p, int n)
+{
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const float v = r < n ? (float)p[r] : 0.0f;
+        if (!(fabsf(v) < -NEG_INF)) x[r] += v;
+    }
+}
+
 // The tile that is read and the one that is being loaded come to a step as two
 // restricted pointers: only so does the compiler know that the loads need not
 // have arrived before the reads.
@@ -229,6 +248,7 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_fwd_kernel(AttnArgs
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NQ, WORDS = BK * L::CHUNKS;
     extern __shared__ uint4 lds[];   // [2][k tile, v tile]
+    __shared__ int found;            // whether put() made anything zero
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const L tile_of;
     const QueryTile w = query_tile<COLS>(A);
@@ -255,23 +275,27 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_fwd_kernel(AttnArgs
         for (int d = 0; d < DT; d++) o[d][n] = f4{0, 0, 0, 0};
     }
 
+    if (threadIdx.x == 0) found = 0;
+    bool met = false;   // by this thread
     Stage<T, DP, BK, F> sk, sv;
     auto fetch = [&](int t, uint4* to) __attribute__((always_inline)) {
-        sk.fetch(to, kb + (int64_t)t * BK * A.ks.t, A.ks.t, w.len - t * BK, A.D);
-        sv.fetch(to + WORDS, vb + (int64_t)t * BK * A.vs.t, A.vs.t, w.len - t * BK, A.D);
+        sk.fetch(to, kb + (int64_t)t * BK * A.ks.t, A.ks.t, w.seen_max - t * BK, A.D);
+        sv.fetch(to + WORDS, vb + (int64_t)t * BK * A.vs.t, A.vs.t, w.seen_max - t * BK, A.D);
     };
-    auto put = [&](uint4* to) {
+    auto put = [&](int t, uint4* to, bool cuts) __attribute__((always_inline)) {
         sk.put(to);
-        sv.put(to + WORDS);
+        met |= sv.put(to + WORDS, cuts && (t + 1) * BK > w.seen_min);
     };
     if (w.t0 < w.t1) {
 #pragma unroll
         for (int k = 0; k < 4; k++) sk.clear(lds + k * WORDS, A.D);
         fetch(w.t0, lds);
-        put(lds);
+        put(w.t0, lds, true);
     }
     __syncthreads();
-    auto step = [&](int t, const uint4* __restrict__ kt, uint4* __restrict__ next) __attribute__((always_inline)) {
+    auto step = [&](auto cuts, int t, const uint4* __restrict__ kt, uint4* __restrict__ next)
+                    __attribute__((always_inline)) {
+        constexpr bool CUTS = decltype(cuts)::value;
         const uint4* vt = kt + WORDS;
         const int k0 = t * BK;
         if (t + 1 < w.t1) fetch(t + 1, next);
@@ -287,7 +311,9 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_fwd_kernel(AttnArgs
                 for (int n = 0; n < NQ; n++) s[u][n] = gs::mma(a, q[n][c], s[u][n]);
             }
         }
-        if (k0 + BK > w.seen_min) {
+        // the parts stay apart, as the mask's branch keeps them (577 x 1025: 33 -> 31 us)
+        if constexpr (!CUTS) __builtin_amdgcn_sched_barrier(0);
+        if (CUTS && k0 + BK > w.seen_min) {
 #pragma unroll
             for (int n = 0; n < NQ; n++)
 #pragma unroll
@@ -337,11 +363,31 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_fwd_kernel(AttnArgs
                 for (int n = 0; n < NQ; n++) o[d][n] = gs::mma(a, p[n], o[d][n]);
             }
         }
-        if (t + 1 < w.t1) put(next);
+        if (t + 1 < w.t1) put(t + 1, next, CUTS);
         __syncthreads();
     };
-    for (int t = w.t0; t < w.t1; t++)
-        step(t, lds + ((t - w.t0) & 1) * 2 * WORDS, lds + ((t + 1 - w.t0) & 1) * 2 * WORDS);
+    // tiles that no mask cuts, and whose next is none that one cuts, take a loop of
+    // their own; at D <= 64 one loop schedules better (4096 keys of 64: 217 us, 226
+    // in two; 8192 causal of 128: 330 and 326)
+    int t = w.t0;
+    if constexpr (DP > 64)
+        for (const int whole = min(w.t1, w.seen_min / BK) - 1; t < whole; t++)
+            step(std::false_type{}, t, lds + ((t - w.t0) & 1) * 2 * WORDS, lds + ((t + 1 - w.t0) & 1) * 2 * WORDS);
+    for (; t < w.t1; t++)
+        step(std::true_type{}, t, lds + ((t - w.t0) & 1) * 2 * WORDS, lds + ((t + 1 - w.t0) & 1) * 2 * WORDS);
+    if (met) found = 1;
+    __syncthreads();
+    if (found) {
+        // keys of the cut tiles
+        const int from = max(w.t0 * BK, w.seen_min / BK * BK);
+#pragma unroll
+        for (int n = 0; n < NQ; n++)
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma nounroll
+                for (int k = from; k < min(w.t1 * BK, col[n].seen); k++)
+                    add_rest(o[d][n], vb + (int64_t)k * A.vs.t + 16 * d + 4 * g, A.D - 16 * d - 4 * g);
+    }
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const float sum = column_sum(l[n]);
@@ -443,6 +489,7 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dq_kernel(AttnArgs 
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NQ, WORDS = BK * L::CHUNKS;
     extern __shared__ uint4 lds[];
+    __shared__ int found;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const L tile_of;
     const QueryTile w = query_tile<COLS>(A);
@@ -484,26 +531,31 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dq_kernel(AttnArgs 
         for (int d2 = 0; d2 < DT; d2++) acc[d2][n] = f4{0, 0, 0, 0};
     }
 
+    if (threadIdx.x == 0) found = 0;
+    bool met = false;   // by this thread
     Stage<T, DP, BK, F> sk, sv;
     auto fetch = [&](int t, uint4* to) __attribute__((always_inline)) {
-        sk.fetch(to, kb + (int64_t)t * BK * A.ks.t, A.ks.t, w.len - t * BK, A.D);
-        sv.fetch(to + WORDS, vb + (int64_t)t * BK * A.vs.t, A.vs.t, w.len - t * BK, A.D);
+        sk.fetch(to, kb + (int64_t)t * BK * A.ks.t, A.ks.t, w.seen_max - t * BK, A.D);
+        sv.fetch(to + WORDS, vb + (int64_t)t * BK * A.vs.t, A.vs.t, w.seen_max - t * BK, A.D);
     };
-    auto put = [&](uint4* to) {
-        sk.put(to);
+    auto put = [&](int t, uint4* to, bool cuts) __attribute__((always_inline)) {
+        met |= sk.put(to, cuts && (t + 1) * BK > w.seen_min);
         sv.put(to + WORDS);
     };
     if (w.t0 < w.t1) {
 #pragma unroll
         for (int k = 0; k < 4; k++) sk.clear(lds + k * WORDS, A.D);
         fetch(w.t0, lds);
-        put(lds);
+        put(w.t0, lds, true);
     }
     __syncthreads();
-    auto step = [&](int t, const uint4* __restrict__ kt, uint4* __restrict__ next) __attribute__((always_inline)) {
+    auto step = [&](auto cuts, int t, const uint4* __restrict__ kt, uint4* __restrict__ next)
+                    __attribute__((always_inline)) {
+        constexpr bool CUTS = decltype(cuts)::value;
         const uint4* vt = kt + WORDS;
         const int k0 = t * BK;
-        if (t + 1 < w.t1) fetch(t + 1, next);
+        if (!CUTS || t + 1 < w.t1) fetch(t + 1, next);
+        const bool cut = CUTS && k0 + BK > w.seen_min;
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
             f4 s[2][NQ], dp[2][NQ];
@@ -525,18 +577,21 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dq_kernel(AttnArgs 
                     }
                 }
             }
-            if (k0 + BK > w.seen_min) {
+            if (cut) {
 #pragma unroll
                 for (int n = 0; n < NQ; n++)
 #pragma unroll
                     for (int u = 0; u < 2; u++)
 #pragma unroll
                         for (int r = 0; r < 4; r++)
-                            if (k0 + 32 * kk + 16 * u + 4 * g + r >= col[n].seen) s[u][n][r] = NEG_INF;
+                            if (k0 + 32 * kk + 16 * u + 4 * g + r >= col[n].seen) {
+                                s[u][n][r] = NEG_INF;
+                                dp[u][n][r] = 0.0f;
+                            }
             }
             Frag<T> ds[NQ];
 #pragma unroll
-            for (int n = 0; n < NQ; n++) {
+            for (int n = 0; n < NQ; n++)
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -544,8 +599,8 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dq_kernel(AttnArgs 
                         const float p = exp2_fast(__builtin_fmaf(s[u][n][r], A.c, -lse[n]));
                         s[u][n][r] = p * dp[u][n][r];
                     }
-                ds[n] = gs::frag_of_tiles<T>(s[0][n], s[1][n]);
-            }
+#pragma unroll
+            for (int n = 0; n < NQ; n++) ds[n] = gs::frag_of_tiles<T>(s[0][n], s[1][n]);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
                 const Frag<T> a = tile_of.cols(kt, 32 * kk, 16 * d);
@@ -553,11 +608,31 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dq_kernel(AttnArgs 
                 for (int n = 0; n < NQ; n++) acc[d][n] = gs::mma(a, ds[n], acc[d][n]);
             }
         }
-        if (t + 1 < w.t1) put(next);
+        if (!CUTS || t + 1 < w.t1) put(t + 1, next, CUTS);
         __syncthreads();
     };
-    for (int t = w.t0; t < w.t1; t++)
-        step(t, lds + ((t - w.t0) & 1) * 2 * WORDS, lds + ((t + 1 - w.t0) & 1) * 2 * WORDS);
+    // as in the forward, at every D (4096 keys of 64: 219 us, in one loop 230)
+    int t = w.t0;
+    for (const int whole = min(w.t1, w.seen_min / BK) - 1; t < whole; t++)
+        step(std::false_type{}, t, lds + ((t - w.t0) & 1) * 2 * WORDS, lds + ((t + 1 - w.t0) & 1) * 2 * WORDS);
+    for (; t < w.t1; t++)
+        step(std::true_type{}, t, lds + ((t - w.t0) & 1) * 2 * WORDS, lds + ((t + 1 - w.t0) & 1) * 2 * WORDS);
+    if (met) found = 1;
+    __syncthreads();
+    if (found) {
+        // a query that sees a key that is not finite has no gradient that is
+        const int from = max(w.t0 * BK, w.seen_min / BK * BK);
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            float x = 0.0f;
+#pragma nounroll
+            for (int k = from; k < min(w.t1 * BK, col[n].seen); k++)
+#pragma nounroll
+                for (int d = 0; d < A.D; d++) x += 0.0f * (float)kb[(int64_t)k * A.ks.t + d];
+#pragma unroll
+            for (int d = 0; d < DT; d++) acc[d][n] += x;
+        }
+    }
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         if (!col[n].valid) continue;
@@ -584,12 +659,14 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
     using L = Tile<T, DP>;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NK, WORDS = QT * L::CHUNKS, BUF = 2 * WORDS + QT / 2;
     extern __shared__ uint4 lds[];   // [2][q tile, do tile, lse[QT], -delta[QT]]
+    __shared__ int found;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const L tile_of;
     const Share share = share_of(A, A.B * A.Hkv);
     const int split = share.split, tile = share.tile, bh = share.bh;   // causal: the first keys are seen most
-    const int b = bh / A.Hkv, hk = bh % A.Hkv, len = length_of(A, b), key0 = tile * COLS;
+    const int b = bh / A.Hkv, hk = bh % A.Hkv, key0 = tile * COLS;
     const int64_t start = start_of(A, b);
+    const int len = seen_of(A, length_of(A, b), start, A.Tq - 1);   // keys that the last query sees
 
     Frag<T> k[NK][KC], v[NK][KC];
     f4 dk[DT][NK], dv[DT][NK];
@@ -617,6 +694,8 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
     const int per_head = tiles - from, total = per_head * A.G, per = (total + A.splits - 1) / A.splits;
     const int e0 = min(total, split * per), e1 = min(total, e0 + per);
 
+    if (threadIdx.x == 0) found = 0;
+    bool met = false;   // by this thread
     Stage<T, DP, QT, F> sq, sg;
     // threads 0 .. QT - 1: lse, QT .. 2 QT - 1: delta, as loaded; put() finishes them,
     // so that nothing waits for them, and the tiles' loads before them, until then
@@ -634,9 +713,10 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
             stat = *((is_lse ? A.lse : A.delta) + row);
         }
     };
-    auto put = [&](uint4* to) {
-        sq.put(to);
-        sg.put(to + WORDS);
+    auto put = [&](int e, uint4* to) __attribute__((always_inline)) {
+        const bool part = A.causal && start + (from + e % per_head) * QT < (int64_t)key0 + COLS - 1;
+        met |= sq.put(to, part);
+        met |= sg.put(to + WORDS, part);
         if (threadIdx.x < 2 * QT)
             ((float*)(to + 2 * WORDS))[threadIdx.x] = is_lse ? (real ? stat : -NEG_INF) : real ? -stat : 0.0f;
     };
@@ -644,7 +724,7 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
 #pragma unroll
         for (int k = 0; k < 4; k++) sq.clear(lds + k / 2 * BUF + k % 2 * WORDS, A.D);
         fetch(e0, lds);
-        put(lds);
+        put(e0, lds);
     }
     __syncthreads();
     auto step = [&](int e, const uint4* __restrict__ qt, uint4* __restrict__ next) __attribute__((always_inline)) {
@@ -677,15 +757,6 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
                     }
                 }
             }
-            if (part) {
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int n = 0; n < NK; n++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            if (32 * kk + 16 * u + 4 * g + r < sees + key[n] - key0) s[u][n][r] = NEG_INF;
-            }
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int r0 = 32 * kk + 16 * u + 4 * g;
@@ -698,6 +769,15 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
                         s[u][n][r] = p;
                         dp[u][n][r] = p * dp[u][n][r];
                     }
+            }
+            if (part) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int n = 0; n < NK; n++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (32 * kk + 16 * u + 4 * g + r < sees + key[n] - key0) s[u][n][r] = dp[u][n][r] = 0.0f;
             }
             Frag<T> fp[NK], fs[NK];
 #pragma unroll
@@ -715,10 +795,29 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
                 }
             }
         }
-        if (e + 1 < e1) put(next);
+        if (e + 1 < e1) put(e + 1, next);
         __syncthreads();
     };
     for (int e = e0; e < e1; e++) step(e, lds + ((e - e0) & 1) * BUF, lds + ((e + 1 - e0) & 1) * BUF);
+    if (met) found = 1;
+    __syncthreads();
+    if (found) {
+        // dv; to dk such a query's delta or lse has brought it already
+#pragma unroll
+        for (int n = 0; n < NK; n++)
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma nounroll
+                for (int e = e0; e < e1; e++) {
+                    const int h = hk * A.G + e / per_head, q0 = (from + e % per_head) * QT;
+                    if (start + q0 >= (int64_t)key0 + COLS - 1) continue;   // not cut
+                    const int64_t first_row = (int64_t)key[n] - start;
+#pragma nounroll
+                    for (int r = (int)max((int64_t)q0, first_row); r < min(A.Tq, q0 + QT); r++)
+                        add_rest(dv[d][n], (const T*)A.dout + b * A.dos.b + h * A.dos.h + (int64_t)r * A.dos.t + 16 * d +
+                                               4 * g, A.D - 16 * d - 4 * g);
+                }
+    }
 #pragma unroll
     for (int n = 0; n < NK; n++) {
         if (key[n] >= A.Tk) continue;
@@ -1063,7 +1162,7 @@ extern "C" int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, i
         A.out0 = dq;
         A.s0 = strides_of(dq_strides);
         A.splits = p.splits_q;
-            A.part = A.splits > 1 ? part : nullptr;
+        A.part = A.splits > 1 ? part : nullptr;
         if (int rc = run<DQ>(type, A, p.nq, stream)) return rc;
         if (A.splits > 1) {
             add_all(1, Hq, Tq);

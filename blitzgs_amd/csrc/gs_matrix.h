@@ -238,15 +238,60 @@ struct Stage {
             if ((Tile<T, DP>::chunk(row, id % CHUNKS) - row * CHUNKS) * V >= D) t[id] = make_uint4(0, 0, 0, 0);
         }
     }
-    // Ends it; a barrier comes before the tile is read.
-    __device__ __forceinline__ void put(uint4* t) const
+    // Ends it; a barrier comes before the tile is read.  With `scrub`, infinities and
+    // NaN become zero; whether this thread met one.
+    __device__ __forceinline__ bool put(uint4* t, bool scrub = false)
     {
-        if constexpr (F == DIRECT) return;
+        bool found = false;
+        if constexpr (F == DIRECT) {
+            if (!scrub) return false;
+            // a thread looks at what its own loads bring, once they are there
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < CPT; k++) {
+                Vec<T> x = __builtin_bit_cast(Vec<T>, t[threadIdx.x + 256 * k]);
+                if (finite(x)) continue;
+                found = true;
+                t[threadIdx.x + 256 * k] = __builtin_bit_cast(uint4, scrubbed(x));
+            }
+            return found;
+        }
 #pragma unroll
         for (int k = 0; k < CPT; k++) {
             const int id = threadIdx.x + 256 * k;
+            if (scrub && !finite(r[k])) {
+                found = true;
+                r[k] = scrubbed(r[k]);
+            }
             t[Tile<T, DP>::chunk(id / CHUNKS, id % CHUNKS)] = __builtin_bit_cast(uint4, r[k]);
         }
+        return found;
+    }
+
+private:
+    static constexpr uint32_t EXPONENT = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, bf16) ? 0x7f80u : 0x7c00u;
+
+    __device__ __forceinline__ static bool finite(const Vec<T>& x)
+    {
+        typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+        const uint4 w = __builtin_bit_cast(uint4, x);
+        if constexpr (sizeof(T) == 4) {
+            constexpr uint32_t M = 0x7fffffffu;
+            return max(max(w.x & M, w.y & M), max(w.z & M, w.w & M)) < EXPONENT;
+        } else {
+            constexpr uint32_t M = 0x7fff7fffu;
+            auto larger = [](us2 a, us2 b) { return __builtin_elementwise_max(a, b); };
+            const us2 top = larger(larger(__builtin_bit_cast(us2, w.x & M), __builtin_bit_cast(us2, w.y & M)),
+                                   larger(__builtin_bit_cast(us2, w.z & M), __builtin_bit_cast(us2, w.w & M)));
+            return max(top[0], top[1]) < EXPONENT;
+        }
+    }
+    __device__ __forceinline__ static Vec<T> scrubbed(Vec<T> x)
+    {
+#pragma unroll
+        for (int e = 0; e < V; e++)
+            if (!(__builtin_fabsf((float)x.v[e]) < __builtin_inff())) x.v[e] = (T)0.0f;
+        return x;
     }
 };
 

@@ -675,9 +675,10 @@ int gs_layer_norm_backward(int type, int param_type, int64_t rows, int width, co
  * elements, of its batch, head and token dimension; D is contiguous.
  *   Query i of batch b sees key j when j < key_lengths[b] (device int32 (B),
  * clamped to [0, Tk]; NULL: Tk) and, if causal, j <= i + query_start[b]
- * (device int32 (B); NULL: Tk - Tq).  Keys from key_lengths on are not read; a
- * row that sees no key gives zeros.  Among the keys below the length, values
- * that a row does not see must be finite.
+ * (device int32 (B); NULL: Tk - Tq).  Keys that no query sees, those from
+ * key_lengths on among them, are not read; a row that sees no key gives zeros.  A
+ * NaN or an infinity reaches only the queries that see its key and, in the
+ * backward, the keys that its query sees.
  *   lse (B, Hq, Tq) fp32, may be NULL: the base-2 logarithm of each row's sum of
  * exponentials (+inf for a row that sees no key), which the backward takes.
  *   o_rest, with o's strides and type, may be NULL: o's value before its
@@ -685,8 +686,8 @@ int gs_layer_norm_backward(int type, int param_type, int64_t rows, int width, co
  * GS_F32 there is nothing to keep.
  *   The backward writes dq, and dk and dv unless both are NULL.
  *   The workspace's size (gs_attention_workspace_bytes; 0: none is needed, or
- * the arguments are invalid) depends on the sizes and on `unequal`: whether the call is causal or is given
- * key_lengths.  Results do not depend on the order of execution. */
+ * the arguments are invalid) depends on the sizes and on `unequal`: whether the
+ * call is causal or is given key_lengths.  Results do not depend on the order of execution. */
 size_t gs_attention_workspace_bytes(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D,
                                     int unequal, int backward);
 int gs_attention_forward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, const void* q,

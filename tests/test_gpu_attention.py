@@ -269,3 +269,97 @@ def test_refusals(gpu):
     wide = torch.zeros((1, 1, 2, 129), device="cuda")
     with pytest.raises(RuntimeError, match="head dimension"):
         attention(wide, wide, wide)
+
+
+# What a NaN or an infinity in one token reaches: the queries that see the key, and
+# the keys that the query sees.  Everything else is what it is without, to the bit
+# where no row's scores change, else (the running base moves for several rows
+# together) within the bound.
+SPOILED = [float("nan"), float("inf"), float("-inf")]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("Tq,D", [(1, 64), (1, 128), (5, 40), (70, 64), (3, 33)])
+def test_the_unused_end_of_a_cache_is_not_read(gpu, t, Tq, D):
+    B, Tk = 3, 300
+    q, k, v, do = _inputs(t, B, 4, 2, Tq, Tk, D)
+    start = _int(0, 17, 200)
+    how = dict(causal=True, query_start=start)
+    for b in range(B):
+        k[b, :, int(start[b]) + Tq:] = 0
+        v[b, :, int(start[b]) + Tq:] = 0
+    clean = _run(q, k, v, do, **how)
+    for spoil in SPOILED:
+        for b in range(B):
+            k[b, :, int(start[b]) + Tq:] = spoil
+            v[b, :, int(start[b]) + Tq:] = spoil
+        got = _run(q, k, v, do, **how)
+        for name in got:
+            assert torch.equal(got[name], clean[name]), (name, spoil)
+        assert torch.equal(_run(q, k, v, **how)["o"], clean["o"])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T,D", [(40, 32), (200, 64), (130, 128), (100, 80), (70, 31)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_what_a_later_key_holds_does_not_reach_earlier_queries(gpu, t, T, D, which):
+    at = T // 2 + 3
+    q, k, v, do = _inputs(t, 1, 4, 2, T, T, D)
+    clean = _run(q, k, v, causal=True)["o"]
+    want = attention_64(q, k, v, True, None, None, 1.0 / math.sqrt(D), do)
+    for spoil in SPOILED:
+        x = dict(k=k.clone(), v=v.clone())
+        x[which][0, 1, at, D // 2] = spoil
+        got = _run(q, x["k"], x["v"], do, causal=True)
+        for name in ("o", "dq"):
+            within(got[name][:, :2], *(w[:, :2] for w in want[name]), f"{spoil}: {name} of the other key head's queries")
+            within(got[name][:, :, :at], *(w[:, :, :at] for w in want[name]), f"{spoil}: {name} of earlier queries")
+        for name in ("dk", "dv"):
+            within(got[name][:, :1], *(w[:, :1] for w in want[name]), f"{spoil}: {name} of the other key head")
+        o = got["o"]
+        if which == "v":
+            assert torch.equal(o[:, :, :at], clean[:, :, :at])
+            rest = [d for d in range(D) if d != D // 2]
+            assert torch.equal(o[..., rest], clean[..., rest])
+            column = o[:, 2:, at:, D // 2].float()
+            assert torch.isnan(column).all() if math.isnan(spoil) else (column == spoil).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T,D", [(40, 32), (200, 64), (130, 128), (70, 31)])
+@pytest.mark.parametrize("which", ["q", "do"])
+def test_what_an_earlier_query_holds_does_not_reach_later_keys(gpu, t, T, D, which):
+    at = T // 2 - 5
+    q, k, v, do = _inputs(t, 1, 4, 2, T, T, D)
+    want = attention_64(q, k, v, True, None, None, 1.0 / math.sqrt(D), do)
+    for spoil in SPOILED:
+        x = dict(q=q.clone(), do=do.clone())
+        x[which][0, 3, at] = spoil
+        got = _run(x["q"], k, v, x["do"], causal=True)
+        others = [i for i in range(T) if i != at]
+        within(got["dq"][:, :, others], *(w[:, :, others] for w in want["dq"]), f"{spoil}: dq")
+        for name in ("dk", "dv"):
+            within(got[name][:, :1], *(w[:, :1] for w in want[name]), f"{spoil}: {name} of the other key head")
+            within(got[name][:, :, at + 1:], *(w[:, :, at + 1:] for w in want[name]), f"{spoil}: {name}, later keys")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("D", [31, 64, 128])
+def test_what_rows_that_see_nothing_hold_reaches_nothing(gpu, t, D):
+    q, k, v, do = _inputs(t, 2, 4, 2, 50, 90, D)
+    how = dict(causal=True, query_start=_int(-20, -50))             # 20 empty rows, 50 empty rows
+    q[0, :, :20] = 0
+    do[0, :, :20] = 0
+    q[1] = 0
+    do[1] = 0
+    clean = _run(q, k, v, do, **how)
+    for spoil in SPOILED:
+        q[0, :, :20] = spoil
+        do[0, :, :20] = spoil
+        q[1] = spoil
+        do[1] = spoil
+        got = _run(q, k, v, do, **how)
+        for name in got:
+            assert torch.equal(got[name], clean[name]), (name, spoil)
+        assert not got["o"][0, :, :20].any() and not got["dq"][0, :, :20].any()
+        assert not any(got[name][1].any() for name in got)
