@@ -57,8 +57,9 @@ class OrthogonalMomentum(torch.optim.Optimizer):
         m = momentum m + g,   u = g + momentum m (nesterov) or m
         p = (1 - lr weight_decay) p - lr sqrt(max(1, rows / columns)) orthogonalise(u)
 
-    The state is one fp32 tensor per parameter, 'momentum_buffer'.  Parameters
-    of one shape and type in a group go through the device together."""
+    The state is one fp32 tensor per parameter, 'momentum_buffer', in a saved
+    state too.  Parameters of one shape and type in a group go through the device
+    together."""
 
     def __init__(self, params, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
         if not lr >= 0.0 or not 0.0 <= momentum < 1.0 or not weight_decay >= 0.0:
@@ -68,6 +69,39 @@ class OrthogonalMomentum(torch.optim.Optimizer):
             raise ValueError(f"steps must be an integer from 1 to 32, got {steps!r}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       steps=steps))
+
+    def load_state_dict(self, state_dict):
+        # torch's loading casts a state to its parameter's type, so the buffers are
+        # taken once more from what it loads: after all hooks that may change that,
+        # and before any that look at the result
+        loaded = {}
+
+        def restore(_):
+            ours = (p for group in self.param_groups for p in group["params"])
+            for key, p in zip((k for group in loaded["param_groups"] for k in group["params"]), ours):
+                buffer = loaded["state"].get(key, {}).get("momentum_buffer")
+                if isinstance(buffer, torch.Tensor):
+                    buffer = buffer.detach().to(p.device, torch.float32, copy=True)
+                    self.state[p]["momentum_buffer"] = buffer.contiguous()
+
+        hooks = [self.register_load_state_dict_pre_hook(lambda _, state: loaded.update(state)),
+                 self.register_load_state_dict_post_hook(restore, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _buffer(self, p):
+        state = self.state[p]
+        if "momentum_buffer" not in state:
+            state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
+        m = state["momentum_buffer"]
+        if (not isinstance(m, torch.Tensor) or m.dtype != torch.float32 or m.shape != p.shape or m.device != p.device
+                or not m.is_contiguous()):
+            raise RuntimeError(f"momentum_buffer must be a contiguous float32 tensor of shape {tuple(p.shape)} on "
+                               f"{p.device}")
+        return m
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -85,26 +119,21 @@ class OrthogonalMomentum(torch.optim.Optimizer):
                     raise RuntimeError(f"OrthogonalMomentum takes matrices, got shape {tuple(p.shape)}")
                 if not p.is_contiguous() or p.grad.dtype != p.dtype or p.grad.is_sparse:
                     raise RuntimeError("parameters must be contiguous, with dense gradients of their type")
-                alike.setdefault((p.device, p.dtype, tuple(p.shape)), []).append(p)
-            for (device, dtype, shape), params in alike.items():
-                for i in range(0, len(params), _MAX_PER_CALL):
+                alike.setdefault((p.device, p.dtype, tuple(p.shape)), []).append((p, self._buffer(p)))
+            for (device, dtype, shape), pairs in alike.items():
+                for i in range(0, len(pairs), _MAX_PER_CALL):
                     with _t.on_device(device):
-                        self._update(group, params[i:i + _MAX_PER_CALL], device, dtype, shape)
+                        self._update(group, *zip(*pairs[i:i + _MAX_PER_CALL]), device, dtype, shape)
         return loss
 
-    def _update(self, group, params, device, dtype, shape):
+    def _update(self, group, params, momenta, device, dtype, shape):
         lib, code, n = _t.load(), _t.DTYPE_CODES[dtype], len(params)
         stream, size = _t.stream(device), shape[0] * shape[1]
-        for p in params:
-            if "momentum_buffer" not in self.state[p]:
-                self.state[p]["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
         grads = [p.grad.contiguous() for p in params]
         pointers = lambda ts: (C.c_void_p * n)(*(t.data_ptr() for t in ts))  # noqa: E731
         update = torch.empty((n, *shape), device=device, dtype=torch.float32)
-        _t.check(lib.gs_momentum_update(code, n, size, pointers(grads),
-                                          pointers([self.state[p]["momentum_buffer"] for p in params]),
-                                          group["momentum"], int(group["nesterov"]), _t.ptr(update), stream),
-                   "gs_momentum_update")
+        _t.check(lib.gs_momentum_update(code, n, size, pointers(grads), pointers(momenta), group["momentum"],
+                                          int(group["nesterov"]), _t.ptr(update), stream), "gs_momentum_update")
         update = _orthogonalise(update, group["steps"])
         scale = max(1.0, shape[0] / shape[1]) ** 0.5
         _t.check(lib.gs_momentum_apply(code, n, size, pointers(params), 1.0 - group["lr"] * group["weight_decay"],
