@@ -3,6 +3,7 @@ tensor arguments, streams and workspaces."""
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -47,7 +48,13 @@ def workspace(nbytes, device):
 
 
 def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call has to go through its autograd function: a backward may follow, or
+    a tensor has a forward-mode tangent, which that function refuses."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    # -1 outside all dual levels, where no tensor has a tangent
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 check = _lib.check
