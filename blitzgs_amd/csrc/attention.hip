@@ -236,6 +236,46 @@ __device__ __forceinline__ void add_rest(f4& x, const T* p, int n)
     }
 }
 
+// dS as an operand in float16.  It is as large as the gradients of o over the number of
+// keys, and as the products of those with v, so both ends of float16's range are within
+// reach: gradients of 1e-3 over 4096 keys left dq and dk with an error of 5.3e-3, of 1e4
+// over 64 made them infinite.  So a column's dS is multiplied by a power of two, `up`,
+// and its sum divided by it at the end.  As with the softmax's base, `up` falls when the
+// column's largest dS so far asks for it: that keeps the largest between 2^7 and 2^15,
+// and all of float16's bits in what is at least 2^-21 of it.  The error above becomes
+// 6.9e-4, of which dq's own rounding is 6.6e-4; dq, dk and dv take 4 to 8 % longer in
+// float16 (4096 x 4096, D 64: 214 -> 232 and 314 -> 335 us).
+template <typename T>
+constexpr bool FITS = __is_same(T, gs::f16);
+constexpr float UP = 0x1p60f;      // of columns that have met no dS yet
+constexpr float UP_MOST = 0x1p15f; // of dS up
+
+template <int U, int N, int DT>
+__device__ __forceinline__ void fit(f4 (&ds)[U][N], f4 (&acc)[DT][N], float (&up)[N])
+{
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        float top = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) top = fmaxf(top, fabsf(ds[u][n][r]));
+        if (__any(top * up[n] >= UP_MOST)) {
+            top = column_max(top);
+            // in powers of two: top up comes to between 2^7 and 2^8
+            int to = 8 - __builtin_amdgcn_frexp_expf(top);
+            const int from = __builtin_amdgcn_frexp_expf(up[n]) - 1;
+            to = top * up[n] >= UP_MOST ? min(to, from) : from;
+            up[n] = __builtin_ldexpf(1.0f, to);
+            const float shrink = __builtin_ldexpf(1.0f, to - from);
+#pragma unroll
+            for (int d = 0; d < DT; d++) acc[d][n] *= shrink;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) ds[u][n] *= up[n];
+    }
+}
+
 // The tile that is read and the one that is being loaded come to a step as two
 // restricted pointers: only so does the compiler know that the loads need not
 // have arrived before the reads.
@@ -498,10 +538,11 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dq_kernel(AttnArgs 
 
     Column col[NQ];
     Frag<T> q[NQ][KC], go[NQ][KC];
-    float lse[NQ], delta[NQ];
+    float lse[NQ], delta[NQ], up[NQ];
     f4 acc[DT][NQ];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
+        up[n] = FITS<T> ? UP : 1.0f;
         col[n] = column(A, w, w.tile * COLS + (wave * NQ + n) * 16 + i);
         const T* p = (const T*)A.q + w.b * A.qs.b + col[n].h * A.qs.h + col[n].i * A.qs.t;
         const T* pg = (const T*)A.dout + w.b * A.dos.b + col[n].h * A.dos.h + col[n].i * A.dos.t;
@@ -599,6 +640,7 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dq_kernel(AttnArgs 
                         const float p = exp2_fast(__builtin_fmaf(s[u][n][r], A.c, -lse[n]));
                         s[u][n][r] = p * dp[u][n][r];
                     }
+            if constexpr (FITS<T>) fit(s, acc, up);
 #pragma unroll
             for (int n = 0; n < NQ; n++) ds[n] = gs::frag_of_tiles<T>(s[0][n], s[1][n]);
 #pragma unroll
@@ -636,17 +678,18 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dq_kernel(AttnArgs 
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         if (!col[n].valid) continue;
+        const float scale = A.scale / up[n];
         if (A.part != nullptr) {
             const int64_t rows = (int64_t)A.B * A.Hkv * A.G * A.Tq;
             float* p = A.part + (w.split * rows + (int64_t)w.bh * A.G * A.Tq + col[n].r) * A.D;
 #pragma unroll
             for (int d = 0; d < DT; d++)
-                store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+                store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * scale, A.D - 16 * d - 4 * g);
         } else {
             T* p = (T*)A.out0 + w.b * A.s0.b + col[n].h * A.s0.h + col[n].i * A.s0.t;
 #pragma unroll
             for (int d = 0; d < DT; d++)
-                store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * A.scale, A.D - 16 * d - 4 * g);
+                store4<F == gs::ODD>(p + 16 * d + 4 * g, acc[d][n] * scale, A.D - 16 * d - 4 * g);
         }
     }
 }
@@ -670,9 +713,11 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
 
     Frag<T> k[NK][KC], v[NK][KC];
     f4 dk[DT][NK], dv[DT][NK];
+    float up[NK];
     int key[NK];
 #pragma unroll
     for (int n = 0; n < NK; n++) {
+        up[n] = FITS<T> ? UP : 1.0f;
         key[n] = key0 + (wave * NK + n) * 16 + i;
         const bool held = key[n] < len;
         const T* pk = (const T*)A.k + b * A.ks.b + hk * A.ks.h + (int64_t)(held ? key[n] : 0) * A.ks.t;
@@ -779,6 +824,7 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
                         for (int r = 0; r < 4; r++)
                             if (32 * kk + 16 * u + 4 * g + r < sees + key[n] - key0) s[u][n][r] = dp[u][n][r] = 0.0f;
             }
+            if constexpr (FITS<T>) fit(dp, dk, up);
             Frag<T> fp[NK], fs[NK];
 #pragma unroll
             for (int n = 0; n < NK; n++) {
@@ -822,10 +868,11 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
     for (int n = 0; n < NK; n++) {
         if (key[n] >= A.Tk) continue;
         const bool held = key[n] < len;
+        const float scale = A.scale / up[n];
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             const int at = 16 * d + 4 * g, left = A.D - at;
-            const f4 xk = held ? dk[d][n] * A.scale : f4{0, 0, 0, 0}, xv = held ? dv[d][n] : f4{0, 0, 0, 0};
+            const f4 xk = held ? dk[d][n] * scale : f4{0, 0, 0, 0}, xv = held ? dv[d][n] : f4{0, 0, 0, 0};
             if (A.part != nullptr) {
                 const int64_t rows = (int64_t)A.B * A.Hkv * A.Tk, row = (int64_t)bh * A.Tk + key[n];
                 store4<F == gs::ODD>(A.part + (2 * split * rows + row) * A.D + at, xk, left);
