@@ -276,6 +276,11 @@ __device__ __forceinline__ void fit(f4 (&ds)[U][N], f4 (&acc)[DT][N], float (&up
     }
 }
 
+// P as an operand of dv in float16: about 1 over the number of keys, and float16 has fewer
+// bits below 2^-14 (a probability of 2^-20 was off by up to 3 %).  The lse that dk, dv
+// takes is smaller by P_UP: its P comes to at most 2^10, with all bits from 2^-24 on.
+constexpr float P_UP = 10.0f, P_BACK = 0x1p-10f;
+
 // The tile that is read and the one that is being loaded come to a step as two
 // restricted pointers: only so does the compiler know that the loads need not
 // have arrived before the reads.
@@ -700,6 +705,7 @@ template <typename T, int DP, int NK, int QT, Fill F>
 __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs A)
 {
     using L = Tile<T, DP>;
+    constexpr float p_up = FITS<T> ? P_UP : 0.0f, p_back = FITS<T> ? P_BACK : 1.0f;
     constexpr int KC = DP / 32, DT = DP / 16, COLS = 64 * NK, WORDS = QT * L::CHUNKS, BUF = 2 * WORDS + QT / 2;
     extern __shared__ uint4 lds[];   // [2][q tile, do tile, lse[QT], -delta[QT]]
     __shared__ int found;
@@ -763,7 +769,7 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
         met |= sq.put(to, part);
         met |= sg.put(to + WORDS, part);
         if (threadIdx.x < 2 * QT)
-            ((float*)(to + 2 * WORDS))[threadIdx.x] = is_lse ? (real ? stat : -NEG_INF) : real ? -stat : 0.0f;
+            ((float*)(to + 2 * WORDS))[threadIdx.x] = is_lse ? (real ? stat - p_up : -NEG_INF) : real ? -stat : 0.0f;
     };
     if (e0 < e1) {
 #pragma unroll
@@ -868,11 +874,11 @@ __global__ __launch_bounds__(256, (PER_CU<T, DP>)) void attn_dkv_kernel(AttnArgs
     for (int n = 0; n < NK; n++) {
         if (key[n] >= A.Tk) continue;
         const bool held = key[n] < len;
-        const float scale = A.scale / up[n];
+        const float scale = A.scale / up[n] * p_back;
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             const int at = 16 * d + 4 * g, left = A.D - at;
-            const f4 xk = held ? dk[d][n] * scale : f4{0, 0, 0, 0}, xv = held ? dv[d][n] : f4{0, 0, 0, 0};
+            const f4 xk = held ? dk[d][n] * scale : f4{0, 0, 0, 0}, xv = held ? dv[d][n] * p_back : f4{0, 0, 0, 0};
             if (A.part != nullptr) {
                 const int64_t rows = (int64_t)A.B * A.Hkv * A.Tk, row = (int64_t)bh * A.Tk + key[n];
                 store4<F == gs::ODD>(A.part + (2 * split * rows + row) * A.D + at, xk, left);

@@ -109,3 +109,17 @@ def test_a_gradient_that_is_not_finite_stays_in_its_row(gpu):
         for g, c in zip(got[1:], clean[1:]):
             assert torch.equal(g[:, 0], c[:, 0]) and torch.equal(g[:, 1, 78:], c[:, 1, 78:])
             assert not torch.isfinite(g[0, 1, :78, 5]).any()
+
+
+@pytest.mark.parametrize("D", [32, 128, 33])
+def test_values_of_small_probability(gpu, D):
+    # one key takes nearly all of each row, the others some 2^-20 of it: dv of these
+    # is P^T do all the same.  The bound less what it grants P in float16's steps.
+    Tq, Tk = 1, 40
+    q, k = _rand((1, 2, Tq, D), 1), _rand((1, 2, Tk, D), 2, 0.1)
+    k[:, :, 0] = (q[:, :, 0].float() * 14.0 * math.sqrt(D) / q[:, :, 0].float().square().sum(-1, keepdim=True)).to(T)
+    v, do = _rand((1, 2, Tk, D), 3), _away_from_zero(_rand((1, 2, Tq, D), 4, 2.0 ** 11), 500.0)
+    value, bound = attention_64(q, k, v, False, None, None, 1 / math.sqrt(D), do)["dv"]
+    bound = bound - 1.01 * STEP[T] * do.double().abs().sum(2, keepdim=True).cpu()
+    assert (bound > 0).all() and (value[:, :, 1:].abs() < 2e-2).all() and (value.abs() > 6.2e-5).all()
+    _within(_grads(q, k, v, do)[2], value, bound, "dv")
