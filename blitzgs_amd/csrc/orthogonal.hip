@@ -49,7 +49,7 @@ constexpr float NORM_FLOOR = 1e-7f;
 constexpr float SX = 16384.0f, SA = 8192.0f;
 constexpr int PAD = 64;         // planes are padded to whole tiles of the smaller kind
 constexpr int KT = 32;          // depth of a staged tile
-constexpr int NORM_PARTS = 64;  // partial sums of squares per matrix
+constexpr int NORM_PARTS = 64;  // parts of a matrix's sum of squares
 
 // A matrix in two planes: hi at p, lo `plane` elements on.
 struct Planes {
@@ -85,13 +85,25 @@ __device__ __forceinline__ void split(float x, f16& hi, f16& lo)
     lo = (f16)(x - (float)hi);
 }
 
-// What takes G to the planes of X at the start, and -log2 |X| there.
-__device__ __forceinline__ float start_scale(float norm, float& small)
+// The squares of elements beyond 2^48 (2^32 elements) to 2^64 (one) pass fp32's range, those
+// of SHRINK times them never do.  Where the plain sum does, the matrix is taken times
+// SHRINK; what of that falls below fp32's range is less than 2^-60 of the sum.
+constexpr float SHRINK = 0x1p-90f;
+
+// What takes G to the planes of X at the start: (G pre) scale, and -log2 |X| there.
+struct Start {
+    float pre, scale, small;
+};
+
+// sum, shrunk: of the squares of G's elements, and of SHRINK times them, which is
+// looked at only where sum is infinite
+__device__ __forceinline__ Start start_of(float sum, float shrunk)
 {
-    const float len = norm / (norm + NORM_FLOOR);
+    if (sum == __builtin_inff()) return {SHRINK, SX / __builtin_sqrtf(shrunk), 0.0f};
+    const float norm = __builtin_sqrtf(sum), len = norm / (norm + NORM_FLOOR);
     // squares that underflow: the norm is unknown but below 2^-60
-    small = len > 0.0f ? fminf(-__builtin_log2f(len), 40.0f) : norm == 0.0f ? 20.0f : 0.0f;
-    return __builtin_ldexpf(SX, extra_scale(small, 0)) / (norm + NORM_FLOOR);
+    const float small = len > 0.0f ? fminf(-__builtin_log2f(len), 40.0f) : norm == 0.0f ? 20.0f : 0.0f;
+    return {1.0f, __builtin_ldexpf(SX, extra_scale(small, 0)) / (norm + NORM_FLOOR), small};
 }
 
 // c[v] + a b[v] for operands in two planes; lo lo is below the planes' last bit.
@@ -111,6 +123,8 @@ __device__ __forceinline__ void three(const Frag<f16>& ah, const Frag<f16>& al, 
 
 // ------------------------------------------------------------- the normalised X
 
+// A workgroup's sum over a part of one matrix, in both units: parts holds NORM_PARTS of
+// the one and then of the other for each matrix.
 template <typename T>
 __global__ __launch_bounds__(256) void orth_norm_kernel(const T* __restrict__ g, int64_t size,
                                                         float* __restrict__ parts)
@@ -120,23 +134,37 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(const T* __restrict__ g,
     constexpr int V = gs::Vec<T>::N;
     const int64_t per = ((size + NORM_PARTS - 1) / NORM_PARTS + V - 1) / V * V;
     const int64_t from = per * blockIdx.x, to = from + per < size ? from + per : size;
-    float s = 0.0f;
     const int64_t whole = to - (to - from) % V;
+    auto sum = [&](float pre) __attribute__((always_inline)) {
+        float s = 0.0f;
 #pragma unroll 4
-    for (int64_t i = from + (int64_t)threadIdx.x * V; i < whole; i += 256 * V) {
-        const gs::Vec<T> t = gs::load_vec(p + i);
+        for (int64_t i = from + (int64_t)threadIdx.x * V; i < whole; i += 256 * V) {
+            const gs::Vec<T> t = gs::load_vec(p + i);
 #pragma unroll
-        for (int k = 0; k < V; k++) s = __builtin_fmaf((float)t.v[k], (float)t.v[k], s);
-    }
-    if (from < to && whole + threadIdx.x < to) {
-        const float t = (float)p[whole + threadIdx.x];
-        s = __builtin_fmaf(t, t, s);
-    }
+            for (int k = 0; k < V; k++) {
+                const float x = (float)t.v[k] * pre;
+                s = __builtin_fmaf(x, x, s);
+            }
+        }
+        if (from < to && whole + threadIdx.x < to) {
+            const float x = (float)p[whole + threadIdx.x] * pre;
+            s = __builtin_fmaf(x, x, s);
+        }
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) parts[blockIdx.y * NORM_PARTS + blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
+        if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        __syncthreads();
+        return s;
+    };
+    const float s = sum(1.0f);
+    const float shrunk = s == __builtin_inff() ? sum(SHRINK) : s * SHRINK * SHRINK;
+    if (threadIdx.x == 0) {
+        float* to_parts = parts + blockIdx.y * 2 * NORM_PARTS + blockIdx.x;
+        to_parts[0] = s;
+        to_parts[NORM_PARTS] = shrunk;
+    }
 }
 
 // One 64 x 64 tile of X, from G or its transpose, padded with zeros.
@@ -147,17 +175,20 @@ __global__ __launch_bounds__(256) void orth_split_kernel(const T* __restrict__ g
 {
     __shared__ float tile[64][65];
     const T* p = g + (int64_t)blockIdx.z * rows * cols;
-    float s = 0.0f;
-    for (int k = 0; k < NORM_PARTS; k++) s += parts[blockIdx.z * NORM_PARTS + k];
-    float sm;
-    const float scale = start_scale(__builtin_sqrtf(s), sm);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) small[blockIdx.z] = sm;
+    const float* sums = parts + blockIdx.z * 2 * NORM_PARTS;
+    float s = 0.0f, shrunk = 0.0f;
+    for (int k = 0; k < NORM_PARTS; k++) s += sums[k];
+    if (s == __builtin_inff())
+        for (int k = 0; k < NORM_PARTS; k++) shrunk += sums[NORM_PARTS + k];
+    const Start start = start_of(s, shrunk);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) small[blockIdx.z] = start.small;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int y0 = blockIdx.y * 64, x0 = blockIdx.x * 64;   // of the tile in X
     const int gy = tall ? x0 : y0, gx = tall ? y0 : x0;     // in G
     for (int k = wave; k < 64; k += 4)
         tile[k][lane] =
-            gy + k < rows && gx + lane < cols ? (float)p[(int64_t)(gy + k) * cols + gx + lane] * scale : 0.0f;
+            gy + k < rows && gx + lane < cols
+                ? (float)p[(int64_t)(gy + k) * cols + gx + lane] * start.pre * start.scale : 0.0f;
     __syncthreads();
     f16* out = x.p + blockIdx.z * x.stride;
     for (int k = wave; k < 64; k += 4) {
@@ -496,20 +527,32 @@ __global__ __launch_bounds__(SMALL_THREADS) void orth_small_kernel(const T* __re
     const T* src = update + (int64_t)blockIdx.x * size;
     T* dst = result + (int64_t)blockIdx.x * size;
 
-    float s = 0.0f;
-#pragma unroll 8
-    for (int e = threadIdx.x; e < size; e += SMALL_THREADS) s = __builtin_fmaf((float)src[e], (float)src[e], s);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
     float* sums = (float*)ah;
-    if (lane == 0) sums[wave] = s;
-    for (int e = threadIdx.x; e < 2 * panels * PANEL; e += SMALL_THREADS) xh[e] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    s = 0.0f;
+    auto sum = [&](float pre) __attribute__((always_inline)) {
+        float s = 0.0f;
+#pragma unroll 8
+        for (int e = threadIdx.x; e < size; e += SMALL_THREADS) {
+            const float x = (float)src[e] * pre;
+            s = __builtin_fmaf(x, x, s);
+        }
 #pragma unroll
-    for (int w = 0; w < SMALL_WAVES; w++) s += sums[w];
-    float small;
-    const float scale = start_scale(__builtin_sqrtf(s), small);
+        for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
+        if (lane == 0) sums[wave] = s;
+        __syncthreads();
+        s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < SMALL_WAVES; w++) s += sums[w];
+        return s;
+    };
+    for (int e = threadIdx.x; e < 2 * panels * PANEL; e += SMALL_THREADS) xh[e] = make_uint4(0, 0, 0, 0);
+    const float s = sum(1.0f);
+    float shrunk = 0.0f;
+    if (s == __builtin_inff()) {
+        __syncthreads();   // all have read the first sums
+        shrunk = sum(SHRINK);
+    }
+    const Start start = start_of(s, shrunk);
+    const float small = start.small;
     // a wave takes rows of G, a lane every 64th element of one
 #pragma unroll 2
     for (int r = wave; r < m; r += SMALL_WAVES)
@@ -517,7 +560,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void orth_small_kernel(const T* __re
         for (int c = lane; c < n; c += 64) {
             const int row = tall ? c : r, col = tall ? r : c;
             f16 hi, lo;
-            split((float)src[r * n + c] * scale, hi, lo);
+            split((float)src[r * n + c] * start.pre * start.scale, hi, lo);
             quad<PANEL>(xh, row, col & ~3)[col & 3] = hi;
             quad<PANEL>(xl, row, col & ~3)[col & 3] = lo;
         }
@@ -676,7 +719,7 @@ Layout layout_of(int count, int m, int n)
     const int s = m < n ? m : n, l = m < n ? n : m, t = tile_of(count, s, l);
     L.m = (int)up(s, t);
     L.n = (int)up(l, t);
-    L.parts = up((int64_t)count * (NORM_PARTS + 1) * 4, 256);
+    L.parts = up((int64_t)count * (2 * NORM_PARTS + 1) * 4, 256);
     L.x = up((int64_t)count * L.m * L.n * 4, 256);
     L.sq = up((int64_t)count * L.m * L.m * 4, 256);
     const int64_t tm = L.m / t, tn = L.n / t, sq = count * (tm * (tm + 1) / 2), full = count * tm * tn;
@@ -760,7 +803,7 @@ int orthogonalise(int count, int m, int n, const T* g, int steps, T* out, void* 
     const Layout L = layout_of(count, m, n);
     const int tall = m > n, S = tile_of(count, m < n ? m : n, m < n ? n : m);
     float* parts = (float*)workspace;
-    float* small = parts + (int64_t)count * NORM_PARTS;
+    float* small = parts + (int64_t)count * 2 * NORM_PARTS;
     char* at = (char*)workspace + L.parts;
     const int64_t px = (int64_t)L.m * L.n, pa = (int64_t)L.m * L.m;
     Planes x[2] = {{(f16*)at, px, 2 * px, L.n}, {(f16*)(at + L.x), px, 2 * px, L.n}};
