@@ -138,3 +138,5 @@ class OrthogonalMomentum(torch.optim.Optimizer):
         scale = max(1.0, shape[0] / shape[1]) ** 0.5
         _t.check(lib.gs_momentum_apply(code, n, size, pointers(params), 1.0 - group["lr"] * group["weight_decay"],
                                          group["lr"] * scale, _t.ptr(update), stream), "gs_momentum_apply")
+        # written through their addresses: graphs that saved them are told
+        torch.autograd.graph.increment_version(params)

@@ -1,5 +1,5 @@
 """The token operators among torch's own machinery: what it cannot differentiate is
-refused."""
+refused, and what it has to know of is told."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -28,3 +28,18 @@ def test_a_forward_mode_tangent_is_refused(gpu, which, also_backward, grad_mode)
             args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
             with pytest.raises(NotImplementedError, match="jvp|forward"):
                 op(*args)
+
+
+def test_a_step_is_seen_by_graphs_that_hold_the_weights(gpu):
+    # as with torch's own optimisers: what saved a weight before the step cannot be differentiated after it
+    from blitzgs_amd.orthogonal import OrthogonalMomentum
+    for t in (torch.float32, torch.bfloat16):
+        w = _rand((24, 16), 0, t).requires_grad_(True)
+        opt = OrthogonalMomentum([w], lr=0.1)
+        x = _rand((5, 16), 1, t).requires_grad_(True)
+        y = x @ w.t()
+        w.grad = torch.ones_like(w)
+        opt.step()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        (x @ w.t()).sum().backward()                        # a new graph is fine
