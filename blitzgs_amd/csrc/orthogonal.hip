@@ -936,11 +936,13 @@ extern "C" int gs_momentum_update(int type, int count, int64_t size, const void*
         B.momentum[i] = momenta[i];
     }
     const dim3 grid = grid_of(size, count);
-    if (type == GS_F32)
-        hipLaunchKernelGGL(momentum_kernel<float>, grid, dim3(256), 0, stream, B, size, beta, nesterov, update);
-    else if (type == GS_BF16)
-        hipLaunchKernelGGL(momentum_kernel<gs::bf16>, grid, dim3(256), 0, stream, B, size, beta, nesterov, update);
-    else hipLaunchKernelGGL(momentum_kernel<f16>, grid, dim3(256), 0, stream, B, size, beta, nesterov, update);
+    auto run = [&](auto kernel) {
+        GS_TIMED("momentum_kernel", stream,
+                 hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, B, size, beta, nesterov, update));
+    };
+    if (type == GS_F32) run(momentum_kernel<float>);
+    else if (type == GS_BF16) run(momentum_kernel<gs::bf16>);
+    else run(momentum_kernel<f16>);
     GS_LAUNCH_CHECK("momentum_kernel");
     return GS_OK;
 }
@@ -960,10 +962,13 @@ extern "C" int gs_momentum_apply(int type, int count, int64_t size, void* const*
         B.param[i] = params[i];
     }
     const dim3 grid = grid_of(size, count);
-    if (type == GS_F32) hipLaunchKernelGGL(apply_kernel<float>, grid, dim3(256), 0, stream, B, size, keep, lr, update);
-    else if (type == GS_BF16)
-        hipLaunchKernelGGL(apply_kernel<gs::bf16>, grid, dim3(256), 0, stream, B, size, keep, lr, update);
-    else hipLaunchKernelGGL(apply_kernel<f16>, grid, dim3(256), 0, stream, B, size, keep, lr, update);
+    auto run = [&](auto kernel) {
+        GS_TIMED("apply_kernel", stream,
+                 hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, B, size, keep, lr, update));
+    };
+    if (type == GS_F32) run(apply_kernel<float>);
+    else if (type == GS_BF16) run(apply_kernel<gs::bf16>);
+    else run(apply_kernel<f16>);
     GS_LAUNCH_CHECK("apply_kernel");
     return GS_OK;
 }
