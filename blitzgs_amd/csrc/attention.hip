@@ -1095,7 +1095,7 @@ int check(int type, int B, int Hq, int Hkv, int Tq, int Tk, int D, float scale)
     GS_REQUIRE(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0,
                "attention: the number of query heads (%d) must be a multiple of the number of key heads (%d)", Hq, Hkv);
     GS_REQUIRE(D >= 1 && D <= 128, "attention: the head dimension must be in [1, 128], got %d", D);
-    GS_REQUIRE(scale > 0.0f && scale <= 3.0e38f, "attention: scale must be a positive number");
+    GS_REQUIRE(scale > 0.0f && scale * LOG2E < -NEG_INF, "attention: scale must be a positive number below 2.3e38");
     GS_REQUIRE((int64_t)(Hq / Hkv) * Tq < 0x7fffff00ll && Tk < 0x7fffff00,
                "attention: too many queries or keys for one head");
     GS_REQUIRE((int64_t)B * Hq * Tq < (1ll << 32) && (int64_t)B * Hkv * Tk < (1ll << 32),
