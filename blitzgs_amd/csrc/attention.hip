@@ -26,23 +26,34 @@
 // read once for all of them, and dk and dv are summed over them in registers.
 //
 // Precision.  Scores, softmax statistics and all sums are fp32.  P and dS are
-// rounded to the tensors' type as operands of the second product: it is the
-// matrix core's operand type, and the error is that of rounding v or k.
-// delta is subtracted from numbers of its own size, where a row looks at few
-// keys, so a 16-bit forward also keeps what the rounding of o left, in as many
-// bits again, and delta is formed from both parts.
+// rounded to the tensors' type as operands of the second product, which is the
+// matrix core's operand type.  That adds to the rounding of the results themselves:
+// o and the gradients are off by 0.0024 in bfloat16 and 0.00030 in float16, relative
+// to their size, where rounding alone leaves 0.0017 and 0.00021 (float32: 4.4e-7).
+// delta is subtracted from numbers of its own size, where a row looks at few keys,
+// so a 16-bit forward also keeps what the rounding of o left, and delta is formed
+// from both parts: in bfloat16 as many bits again, in float16 down to 2^-25, which
+// for v of 2^-14 and more is below what the rounding of P has left in o.
 //
 // Bound and figures (bfloat16; a large library product reaches 1240 TFLOP/s on the
-// card, power being the limit).  The forward at D = 64 is bound by the SIMD's
-// issue: per score one fused multiply-add, an exponential at half rate, a sum, a
-// maximum and half a conversion, 65 % of its cycles, beside 33 % matrix work.  The
-// others are near the matrix core's practical rate, dk, dv behind for want of
-// registers: 16 keys a wave at D = 128, two waves per SIMD.
-//   2 x 16 heads, 4096 x 4096, D 64     forward 210 us (654 TFLOP/s), dq 215 (959
-//                                       with its recomputation), dk dv 320 (859)
-//   16 heads on 4, 8192 causal, D 128   330 us (833), 396 (1041), 719 (765)
-//   8 x 32 heads on 8, one query, up to 32768 keys, D 128   111 + 7 us to join
-//                                       the splits (537 MB, 4.6 TB/s in all)
+// card; after 200 passes, the first of which are up to 15 % slower).  Of a SIMD's
+// cycles with work on its CU, the share with vector instructions issued and the share
+// with the matrix core busy:
+//   2 x 16 heads, 4096 x 4096, D 64
+//     forward 183 us (752 TFLOP/s)                        64 %, 32 %
+//     dq 197 us (1046 with its recomputation)             60 %, 50 %
+//     dk, dv 276 us (997)                                 46 %, 42 %
+//   16 heads on 4, 8192 causal, D 128
+//     forward 308 us (891)                                53 %, 42 %
+//     dq 380 us (1084)                                    46 %, 54 %
+//     dk, dv 657 us (836), 22 to add                      32 %, 36 %, and LDS 41 %
+// Neither is full: a wave's products, its exponentials and its second product follow
+// one another, and two or three waves per SIMD do not cover all of that.  dk, dv want
+// registers besides: 16 keys a wave at D = 128.  float16 takes the same but for fit().
+//   8 x 32 heads on 8, one query, up to 32768 keys, D 128
+//     104 us and 6 to join the splits (537 MB, 4.9 TB/s; a large copy: 5.15)
+//   float32, 2 x 16 heads, 4096 x 4096, D 64
+//     1098, 1535 and 2187 us (125, 134 and 126 TFLOP/s; a large library product: 153)
 #include <algorithm>
 #include <type_traits>
 
@@ -243,8 +254,9 @@ __device__ __forceinline__ void add_rest(f4& x, const T* p, int n)
 // and its sum divided by it at the end.  As with the softmax's base, `up` falls when the
 // column's largest dS so far asks for it: that keeps the largest between 2^7 and 2^15,
 // and all of float16's bits in what is at least 2^-21 of it.  The error above becomes
-// 6.9e-4, of which dq's own rounding is 6.6e-4; dq, dk and dv take 4 to 8 % longer in
-// float16 (4096 x 4096, D 64: 214 -> 232 and 314 -> 335 us).
+// 6.9e-4, of which dq's own rounding is 6.6e-4; float16's dq, dk and dv take longer by it:
+// 204 -> 225 and 285 -> 309 us at 2 x 16 heads of 4096 x 4096, D 64; 399 -> 416 and
+// 681 -> 709 at 16 heads on 4 of 8192, causal, D 128.
 template <typename T>
 constexpr bool FITS = __is_same(T, gs::f16);
 constexpr float UP = 0x1p60f;      // of columns that have met no dS yet

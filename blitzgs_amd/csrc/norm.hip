@@ -20,9 +20,10 @@
 // same bits.  All sums and statistics are fp32 whatever the tensors' type;
 // each output is rounded to its type once.
 //
-// 65536 x 1024 bfloat16, fp32 parameters: forward 54 us (268 MB, 4.9 TB/s),
-// backward 85 us (403 MB, 4.7 TB/s) and 4 us for the partial rows; a large copy
-// reaches 5.15 TB/s.
+// 65536 x 1024 bfloat16, fp32 parameters: forward 53 us (268 MB, 5.0 TB/s),
+// backward 83 us (403 MB, 4.8 TB/s) and 4 us for the partial rows; a large copy
+// reaches 5.15 TB/s.  10007 x 513 float32, one element per access: 12, 17 and 4 us
+// (103 MB, 20 us at that rate).
 #include "gs_host.h"
 #include "gs_types.h"
 #include "../../include/blitzgs_amd.h"
@@ -260,7 +261,9 @@ __global__ __launch_bounds__(1024) void norm_columns_kernel(const float* __restr
 // threads per row and accesses per thread: the fewest threads that hold the
 // row in one access each, then a wave with up to 32 elements per lane, then 4
 // and 16 waves.  More elements per lane would spill the backward's five
-// values per element.
+// values per element.  Rows of single elements step from 8 accesses to 12 before 16:
+// 10007 rows of 513 float32 take 19.4 us backward with 12 and 21.1 with 16, of 767
+// 22.6 and 25.0; of 513 bfloat16 24.8 and 27.4.  6 and 24 have not been tried.
 struct Shape {
     int v, lpr, nc;
 };

@@ -25,10 +25,12 @@
 // and stored twice.  The planes are padded to whole tiles with zeros, so the
 // products have no edge cases.
 //
-// Eight 1024 x 4096 fp32 matrices: 2.03 ms, per step X X^T 150 us, B 52 us, B X
-// 194 us (1060 TFLOP/s of float16 products; a large library product reaches 1190
+// Eight 1024 x 4096 fp32 matrices: 2.03 ms, per step X X^T 148 us, B 51 us, B X
+// 189 us (1090 TFLOP/s of float16 products; a large library product reaches 1190
 // on the card).  The symmetric products' 288 tiles leave a second place on most
-// CUs empty: 64-wide tiles were slower (191 us), parts of the depth no faster.
+// CUs empty: 64-wide tiles were slower (191 us for X X^T), and of the 32 tiles beyond
+// one per CU split over all CUs the products took 125 us, but adding them 20 more in
+// a launch of its own.
 #include <algorithm>
 #include <utility>
 
@@ -865,6 +867,9 @@ struct MomentumBatch {
     float* momentum[MAX_PARAMS];
 };
 
+// Bound by memory, an element per thread.  Eight 1024 x 4096 matrices: 96 us (537 MB, 5.6
+// TB/s) and 84 us (403 MB, 4.8) in float32, 94 (5.0) and 77 (3.5: two-byte accesses)
+// in bfloat16, beside 2 ms for the products.
 // m = beta m + g;  update = nesterov ? g + beta m : m, stacked
 template <typename T>
 __global__ __launch_bounds__(256) void momentum_kernel(MomentumBatch B, int64_t size, float beta, int nesterov,
