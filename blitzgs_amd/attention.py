@@ -35,6 +35,10 @@ def _strides(t):
     return (C.c_int64 * 3)(*t.stride()[:3])
 
 
+def _laid(*tensors):
+    return [None if t is None else t.stride() for t in tensors]
+
+
 def _last_contiguous(t):
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
@@ -70,6 +74,7 @@ class _Attention(torch.autograd.Function):
         q, k, v = (_last_contiguous(t.detach()) for t in (q, k, v))
         o, rest, lse, ctx.how = _forward(q, k, v, causal, key_lengths, query_start, scale, True)
         ctx.save_for_backward(q, k, v, o, rest, lse, key_lengths, query_start)
+        ctx.laid = _laid(q, k, v, o, rest, lse, key_lengths, query_start)
         ctx.ws_bytes = _t.load().gs_attention_workspace_bytes(*ctx.how[0], ctx.how[2], 1)
         return o
 
@@ -78,10 +83,16 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, rest, lse, key_lengths, query_start = ctx.saved_tensors
+        saved = ctx.saved_tensors
         sizes, (qs, ks, vs, os), _, scale, causal = ctx.how
+        if _laid(*saved) != ctx.laid:
+            # hooks on saved tensors give them back with the same values, not in the same places
+            saved = [t if t is None else t.contiguous() for t in saved]
+            qs, ks, vs, os = (_strides(t) for t in saved[:4])
+        q, k, v, o, rest, lse, key_lengths, query_start = saved
         do = _last_contiguous(do)
-        dq, dk, dv, beside = _token_major(q), None, None, ks
+        dq, dk, dv = _token_major(q), None, None
+        dqs = beside = _strides(dq)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dk, dv = _token_major(k), _token_major(v)
             beside = _strides(dk)
@@ -89,7 +100,7 @@ class _Attention(torch.autograd.Function):
         _t.check(_t.load().gs_attention_backward(
             *sizes, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, scale, causal, _t.ptr(key_lengths),
             _t.ptr(query_start), o.data_ptr(), os, _t.ptr(rest), lse.data_ptr(), do.data_ptr(), _strides(do),
-            dq.data_ptr(), os, _t.ptr(dk), beside, _t.ptr(dv), beside, _t.ptr(ws), _t.stream(q.device)),
+            dq.data_ptr(), dqs, _t.ptr(dk), beside, _t.ptr(dv), beside, _t.ptr(ws), _t.stream(q.device)),
             "gs_attention_backward")
         return dq, dk, dv, None, None, None, None
 

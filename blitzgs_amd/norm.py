@@ -61,6 +61,9 @@ class _LayerNorm(torch.autograd.Function):
         x, weight, stats = ctx.saved_tensors
         code, param_code, n, width, params = ctx.how
         device = x.device
+        # hooks on saved tensors give them back with the same values, not in the same places
+        stats = stats.contiguous()
+        weight = None if weight is None else weight.contiguous()
         rows, _, apart = _rows(x, width)
         drows, _, dapart = _rows(dy, width)
         dx = torch.empty(x.shape, device=device, dtype=x.dtype)
