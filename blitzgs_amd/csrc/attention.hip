@@ -217,10 +217,22 @@ __device__ __forceinline__ void store4(T* p, f4 v, int n)
     }
 }
 
+// o is a mean of values of v.  The rounding of P can leave it above the largest of them by
+// 2^-11, which takes it from float16's largest numbers to infinity.
+template <typename T>
+__device__ __forceinline__ float mean_of(float x)
+{
+    if constexpr (__is_same(T, gs::f16))
+        return fabsf(x) < -NEG_INF ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x;
+    return x;
+}
+
 // Four neighbours of o, and what their rounding leaves.
 template <bool ODD, typename T>
 __device__ __forceinline__ void store_o(T* p, T* rest, f4 v, int n)
 {
+#pragma unroll
+    for (int r = 0; r < 4; r++) v[r] = mean_of<T>(v[r]);
     store4<ODD>(p, v, n);
     if (rest == nullptr) return;
     f4 left;
@@ -524,7 +536,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void attn_join_kernel(AttnArg
     }
     const uint32_t r = (uint32_t)row, i = r % (uint32_t)A.Tq, bh = r / (uint32_t)A.Tq, Hq = A.Hkv * A.G;
     const int64_t out = bh / Hq * A.s0.b + bh % Hq * A.s0.h + i * A.s0.t;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, x0 = o0 * inv, x1 = o1 * inv;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, x0 = mean_of<T>(o0 * inv), x1 = mean_of<T>(o1 * inv);
     T *o = (T*)A.out0 + out, *rest = (T*)A.rest + out;
     if (lane < A.D) {
         o[lane] = (T)x0;

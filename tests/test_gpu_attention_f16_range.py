@@ -123,3 +123,22 @@ def test_values_of_small_probability(gpu, D):
     bound = bound - 1.01 * STEP[T] * do.double().abs().sum(2, keepdim=True).cpu()
     assert (bound > 0).all() and (value[:, :, 1:].abs() < 2e-2).all() and (value.abs() > 6.2e-5).all()
     _within(_grads(q, k, v, do)[2], value, bound, "dv")
+
+
+@pytest.mark.parametrize("Tq,Tk", [(300, 700), (2, 3000)])
+@pytest.mark.parametrize("D", [64, 128, 33])
+def test_the_largest_values_stay_finite(gpu, Tq, Tk, D):
+    # o is a mean of v: never beyond float16's largest number, which all keys hold here
+    from blitzgs_amd.attention import attention
+    for seed in range(3):
+        q, k = _rand((2, 4, Tq, D), seed, 3.0), _rand((2, 4, Tk, D), 10 + seed, 3.0)
+        for sign in (1.0, -1.0):
+            v = torch.full((2, 4, Tk, D), sign * 65504.0, device="cuda", dtype=T)
+            want, bound = attention_64(q, k, v, False, None, None, 1 / math.sqrt(D))["o"]
+            _within(attention(q, k, v), want, bound, "o")
+            leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+            _within(attention(*leaves).detach(), want, bound, "o kept for a backward")
+    # an infinity is none of these (times a probability that float16 takes for 0, it is a NaN)
+    v[:, :, 5, 3] = float("inf")
+    o = attention(q, k, v)
+    assert not torch.isfinite(o[..., 3]).any() and torch.isfinite(o[..., 4:]).all()
