@@ -17,9 +17,11 @@ infinity reaches the queries that see its key and, in the backward, the keys tha
 its query sees, and no others.
 
 Scores, softmax and all sums are fp32; probabilities are rounded to the
-tensors' type for the product with v.  Nothing of size Tq x Tk is stored: a call
-that needs gradients keeps q, k, v, o, one number per query, and in the 16-bit
-types a second part of o.  Equal inputs give equal bits.
+tensors' type for the product with v.  The sums come before their division by the
+softmax's, so values of v beyond 1e36 / Tk may pass fp32's range; float16's values
+never do.  Nothing of size Tq x Tk is stored: a call that needs gradients keeps q,
+k, v, o, one number per query, and in the 16-bit types a second part of o.  Equal
+inputs give equal bits.
 """
 import ctypes as C
 import math

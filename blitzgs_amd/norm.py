@@ -6,7 +6,8 @@ mean and var (over n, uncorrected) and every sum are fp32 whatever the type of
 x; each output is rounded to its type once.  x is float32, bfloat16 or float16;
 weight and bias (either may be None) have x's type or float32.  The gradients
 of weight and bias are added up in a fixed order, so equal inputs give equal
-bits.
+bits.  A row whose squared deviations pass fp32's range (deviations of 1e18 and
+more) has an infinite variance and becomes bias.
 """
 import torch
 
