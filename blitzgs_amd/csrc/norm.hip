@@ -262,9 +262,10 @@ __global__ __launch_bounds__(1024) void norm_columns_kernel(const float* __restr
 // row in one access each, then a wave with up to 32 elements per lane, then 4
 // and 16 waves.  More elements per lane would spill the backward's five
 // values per element, as 16 waves do already, which leave a lane 128 registers
-// (widths above 8192: up to 656 bytes of scratch a lane backward).  Rows of single elements step from 8 accesses to 12 before 16:
-// 10007 rows of 513 float32 take 19.4 us backward with 12 and 21.1 with 16, of 767
-// 22.6 and 25.0; of 513 bfloat16 24.8 and 27.4.  6 and 24 have not been tried.
+// (widths above 8192: up to 656 bytes of scratch a lane backward).  Rows of
+// single elements step from 8 accesses to 12 before 16: 10007 rows of 513 float32
+// take 19.4 us backward with 12 and 21.1 with 16, of 767 22.6 and 25.0; of 513
+// bfloat16 24.8 and 27.4.  6 and 24 have not been tried.
 struct Shape {
     int v, lpr, nc;
 };
