@@ -33,12 +33,11 @@ from . import _tensors as _t
 MAX_HEAD_DIM = 128
 
 
+_Strides = C.c_int64 * 3
+
+
 def _strides(t):
-    return (C.c_int64 * 3)(*t.stride()[:3])
-
-
-def _laid(*tensors):
-    return [None if t is None else t.stride() for t in tensors]
+    return _Strides(*t.stride()[:3])
 
 
 def _last_contiguous(t):
@@ -61,13 +60,14 @@ def _forward(q, k, v, causal, key_lengths, query_start, scale, grads):
     lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32) if grads else None
     rest = _token_major(q) if grads and q.dtype != torch.float32 else None
     ws = _t.workspace(lib.gs_attention_workspace_bytes(*sizes, unequal, 0), q.device)
-    strides = _strides(q), _strides(k), _strides(v), _strides(o)
+    laid = q.stride(), k.stride(), v.stride(), o.stride()
+    strides = [_Strides(*s[:3]) for s in laid]
     with _t.on_device(q.device):
         _t.check(lib.gs_attention_forward(
             *sizes, q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(), strides[2], scale, int(causal),
             _t.ptr(key_lengths), _t.ptr(query_start), o.data_ptr(), strides[3], _t.ptr(rest), _t.ptr(lse),
             _t.ptr(ws), _t.stream(q.device)), "gs_attention_forward")
-    return o, rest, lse, (sizes, strides, unequal, scale, int(causal))
+    return o, rest, lse, (sizes, strides, laid, unequal, scale, int(causal))
 
 
 class _Attention(torch.autograd.Function):
@@ -76,8 +76,7 @@ class _Attention(torch.autograd.Function):
         q, k, v = (_last_contiguous(t.detach()) for t in (q, k, v))
         o, rest, lse, ctx.how = _forward(q, k, v, causal, key_lengths, query_start, scale, True)
         ctx.save_for_backward(q, k, v, o, rest, lse, key_lengths, query_start)
-        ctx.laid = _laid(q, k, v, o, rest, lse, key_lengths, query_start)
-        ctx.ws_bytes = _t.load().gs_attention_workspace_bytes(*ctx.how[0], ctx.how[2], 1)
+        ctx.ws_bytes = _t.load().gs_attention_workspace_bytes(*ctx.how[0], ctx.how[3], 1)
         return o
 
     # The autograd engine calls this from a thread of its own, on the forward's
@@ -85,16 +84,19 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        saved = ctx.saved_tensors
-        sizes, (qs, ks, vs, os), _, scale, causal = ctx.how
-        if _laid(*saved) != ctx.laid:
-            # hooks on saved tensors give them back with the same values, not in the same places
-            saved = [t if t is None else t.contiguous() for t in saved]
-            qs, ks, vs, os = (_strides(t) for t in saved[:4])
-        q, k, v, o, rest, lse, key_lengths, query_start = saved
+        q, k, v, o, rest, lse, key_lengths, query_start = ctx.saved_tensors
+        sizes, (qs, ks, vs, os), laid, _, scale, causal = ctx.how
         do = _last_contiguous(do)
-        dq, dk, dv = _token_major(q), None, None
-        dqs = beside = _strides(dq)
+        dq, dk, dv, beside = _token_major(q), None, None, ks
+        dqs = os
+        if ((q.stride(), k.stride(), v.stride(), o.stride()) != laid or (rest is not None and rest.stride() != laid[3])
+                or not lse.is_contiguous() or (key_lengths is not None and not key_lengths.is_contiguous())
+                or (query_start is not None and not query_start.is_contiguous())):
+            # hooks on saved tensors give them back with the same values, not in the same places
+            q, k, v, o, lse = (t.contiguous() for t in (q, k, v, o, lse))
+            rest, key_lengths, query_start = (t if t is None else t.contiguous()
+                                              for t in (rest, key_lengths, query_start))
+            qs, ks, vs, os, dqs = (_strides(t) for t in (q, k, v, o, dq))
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dk, dv = _token_major(k), _token_major(v)
             beside = _strides(dk)
