@@ -20,7 +20,10 @@ and, for a network in front of the rasterizer that predicts Gaussians (float32,
 bfloat16, float16):
   blitzgs_amd.norm       : layer_norm
   blitzgs_amd.attention  : attention (shared heads, causal limit, key lengths)
+  blitzgs_amd.rotary     : rotate, norm_rotate (positions and norms of queries and keys)
+  blitzgs_amd.feedforward: feed_forward (the gated block)
   blitzgs_amd.orthogonal : orthogonalise, OrthogonalMomentum (weight matrices' optimiser)
+  blitzgs_amd.adamw      : adamw_update, AdamW (many tensors at once, moments in 32 or 8 bits)
   blitzgs_amd.examples.train_predictor trains such a network with them
 Drop-in packages with the reference's module names live in blitzgs_amd/dropin.
 """

@@ -35,6 +35,12 @@ class AdamGroup(C.Structure):
                 ("M", C.c_int64), ("lr", C.c_float), ("eps", C.c_float)]
 
 
+class AdamWSettings(C.Structure):
+    """gs_adamw_settings (include/blitzgs_amd.h)."""
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("step", C.c_int64), ("seed", C.c_uint32)]
+
+
 _SIGS = {
     "gs_version": (_i, []),
     "gs_last_error": (C.c_char_p, []),
@@ -105,10 +111,20 @@ _SIGS = {
                                                                          _c, _c]),
     "gs_attention_backward": (_i, [_i] * 7 + [_c, C.POINTER(_i64)] * 3 + [_f, _i, _c, _c, _c, C.POINTER(_i64), _c, _c]
                               + [_c, C.POINTER(_i64)] * 4 + [_c, _c]),
+    "gs_rotary_forward": (_i, [_i] * 10 + [_f, _i, _f] + [_c, C.POINTER(_i64)] * 2 + [_c, _c, _c, _i, C.POINTER(_i64), _c]
+                          + [_c, C.POINTER(_i64)] * 2 + [_c]),
+    "gs_rotary_workspace_bytes": (_sz, [_i] * 8),
+    "gs_rotary_backward": (_i, [_i] * 10 + [_f, _i, _f] + [_c, C.POINTER(_i64)] * 2 + [_c, _c, _c, _i, C.POINTER(_i64), _c]
+                           + [_c, C.POINTER(_i64)] * 4 + [_c] * 4),
     "gs_orthogonalise_workspace_bytes": (_sz, [_i, _i, _i]),
     "gs_orthogonalise": (_i, [_i, _i, _i, _i, _c, _i, _c, _c, _c]),
     "gs_momentum_update": (_i, [_i, _i, _i64, C.POINTER(_c), C.POINTER(_c), _f, _i, _c, _c]),
     "gs_momentum_apply": (_i, [_i, _i, _i64, C.POINTER(_c), _f, _f, _c, _c]),
+    "gs_feed_forward_workspace_bytes": (_sz, [_i, _i64, _i, _i, _i, _i]),
+    "gs_feed_forward": (_i, [_i, _i, _i64, _i, _i, _i, _c, _i64] + [_c] * 9),
+    "gs_feed_forward_backward": (_i, [_i, _i, _i64, _i, _i, _i, _c, _i64] + [_c] * 7 + [_i64] + [_c] * 6),
+    "gs_adamw_update": (_i, [_i, _i, _i, C.POINTER(_i64)] + [C.POINTER(_c)] * 6 + [C.POINTER(AdamWSettings), _c]),
+    "gs_adamw_values": (_i, [_i, _i64] + [_c] * 7),
     "gs_diag_math": (_i, [_i, _i, _c, _c, _c]),
     "gs_timing_enable": (_i, [_i]),
     "gs_timing_reset": (_i, []),

@@ -57,5 +57,27 @@ def wants_grad(*tensors):
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+def load_uncast(optimizer, load, state_dict, take):
+    """load(state_dict) of an optimiser whose state keeps its own types: torch's loading
+    casts a state to its parameter's type, so take(state, loaded, parameter) takes from
+    what was loaded once more: after all hooks that may change that, and before any that
+    look at the result."""
+    loaded = {}
+
+    def restore(_):
+        ours = (p for group in optimizer.param_groups for p in group["params"])
+        for key, p in zip((k for group in loaded["param_groups"] for k in group["params"]), ours):
+            if key in loaded["state"]:
+                take(optimizer.state[p], loaded["state"][key], p)
+
+    hooks = [optimizer.register_load_state_dict_pre_hook(lambda _, state: loaded.update(state)),
+             optimizer.register_load_state_dict_post_hook(restore, prepend=True)]
+    try:
+        load(state_dict)
+    finally:
+        for hook in hooks:
+            hook.remove()
+
+
 check = _lib.check
 load = _lib.load

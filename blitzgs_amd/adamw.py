@@ -1,0 +1,199 @@
+"""adamw_update, AdamW: an AdamW step over many tensors at once, with moments in 32
+bits or in 8.
+
+    m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
+    p = (1 - lr weight_decay) p - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+
+Parameters and gradients are float32, bfloat16 or float16, of one type; all arithmetic
+is fp32 and a parameter is rounded to its type once.  SparseGaussianAdam updates the
+per-Gaussian tensors of a scene, OrthogonalMomentum the weight matrices of a network in
+front of it, AdamW what is left of the network, or all of it.
+
+Moments in 8 bits are uint8 tensors of the parameter's shape and one of scales, (2,
+ceil(n / 128)): 128 elements in a row share a power of two, over which a first moment
+is a small float of a sign, four bits of exponent and three of mantissa, a second one
+of five and three.  They are rounded up with the probability of the rest, by bits that
+follow from seed, step, the tensor's place in the call and the element's: equal inputs
+give equal bits.  A step uses the moments before they are rounded.  A moment that is
+infinite or NaN is NaN in 8 bits.
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import _tensors as _t
+from ._lib import AdamWSettings
+
+BLOCK = 128
+
+
+def new_moments(param, bits=32):
+    """(exp_avg, exp_avg_sq, scales) of a parameter at the start; scales is None with 32 bits."""
+    if bits not in (8, 32):
+        raise RuntimeError(f"moments have 8 or 32 bits, got {bits!r}")
+    zeros = lambda *shape, dtype: torch.zeros(shape, device=param.device, dtype=dtype)  # noqa: E731
+    if bits == 32:
+        return zeros(*param.shape, dtype=torch.float32), zeros(*param.shape, dtype=torch.float32), None
+    return (zeros(*param.shape, dtype=torch.uint8), zeros(*param.shape, dtype=torch.uint8),
+            zeros(2, -(-param.numel() // BLOCK), dtype=torch.uint8))
+
+
+def _checked(ts, name, dtype, params):
+    """Contiguous tensors like the parameters, of a type."""
+    if len(ts) != len(params):
+        raise RuntimeError(f"{name} must hold a tensor for each of {len(params)} parameters, got {len(ts)}")
+    for t, p in zip(ts, params):
+        if (not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != p.shape or t.device != p.device
+                or not t.is_contiguous()):
+            raise RuntimeError(f"{name} must hold contiguous {dtype} tensors of the parameters' shapes on {p.device}")
+
+
+def _settings(lr, betas, eps, weight_decay):
+    beta1, beta2 = betas
+    if not (0.0 <= lr < math.inf and 0.0 <= eps < math.inf and 0.0 <= weight_decay < math.inf
+            and 0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise RuntimeError("lr, eps and weight_decay must be finite and not negative and the betas in [0, 1), got "
+                           f"{lr}, {eps}, {weight_decay}, {betas}")
+    return float(lr), float(beta1), float(beta2), float(eps), float(weight_decay)
+
+
+@torch.no_grad()
+def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
+                 scales=None, seed=0):
+    """Step number `step` (from 1 on), in place, over lists of tensors on one device.
+
+    exp_avgs, exp_avg_sqs: float32, or uint8 with a list of scales, as new_moments makes
+    them.  A tensor may not come twice.  In a captured graph every replay is the step, with
+    the rates and the seed, that was captured."""
+    params, grads = list(params), list(grads)
+    how = _settings(lr, betas, eps, weight_decay)
+    if not isinstance(step, int) or not 1 <= step < 2 ** 53:
+        raise RuntimeError(f"step must be an integer from 1 to 2^53, got {step!r}")
+    if not isinstance(seed, int):
+        raise RuntimeError(f"seed must be an integer, got {seed!r}")
+    if not params:
+        return
+    first = params[0]
+    _t.require_tensor(first, "params")
+    _checked(params, "params", first.dtype, params)
+    device = first.device
+    for p in params:
+        if p.device != device:
+            raise RuntimeError(f"params must be on one device, got {device} and {p.device}")
+    for g in grads:
+        if isinstance(g, torch.Tensor) and g.is_sparse:
+            raise RuntimeError("gradients must be dense")
+    grads = [g.contiguous() if isinstance(g, torch.Tensor) else g for g in grads]
+    _checked(grads, "grads", first.dtype, params)
+    moment = torch.float32 if scales is None else torch.uint8
+    _checked(exp_avgs, "exp_avgs", moment, params)
+    _checked(exp_avg_sqs, "exp_avg_sqs", moment, params)
+    n = len(params)
+    pointers = lambda addresses: (C.c_void_p * n)(*addresses)  # noqa: E731
+    written = [[t.data_ptr() for t in ts] for ts in (params, exp_avgs, exp_avg_sqs)]
+    low = high = None
+    if scales is not None:
+        if len(scales) != n:
+            raise RuntimeError(f"scales must hold a tensor for each of {n} parameters, got {len(scales)}")
+        for s, p in zip(scales, params):
+            if (not isinstance(s, torch.Tensor) or s.dtype != torch.uint8 or s.device != device
+                    or s.shape != (2, -(-p.numel() // BLOCK)) or (s.shape[1] > 1 and s.stride(1) != 1)):
+                raise RuntimeError(f"scales must hold uint8 tensors of shape (2, ceil(n / {BLOCK})) with contiguous rows "
+                                   f"on {device}")
+        written += [[s.data_ptr() for s in scales], [s.data_ptr() + s.stride(0) for s in scales]]
+        low, high = (pointers(a) for a in written[3:])
+    sizes = [p.numel() for p in params]
+    addresses = [a for column in written for a, size in zip(column, sizes) if size]
+    if len(set(addresses)) != len(addresses):
+        raise RuntimeError("a tensor may not come twice in a call")
+    with _t.on_device(device):
+        _t.check(_t.load().gs_adamw_update(
+            _t.DTYPE_CODES[first.dtype], 32 if scales is None else 8, n, (C.c_int64 * n)(*sizes), pointers(written[0]),
+            pointers([g.data_ptr() for g in grads]), pointers(written[1]), pointers(written[2]), low, high,
+            C.byref(AdamWSettings(*how, step, seed & 0xFFFFFFFF)), _t.stream(device)), "gs_adamw_update")
+    # written through their addresses: graphs that saved them are told
+    torch.autograd.graph.increment_version(params)
+
+
+@torch.no_grad()
+def moment_values(exp_avg, exp_avg_sq, scales, dtype=torch.float32):
+    """The values that 8-bit moments stand for, float32 or (which holds them whole) bfloat16."""
+    for name, t in (("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq), ("scales", scales)):
+        if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.device != exp_avg.device):
+            raise RuntimeError(f"{name} must be a uint8 HIP device tensor (of exp_avg's device)")
+    n = exp_avg.numel()
+    if exp_avg_sq.shape != exp_avg.shape or scales.shape != (2, -(-n // BLOCK)):
+        raise RuntimeError(f"exp_avg_sq must have exp_avg's shape and scales (2, {-(-n // BLOCK)}), got "
+                           f"{tuple(exp_avg_sq.shape)} and {tuple(scales.shape)}")
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"dtype must be torch.float32 or torch.bfloat16, got {dtype}")
+    m, v, scales = exp_avg.contiguous(), exp_avg_sq.contiguous(), scales.contiguous()
+    out = [torch.empty(exp_avg.shape, device=exp_avg.device, dtype=dtype) for _ in range(2)]
+    with _t.on_device(exp_avg.device):
+        _t.check(_t.load().gs_adamw_values(
+            _t.DTYPE_CODES[dtype], n, m.data_ptr(), v.data_ptr(), scales.data_ptr(), scales.data_ptr() + scales.stride(0),
+            out[0].data_ptr(), out[1].data_ptr(), _t.stream(exp_avg.device)), "gs_adamw_values")
+    return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW whose step takes all tensors of a group through the device together.
+
+    bits: 32 or 8, of the moments.  State per parameter: 'step' (an integer), 'exp_avg',
+    'exp_avg_sq' and, with 8 bits, 'scales'; a state with another number of bits than the
+    group's is refused by the step.  Steps are counted on the host, so a step cannot be
+    captured in a graph; adamw_update can."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, bits=32, seed=0):
+        try:
+            _settings(lr, betas, eps, weight_decay)
+        except RuntimeError as e:
+            raise ValueError(str(e)) from None
+        if bits not in (8, 32) or not isinstance(seed, int):
+            raise ValueError(f"bits must be 8 or 32 and seed an integer, got {bits!r} and {seed!r}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits, seed=seed))
+
+    def load_state_dict(self, state_dict):
+        def take(state, loaded, p):
+            for name in ("exp_avg", "exp_avg_sq", "scales"):
+                if isinstance(loaded.get(name), torch.Tensor):
+                    state[name] = loaded[name].detach().to(p.device, copy=True).contiguous()
+            if "step" in loaded:
+                state["step"] = int(loaded["step"])
+
+        _t.load_uncast(self, super().load_state_dict, state_dict, take)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls = []
+        for group in self.param_groups:
+            alike = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if not state:
+                    state["step"] = 0
+                    state["exp_avg"], state["exp_avg_sq"], scales = new_moments(p, group["bits"])
+                    if scales is not None:
+                        state["scales"] = scales
+                if ("scales" in state) != (group["bits"] == 8):
+                    raise RuntimeError(f"a parameter's state has not the {group['bits']} bits of its group")
+                alike.setdefault((p.device, p.dtype, state["step"]), []).append((p, state))
+            calls += [(group, *key, pairs) for key, pairs in alike.items()]
+        if calls and calls[0][1].type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW counts its steps on the host and cannot be captured; adamw_update can")
+        for i, (group, _, _, step, pairs) in enumerate(calls):
+            params, states = zip(*pairs)
+            adamw_update(params, [p.grad for p in params], [s["exp_avg"] for s in states],
+                         [s["exp_avg_sq"] for s in states], step + 1, group["lr"], group["betas"], group["eps"],
+                         group["weight_decay"], [s["scales"] for s in states] if group["bits"] == 8 else None,
+                         group["seed"] + i)
+            for s in states:
+                s["step"] = step + 1
+        return loss

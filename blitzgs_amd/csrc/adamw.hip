@@ -1,0 +1,343 @@
+// One AdamW step over many tensors, moments in 32 bits or in 8.
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr decay) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+//
+// Every element is read and written once, so the step is bound by memory: 28
+// bytes an element with all in fp32, 16 with 8-bit moments, 10 with 16-bit
+// parameters beside them.  A launch takes up to MAX_TENSORS tensors, whose
+// addresses travel in its arguments; a workgroup finds its tensor by their first
+// workgroups and walks CHUNK elements at a time, eight neighbours to a lane.
+//
+// 8 bits.  BLOCK_8 neighbours share a power of two 2^e, that of the largest.  A
+// number over it is below 2 and is held as a small float with three bits of
+// mantissa: m with a sign and a 4-bit exponent (1 is exponent 14), v, which is
+// never negative, with a 5-bit one (1 is exponent 30).  b2 = 0.999 moves v by a
+// thousandth a step where a code's neighbours are a sixteenth away: to nearest it
+// would never move, so the rest is rounded up with its own probability, by 16
+// bits of a hash of the tensor's key and the element's index.  A code of all ones
+// (bar the sign) is NaN, which infinities become too; they leave their block's
+// power of two alone.  The step itself uses m and v before they are rounded.
+//
+// A code shifted to fp32's exponent is the number up to a power of two, below the
+// smallest exponent too, where both are subnormal: decoding and encoding are
+// multiplications by powers of two, without cases.
+#include <math.h>
+
+#include "gs_host.h"
+#include "gs_types.h"
+#include "../../include/blitzgs_amd.h"
+
+namespace {
+
+constexpr int MAX_TENSORS = 48;
+constexpr int THREADS = 256;
+constexpr int V = 8;                       // elements of a lane
+constexpr int CHUNK = THREADS * V;
+constexpr int BLOCK_8 = 128;               // elements that share a power of two: 16 lanes
+constexpr int TOP_M = 14, TOP_V = 30;      // exponent codes of 1
+
+struct Tensor {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    uint8_t* ms;
+    uint8_t* vs;
+    int64_t size;
+    uint32_t key;
+    uint32_t first;                        // workgroup
+};
+
+struct AdamArgs {
+    Tensor t[MAX_TENSORS];
+    int count;
+    int chunks;                            // of a workgroup
+    float b1, c1, b2, c2;                  // c = 1 - b
+    float keep, rate, root, eps;           // 1 - lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+};
+
+__host__ __device__ inline uint32_t scrambled(uint32_t x)
+{
+    // xor-shifts between products with the fractional parts of sqrt(2) and sqrt(3)
+    x ^= x >> 16;
+    x *= 0x6A09E667u;
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+constexpr uint32_t PHI = 0x9E3779B9u;      // of the golden ratio
+
+__device__ __forceinline__ float power(uint32_t biased)   // 2^(biased - 127)
+{
+    return __uint_as_float(biased == 0 ? 0x00400000u : biased << 23);
+}
+__device__ __forceinline__ float over_power(uint32_t biased)   // 2^(127 - biased)
+{
+    return __uint_as_float(biased >= 254 ? 0x00400000u : (254u - biased) << 23);
+}
+
+template <int TOP, bool SIGN>
+__device__ __forceinline__ float decoded(uint32_t code, float unit)
+{
+    constexpr uint32_t ONES = SIGN ? 127u : 255u;
+    const uint32_t c = code & ONES;
+    const float x = __uint_as_float(c << 20) * __uint_as_float((254u - TOP) << 23) * unit;
+    const float y = c == ONES ? __builtin_nanf("") : x;
+    return SIGN && (code & 128u) ? -y : y;
+}
+
+// x over its block's power of two, rounded up where its rest and draw / 2^16 make a step
+template <int TOP, bool SIGN>
+__device__ __forceinline__ uint32_t encoded(float x, float over, uint32_t draw)
+{
+    const float size = __builtin_fabsf(x) * over * __uint_as_float((uint32_t)TOP << 23);
+    uint32_t c = (__float_as_uint(size) + (draw << 4)) >> 20;
+    if (!(__builtin_fabsf(x) < __builtin_inff())) c = SIGN ? 127u : 255u;
+    return SIGN ? c | (c > 0 && x < 0.0f ? 128u : 0u) : c;
+}
+
+template <typename T, int BITS, bool WHOLE>
+__device__ __forceinline__ void step(const AdamArgs& A, const Tensor& t, int64_t at)
+{
+    T* p = (T*)t.p + at;
+    const T* g = (const T*)t.g + at;
+    const int n = WHOLE ? V : (int)(t.size - at < V ? t.size - at : V);   // may be negative
+    auto get = [&](const auto* from, auto& to) __attribute__((always_inline)) {
+        if constexpr (WHOLE) {
+            __builtin_memcpy(&to, from, sizeof(to));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (i < n) to[i] = from[i];
+        }
+    };
+    auto put = [&](auto* to, const auto& from) __attribute__((always_inline)) {
+        if constexpr (WHOLE) {
+            __builtin_memcpy(to, &from, sizeof(from));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (i < n) to[i] = from[i];
+        }
+    };
+    T tp[V] = {}, tg[V] = {};
+    float m[V] = {}, v[V] = {};
+    get((const T*)p, tp);
+    get(g, tg);
+    const int64_t block = at / BLOCK_8;
+    if constexpr (BITS == 32) {
+        get((const float*)t.m + at, m);
+        get((const float*)t.v + at, v);
+    } else {
+        uint8_t cm[V] = {}, cv[V] = {};
+        get((const uint8_t*)t.m + at, cm);
+        get((const uint8_t*)t.v + at, cv);
+        const float um = power(n > 0 ? t.ms[block] : 0), uv = power(n > 0 ? t.vs[block] : 0);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            m[i] = decoded<TOP_M, true>(cm[i], um);
+            v[i] = decoded<TOP_V, false>(cv[i], uv);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float gi = (float)tg[i];
+        m[i] = __builtin_fmaf(A.b1, m[i], A.c1 * gi);
+        v[i] = __builtin_fmaf(A.b2, v[i], A.c2 * gi * gi);
+        const float by = __builtin_fmaf(__builtin_sqrtf(v[i]), A.root, A.eps);
+        tp[i] = (T)__builtin_fmaf((float)tp[i], A.keep, -(A.rate * (m[i] / by)));
+    }
+    put(p, tp);
+    if constexpr (BITS == 32) {
+        put((float*)t.m + at, m);
+        put((float*)t.v + at, v);
+    } else {
+        // elements beyond the last are zero and change no maximum
+        uint32_t lm = 0, lv = 0;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const uint32_t a = __float_as_uint(m[i]) & 0x7fffffffu, b = __float_as_uint(v[i]) & 0x7fffffffu;
+            lm = max(lm, WHOLE || i < n ? (a < 0x7f800000u ? a : 0u) : 0u);
+            lv = max(lv, WHOLE || i < n ? (b < 0x7f800000u ? b : 0u) : 0u);
+        }
+#pragma unroll
+        for (int d = 1; d < BLOCK_8 / V; d <<= 1) {
+            lm = max(lm, (uint32_t)__shfl_xor((int)lm, d, 64));
+            lv = max(lv, (uint32_t)__shfl_xor((int)lv, d, 64));
+        }
+        const uint32_t em = lm >> 23, ev = lv >> 23;
+        const float om = over_power(em), ov = over_power(ev);
+        uint32_t place = (uint32_t)at * PHI + t.key + (uint32_t)(at >> 32) * 0x6A09E667u;
+        uint8_t cm[V], cv[V];
+#pragma unroll
+        for (int i = 0; i < V; i++, place += PHI) {
+            const uint32_t draw = scrambled(place);
+            cm[i] = (uint8_t)encoded<TOP_M, true>(m[i], om, draw & 0xffffu);
+            cv[i] = (uint8_t)encoded<TOP_V, false>(v[i], ov, draw >> 16);
+        }
+        put((uint8_t*)t.m + at, cm);
+        put((uint8_t*)t.v + at, cv);
+        if (n > 0 && at % BLOCK_8 == 0) {
+            t.ms[block] = (uint8_t)em;
+            t.vs[block] = (uint8_t)ev;
+        }
+    }
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(THREADS) void adamw_kernel(AdamArgs A)
+{
+    int lo = 0, hi = A.count - 1;          // the last tensor that begins at or before this workgroup
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (A.t[mid].first <= blockIdx.x) lo = mid; else hi = mid - 1;
+    }
+    const Tensor t = A.t[lo];
+    const int64_t begin = (int64_t)(blockIdx.x - t.first) * A.chunks * CHUNK;
+    for (int c = 0; c < A.chunks; c++) {
+        const int64_t from = begin + (int64_t)c * CHUNK;
+        if (from >= t.size) return;
+        // the lanes of a block of 128 go the same way
+        if (from + CHUNK <= t.size)
+            step<T, BITS, true>(A, t, from + threadIdx.x * V);
+        else
+            step<T, BITS, false>(A, t, from + threadIdx.x * V);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void adamw_values_kernel(int64_t size, const uint8_t* __restrict__ m,
+                                                               const uint8_t* __restrict__ v,
+                                                               const uint8_t* __restrict__ ms,
+                                                               const uint8_t* __restrict__ vs, T* __restrict__ mo,
+                                                               T* __restrict__ vo)
+{
+    for (int64_t at = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * V; at < size;
+         at += (int64_t)gridDim.x * CHUNK) {
+        const float um = power(ms[at / BLOCK_8]), uv = power(vs[at / BLOCK_8]);
+        if (at + V <= size) {
+            uint8_t cm[V], cv[V];
+            __builtin_memcpy(cm, m + at, V);
+            __builtin_memcpy(cv, v + at, V);
+            T tm[V], tv[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                tm[i] = (T)decoded<TOP_M, true>(cm[i], um);
+                tv[i] = (T)decoded<TOP_V, false>(cv[i], uv);
+            }
+            __builtin_memcpy(mo + at, tm, sizeof(tm));
+            __builtin_memcpy(vo + at, tv, sizeof(tv));
+        } else {
+            for (int64_t i = at; i < size; i++) {
+                mo[i] = (T)decoded<TOP_M, true>(m[i], um);
+                vo[i] = (T)decoded<TOP_V, false>(v[i], uv);
+            }
+        }
+    }
+}
+
+template <typename T>
+void launch(int bits, const AdamArgs& A, unsigned blocks, hipStream_t stream)
+{
+    if (bits == 32)
+        GS_TIMED("adamw_kernel", stream,
+                 hipLaunchKernelGGL((adamw_kernel<T, 32>), dim3(blocks), dim3(THREADS), 0, stream, A));
+    else
+        GS_TIMED("adamw_kernel", stream,
+                 hipLaunchKernelGGL((adamw_kernel<T, 8>), dim3(blocks), dim3(THREADS), 0, stream, A));
+}
+
+}  // namespace
+
+extern "C" int gs_adamw_update(int type, int bits, int count, const int64_t* sizes, void* const* params,
+                               const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
+                               uint8_t* const* exp_avg_scales, uint8_t* const* exp_avg_sq_scales,
+                               const gs_adamw_settings* settings, hipStream_t stream)
+{
+    gs::clear_error();
+    GS_REQUIRE(gs::dtype_known(type), "adamw: unknown element type %d", type);
+    GS_REQUIRE(bits == 8 || bits == 32, "adamw: moments have 8 or 32 bits, not %d", bits);
+    GS_REQUIRE(count >= 0, "adamw: count must not be negative");
+    GS_REQUIRE(settings != nullptr, "adamw: the settings must be non-null");
+    const double lr = settings->lr, beta1 = settings->beta1, beta2 = settings->beta2;
+    GS_REQUIRE(settings->step >= 1, "adamw: step must be at least 1");
+    GS_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw: the betas must be in [0, 1)");
+    GS_REQUIRE(lr >= 0.0 && settings->eps >= 0.0 && settings->weight_decay >= 0.0,
+               "adamw: lr, eps and weight_decay must not be negative");
+    if (count == 0) return GS_OK;
+    GS_REQUIRE(sizes && params && grads && exp_avgs && exp_avg_sqs, "adamw: the arrays must be non-null");
+    GS_REQUIRE(bits == 32 || (exp_avg_scales && exp_avg_sq_scales), "adamw: 8-bit moments need their scales");
+    for (int i = 0; i < count; i++) {
+        GS_REQUIRE(sizes[i] >= 0 && sizes[i] < (1ll << 40), "adamw: tensor %d has an impossible size", i);
+        if (sizes[i] == 0) continue;
+        GS_REQUIRE(params[i] && grads[i] && exp_avgs[i] && exp_avg_sqs[i], "adamw: tensor %d has a null pointer", i);
+        GS_REQUIRE(bits == 32 || (exp_avg_scales[i] && exp_avg_sq_scales[i]), "adamw: tensor %d has no scales", i);
+    }
+    AdamArgs A;
+    A.b1 = (float)beta1;
+    A.c1 = (float)(1.0 - beta1);
+    A.b2 = (float)beta2;
+    A.c2 = (float)(1.0 - beta2);
+    A.keep = (float)(1.0 - lr * settings->weight_decay);
+    A.rate = (float)(lr / (1.0 - pow(beta1, (double)settings->step)));
+    A.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)settings->step)));
+    A.eps = (float)settings->eps;
+    const uint32_t start = scrambled((uint32_t)settings->step * PHI + settings->seed);
+    A.chunks = 1;
+    for (int i = 0; i < count;) {
+        uint64_t blocks = 0;
+        A.count = 0;
+        for (; i < count && A.count < MAX_TENSORS; i++) {
+            if (sizes[i] == 0) continue;
+            const uint64_t n = ((uint64_t)sizes[i] + (uint64_t)A.chunks * CHUNK - 1) / ((uint64_t)A.chunks * CHUNK);
+            if (A.count > 0 && blocks + n > 0x7fffffffu) break;
+            Tensor& t = A.t[A.count++];
+            t.p = params[i];
+            t.g = grads[i];
+            t.m = exp_avgs[i];
+            t.v = exp_avg_sqs[i];
+            t.ms = bits == 8 ? exp_avg_scales[i] : nullptr;
+            t.vs = bits == 8 ? exp_avg_sq_scales[i] : nullptr;
+            t.size = sizes[i];
+            t.key = scrambled((uint32_t)i * PHI + start);
+            t.first = (uint32_t)blocks;
+            blocks += n;
+        }
+        if (blocks == 0) continue;
+        if (type == GS_F32)
+            launch<float>(bits, A, (unsigned)blocks, stream);
+        else if (type == GS_BF16)
+            launch<gs::bf16>(bits, A, (unsigned)blocks, stream);
+        else
+            launch<gs::f16>(bits, A, (unsigned)blocks, stream);
+        GS_LAUNCH_CHECK("adamw_kernel");
+    }
+    return GS_OK;
+}
+
+extern "C" int gs_adamw_values(int type, int64_t size, const uint8_t* exp_avg, const uint8_t* exp_avg_sq,
+                               const uint8_t* exp_avg_scale, const uint8_t* exp_avg_sq_scale, void* exp_avg_out,
+                               void* exp_avg_sq_out, hipStream_t stream)
+{
+    gs::clear_error();
+    GS_REQUIRE(type == GS_F32 || type == GS_BF16, "adamw: values are float32 or bfloat16, not type %d", type);
+    GS_REQUIRE(size >= 0, "adamw: size must not be negative");
+    if (size == 0) return GS_OK;
+    GS_REQUIRE(exp_avg && exp_avg_sq && exp_avg_scale && exp_avg_sq_scale && exp_avg_out && exp_avg_sq_out,
+               "adamw: the moments and their values must be non-null");
+    const int64_t n = (size + CHUNK - 1) / CHUNK;
+    const dim3 blocks((unsigned)(n < 65536 ? n : 65536));
+    if (type == GS_F32)
+        GS_TIMED("adamw_values_kernel", stream,
+                 hipLaunchKernelGGL((adamw_values_kernel<float>), blocks, dim3(THREADS), 0, stream, size, exp_avg,
+                                    exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, (float*)exp_avg_out,
+                                    (float*)exp_avg_sq_out));
+    else
+        GS_TIMED("adamw_values_kernel", stream,
+                 hipLaunchKernelGGL((adamw_values_kernel<gs::bf16>), blocks, dim3(THREADS), 0, stream, size, exp_avg,
+                                    exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, (gs::bf16*)exp_avg_out,
+                                    (gs::bf16*)exp_avg_sq_out));
+    GS_LAUNCH_CHECK("adamw_values_kernel");
+    return GS_OK;
+}

@@ -71,26 +71,12 @@ class OrthogonalMomentum(torch.optim.Optimizer):
                                       steps=steps))
 
     def load_state_dict(self, state_dict):
-        # torch's loading casts a state to its parameter's type, so the buffers are
-        # taken once more from what it loads: after all hooks that may change that,
-        # and before any that look at the result
-        loaded = {}
+        def take(state, loaded, p):
+            buffer = loaded.get("momentum_buffer")
+            if isinstance(buffer, torch.Tensor):
+                state["momentum_buffer"] = buffer.detach().to(p.device, torch.float32, copy=True).contiguous()
 
-        def restore(_):
-            ours = (p for group in self.param_groups for p in group["params"])
-            for key, p in zip((k for group in loaded["param_groups"] for k in group["params"]), ours):
-                buffer = loaded["state"].get(key, {}).get("momentum_buffer")
-                if isinstance(buffer, torch.Tensor):
-                    buffer = buffer.detach().to(p.device, torch.float32, copy=True)
-                    self.state[p]["momentum_buffer"] = buffer.contiguous()
-
-        hooks = [self.register_load_state_dict_pre_hook(lambda _, state: loaded.update(state)),
-                 self.register_load_state_dict_post_hook(restore, prepend=True)]
-        try:
-            super().load_state_dict(state_dict)
-        finally:
-            for hook in hooks:
-                hook.remove()
+        _t.load_uncast(self, super().load_state_dict, state_dict, take)
 
     def _buffer(self, p):
         state = self.state[p]

@@ -1,0 +1,203 @@
+"""rotate, norm_rotate: rotary positions of queries and keys, alone or after the RMS
+norm of every head, in one pass, with their gradients.
+
+    u = x, or weight x / sqrt(mean(x^2) + eps) over the head's D elements
+    y1 = magnitude (u1 cos - u2 sin),  y2 = magnitude (u1 sin + u2 cos)
+
+for N pairs of elements, (i, i + N) or, interleaved, (2 i, 2 i + 1), by the angle
+position * frequency of the pair; elements from 2 N on are u.  q is (B, Hq, T, D), k
+(B, Hk, T, D) or None, as attention takes them: float32, bfloat16 or float16, one
+type for both, D from 1 to 256, any strides with the last dimension contiguous.
+Results lie in memory as (B, T, H, D).  Weights have the rows' type or float32.
+
+positions are int32 or int64, (T,) or (B, T).  Tokens of an image or a volume have
+several, (T, axes) or (B, T, axes), with frequencies of shape (axes, pairs): each
+axis turns pairs of its own.
+
+frequencies are int64, in 2^-64ths of a turn per position: position * frequency is
+formed modulo a turn, without error however far the position, and its cosine and sine
+in float32.  rotary_frequencies makes the usual ones, also scaled for contexts longer
+than those of the training, as_turns makes them from any angles.
+
+Sums are fp32, each output is rounded to its type once.  A row whose squares pass
+fp32's range (elements of 1e18 and more) becomes zero under the norm.  The weights'
+gradients are added up in a fixed order: equal inputs give equal bits.
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import _tensors as _t
+
+MAX_HEAD_DIM = 256
+
+_Strides = C.c_int64 * 3
+
+
+def as_turns(radians, device=None):
+    """Angles per position (a tensor or sequence of numbers, in radians) as frequencies."""
+    if not isinstance(radians, torch.Tensor):
+        radians, device = torch.tensor(radians, dtype=torch.float64), "cuda" if device is None else device
+    turns = radians.detach().to("cpu", torch.float64) / (2 * math.pi)
+    if not bool(torch.isfinite(turns).all()):
+        raise RuntimeError("frequencies must be finite")
+    # whole turns do not count: what is left, in [-1/2, 1/2), as a 64-bit integer
+    turns = turns - torch.floor(turns + 0.5)
+    return torch.clamp(turns * 2.0 ** 64, -2.0 ** 63, 2.0 ** 63 - 1024).to(torch.int64).to(
+        radians.device if device is None else device)
+
+
+def rotary_frequencies(pairs, base=10000.0, factor=1.0, trained=None, ramp=(1.0, 32.0), axes=1, device="cuda"):
+    """The frequencies base^(-i / pairs) radians per position, i in 0 .. pairs - 1: (pairs,), or (axes, pairs).
+
+    factor > 1 stretches them for contexts that much longer: all of them, or, with
+    `trained` (the positions of the training), only the slow ones: a pair that turns fewer
+    than ramp[0] times over them is divided by factor, one that turns more than ramp[1]
+    times is left as it is, and between the two the share falls linearly."""
+    if pairs < 1 or axes < 1:
+        raise RuntimeError(f"pairs and axes must be at least 1, got {pairs} and {axes}")
+    if not 0.0 < base < math.inf or not 0.0 < factor < math.inf:
+        raise RuntimeError(f"base and factor must be positive numbers, got {base} and {factor}")
+    radians = torch.tensor([base ** (-i / pairs) for i in range(pairs)], dtype=torch.float64)
+    if trained is None:
+        radians = radians / factor
+    else:
+        slow, fast = ramp
+        if not trained > 0 or not 0.0 <= slow < fast:
+            raise RuntimeError(f"trained must be positive and ramp two rising numbers, got {trained} and {ramp}")
+        kept = ((radians * trained / (2 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        radians = radians * (kept + (1.0 - kept) / factor)
+    turns = as_turns(radians, device)
+    return turns if axes == 1 else turns.expand(axes, pairs).contiguous()
+
+
+def _last_contiguous(t):
+    return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _strides(t):
+    return None if t is None else _Strides(*t.stride()[:3])
+
+
+def _token_major(like):
+    B, H, T, D = like.shape
+    return torch.empty_strided((B, H, T, D), (T * H * D, D, H * D, 1), device=like.device, dtype=like.dtype)
+
+
+class _How:
+    """What a call passes to the library beside its tensors."""
+
+    def __init__(self, q, k, weight, frequencies, interleaved, magnitude, norm, eps):
+        B, Hq, T, D = q.shape
+        code = _t.DTYPE_CODES[q.dtype]
+        axes, pairs = (1, frequencies.shape[0]) if frequencies.dim() == 1 else frequencies.shape
+        self.sizes = code, B, Hq, 0 if k is None else k.shape[1], T, D, axes, pairs
+        self.params = q.dtype if weight is None else weight.dtype
+        self.first = code, _t.DTYPE_CODES[self.params], *self.sizes[1:], interleaved, magnitude, norm, eps
+
+    def angles(self, positions, frequencies):
+        B, T, axes = self.sizes[1], self.sizes[4], self.sizes[6]
+        strides = list(positions.stride())
+        if frequencies.dim() == 1:
+            strides.append(0)
+        if len(strides) == 2:
+            strides.insert(0, 0)
+        return positions.data_ptr(), int(positions.dtype == torch.int64), _Strides(*strides), frequencies.data_ptr()
+
+
+def _forward(q, k, qw, kw, positions, frequencies, how):
+    qy, ky = _token_major(q), None if k is None else _token_major(k)
+    with _t.on_device(q.device):
+        _t.check(_t.load().gs_rotary_forward(
+            *how.first, q.data_ptr(), _strides(q), _t.ptr(k), _strides(k), _t.ptr(qw), _t.ptr(kw),
+            *how.angles(positions, frequencies), qy.data_ptr(), _strides(qy), _t.ptr(ky), _strides(ky),
+            _t.stream(q.device)), "gs_rotary_forward")
+    return qy, ky
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, positions, frequencies, how):
+        q, k = _last_contiguous(q.detach()), None if k is None else _last_contiguous(k.detach())
+        ctx.how, ctx.like = how, (q.shape, None if k is None else k.shape, q.dtype)
+        norm = how.first[-2]
+        ctx.save_for_backward(*((q, k) if norm else (None, None)), qw, kw, positions, frequencies)
+        return _forward(q, k, qw, kw, positions, frequencies, how)
+
+    # The autograd engine calls this from a thread of its own, on the forward's
+    # device and stream.
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dqy, dky):
+        # hooks on saved tensors give them back with the same values, not in the same places
+        q, k, qw, kw, positions, frequencies = ctx.saved_tensors
+        q, k, dqy, dky = (_last_contiguous(t) for t in (q, k, dqy, dky))
+        qw, kw, frequencies = (t if t is None else t.contiguous() for t in (qw, kw, frequencies))
+        how, need = ctx.how, ctx.needs_input_grad
+        device, norm = frequencies.device, how.first[-2]
+        dq = _token_major(dqy) if need[0] or need[2] else None
+        dk = _token_major(dky) if dky is not None and (need[1] or need[3]) else None
+        dqw = torch.empty(qw.shape, device=device, dtype=how.params) if need[2] else None
+        dkw = torch.empty(kw.shape, device=device, dtype=how.params) if need[3] and dk is not None else None
+        lib = _t.load()
+        ws = _t.workspace(lib.gs_rotary_workspace_bytes(*how.sizes), device) if norm and (need[2] or need[3]) else None
+        _t.check(lib.gs_rotary_backward(
+            *how.first, _t.ptr(q), _strides(q), _t.ptr(k), _strides(k), _t.ptr(qw), _t.ptr(kw),
+            *how.angles(positions, frequencies), dqy.data_ptr(), _strides(dqy), _t.ptr(dky), _strides(dky),
+            _t.ptr(dq), _strides(dq), _t.ptr(dk), _strides(dk), _t.ptr(dqw), _t.ptr(dkw), _t.ptr(ws),
+            _t.stream(device)), "gs_rotary_backward")
+        return dq if need[0] else None, dk if need[1] else None, dqw, dkw, None, None, None
+
+
+def _call(q, k, qw, kw, positions, frequencies, interleaved, magnitude, norm, eps):
+    _t.require_tensor(q, "q")
+    if q.dim() != 4 or not 1 <= q.shape[3] <= MAX_HEAD_DIM:
+        raise RuntimeError(f"q must have dimensions (B, H, T, D) with D of 1 to {MAX_HEAD_DIM}, got shape "
+                           f"{tuple(q.shape)}")
+    B, _, T, D = q.shape
+    if k is not None:
+        _t.require_tensor(k, "k", device=q.device)
+        if k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (B, T, D):
+            raise RuntimeError("k must have q's type, batch, tokens and head dimension; got q "
+                               f"{tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}")
+    if (not isinstance(frequencies, torch.Tensor) or frequencies.dtype != torch.int64 or frequencies.device != q.device
+            or frequencies.dim() not in (1, 2) or frequencies.numel() == 0 or 2 * frequencies.numel() > D):
+        raise RuntimeError(f"frequencies must be an int64 tensor of shape (pairs,) or (axes, pairs) on {q.device}, of at "
+                           f"most D / 2 = {D // 2} pairs in all")
+    ends = ((T,), (B, T)) if frequencies.dim() == 1 else ((T, frequencies.shape[0]), (B, T, frequencies.shape[0]))
+    if (not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64)
+            or positions.device != q.device or tuple(positions.shape) not in ends):
+        raise RuntimeError(f"positions must be an int32 or int64 tensor of shape {ends[0]} or {ends[1]} on {q.device}")
+    if not abs(magnitude) <= 3e38:
+        raise RuntimeError(f"magnitude must be a number of at most 3e38, got {magnitude}")
+    if not 0.0 <= eps < math.inf:
+        raise RuntimeError(f"eps must be a finite number of at least 0, got {eps}")
+    for name, w in (("q_weight", qw), ("k_weight", kw)):
+        if w is None:
+            continue
+        _t.require_tensor(w, name, device=q.device)
+        if w.shape != (D,) or w.dtype not in (q.dtype, torch.float32):
+            raise RuntimeError(f"{name} must have shape ({D},) and be {q.dtype} or torch.float32, got "
+                               f"{tuple(w.shape)} {w.dtype}")
+    if qw is not None and kw is not None and qw.dtype != kw.dtype:
+        raise RuntimeError(f"q_weight and k_weight must have one type, got {qw.dtype} and {kw.dtype}")
+    if kw is not None and k is None:
+        raise RuntimeError("k_weight needs k")
+    qw, kw = (None if w is None else w.contiguous() for w in (qw, kw))
+    frequencies = frequencies.contiguous()
+    how = _How(q, k, kw if qw is None else qw, frequencies, int(bool(interleaved)), float(magnitude), norm, float(eps))
+    if _t.wants_grad(q, k, qw, kw):
+        return _Rotary.apply(q, k, qw, kw, positions, frequencies, how)
+    return _forward(_last_contiguous(q), _last_contiguous(k), qw, kw, positions, frequencies, how)
+
+
+def rotate(q, k, positions, frequencies, interleaved=False, magnitude=1.0):
+    """q and k (or None) rotated to their positions; differentiable in both.  Returns the two."""
+    return _call(q, k, None, None, positions, frequencies, interleaved, magnitude, 0, 0.0)
+
+
+def norm_rotate(q, k, q_weight, k_weight, positions, frequencies, interleaved=False, magnitude=1.0, eps=1e-6):
+    """The same of each head's rows over their root mean square, times weights (D,) or None; differentiable in q, k
+    and the weights."""
+    return _call(q, k, q_weight, k_weight, positions, frequencies, interleaved, magnitude, 1, eps)

@@ -706,6 +706,65 @@ int gs_attention_backward(int type, int B, int Hq, int Hkv, int Tq, int Tk, int 
                           const int64_t* dk_strides, void* dv, const int64_t* dv_strides,
                           void* workspace, gs_stream_t stream);
 
+/* Rotary positions of queries and keys, q (B, Hq, T, D) and k (B, Hk, T, D), D from
+ * 1 to 256: element pairs are rotated by position * frequency, times magnitude, of
+ * N = axes * pairs pairs (2 N <= D), pair i of elements (i, i + N) or, interleaved,
+ * (2 i, 2 i + 1); elements from 2 N on are not rotated.  Pair i turns with axis
+ * i / pairs.  With `norm` each row of D elements is first divided by
+ * sqrt(mean(x^2) + eps) and multiplied by its weight (D, of param_type: `type` or
+ * GS_F32; NULL: ones).
+ *   frequencies (N): 2^-64ths of a turn per position; position * frequency is
+ * formed modulo 2^64, so no position is too far.  positions: int32, or int64 with
+ * `wide`; position_strides of batch, token and axis, in elements, any may be 0.
+ *   Tensors come with three strides in elements, of batch, head and token; D is
+ * contiguous; outputs may not overlap inputs.  A side without heads is left out.
+ *   Backward: from the gradients of the outputs, dq and dk (either may be NULL: not
+ * formed) and, with norm, the weights' gradients unless NULL, each together with
+ * its rows', added up in a fixed order through the workspace of
+ * gs_rotary_workspace_bytes.  Without norm q and k are not read. */
+int gs_rotary_forward(int type, int param_type, int B, int Hq, int Hk, int T, int D, int axes,
+                      int pairs, int interleaved, float magnitude, int norm, float eps,
+                      const void* q, const int64_t* q_strides, const void* k,
+                      const int64_t* k_strides, const void* q_weight, const void* k_weight,
+                      const void* positions, int wide, const int64_t* position_strides,
+                      const int64_t* frequencies, void* q_out, const int64_t* q_out_strides,
+                      void* k_out, const int64_t* k_out_strides, gs_stream_t stream);
+size_t gs_rotary_workspace_bytes(int type, int B, int Hq, int Hk, int T, int D, int axes,
+                                 int pairs);
+int gs_rotary_backward(int type, int param_type, int B, int Hq, int Hk, int T, int D, int axes,
+                       int pairs, int interleaved, float magnitude, int norm, float eps,
+                       const void* q, const int64_t* q_strides, const void* k,
+                       const int64_t* k_strides, const void* q_weight, const void* k_weight,
+                       const void* positions, int wide, const int64_t* position_strides,
+                       const int64_t* frequencies, const void* dq_out,
+                       const int64_t* dq_out_strides, const void* dk_out,
+                       const int64_t* dk_out_strides, void* dq, const int64_t* dq_strides,
+                       void* dk, const int64_t* dk_strides, void* dq_weight, void* dk_weight,
+                       void* workspace, gs_stream_t stream);
+
+/* The gated feed-forward block: y = (act(x gate^T) * (x up^T)) down^T of x (rows,
+ * width), gate and up (hidden, width), down (out, hidden), y (rows, out); act is
+ * GS_SILU, a / (1 + exp(-a)), or GS_GELU, a (1 + erf(a / sqrt(2))) / 2.  x's (and
+ * dy's) rows are x_stride elements apart and contiguous inside, all else is
+ * contiguous.  h (rows, hidden) is written: act(a) * b of a = x gate^T, b = x up^T,
+ * rounded to `type`; a and b (rows, hidden) too, for the backward, or both NULL.
+ *   Backward, from a, b and h: dx, dgate, dup, ddown, each unless NULL.
+ *   workspace: 256-byte aligned, of gs_feed_forward_workspace_bytes (0: none is
+ * needed, or the arguments are invalid). */
+#define GS_SILU 0
+#define GS_GELU 1
+size_t gs_feed_forward_workspace_bytes(int type, int64_t rows, int width, int hidden, int out,
+                                       int backward);
+int gs_feed_forward(int type, int activation, int64_t rows, int width, int hidden, int out,
+                    const void* x, int64_t x_stride, const void* gate, const void* up,
+                    const void* down, void* a, void* b, void* h, void* y, void* workspace,
+                    gs_stream_t stream);
+int gs_feed_forward_backward(int type, int activation, int64_t rows, int width, int hidden, int out,
+                             const void* x, int64_t x_stride, const void* gate, const void* up,
+                             const void* down, const void* a, const void* b, const void* h,
+                             const void* dy, int64_t dy_stride, void* dx, void* dgate, void* dup,
+                             void* ddown, void* workspace, gs_stream_t stream);
+
 /* The orthogonalised update of `count` matrices (m, n), contiguous: `steps` (1
  * to 32) steps of A = X X^T, X = a X + (b A + c A A) X with (a, b, c) =
  * (3.4445, -4.7750, 2.0315) from X = update / (|update|_F + 1e-7), over the
@@ -727,6 +786,41 @@ int gs_momentum_update(int type, int count, int64_t size, const void* const* gra
                        gs_stream_t stream);
 int gs_momentum_apply(int type, int count, int64_t size, void* const* params, float keep, float lr,
                       const float* update, gs_stream_t stream);
+
+/* One AdamW step, number `step` (from 1 on) of host-side `settings`, over `count`
+ * tensors; the arrays are host arrays, of sizes in elements and of device pointers to contiguous tensors:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay)
+ *       - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * params and grads are of `type`, the moments of 32 bits (float32) or 8.  With 8
+ * the elements of a tensor share in blocks of 128 a power of two 2^(scale - 127),
+ * one byte each in exp_avg_scales and exp_avg_sq_scales (NULL with 32 bits), that of
+ * the block's largest (scale 0: 2^-127 or less); a first moment's byte is a sign, four bits of exponent (1 is
+ * 14) and three of mantissa, a second one's five (1 is 30) and three, both with
+ * subnormals, and all ones (the sign apart) is NaN.  Bytes and scales of zero are a
+ * moment of zero.  They are rounded up with the probability of what is left, by
+ * 16 bits each of s(s(i phi + s(step phi + seed)) + element phi), modulo 2^32,
+ * where i is the tensor's place in the arrays, phi = 0x9E3779B9 and
+ *   s(x): x ^= x >> 16; x *= 0x6A09E667; x ^= x >> 15; x *= 0xBB67AE85; x ^= x >> 16.
+ * Tensors may not overlap.
+ *   gs_adamw_values: the values of 8-bit moments, GS_F32 or GS_BF16. */
+typedef struct gs_adamw_settings {
+    double lr;
+    double beta1;
+    double beta2;
+    double eps;
+    double weight_decay;
+    int64_t step;
+    uint32_t seed;
+} gs_adamw_settings;
+
+int gs_adamw_update(int type, int bits, int count, const int64_t* sizes, void* const* params,
+                    const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
+                    uint8_t* const* exp_avg_scales, uint8_t* const* exp_avg_sq_scales,
+                    const gs_adamw_settings* settings, gs_stream_t stream);
+int gs_adamw_values(int type, int64_t size, const uint8_t* exp_avg, const uint8_t* exp_avg_sq,
+                    const uint8_t* exp_avg_scale, const uint8_t* exp_avg_sq_scale,
+                    void* exp_avg_out, void* exp_avg_sq_out, gs_stream_t stream);
 
 /* ------------------------------------------------------------------------ *
  * Per-kernel timing (the counterpart of the reference's MyTimerOnGPU,
