@@ -19,6 +19,8 @@
 // Sums are fp32.  Rounded to the tensors' type: each output once, h, and for the
 // backward a, b, da and db, since they are operands of the next product: float16's
 // range holds for them too.
+#include <atomic>
+
 #include "gs_host.h"
 #include "gs_matrix.h"
 #include "../../include/blitzgs_amd.h"
@@ -53,6 +55,15 @@ struct FeedArgs {
 
 __device__ __align__(16) const uint32_t zeros[4] = {0, 0, 0, 0};
 
+// All waves' loads to LDS are there, and all waves are done with what they read: a
+// barrier alone waits for neither where the compiler sees that this wave's own reads
+// need not.
+__device__ __forceinline__ void arrived()
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // act(a) and its derivative
 __device__ __forceinline__ void activation(int act, float a, float& value, float& slope)
 {
@@ -75,12 +86,15 @@ __device__ __forceinline__ void activation(int act, float a, float& value, float
 //   DIRECT: straight to LDS, 16 bytes at a time; chunks are whole and aligned.  What
 //           lies beyond the depth comes from `zeros`; beyond the last row or column
 //           the last one comes again, whose results nobody keeps.
-//   else:   through registers, element by element at the edges
+//   else:   through registers, element by element
 template <typename T, int S, bool DOWN, int THREADS, bool DIRECT>
 struct Operand {
     static constexpr int KT = 128 / (int)sizeof(T), V = gs::Vec<T>::N, CH = S * 8 / THREADS;
-    static_assert(CH >= 1, "a chunk per thread");
+    static_assert(CH >= 1 && THREADS % 256 == 0, "a chunk per thread, 32 rows or more per access");
     using L = gs::Tile<T, KT>;
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+
+    uint32_t at[CH];   // bytes from the tile's corner
 
     // place `id` of the tile holds k (or the chunk of k from there) and row of the result
     __device__ static __forceinline__ void place(int id, int& row, int& k)
@@ -95,36 +109,62 @@ struct Operand {
             k = col;
         }
     }
-
-    // Fetches the tile whose depth begins at k0.  pick(row): the pointer to a row of the result's
-    // operand (along), or to its column in row 0 (DOWN).
-    template <typename Pick>
-    __device__ static __forceinline__ void fetch(uint4* to, int k0, int depth, int limit, int64_t ld, Pick pick)
+    // map(row): the place of the result's row among the operand's rows (DOWN: columns), of which there are `limit`
+    template <typename Map>
+    __device__ __forceinline__ Operand(int64_t ld, int limit, Map map)
     {
-        typedef const __attribute__((address_space(1))) void* global_ptr;
-        typedef __attribute__((address_space(3))) void* lds_ptr;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             int row, k;
             place(threadIdx.x + THREADS * c, row, k);
-            k += k0;
-            if constexpr (DIRECT) {
-                const T* p = DOWN ? pick(row) + (int64_t)k * ld : pick(row) + k;
-                const void* from = k < depth ? (const void*)p : (const void*)zeros;
-                __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(to + THREADS * c + (threadIdx.x & ~63u)),
-                                                 16, 0, 0);
-            } else {
-                gs::Vec<T> v = {};
+            row = map(row);
+            if constexpr (DOWN) at[c] = (uint32_t)(((int64_t)k * ld + min(row, limit - V)) * (int)sizeof(T));
+            else at[c] = (uint32_t)(((int64_t)min(row, limit - 1) * ld + k) * (int)sizeof(T));
+        }
+    }
+    // DIRECT: the tile at `from`, of which `depth` is there
+    __device__ __forceinline__ void fetch(uint4* to, const T* from, int depth) const
+    {
+        const char* base = (const char*)from;
+        uint4* mine = to + (threadIdx.x & ~63u);   // + 16 bytes per lane
+        // As buffer loads: the compiler takes global ones to LDS for accesses of any kind, and
+        // waits for all LDS reads while one is under way.  Their offsets are below `span`.
+        const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x27000);
+        if (depth >= KT) {
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    if constexpr (DOWN) {
-                        if (k < depth && row + e < limit) v.v[e] = pick(row)[(int64_t)k * ld + e];
-                    } else {
-                        if (k + e < depth && row < limit) v.v[e] = pick(row)[k + e];
-                    }
-                }
-                to[threadIdx.x + THREADS * c] = __builtin_bit_cast(uint4, v);
+            for (int c = 0; c < CH; c++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(all, (lds_ptr)(mine + THREADS * c), 16, (int)at[c], 0, 0, 0);
+        } else {
+            const __amdgpu_buffer_rsrc_t none = __builtin_amdgcn_make_buffer_rsrc((void*)zeros, 0, 16, 0x27000);
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                int row, k;
+                place(threadIdx.x + THREADS * c, row, k);
+                if (k < depth)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(all, (lds_ptr)(mine + THREADS * c), 16, (int)at[c], 0, 0, 0);
+                else
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(none, (lds_ptr)(mine + THREADS * c), 16, 0, 0, 0, 0);
             }
+        }
+    }
+    // else: the same, of which `limit` rows (DOWN: columns) are there
+    template <typename Map>
+    __device__ static __forceinline__ void gather(uint4* to, const T* from, int depth, int64_t ld, int limit, Map map)
+    {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            int row, k;
+            place(threadIdx.x + THREADS * c, row, k);
+            gs::Vec<T> v = {};
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                if constexpr (DOWN) {
+                    if (k < depth && map(row) + e < limit) v.v[e] = from[(int64_t)k * ld + map(row) + e];
+                } else {
+                    if (k + e < depth && map(row) < limit) v.v[e] = from[(int64_t)map(row) * ld + k + e];
+                }
+            }
+            to[threadIdx.x + THREADS * c] = __builtin_bit_cast(uint4, v);
         }
     }
 };
@@ -159,23 +199,26 @@ __device__ __forceinline__ void get(const T* p, float* v, int n)
     for (int i = 0; i < N; i++) v[i] = (float)t[i];
 }
 
-// S x S of the result; waves in a grid of WM x WN.
-template <typename T, Kind K, bool LDOWN, bool RDOWN, int S, int WM, int WN, bool DIRECT>
-__global__ __launch_bounds__(64 * WM * WN, S == 256 ? 2 : 1) void feed_kernel(FeedArgs A)
+// SM x SN of the result; waves in a grid of WM x WN.
+template <typename T, Kind K, bool LDOWN, bool RDOWN, int SM, int SN, int WM, int WN, bool DIRECT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void feed_kernel(FeedArgs A)
 {
-    constexpr int THREADS = 64 * WM * WN, KT = 128 / (int)sizeof(T), WORDS = S * 8;
-    constexpr int HM = S / WM, HN = S / WN, MT = HM / 16, NT = HN / 16;   // of a wave
-    using OL = Operand<T, S, LDOWN, THREADS, DIRECT>;
-    using OR = Operand<T, S, RDOWN, THREADS, DIRECT>;
+    constexpr int THREADS = 64 * WM * WN, KT = 128 / (int)sizeof(T), LW = SM * 8, RW = SN * 8;
+    constexpr int HM = SM / WM, HN = SN / WN, MT = HM / 16, NT = HN / 16;   // of a wave
+    using OL = Operand<T, SM, LDOWN, THREADS, DIRECT>;
+    using OR = Operand<T, SN, RDOWN, THREADS, DIRECT>;
     extern __shared__ uint4 lds[];                   // [2][left, right]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int which = 0;
     const uint32_t place = gs::xcd_item(blockIdx.x, gridDim.x);
     while (which + 1 < A.count && (int)place >= A.p[which + 1].first) which++;
     const Product& P = A.p[which];
     const int item = (int)place - P.first, tile_item = item / A.splits, split = item % A.splits;
-    const int tm = tile_item % P.tiles_m, tn = tile_item / P.tiles_m;
-    const int m0 = tm * S, n0 = tn * (K == HIDDEN ? S / 2 : S);
+    // runs of eight rows of tiles: the 32 tiles that an XCD works on at a time are 8 x 4
+    const int run = tile_item / (8 * P.tiles_n), high = min(8, P.tiles_m - 8 * run), in_run = tile_item - run * 8 * P.tiles_n;
+    const int tm = 8 * run + in_run % high, tn = in_run / high;
+    const int m0 = tm * SM, n0 = tn * (K == HIDDEN ? SN / 2 : SN);
     const int wm = wave % WM * HM, wn = wave / WM * HN;
 
     f4 acc[NT][MT];
@@ -186,59 +229,109 @@ __global__ __launch_bounds__(64 * WM * WN, S == 256 ? 2 : 1) void feed_kernel(Fe
 
     const int per = (P.depth + KT - 1) / KT, all = K == SUM ? 2 * per : per;
     const int begin = (int)((int64_t)all * split / A.splits), end = (int)((int64_t)all * (split + 1) / A.splits);
-    const gs::Tile<T, KT> tile;
-    auto fetch = [&](int t, uint4* to) __attribute__((always_inline)) {
-        const int second = K == SUM && t >= per;
-        const int k0 = (t - second * per) * KT;
-        const T* l = (const T*)P.l[second];
-        const T* r = (const T*)P.r[second];
-        OL::fetch(to, k0, P.depth, P.rows - m0, P.lld, [&](int row) {
-            const int at = m0 + row;
-            if constexpr (LDOWN) return l + (DIRECT ? min(at, P.rows - OL::V) : at);
-            else return l + (int64_t)(DIRECT ? min(at, P.rows - 1) : at) * P.lld;
-        });
-        OR::fetch(to + WORDS, k0, P.depth, K == HIDDEN ? S : P.cols - n0, P.rld, [&](int row) {
-            if constexpr (K == HIDDEN) {
-                // 16 of the gate's rows, then 16 of up's; rows beyond the last hold the last again
-                const int at = min(n0 + row / 32 * 16 + row % 16, P.cols - 1);
-                return (const T*)P.r[row / 16 % 2] + (int64_t)at * P.rld;
-            } else {
-                const int at = n0 + row;
-                if constexpr (RDOWN) return r + (DIRECT ? min(at, P.cols - OR::V) : at);
-                else return r + (int64_t)(DIRECT ? min(at, P.cols - 1) : at) * P.rld;
-            }
-        });
-    };
-    // two restricted pointers tell the compiler that the loads need not have arrived
-    // before the reads
-    auto step = [&](int t, const uint4* __restrict__ at, uint4* __restrict__ next) __attribute__((always_inline)) {
-        __syncthreads();   // tile t is there for all waves, and all are done with tile t - 1
-        if (t + 1 < end) fetch(t + 1, next);
-#pragma unroll
-        for (int k = 0; k < KT; k += 32) {
-            Frag<T> l[MT];
-#pragma unroll
-            for (int v = 0; v < MT; v++) {
-                const int row = wm + 16 * v;
-                if constexpr (LDOWN) l[v] = tile.cols(at + row / KT * (8 * KT), k, row % KT);
-                else l[v] = tile.rows(at, row, k);
-            }
-#pragma unroll
-            for (int u = 0; u < NT; u++) {
-                const int row = wn + 16 * u;
-                Frag<T> r;
-                if constexpr (RDOWN) r = tile.cols(at + WORDS + row / KT * (8 * KT), k, row % KT);
-                else r = tile.rows(at + WORDS, row, k);
-#pragma unroll
-                for (int v = 0; v < MT; v++) acc[u][v] = gs::mma(r, l[v], acc[u][v]);
-            }
+    // 16 rows of the gate, then 16 of up; a wave's eight rows of an access are of one
+    const int which_r = K == HIDDEN ? wave / 2 % 2 : 0;
+    auto left = [](int row) { return row; };
+    auto right = [](int row) { return K == HIDDEN ? row / 32 * 16 + row % 16 : row; };
+    const int lrows = P.rows - m0, rrows = P.cols - n0;
+    const OL ol(P.lld, lrows, left);
+    const OR orr(P.rld, rrows, right);
+    // The next tile's corners, how much of the depth is left there, and the steps to the
+    // tile after it; held in registers, so that the loop reads no arguments (whose loads
+    // would be waited for together with those from LDS).
+    const int second = K == SUM && begin >= per, k0 = (begin - second * per) * KT;
+    const T* lp = (const T*)P.l[second] + (LDOWN ? (int64_t)k0 * P.lld + m0 : (int64_t)m0 * P.lld + k0);
+    const T* rp = (const T*)P.r[second + which_r] + (RDOWN ? (int64_t)k0 * P.rld + n0 : (int64_t)n0 * P.rld + k0);
+    const T* lp2 = (const T*)P.l[1] + (LDOWN ? m0 : (int64_t)m0 * P.lld);
+    const T* rp2 = (const T*)P.r[1] + (RDOWN ? n0 : (int64_t)n0 * P.rld);
+    int64_t lstep = LDOWN ? KT * P.lld : KT, rstep = RDOWN ? KT * P.rld : KT;
+    int depth = P.depth, rest = depth - k0;
+    if (DIRECT) asm volatile("" : "+s"(lp), "+s"(rp), "+s"(lstep), "+s"(rstep), "+s"(rest));
+    if (DIRECT && K == SUM) asm volatile("" : "+s"(lp2), "+s"(rp2), "+s"(depth));
+    auto fetch = [&](uint4* to) __attribute__((always_inline)) {
+        if constexpr (DIRECT) {
+            ol.fetch(to, lp, rest);
+            orr.fetch(to + LW, rp, rest);
+        } else {
+            OL::gather(to, lp, rest, P.lld, lrows, left);
+            OR::gather(to + LW, rp, rest, P.rld, rrows, right);
+        }
+        lp += lstep;
+        rp += rstep;
+        rest -= KT;
+        if (K == SUM && rest <= 0) {
+            lp = lp2;
+            rp = rp2;
+            rest = depth;
         }
     };
-    if (begin < end) fetch(begin, lds);
-    for (int t = begin; t < end; t++)
-        step(t, lds + (t - begin) % 2 * 2 * WORDS, lds + (t - begin + 1) % 2 * 2 * WORDS);
+    const gs::Tile<T, KT> tile;
+    auto get_l = [&](const uint4* at, int k, int v) __attribute__((always_inline)) {
+        const int row = wm + 16 * v;
+        if constexpr (LDOWN) return tile.cols(at + row / KT * (8 * KT), k, row % KT);
+        else return tile.rows(at, row, k);
+    };
+    auto get_r = [&](const uint4* at, int k, int u) __attribute__((always_inline)) {
+        const int row = wn + 16 * u;
+        if constexpr (RDOWN) return tile.cols(at + LW + row / KT * (8 * KT), k, row % KT);
+        else return tile.rows(at + LW, row, k);
+    };
+    // A tile is STEPS steps of 32 of the depth and half of the wave's columns.  A step's
+    // operands are read from LDS during the step before, its first step's behind the
+    // barrier after which the tile is there and the one before it is free; a tile's loads
+    // are under way for a whole tile.  Left to itself the compiler reads just before it
+    // multiplies.
+    constexpr int KS = KT / 32, STEPS = 2 * KS, NH = NT / 2;
+    Frag<T> l[2][MT], r[2][NH];
+    // Restricted pointers tell the compiler that loads into one need not have arrived
+    // before reads of the other.
+    auto body = [&](int t, uint4* __restrict__ cur, uint4* __restrict__ next) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const int k = s / 2, h = s % 2;
+            if (s + 1 < STEPS) {
+#pragma unroll
+                for (int u = 0; u < NH; u++) r[(s + 1) % 2][u] = get_r(cur, (s + 1) / 2 * 32, (s + 1) % 2 * NH + u);
+                if (h == 1)
+#pragma unroll
+                    for (int v = 0; v < MT; v++) l[(k + 1) % 2][v] = get_l(cur, (k + 1) * 32, v);
+            } else if (t + 1 < end) {
+                arrived();
+                if (t + 2 < end) fetch(cur);
+#pragma unroll
+                for (int u = 0; u < NH; u++) r[(s + 1) % 2][u] = get_r(next, 0, u);
+#pragma unroll
+                for (int v = 0; v < MT; v++) l[(k + 1) % 2][v] = get_l(next, 0, v);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < NH; u++)
+#pragma unroll
+                for (int v = 0; v < MT; v++)
+                    acc[h * NH + u][v] = gs::mma(r[s % 2][u], l[k % 2][v], acc[h * NH + u][v]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (KS % 2 == 1) {
+#pragma unroll
+            for (int v = 0; v < MT; v++) l[0][v] = l[1][v];
+        }
+    };
+    auto walk = [&](uint4* __restrict__ one, uint4* __restrict__ two) __attribute__((always_inline)) {
+        fetch(one);
+        arrived();
+        if (begin + 1 < end) fetch(two);
+#pragma unroll
+        for (int u = 0; u < NH; u++) r[0][u] = get_r(one, 0, u);
+#pragma unroll
+        for (int v = 0; v < MT; v++) l[0][v] = get_l(one, 0, v);
+        for (int t = begin; t < end; t += 2) {
+            body(t, one, two);
+            if (t + 1 < end) body(t + 1, two, one);
+        }
+    };
+    if (begin < end) walk(lds, lds + LW + RW);
 
-    // lane: row 16 v + i of the result, columns 16 u + 4 g .. + 3
+    // a lane holds row 16 v + i, columns 16 u + 4 g .. + 3
     if (A.splits > 1) {
         f4* part = (f4*)A.part + (int64_t)place * (NT * MT * THREADS) + threadIdx.x;
 #pragma unroll
@@ -247,89 +340,133 @@ __global__ __launch_bounds__(64 * WM * WN, S == 256 ? 2 : 1) void feed_kernel(Fe
             for (int v = 0; v < MT; v++) part[(u * MT + v) * THREADS] = acc[u][v];
         return;
     }
+    // Results leave as whole rows, 16 rows of the wave's columns at a time: through LDS,
+    // eight neighbours to a lane.  In the lanes' own pieces of 8 bytes the forward's
+    // three results and the backward's two, with the two that they read, took as long
+    // as the products.
+    constexpr int C = (K == HIDDEN ? HN / 2 : HN) / 8, RP = 64 / C, LD = HN + 4;   // lanes and rows of a pass
+    static_assert(C >= 4 && C <= 64, "whole rows of lanes");
+    float* own = (float*)lds + wave * (16 * LD);
+    const int c8 = lane % C * 8, col = (K == HIDDEN ? n0 + wn / 2 : n0 + wn) + c8, n = P.cols - col;
+    __syncthreads();   // all waves are done with the tiles
 #pragma unroll
     for (int v = 0; v < MT; v++) {
-        const int row = m0 + wm + 16 * v + i;
-        if (row >= P.rows) continue;
+        const int row0 = m0 + wm + 16 * v;
+        // before the exchange: what the result is multiplied with
+        float in[16 / RP][2][8];
+        if constexpr (K == GRAD) {
 #pragma unroll
-        for (int u = 0; u < NT; u += K == HIDDEN ? 2 : 1) {
-            const int col = K == HIDDEN ? n0 + (wn + 16 * u) / 2 + 4 * g : n0 + wn + 16 * u + 4 * g;
-            const int n = P.cols - col;
-            if (n <= 0) continue;
+            for (int p = 0; p < 16 / RP; p++) {
+                const int row = row0 + p * RP + lane / C;
+                const int64_t at = (int64_t)row * P.old + col;
+#pragma unroll
+                for (int w = 0; w < 2; w++) get<T, 8>((const T*)P.in[w] + at, in[p][w], row < P.rows ? n : 0);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int u = 0; u < NT; u++) *(f4*)(own + i * LD + 16 * u + 4 * g) = acc[u][v];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int p = 0; p < 16 / RP; p++) {
+            const int r = p * RP + lane / C, row = row0 + r;
+            const float* from = own + r * LD;
             const int64_t at = (int64_t)row * P.old + col;
-            float o[4];
+            const int here = row < P.rows ? n : 0;
+            float o[8], d[8];
             if constexpr (K == HIDDEN) {
+                // 16 of a and 16 of b in turn
+                const float* f = from + c8 / 16 * 32 + c8 % 16;
+                float a[8], b[8];
+                __builtin_memcpy(a, f, 32);
+                __builtin_memcpy(b, f + 16, 32);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float value, slope;
-                    activation(A.act, acc[u][v][e], value, slope);
-                    o[e] = value * acc[u + 1][v][e];
-                }
-                put<T, 4>((T*)P.out[0] + at, o, n);
-                if (P.out[1] != nullptr) {
-#pragma unroll
-                    for (int w = 0; w < 2; w++) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[e] = acc[u + w][v][e];
-                        put<T, 4>((T*)P.out[1 + w] + at, o, n);
-                    }
-                }
-            } else if constexpr (K == GRAD) {
-                float a[4], b[4], d[4];
-                get<T, 4>((const T*)P.in[0] + at, a, n);
-                get<T, 4>((const T*)P.in[1] + at, b, n);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
+                for (int e = 0; e < 8; e++) {
                     float value, slope;
                     activation(A.act, a[e], value, slope);
-                    o[e] = acc[u][v][e] * b[e] * slope;
-                    d[e] = acc[u][v][e] * value;
+                    o[e] = value * b[e];
                 }
-                put<T, 4>((T*)P.out[0] + at, o, n);
-                put<T, 4>((T*)P.out[1] + at, d, n);
-            } else {
+                put<T, 8>((T*)P.out[0] + at, o, here);
+                if (P.out[1] != nullptr) {
+                    put<T, 8>((T*)P.out[1] + at, a, here);
+                    put<T, 8>((T*)P.out[2] + at, b, here);
+                }
+            } else if constexpr (K == GRAD) {
+                __builtin_memcpy(d, from + c8, 32);
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[e] = acc[u][v][e];
-                put<T, 4>((T*)P.out[0] + at, o, n);
+                for (int e = 0; e < 8; e++) {
+                    float value, slope;
+                    activation(A.act, in[p][0][e], value, slope);
+                    o[e] = d[e] * in[p][1][e] * slope;
+                    d[e] = d[e] * value;
+                }
+                put<T, 8>((T*)P.out[0] + at, o, here);
+                put<T, 8>((T*)P.out[1] + at, d, here);
+            } else {
+                __builtin_memcpy(o, from + c8, 32);
+                put<T, 8>((T*)P.out[0] + at, o, here);
             }
         }
     }
 }
 
-template <typename T, Kind K, bool LDOWN, bool RDOWN>
-int launch_tiles(FeedArgs& A, bool direct, hipStream_t stream)
+template <typename T, Kind K, bool LDOWN, bool RDOWN, int SM, int SN, int WM, int WN, bool DIRECT>
+int launch_tiles(FeedArgs& A, hipStream_t stream)
 {
-    constexpr int S = 128;
     int blocks = 0;
     for (int i = 0; i < A.count; i++) {
         Product& P = A.p[i];
-        P.tiles_m = (P.rows + S - 1) / S;
-        P.tiles_n = (P.cols + (K == HIDDEN ? S / 2 : S) - 1) / (K == HIDDEN ? S / 2 : S);
+        P.tiles_m = (P.rows + SM - 1) / SM;
+        P.tiles_n = (P.cols + (K == HIDDEN ? SN / 2 : SN) - 1) / (K == HIDDEN ? SN / 2 : SN);
         P.first = blocks;
         const int64_t n = (int64_t)P.tiles_m * P.tiles_n * A.splits;
         GS_REQUIRE(n + blocks < 0x7fffffff, "feed forward: too many tiles");
         blocks += (int)n;
     }
     if (blocks == 0) return GS_OK;
-    const size_t lds = 4 * S * 128;
-    if (direct)
-        GS_TIMED("feed_kernel", stream,
-                 hipLaunchKernelGGL((feed_kernel<T, K, LDOWN, RDOWN, S, 2, 2, true>), dim3(blocks), dim3(256), lds,
-                                    stream, A));
-    else
-        GS_TIMED("feed_kernel", stream,
-                 hipLaunchKernelGGL((feed_kernel<T, K, LDOWN, RDOWN, S, 2, 2, false>), dim3(blocks), dim3(256), lds,
-                                    stream, A));
+    constexpr size_t LDS = 2 * (SM + SN) * 128;
+    auto kernel = feed_kernel<T, K, LDOWN, RDOWN, SM, SN, WM, WN, DIRECT>;
+    if constexpr (LDS > 65536) {
+        // on the current device; a driver call, so once a device
+        static std::atomic<uint64_t> told{0};
+        int device = 0;
+        GS_HIP(hipGetDevice(&device));
+        const uint64_t bit = 1ull << (device & 63);
+        if (!(told.load() & bit)) {
+            GS_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+            told |= bit;
+        }
+    }
+    GS_TIMED("feed_kernel", stream,
+             hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WM * WN), LDS, stream, A));
     GS_LAUNCH_CHECK("feed_kernel");
     return GS_OK;
+}
+
+template <typename T, Kind K, bool LDOWN, bool RDOWN>
+int launch_shape(FeedArgs& A, bool direct, hipStream_t stream)
+{
+    if constexpr (sizeof(T) == 2) {
+        if (direct) {
+            int64_t n = 0;
+            for (int i = 0; i < A.count; i++)
+                n += (int64_t)((A.p[i].rows + 255) / 256) * ((A.p[i].cols + (K == HIDDEN ? 127 : 255)) / (K == HIDDEN ? 128 : 256));
+            if (n >= 160) return launch_tiles<T, K, LDOWN, RDOWN, 256, 256, 4, 2, true>(A, stream);
+            if (n >= 64) return launch_tiles<T, K, LDOWN, RDOWN, 256, 128, 4, 2, true>(A, stream);
+        }
+    }
+    if (direct) return launch_tiles<T, K, LDOWN, RDOWN, 128, 128, 2, 2, true>(A, stream);
+    return launch_tiles<T, K, LDOWN, RDOWN, 128, 128, 2, 2, false>(A, stream);
 }
 
 template <Kind K, bool LDOWN, bool RDOWN>
 int launch(int type, FeedArgs& A, bool direct, hipStream_t stream)
 {
-    if (type == GS_F32) return launch_tiles<float, K, LDOWN, RDOWN>(A, direct, stream);
-    if (type == GS_BF16) return launch_tiles<gs::bf16, K, LDOWN, RDOWN>(A, direct, stream);
-    return launch_tiles<gs::f16, K, LDOWN, RDOWN>(A, direct, stream);
+    if (type == GS_F32) return launch_shape<float, K, LDOWN, RDOWN>(A, direct, stream);
+    if (type == GS_BF16) return launch_shape<gs::bf16, K, LDOWN, RDOWN>(A, direct, stream);
+    return launch_shape<gs::f16, K, LDOWN, RDOWN>(A, direct, stream);
 }
 
 constexpr int MAX_SIDE = 1 << 24;
