@@ -20,6 +20,7 @@
 // backward a, b, da and db, since they are operands of the next product: float16's
 // range holds for them too.
 #include <atomic>
+#include <type_traits>
 
 #include "gs_host.h"
 #include "gs_matrix.h"
@@ -55,20 +56,24 @@ struct FeedArgs {
 
 __device__ __align__(16) const uint32_t zeros[4] = {0, 0, 0, 0};
 
-// All waves' loads to LDS are there, and all waves are done with what they read: a
-// barrier alone waits for neither where the compiler sees that this wave's own reads
-// need not.
+// All waves' loads to LDS but their last N are there, and all waves are done with what
+// they read.  In one piece: the compiler's own barrier waits for all loads.
+template <int N>
 __device__ __forceinline__ void arrived()
 {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// act(a) and its derivative
+// act(a) and its derivative.  For the 16-bit types, whose results are rounded to 2^-9 and
+// more, with the hardware's exponential and reciprocal (off by 2^-20 of the value for |a|
+// up to 16, where the sigmoid is 1e-7): the exact ones took a quarter of the backward's
+// first product.
+template <typename T>
 __device__ __forceinline__ void activation(int act, float a, float& value, float& slope)
 {
     if (act == GS_SILU) {
-        const float s = 1.0f / (1.0f + expf(-a));
+        const float s = sizeof(T) == 2 ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a * -1.44269504f))
+                                       : 1.0f / (1.0f + expf(-a));
         value = a * s;
         slope = s * __builtin_fmaf(a, 1.0f - s, 1.0f);
     } else {
@@ -79,57 +84,59 @@ __device__ __forceinline__ void activation(int act, float a, float& value, float
     }
 }
 
-// An operand's tiles of S rows of the result by KT of the depth, KT elements being
-// 128 bytes.  Along: S rows of 128 bytes.  DOWN: KT rows of S elements, as S / KT
-// tiles of KT columns, the rows in the order in which Tile::cols takes them as
-// k = 8 g + j.
+// An operand's tiles of S rows of the result by KT of the depth, as tiles of rows of W
+// elements, 128 bytes.  Along: KT / W tiles of S rows.  DOWN: S / W tiles of KT rows, which
+// lie in the order in which Tile::cols takes them as k = 8 g + j.
 //   DIRECT: straight to LDS, 16 bytes at a time; chunks are whole and aligned.  What
 //           lies beyond the depth comes from `zeros`; beyond the last row or column
 //           the last one comes again, whose results nobody keeps.
-//   else:   through registers, element by element
-template <typename T, int S, bool DOWN, int THREADS, bool DIRECT>
+//   else:   through registers, from any address; what lies beyond is zero
+template <typename T, int S, int KT, bool DOWN, int THREADS, bool DIRECT>
 struct Operand {
-    static constexpr int KT = 128 / (int)sizeof(T), V = gs::Vec<T>::N, CH = S * 8 / THREADS;
-    static_assert(CH >= 1 && THREADS % 256 == 0, "a chunk per thread, 32 rows or more per access");
-    using L = gs::Tile<T, KT>;
+    static constexpr int V = gs::Vec<T>::N, W = 128 / (int)sizeof(T), ROWS = DOWN ? KT : S;
+    static constexpr int WORDS = S * KT / V, CH = WORDS / THREADS;
+    static_assert(WORDS % THREADS == 0 && THREADS % 256 == 0, "whole accesses, of 32 rows or more");
+    static_assert(KT % W == 0 && S % (DOWN ? W : 16) == 0, "whole tiles");
+    using L = gs::Tile<T, W>;
     typedef __attribute__((address_space(3))) void* lds_ptr;
 
-    uint32_t at[CH];   // bytes from the tile's corner
+    uint32_t at[DIRECT ? CH : 1];   // bytes from the tile's corner
 
     // place `id` of the tile holds k (or the chunk of k from there) and row of the result
     __device__ static __forceinline__ void place(int id, int& row, int& k)
     {
-        const int r = DOWN ? id / 8 % KT : id / 8, col = (L::chunk(r, id % 8) - r * 8) * V;
+        const int r = id / 8 % ROWS, col = (L::chunk(r, id % 8) - r * 8) * V, sub = id / (8 * ROWS) * W;
         if constexpr (DOWN) {
             const int q = r % 32;
-            row = id / (8 * KT) * KT + col;
+            row = sub + col;
             k = r / 32 * 32 + 8 * (q % 16 / 4) + 4 * (q / 16) + q % 4;
         } else {
             row = r;
-            k = col;
+            k = sub + col;
         }
     }
     // map(row): the place of the result's row among the operand's rows (DOWN: columns), of which there are `limit`
     template <typename Map>
     __device__ __forceinline__ Operand(int64_t ld, int limit, Map map)
     {
+        if constexpr (DIRECT) {
 #pragma unroll
-        for (int c = 0; c < CH; c++) {
-            int row, k;
-            place(threadIdx.x + THREADS * c, row, k);
-            row = map(row);
-            if constexpr (DOWN) at[c] = (uint32_t)(((int64_t)k * ld + min(row, limit - V)) * (int)sizeof(T));
-            else at[c] = (uint32_t)(((int64_t)min(row, limit - 1) * ld + k) * (int)sizeof(T));
+            for (int c = 0; c < CH; c++) {
+                int row, k;
+                place(threadIdx.x + THREADS * c, row, k);
+                row = map(row);
+                if constexpr (DOWN) at[c] = (uint32_t)(((int64_t)k * ld + min(row, limit - V)) * (int)sizeof(T));
+                else at[c] = (uint32_t)(((int64_t)min(row, limit - 1) * ld + k) * (int)sizeof(T));
+            }
         }
     }
-    // DIRECT: the tile at `from`, of which `depth` is there
+    // DIRECT: the tile at `from`, of which `depth` is there.  As buffer loads: the compiler
+    // takes global ones to LDS for accesses of any kind, and waits for all LDS reads while
+    // one is under way.
     __device__ __forceinline__ void fetch(uint4* to, const T* from, int depth) const
     {
-        const char* base = (const char*)from;
         uint4* mine = to + (threadIdx.x & ~63u);   // + 16 bytes per lane
-        // As buffer loads: the compiler takes global ones to LDS for accesses of any kind, and
-        // waits for all LDS reads while one is under way.  Their offsets are below `span`.
-        const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x27000);
+        const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, -1, 0x27000);
         if (depth >= KT) {
 #pragma unroll
             for (int c = 0; c < CH; c++)
@@ -147,35 +154,54 @@ struct Operand {
             }
         }
     }
-    // else: the same, of which `limit` rows (DOWN: columns) are there
+    // else: the same to registers, of which `limit` rows (DOWN: columns) are there, and from there to LDS
     template <typename Map>
-    __device__ static __forceinline__ void gather(uint4* to, const T* from, int depth, int64_t ld, int limit, Map map)
+    __device__ static __forceinline__ void gather(gs::Vec<T> (&v)[CH], const T* from, int depth, int64_t ld, int limit,
+                                                  Map map)
     {
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             int row, k;
             place(threadIdx.x + THREADS * c, row, k);
-            gs::Vec<T> v = {};
+            row = map(row);
+            const T* p = DOWN ? from + (int64_t)k * ld + row : from + (int64_t)row * ld + k;
+            const int n = DOWN ? (k < depth ? limit - row : 0) : (row < limit ? depth - k : 0);
+            v[c] = {};
+            if (n >= V) {
+                v[c] = gs::load_vec(p);
+            } else {
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                if constexpr (DOWN) {
-                    if (k < depth && map(row) + e < limit) v.v[e] = from[(int64_t)k * ld + map(row) + e];
-                } else {
-                    if (k + e < depth && map(row) < limit) v.v[e] = from[(int64_t)map(row) * ld + k + e];
-                }
+                for (int e = 0; e < V; e++)
+                    if (e < n) v[c].v[e] = p[e];
             }
-            to[threadIdx.x + THREADS * c] = __builtin_bit_cast(uint4, v);
         }
+    }
+    __device__ static __forceinline__ void settle(const gs::Vec<T> (&v)[CH], uint4* to)
+    {
+#pragma unroll
+        for (int c = 0; c < CH; c++) to[threadIdx.x + THREADS * c] = __builtin_bit_cast(uint4, v[c]);
     }
 };
 
 template <typename T, int N>
+struct Raw {
+    T v[N];
+};
+
+template <typename T, int N, bool WHOLE>
 __device__ __forceinline__ void put(T* p, const float* v, int n)
 {
+    // in pairs, which the conversion instruction takes
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
     T t[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) t[i] = (T)v[i];
-    if (n >= N) {
+    for (int i = 0; i < N; i += 2) {
+        const t2 two = __builtin_convertvector(f2{v[i], v[i + 1]}, t2);
+        t[i] = two[0];
+        t[i + 1] = two[1];
+    }
+    if (WHOLE || n >= N) {
         __builtin_memcpy(p, t, sizeof(t));
     } else {
 #pragma unroll
@@ -184,104 +210,229 @@ __device__ __forceinline__ void put(T* p, const float* v, int n)
     }
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void get(const T* p, float* v, int n)
+template <typename T, int N, bool WHOLE>
+__device__ __forceinline__ Raw<T, N> get(const T* p, int n)
 {
-    T t[N] = {};
-    if (n >= N) {
-        __builtin_memcpy(t, p, sizeof(t));
+    Raw<T, N> t = {};
+    if (WHOLE || n >= N) {
+        __builtin_memcpy(&t, p, sizeof(t));
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++)
-            if (i < n) t[i] = p[i];
+            if (i < n) t.v[i] = p[i];
     }
-#pragma unroll
-    for (int i = 0; i < N; i++) v[i] = (float)t[i];
+    return t;
 }
 
-// SM x SN of the result; waves in a grid of WM x WN.
-template <typename T, Kind K, bool LDOWN, bool RDOWN, int SM, int SN, int WM, int WN, bool DIRECT>
-__global__ __launch_bounds__(64 * WM * WN, 2) void feed_kernel(FeedArgs A)
-{
-    constexpr int THREADS = 64 * WM * WN, KT = 128 / (int)sizeof(T), LW = SM * 8, RW = SN * 8;
-    constexpr int HM = SM / WM, HN = SN / WN, MT = HM / 16, NT = HN / 16;   // of a wave
-    using OL = Operand<T, SM, LDOWN, THREADS, DIRECT>;
-    using OR = Operand<T, SN, RDOWN, THREADS, DIRECT>;
-    extern __shared__ uint4 lds[];                   // [2][left, right]
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int which = 0;
-    const uint32_t place = gs::xcd_item(blockIdx.x, gridDim.x);
-    while (which + 1 < A.count && (int)place >= A.p[which + 1].first) which++;
-    const Product& P = A.p[which];
-    const int item = (int)place - P.first, tile_item = item / A.splits, split = item % A.splits;
-    // runs of eight rows of tiles: the 32 tiles that an XCD works on at a time are 8 x 4
-    const int run = tile_item / (8 * P.tiles_n), high = min(8, P.tiles_m - 8 * run), in_run = tile_item - run * 8 * P.tiles_n;
-    const int tm = 8 * run + in_run % high, tn = in_run / high;
-    const int m0 = tm * SM, n0 = tn * (K == HIDDEN ? SN / 2 : SN);
-    const int wm = wave % WM * HM, wn = wave / WM * HN;
+// How 16 rows of a wave's HN columns leave: through LDS, eight neighbours to a lane, as
+// whole rows.  In the lanes' own pieces of 8 bytes the forward's three results and the
+// backward's two, with the two that they read, took as long as the products.
+template <typename T, Kind K, int HN>
+struct Leave {
+    static constexpr int C = (K == HIDDEN ? HN / 2 : HN) / 8, RP = 64 / C, PASSES = 16 / RP;   // lanes, rows of a pass
+    static constexpr int LD = HN + 4;
+    static_assert(C >= 4 && C <= 64, "whole rows of lanes");
+    using In = Raw<T, 8>[PASSES][2];
 
-    f4 acc[NT][MT];
-#pragma unroll
-    for (int u = 0; u < NT; u++)
-#pragma unroll
-        for (int v = 0; v < MT; v++) acc[u][v] = f4{0, 0, 0, 0};
+    float* own;          // 16 rows of LD floats of the wave's
+    int lane, act, rows, n;
+    int64_t old;
+    T *out0, *out1, *out2;
+    const T *in0, *in1;
+    bool also;
 
-    const int per = (P.depth + KT - 1) / KT, all = K == SUM ? 2 * per : per;
-    const int begin = (int)((int64_t)all * split / A.splits), end = (int)((int64_t)all * (split + 1) / A.splits);
-    // 16 rows of the gate, then 16 of up; a wave's eight rows of an access are of one
-    const int which_r = K == HIDDEN ? wave / 2 % 2 : 0;
-    auto left = [](int row) { return row; };
-    auto right = [](int row) { return K == HIDDEN ? row / 32 * 16 + row % 16 : row; };
-    const int lrows = P.rows - m0, rrows = P.cols - n0;
-    const OL ol(P.lld, lrows, left);
-    const OR orr(P.rld, rrows, right);
-    // The next tile's corners, how much of the depth is left there, and the steps to the
-    // tile after it; held in registers, so that the loop reads no arguments (whose loads
-    // would be waited for together with those from LDS).
-    const int second = K == SUM && begin >= per, k0 = (begin - second * per) * KT;
-    const T* lp = (const T*)P.l[second] + (LDOWN ? (int64_t)k0 * P.lld + m0 : (int64_t)m0 * P.lld + k0);
-    const T* rp = (const T*)P.r[second + which_r] + (RDOWN ? (int64_t)k0 * P.rld + n0 : (int64_t)n0 * P.rld + k0);
-    const T* lp2 = (const T*)P.l[1] + (LDOWN ? m0 : (int64_t)m0 * P.lld);
-    const T* rp2 = (const T*)P.r[1] + (RDOWN ? n0 : (int64_t)n0 * P.rld);
-    int64_t lstep = LDOWN ? KT * P.lld : KT, rstep = RDOWN ? KT * P.rld : KT;
-    int depth = P.depth, rest = depth - k0;
-    if (DIRECT) asm volatile("" : "+s"(lp), "+s"(rp), "+s"(lstep), "+s"(rstep), "+s"(rest));
-    if (DIRECT && K == SUM) asm volatile("" : "+s"(lp2), "+s"(rp2), "+s"(depth));
-    auto fetch = [&](uint4* to) __attribute__((always_inline)) {
-        if constexpr (DIRECT) {
-            ol.fetch(to, lp, rest);
-            orr.fetch(to + LW, rp, rest);
-        } else {
-            OL::gather(to, lp, rest, P.lld, lrows, left);
-            OR::gather(to + LW, rp, rest, P.rld, rrows, right);
+    __device__ __forceinline__ Leave(const Product& P, int act, float* own, int first)
+        : own(own), lane(threadIdx.x & 63), act(act), rows(P.rows), old(P.old), also(P.out[1] != nullptr)
+    {
+        const int col = first + lane % C * 8;
+        n = P.cols - col;
+        out0 = (T*)P.out[0] + col;
+        out1 = (T*)P.out[1] + col;
+        out2 = (T*)P.out[2] + col;
+        in0 = (const T*)P.in[0] + col;
+        in1 = (const T*)P.in[1] + col;
+    }
+    // elements of this lane's eight that are there; WHOLE: all of the tile are
+    template <bool WHOLE>
+    __device__ __forceinline__ int here(int row) const
+    {
+        return WHOLE ? 8 : row < rows ? n : 0;
+    }
+    // what the rows from row0 on are multiplied with
+    template <bool WHOLE>
+    __device__ __forceinline__ void ask(In& in, int row0) const
+    {
+        if constexpr (K == GRAD) {
+#pragma unroll
+            for (int p = 0; p < PASSES; p++) {
+                const int row = row0 + p * RP + lane / C;
+                in[p][0] = get<T, 8, WHOLE>(in0 + row * old, here<WHOLE>(row));
+                in[p][1] = get<T, 8, WHOLE>(in1 + row * old, here<WHOLE>(row));
+            }
         }
-        lp += lstep;
-        rp += rstep;
+    }
+    template <bool WHOLE>
+    __device__ __forceinline__ void give(const In& in, const f4 (&acc)[HN / 16], int row0) const
+    {
+        const int i = lane & 15, g = lane >> 4, c8 = lane % C * 8;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int u = 0; u < HN / 16; u++) *(f4*)(own + i * LD + 16 * u + 4 * g) = acc[u];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) {
+            const int r = p * RP + lane / C, row = row0 + r, count = here<WHOLE>(row);
+            const float* from = own + r * LD;
+            const int64_t at = row * old;
+            float o[8], d[8];
+            if constexpr (K == HIDDEN) {
+                // 16 of a and 16 of b in turn
+                const float* f = from + c8 / 16 * 32 + c8 % 16;
+                float a[8], b[8];
+                __builtin_memcpy(a, f, 32);
+                __builtin_memcpy(b, f + 16, 32);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float value, slope;
+                    activation<T>(act, a[e], value, slope);
+                    o[e] = value * b[e];
+                }
+                put<T, 8, WHOLE>(out0 + at, o, count);
+                if (also) {
+                    put<T, 8, WHOLE>(out1 + at, a, count);
+                    put<T, 8, WHOLE>(out2 + at, b, count);
+                }
+            } else if constexpr (K == GRAD) {
+                __builtin_memcpy(d, from + c8, 32);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float value, slope;
+                    activation<T>(act, (float)in[p][0].v[e], value, slope);
+                    o[e] = d[e] * (float)in[p][1].v[e] * slope;
+                    d[e] = d[e] * value;
+                }
+                put<T, 8, WHOLE>(out0 + at, o, count);
+                put<T, 8, WHOLE>(out1 + at, d, count);
+            } else {
+                __builtin_memcpy(o, from + c8, 32);
+                put<T, 8, WHOLE>(out0 + at, o, count);
+            }
+        }
+    }
+};
+
+// The product and the tile of it that a workgroup has.  Consecutive tiles are in runs of
+// eight rows of tiles, and those of an XCD consecutive: the 32 that it works on at a time
+// are 8 x 4, whose operands its L2 holds (the down projection of 8192 x 1024 x 4096 took
+// 103 us with whole columns of tiles, 76 so).
+struct Place {
+    int which, tm, tn, split;
+};
+
+__device__ __forceinline__ Place place_of(const FeedArgs& A)
+{
+    const uint32_t place = gs::xcd_item(blockIdx.x, gridDim.x);
+    Place p;
+    p.which = 0;
+    while (p.which + 1 < A.count && (int)place >= A.p[p.which + 1].first) p.which++;
+    const Product& P = A.p[p.which];
+    const int item = (int)place - P.first, tile = item / A.splits;
+    p.split = item % A.splits;
+    const int run = tile / (8 * P.tiles_n), high = min(8, P.tiles_m - 8 * run), in_run = tile - run * 8 * P.tiles_n;
+    p.tm = 8 * run + in_run % high;
+    p.tn = in_run / high;
+    return p;
+}
+
+// Where an operand's next tile begins, how much of the depth is left there, and the steps
+// to the tile after it; held in registers, so that the loops read no arguments (whose
+// loads would be waited for together with those from LDS).
+template <typename T, Kind K, int KT, bool LDOWN, bool RDOWN>
+struct Walk {
+    const T *l, *r, *l2, *r2;
+    int64_t lstep, rstep;
+    int depth, rest;
+
+    __device__ __forceinline__ Walk(const Product& P, int m0, int n0, int which_r, int begin)
+    {
+        const int per = (P.depth + KT - 1) / KT, second = K == SUM && begin >= per, k0 = (begin - second * per) * KT;
+        l = (const T*)P.l[second] + (LDOWN ? (int64_t)k0 * P.lld + m0 : (int64_t)m0 * P.lld + k0);
+        r = (const T*)P.r[second + which_r] + (RDOWN ? (int64_t)k0 * P.rld + n0 : (int64_t)n0 * P.rld + k0);
+        l2 = (const T*)P.l[1] + (LDOWN ? m0 : (int64_t)m0 * P.lld);
+        r2 = (const T*)P.r[1] + (RDOWN ? n0 : (int64_t)n0 * P.rld);
+        lstep = LDOWN ? KT * P.lld : KT;
+        rstep = RDOWN ? KT * P.rld : KT;
+        depth = P.depth;
+        rest = depth - k0;
+        asm volatile("" : "+s"(l), "+s"(r), "+s"(lstep), "+s"(rstep), "+s"(rest));
+        if (K == SUM) asm volatile("" : "+s"(l2), "+s"(r2), "+s"(depth));
+    }
+    __device__ __forceinline__ void next()
+    {
+        l += lstep;
+        r += rstep;
         rest -= KT;
         if (K == SUM && rest <= 0) {
-            lp = lp2;
-            rp = rp2;
+            l = l2;
+            r = r2;
             rest = depth;
         }
+    }
+};
+
+// 16-bit types, whole aligned chunks: SM x SN of the result, waves in a grid of WM x WN.
+template <typename T, Kind K, bool LDOWN, bool RDOWN, int SM, int SN, int WM, int WN, int BUFFERS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void feed_kernel(FeedArgs A)
+{
+    constexpr int THREADS = 64 * WM * WN, KT = 64;
+    constexpr int HM = SM / WM, HN = SN / WN, MT = HM / 16, NT = HN / 16;   // of a wave
+    using OL = Operand<T, SM, KT, LDOWN, THREADS, true>;
+    using OR = Operand<T, SN, KT, RDOWN, THREADS, true>;
+    static_assert((!LDOWN || HM % OL::W == 0) && (!RDOWN || HN % OR::W == 0), "a wave's columns are whole tiles");
+    constexpr int LW = OL::WORDS, RW = OR::WORDS, LOADS = OL::CH + OR::CH;
+    extern __shared__ uint4 lds[];                   // [BUFFERS][left, right]
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Place at = place_of(A);
+    const Product& P = A.p[at.which];
+    const int m0 = at.tm * SM, n0 = at.tn * (K == HIDDEN ? SN / 2 : SN);
+    const int wm = wave % WM * HM, wn = wave / WM * HN;
+
+    f4 acc[MT][NT];
+#pragma unroll
+    for (int v = 0; v < MT; v++)
+#pragma unroll
+        for (int u = 0; u < NT; u++) acc[v][u] = f4{0, 0, 0, 0};
+
+    const int end = (K == SUM ? 2 : 1) * ((P.depth + KT - 1) / KT);
+    // 16 rows of the gate, then 16 of up; a wave's eight rows of an access are of one
+    const OL ol(P.lld, P.rows - m0, [](int row) { return row; });
+    const OR orr(P.rld, P.cols - n0, [](int row) { return K == HIDDEN ? row / 32 * 16 + row % 16 : row; });
+    Walk<T, K, KT, LDOWN, RDOWN> walk(P, m0, n0, K == HIDDEN ? wave / 2 % 2 : 0, 0);
+    auto fetch = [&](uint4* to) __attribute__((always_inline)) {
+        ol.fetch(to, walk.l, walk.rest);
+        orr.fetch(to + LW, walk.r, walk.rest);
+        walk.next();
     };
-    const gs::Tile<T, KT> tile;
-    auto get_l = [&](const uint4* at, int k, int v) __attribute__((always_inline)) {
+    const gs::Tile<T, OL::W> tile;
+    auto get_l = [&](const uint4* from, int k, int v) __attribute__((always_inline)) {
         const int row = wm + 16 * v;
-        if constexpr (LDOWN) return tile.cols(at + row / KT * (8 * KT), k, row % KT);
-        else return tile.rows(at, row, k);
+        if constexpr (LDOWN) return tile.cols(from + row / OL::W * (8 * KT), k, row % OL::W);
+        else return tile.rows(from, row, k);
     };
-    auto get_r = [&](const uint4* at, int k, int u) __attribute__((always_inline)) {
+    auto get_r = [&](const uint4* from, int k, int u) __attribute__((always_inline)) {
         const int row = wn + 16 * u;
-        if constexpr (RDOWN) return tile.cols(at + LW + row / KT * (8 * KT), k, row % KT);
-        else return tile.rows(at + LW, row, k);
+        if constexpr (RDOWN) return tile.cols(from + LW + row / OR::W * (8 * KT), k, row % OR::W);
+        else return tile.rows(from + LW, row, k);
     };
-    // A tile is STEPS steps of 32 of the depth and half of the wave's columns.  A step's
+    // A tile is four steps of 32 of the depth and half of the wave's columns.  A step's
     // operands are read from LDS during the step before, its first step's behind the
-    // barrier after which the tile is there and the one before it is free; a tile's loads
-    // are under way for a whole tile.  Left to itself the compiler reads just before it
-    // multiplies.
-    constexpr int KS = KT / 32, STEPS = 2 * KS, NH = NT / 2;
+    // barrier after which the tile is there and the one before it is free: left to itself
+    // the compiler reads just before it multiplies.  The loads of the tile BUFFERS on go
+    // out there too, all at once: spread between the products they came too late (down
+    // projection of 8192 x 1024 x 4096, two buffers, 83 us instead of 72).
+    constexpr int STEPS = 4, NH = NT / 2;
     Frag<T> l[2][MT], r[2][NH];
     // Restricted pointers tell the compiler that loads into one need not have arrived
     // before reads of the other.
@@ -296,8 +447,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void feed_kernel(FeedArgs A)
 #pragma unroll
                     for (int v = 0; v < MT; v++) l[(k + 1) % 2][v] = get_l(cur, (k + 1) * 32, v);
             } else if (t + 1 < end) {
-                arrived();
-                if (t + 2 < end) fetch(cur);
+                if (BUFFERS == 3 && t + 2 < end) arrived<LOADS>(); else arrived<0>();
+                if (t + BUFFERS < end) fetch(cur);
 #pragma unroll
                 for (int u = 0; u < NH; u++) r[(s + 1) % 2][u] = get_r(next, 0, u);
 #pragma unroll
@@ -308,141 +459,330 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void feed_kernel(FeedArgs A)
             for (int u = 0; u < NH; u++)
 #pragma unroll
                 for (int v = 0; v < MT; v++)
-                    acc[h * NH + u][v] = gs::mma(r[s % 2][u], l[k % 2][v], acc[h * NH + u][v]);
+                    acc[v][h * NH + u] = gs::mma(r[s % 2][u], l[k % 2][v], acc[v][h * NH + u]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (KS % 2 == 1) {
-#pragma unroll
-            for (int v = 0; v < MT; v++) l[0][v] = l[1][v];
-        }
     };
-    auto walk = [&](uint4* __restrict__ one, uint4* __restrict__ two) __attribute__((always_inline)) {
+    auto first = [&](const uint4* from) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NH; u++) r[0][u] = get_r(from, 0, u);
+#pragma unroll
+        for (int v = 0; v < MT; v++) l[0][v] = get_l(from, 0, v);
+    };
+    auto walk2 = [&](uint4* __restrict__ one, uint4* __restrict__ two) __attribute__((always_inline)) {
         fetch(one);
-        arrived();
-        if (begin + 1 < end) fetch(two);
-#pragma unroll
-        for (int u = 0; u < NH; u++) r[0][u] = get_r(one, 0, u);
-#pragma unroll
-        for (int v = 0; v < MT; v++) l[0][v] = get_l(one, 0, v);
-        for (int t = begin; t < end; t += 2) {
+        arrived<0>();
+        if (1 < end) fetch(two);
+        first(one);
+        for (int t = 0; t < end; t += 2) {
             body(t, one, two);
             if (t + 1 < end) body(t + 1, two, one);
         }
     };
-    if (begin < end) walk(lds, lds + LW + RW);
+    auto walk3 = [&](uint4* __restrict__ one, uint4* __restrict__ two, uint4* __restrict__ three)
+                     __attribute__((always_inline)) {
+        fetch(one);
+        if (1 < end) fetch(two);
+        if (1 < end) arrived<LOADS>(); else arrived<0>();
+        if (2 < end) fetch(three);
+        first(one);
+        for (int t = 0; t < end; t += 3) {
+            body(t, one, two);
+            if (t + 1 < end) body(t + 1, two, three);
+            if (t + 2 < end) body(t + 2, three, one);
+        }
+    };
+    if constexpr (BUFFERS == 3) walk3(lds, lds + LW + RW, lds + 2 * (LW + RW));
+    else walk2(lds, lds + LW + RW);
 
-    // a lane holds row 16 v + i, columns 16 u + 4 g .. + 3
-    if (A.splits > 1) {
-        f4* part = (f4*)A.part + (int64_t)place * (NT * MT * THREADS) + threadIdx.x;
+    using Out = Leave<T, K, HN>;
+    const Out out(P, A.act, (float*)lds + wave * (16 * Out::LD), K == HIDDEN ? n0 + wn / 2 : n0 + wn);
+    auto finish = [&](auto whole) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        // two rounds of 16 rows ahead
+        typename Out::In in[2];
+        out.template ask<WHOLE>(in[0], m0 + wm);
+        if (MT > 1) out.template ask<WHOLE>(in[1], m0 + wm + 16);
+        arrived<0>();   // all waves are done with the tiles
 #pragma unroll
-        for (int u = 0; u < NT; u++)
-#pragma unroll
-            for (int v = 0; v < MT; v++) part[(u * MT + v) * THREADS] = acc[u][v];
-        return;
-    }
-    // Results leave as whole rows, 16 rows of the wave's columns at a time: through LDS,
-    // eight neighbours to a lane.  In the lanes' own pieces of 8 bytes the forward's
-    // three results and the backward's two, with the two that they read, took as long
-    // as the products.
-    constexpr int C = (K == HIDDEN ? HN / 2 : HN) / 8, RP = 64 / C, LD = HN + 4;   // lanes and rows of a pass
-    static_assert(C >= 4 && C <= 64, "whole rows of lanes");
-    float* own = (float*)lds + wave * (16 * LD);
-    const int c8 = lane % C * 8, col = (K == HIDDEN ? n0 + wn / 2 : n0 + wn) + c8, n = P.cols - col;
-    __syncthreads();   // all waves are done with the tiles
-#pragma unroll
-    for (int v = 0; v < MT; v++) {
-        const int row0 = m0 + wm + 16 * v;
-        // before the exchange: what the result is multiplied with
-        float in[16 / RP][2][8];
-        if constexpr (K == GRAD) {
-#pragma unroll
-            for (int p = 0; p < 16 / RP; p++) {
-                const int row = row0 + p * RP + lane / C;
-                const int64_t at = (int64_t)row * P.old + col;
-#pragma unroll
-                for (int w = 0; w < 2; w++) get<T, 8>((const T*)P.in[w] + at, in[p][w], row < P.rows ? n : 0);
-            }
+        for (int v = 0; v < MT; v++) {
+            out.template give<WHOLE>(in[v % 2], acc[v], m0 + wm + 16 * v);
+            if (v + 2 < MT) out.template ask<WHOLE>(in[v % 2], m0 + wm + 16 * (v + 2));
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int u = 0; u < NT; u++) *(f4*)(own + i * LD + 16 * u + 4 * g) = acc[u][v];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int p = 0; p < 16 / RP; p++) {
-            const int r = p * RP + lane / C, row = row0 + r;
-            const float* from = own + r * LD;
-            const int64_t at = (int64_t)row * P.old + col;
-            const int here = row < P.rows ? n : 0;
-            float o[8], d[8];
-            if constexpr (K == HIDDEN) {
-                // 16 of a and 16 of b in turn
-                const float* f = from + c8 / 16 * 32 + c8 % 16;
-                float a[8], b[8];
-                __builtin_memcpy(a, f, 32);
-                __builtin_memcpy(b, f + 16, 32);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    float value, slope;
-                    activation(A.act, a[e], value, slope);
-                    o[e] = value * b[e];
-                }
-                put<T, 8>((T*)P.out[0] + at, o, here);
-                if (P.out[1] != nullptr) {
-                    put<T, 8>((T*)P.out[1] + at, a, here);
-                    put<T, 8>((T*)P.out[2] + at, b, here);
-                }
-            } else if constexpr (K == GRAD) {
-                __builtin_memcpy(d, from + c8, 32);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    float value, slope;
-                    activation(A.act, in[p][0][e], value, slope);
-                    o[e] = d[e] * in[p][1][e] * slope;
-                    d[e] = d[e] * value;
-                }
-                put<T, 8>((T*)P.out[0] + at, o, here);
-                put<T, 8>((T*)P.out[1] + at, d, here);
-            } else {
-                __builtin_memcpy(o, from + c8, 32);
-                put<T, 8>((T*)P.out[0] + at, o, here);
-            }
-        }
-    }
+    };
+    if (P.rows - m0 >= SM && P.cols - n0 >= (K == HIDDEN ? SN / 2 : SN))
+        finish(std::true_type{});
+    else
+        finish(std::false_type{});
 }
 
-template <typename T, Kind K, bool LDOWN, bool RDOWN, int SM, int SN, int WM, int WN, bool DIRECT>
-int launch_tiles(FeedArgs& A, hipStream_t stream)
+// Few tiles, fp32, or chunks that are not whole: 64 x 64 of the result, of whose depth of
+// 128 a turn each of four waves takes a quarter, so that a short depth keeps a workgroup
+// busy and 64 columns fill its transposing reads.  The waves' sums meet at the end, in
+// order.  With splits > 1 a workgroup has a part of the depth and leaves its sums in
+// memory for feed_join_kernel.
+constexpr int SS = 64, SKT = 128;
+
+template <typename T, Kind K, bool LDOWN, bool RDOWN, bool DIRECT>
+__global__ __launch_bounds__(256, 1) void feed_small_kernel(FeedArgs A)
 {
-    int blocks = 0;
-    for (int i = 0; i < A.count; i++) {
-        Product& P = A.p[i];
-        P.tiles_m = (P.rows + SM - 1) / SM;
-        P.tiles_n = (P.cols + (K == HIDDEN ? SN / 2 : SN) - 1) / (K == HIDDEN ? SN / 2 : SN);
-        P.first = blocks;
-        const int64_t n = (int64_t)P.tiles_m * P.tiles_n * A.splits;
-        GS_REQUIRE(n + blocks < 0x7fffffff, "feed forward: too many tiles");
-        blocks += (int)n;
-    }
-    if (blocks == 0) return GS_OK;
-    constexpr size_t LDS = 2 * (SM + SN) * 128;
-    auto kernel = feed_kernel<T, K, LDOWN, RDOWN, SM, SN, WM, WN, DIRECT>;
-    if constexpr (LDS > 65536) {
-        // on the current device; a driver call, so once a device
-        static std::atomic<uint64_t> told{0};
-        int device = 0;
-        GS_HIP(hipGetDevice(&device));
-        const uint64_t bit = 1ull << (device & 63);
-        if (!(told.load() & bit)) {
-            GS_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-            told |= bit;
+    using OL = Operand<T, SS, SKT, LDOWN, 256, DIRECT>;
+    using OR = Operand<T, SS, SKT, RDOWN, 256, DIRECT>;
+    constexpr int WORDS = OL::WORDS, LOADS = 2 * OL::CH, N = SS / 16;
+    constexpr int BUFFERS = DIRECT && sizeof(T) == 2 ? 3 : 2;
+    extern __shared__ uint4 lds[];                   // [BUFFERS][left, right]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Place at = place_of(A);
+    const Product& P = A.p[at.which];
+    const int m0 = at.tm * SS, n0 = at.tn * (K == HIDDEN ? SS / 2 : SS);
+    const int all = (K == SUM ? 2 : 1) * ((P.depth + SKT - 1) / SKT);
+    const int begin = (int)((int64_t)all * at.split / A.splits), end = (int)((int64_t)all * (at.split + 1) / A.splits);
+
+    f4 acc[N][N];
+#pragma unroll
+    for (int v = 0; v < N; v++)
+#pragma unroll
+        for (int u = 0; u < N; u++) acc[v][u] = f4{0, 0, 0, 0};
+
+    auto left = [](int row) { return row; };
+    auto right = [](int row) { return K == HIDDEN ? row / 32 * 16 + row % 16 : row; };
+    const int lrows = P.rows - m0, rrows = P.cols - n0;
+    const OL ol(P.lld, lrows, left);
+    const OR orr(P.rld, rrows, right);
+    Walk<T, K, SKT, LDOWN, RDOWN> walk(P, m0, n0, K == HIDDEN ? wave / 2 % 2 : 0, begin);
+    const int64_t lld = P.lld, rld = P.rld;
+    // a wave's quarter of the depth: a tile of 128 bytes, or half of one
+    const gs::Tile<T, OL::W> tile;
+    const int mine = sizeof(T) == 4 ? 0 : wave & 1 ? tile.row_at[OL::L::RB - 1] : tile.row_at[0];
+    auto along = [&](const uint4* from, int v) __attribute__((always_inline)) {
+        const uint4* t = from + 32 * wave / OL::W * (8 * SS);
+        if constexpr (sizeof(T) == 4) {
+            return tile.rows(t, 16 * v, 0);
+        } else {
+            Frag<T> f;
+            f.v = __builtin_bit_cast(gs::s8, t[mine + 16 * v * 8]);
+            return f;
+        }
+    };
+    auto down = [&](const uint4* from, int u) __attribute__((always_inline)) {
+        return tile.cols(from + 16 * u / OL::W * (8 * SKT) + 32 * 8 * wave, 0, 16 * u % OL::W);
+    };
+    auto multiply = [&](const uint4* from) __attribute__((always_inline)) {
+        Frag<T> l[N], r[N];
+#pragma unroll
+        for (int v = 0; v < N; v++) {
+            if constexpr (LDOWN) l[v] = down(from, v);
+            else l[v] = along(from, v);
+        }
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            if constexpr (RDOWN) r[u] = down(from + WORDS, u);
+            else r[u] = along(from + WORDS, u);
+        }
+#pragma unroll
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int v = 0; v < N; v++) acc[v][u] = gs::mma(r[u], l[v], acc[v][u]);
+    };
+    if constexpr (DIRECT) {
+        auto fetch = [&](uint4* to) __attribute__((always_inline)) {
+            ol.fetch(to, walk.l, walk.rest);
+            orr.fetch(to + WORDS, walk.r, walk.rest);
+            walk.next();
+        };
+        // behind the barrier `cur` is there, and `far`, which the turn before read, is free
+        auto body = [&](int t, uint4* __restrict__ cur, uint4* __restrict__ far) __attribute__((always_inline)) {
+            if (BUFFERS == 3 && t + 1 < end) arrived<LOADS>(); else arrived<0>();
+            if (t + BUFFERS - 1 < end) fetch(far);
+            multiply(cur);
+        };
+        auto walk2 = [&](uint4* __restrict__ one, uint4* __restrict__ two) __attribute__((always_inline)) {
+            fetch(one);
+            for (int t = begin; t < end; t += 2) {
+                body(t, one, two);
+                if (t + 1 < end) body(t + 1, two, one);
+            }
+        };
+        auto walk3 = [&](uint4* __restrict__ one, uint4* __restrict__ two, uint4* __restrict__ three)
+                         __attribute__((always_inline)) {
+            fetch(one);
+            if (begin + 1 < end) fetch(two);
+            for (int t = begin; t < end; t += 3) {
+                body(t, one, three);
+                if (t + 1 < end) body(t + 1, two, one);
+                if (t + 2 < end) body(t + 2, three, two);
+            }
+        };
+        if (begin < end) {
+            if constexpr (BUFFERS == 3) walk3(lds, lds + 2 * WORDS, lds + 4 * WORDS);
+            else walk2(lds, lds + 2 * WORDS);
+        }
+    } else {
+        gs::Vec<T> lv[OL::CH], rv[OR::CH];
+        auto gather = [&]() __attribute__((always_inline)) {
+            OL::gather(lv, walk.l, walk.rest, lld, lrows, left);
+            // the right operand's rows of HIDDEN are of two tensors, by the wave
+            OR::gather(rv, walk.r, walk.rest, rld, rrows, right);
+            walk.next();
+        };
+        if (begin < end) gather();
+        for (int t = begin; t < end; t++) {
+            uint4* cur = lds + (t - begin) % 2 * 2 * WORDS;
+            OL::settle(lv, cur);
+            OR::settle(rv, cur + WORDS);
+            __syncthreads();   // the other tile was read before the barrier of the turn before
+            if (t + 1 < end) gather();
+            multiply(cur);
         }
     }
+    // wave w takes the rows 16 w .. 16 w + 15 of all four waves' sums
+    f4* meet = (f4*)lds;
+    arrived<0>();
+#pragma unroll
+    for (int v = 0; v < N; v++)
+#pragma unroll
+        for (int u = 0; u < N; u++) meet[((wave * N + v) * N + u) * 64 + lane] = acc[v][u];
+    arrived<0>();
+    f4 sum[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+        sum[u] = meet[((0 * N + wave) * N + u) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < 4; w++) sum[u] += meet[((w * N + wave) * N + u) * 64 + lane];
+    }
+    if (A.splits > 1) {
+        const int64_t tile_of = (int64_t)at.tm * P.tiles_n + at.tn + P.first / A.splits;
+        f4* part = (f4*)A.part + (tile_of * A.splits + at.split) * (N * 256) + threadIdx.x;
+#pragma unroll
+        for (int u = 0; u < N; u++) part[u * 256] = sum[u];
+        return;
+    }
+    arrived<0>();
+    using Out = Leave<T, K, SS>;
+    const Out out(P, A.act, (float*)lds + wave * (16 * Out::LD), n0);
+    typename Out::In in;
+    out.template ask<false>(in, m0 + 16 * wave);
+    out.template give<false>(in, sum, m0 + 16 * wave);
+}
+
+// A tile's parts of the depth, added in order.
+template <typename T>
+__global__ __launch_bounds__(256) void feed_join_kernel(FeedArgs A)
+{
+    constexpr int N = SS / 16;
+    using Out = Leave<T, PLAIN, SS>;
+    __shared__ float lds[4 * 16 * Out::LD];
+    int which = 0;
+    while (which + 1 < A.count && (int)blockIdx.x >= A.p[which + 1].first / A.splits) which++;
+    const Product& P = A.p[which];
+    const int tile = blockIdx.x - P.first / A.splits, tm = tile / P.tiles_n, tn = tile % P.tiles_n, wave = threadIdx.x >> 6;
+    const f4* part = (const f4*)A.part + (int64_t)blockIdx.x * A.splits * (N * 256) + threadIdx.x;
+    f4 sum[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) sum[u] = part[u * 256];
+    for (int s = 1; s < A.splits; s++)
+#pragma unroll
+        for (int u = 0; u < N; u++) sum[u] += part[(int64_t)(s * N + u) * 256];
+    const Out out(P, A.act, lds + wave * (16 * Out::LD), tn * SS);
+    typename Out::In in;
+    out.template give<false>(in, sum, tm * SS + 16 * wave);
+}
+
+// Lays the products' tiles of SM x SN out one after the other; the workgroups, or -1.
+template <Kind K>
+int64_t lay_out(FeedArgs& A, int sm, int sn)
+{
+    int64_t blocks = 0;
+    for (int i = 0; i < A.count; i++) {
+        Product& P = A.p[i];
+        const int n = K == HIDDEN ? sn / 2 : sn;
+        P.tiles_m = (P.rows + sm - 1) / sm;
+        P.tiles_n = (P.cols + n - 1) / n;
+        P.first = (int)blocks;
+        blocks += (int64_t)P.tiles_m * P.tiles_n * A.splits;
+        if (blocks > 0x7fffffff) return -1;
+    }
+    return blocks;
+}
+
+// A kernel with more LDS than 64 KB says so once a device.
+template <typename F>
+int allow_lds(F kernel, size_t bytes, std::atomic<uint64_t>& told)
+{
+    int device = 0;
+    GS_HIP(hipGetDevice(&device));
+    const uint64_t bit = 1ull << (device & 63);
+    if (device > 63 || !(told.load() & bit)) {
+        GS_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        told |= bit;
+    }
+    return GS_OK;
+}
+
+template <typename T, Kind K, bool LDOWN, bool RDOWN, int SM, int SN, int WM, int WN, int BUFFERS>
+int launch_large(FeedArgs& A, hipStream_t stream)
+{
+    const int64_t blocks = lay_out<K>(A, SM, SN);
+    GS_REQUIRE(blocks >= 0, "feed forward: too many tiles");
+    constexpr size_t LDS = (size_t)BUFFERS * (SM + SN) * 128;
+    auto kernel = feed_kernel<T, K, LDOWN, RDOWN, SM, SN, WM, WN, BUFFERS>;
+    static std::atomic<uint64_t> told{0};
+    if (int rc = allow_lds(kernel, LDS, told)) return rc;
     GS_TIMED("feed_kernel", stream,
-             hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WM * WN), LDS, stream, A));
+             hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WM * WN), LDS, stream, A));
     GS_LAUNCH_CHECK("feed_kernel");
     return GS_OK;
+}
+
+template <typename T, Kind K, bool LDOWN, bool RDOWN, bool DIRECT>
+int launch_small(FeedArgs& A, hipStream_t stream)
+{
+    const int64_t blocks = lay_out<K>(A, SS, SS);
+    GS_REQUIRE(blocks >= 0, "feed forward: too many tiles");
+    constexpr size_t LDS = (size_t)(DIRECT && sizeof(T) == 2 ? 3 : 2) * 2 * SS * SKT * sizeof(T);
+    auto kernel = feed_small_kernel<T, K, LDOWN, RDOWN, DIRECT>;
+    static std::atomic<uint64_t> told{0};
+    if (int rc = allow_lds(kernel, LDS, told)) return rc;
+    GS_TIMED("feed_small_kernel", stream,
+             hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), LDS, stream, A));
+    GS_LAUNCH_CHECK("feed_small_kernel");
+    if constexpr (K == PLAIN || K == SUM) {
+        if (A.splits > 1) {
+            GS_TIMED("feed_join_kernel", stream,
+                     hipLaunchKernelGGL(feed_join_kernel<T>, dim3((unsigned)(blocks / A.splits)), dim3(256), 0, stream, A));
+            GS_LAUNCH_CHECK("feed_join_kernel");
+        }
+    }
+    return GS_OK;
+}
+
+constexpr int CUS = 256;
+
+int64_t tiles_of(int64_t m, int64_t n, int sm, int sn) { return (m + sm - 1) / sm * ((n + sn - 1) / sn); }
+
+// Parts of the depth for `tiles` small tiles: while there are fewer than CUs, and three
+// turns or more in a part, of which one takes about what adding it up does.
+int splits_of(int64_t tiles, int64_t turns)
+{
+    int64_t n = tiles > 0 ? CUS / tiles : 1;
+    if (n > turns / 3) n = turns / 3;
+    return (int)(n < 1 ? 1 : n);
+}
+
+// Microseconds that a launch takes with tiles of sm x sn: rounds of tiles, a turn of 64 of
+// the depth each, what begins and ends a tile.  Two 128 x 128 workgroups share a CU, so one
+// ends while the other multiplies; a 256 x 256 one is alone.  Measured, bfloat16, 8192 x
+// 1024 x 4096, with 256 x 256, 256 x 128 (three buffers), 128 x 128 and 64 x 64:
+//   HIDDEN 155, 189, 184, 478   GRAD 141, 133, 124, 296   SUM 190, 123, 157, 277
+//   y 96, 65, 74, 143           weights' gradients 188, 237, 260, 427
+template <Kind K, bool LDOWN>
+double estimate(const FeedArgs& A, int sm, int sn, double turn, double ends)
+{
+    int64_t tiles = 0;
+    for (int i = 0; i < A.count; i++)
+        tiles += tiles_of(A.p[i].rows, A.p[i].cols, sm, K == HIDDEN ? sn / 2 : sn);
+    const double turns = (K == SUM ? 2 : 1) * ((A.p[0].depth + 63) / 64);
+    return (double)((tiles + CUS - 1) / CUS) * (turn * turns + ends);
 }
 
 template <typename T, Kind K, bool LDOWN, bool RDOWN>
@@ -450,15 +790,21 @@ int launch_shape(FeedArgs& A, bool direct, hipStream_t stream)
 {
     if constexpr (sizeof(T) == 2) {
         if (direct) {
-            int64_t n = 0;
-            for (int i = 0; i < A.count; i++)
-                n += (int64_t)((A.p[i].rows + 255) / 256) * ((A.p[i].cols + (K == HIDDEN ? 127 : 255)) / (K == HIDDEN ? 128 : 256));
-            if (n >= 160) return launch_tiles<T, K, LDOWN, RDOWN, 256, 256, 4, 2, true>(A, stream);
-            if (n >= 64) return launch_tiles<T, K, LDOWN, RDOWN, 256, 128, 4, 2, true>(A, stream);
+            const double large = estimate<K, LDOWN>(A, 256, 256, 1.4, K == GRAD ? 48 : K == HIDDEN ? 15 : 7),
+                         wide = estimate<K, LDOWN>(A, 256, 128, 0.98, K == GRAD ? 18 : K == HIDDEN ? 9 : 5),
+                         middle = estimate<K, LDOWN>(A, 128, 128, LDOWN ? 0.68 : 0.58, K == GRAD ? 6 : 2) + 3,
+                         small = estimate<K, LDOWN>(A, 64, 64, 0.28, 1.5) / A.splits + (A.splits > 1 ? 7 : 3);
+            const int splits = A.splits;
+            A.splits = 1;
+            if (large <= wide && large <= middle && large <= small)
+                return launch_large<T, K, LDOWN, RDOWN, 256, 256, 4, 2, 2>(A, stream);
+            if (wide <= middle && wide <= small) return launch_large<T, K, LDOWN, RDOWN, 256, 128, 4, 2, 3>(A, stream);
+            if (middle <= small) return launch_large<T, K, LDOWN, RDOWN, 128, 128, 2, 2, 2>(A, stream);
+            A.splits = splits;
         }
     }
-    if (direct) return launch_tiles<T, K, LDOWN, RDOWN, 128, 128, 2, 2, true>(A, stream);
-    return launch_tiles<T, K, LDOWN, RDOWN, 128, 128, 2, 2, false>(A, stream);
+    if (direct) return launch_small<T, K, LDOWN, RDOWN, true>(A, stream);
+    return launch_small<T, K, LDOWN, RDOWN, false>(A, stream);
 }
 
 template <Kind K, bool LDOWN, bool RDOWN>
@@ -484,19 +830,38 @@ int check(int type, int activation, int64_t rows, int width, int hidden, int out
 // Whether rows of `n` elements, `ld` apart from p on, are whole 16-byte pieces
 bool whole(const void* p, int64_t ld, int n, int type)
 {
+    // a tile's 256 rows are less than 2^31 bytes
     const int v = 16 / gs::dtype_bytes(type);
-    return (uintptr_t)p % 16 == 0 && ld % v == 0 && n % v == 0;
+    return (uintptr_t)p % 16 == 0 && ld % v == 0 && n % v == 0 && ld < 1 << 21;
 }
 
 size_t padded(size_t n) { return (n + 255) / 256 * 256; }
+
+// Sets A's parts of the depth.
+void split(FeedArgs& A, int64_t turns, void* part)
+{
+    int64_t tiles = 0;
+    for (int i = 0; i < A.count; i++) tiles += tiles_of(A.p[i].rows, A.p[i].cols, SS, SS);
+    A.splits = splits_of(tiles, turns);
+    A.part = (float*)part;
+}
+
+int64_t turns_of(int64_t depth) { return (depth + SKT - 1) / SKT; }
+
+// What the parts take: no more of them than CUs, of any products of a launch.
+constexpr size_t PART_BYTES = (size_t)CUS * SS * SS * sizeof(float);
 
 }  // namespace
 
 extern "C" size_t gs_feed_forward_workspace_bytes(int type, int64_t rows, int width, int hidden, int out, int backward)
 {
     if (check(type, GS_SILU, rows, width, hidden, out) != GS_OK) return 0;
-    if (!backward) return 0;
-    return 2 * padded((size_t)rows * hidden * gs::dtype_bytes(type)) + 256;
+    if (!backward) return splits_of(tiles_of(rows, out, SS, SS), turns_of(hidden)) > 1 ? PART_BYTES : 0;
+    // the weights' gradients are split alone or together, as many as are asked for
+    const bool parts = splits_of(tiles_of(rows, width, SS, SS), 2 * turns_of(hidden)) > 1 ||
+                       splits_of(tiles_of(hidden, width, SS, SS), turns_of(rows)) > 1 ||
+                       splits_of(tiles_of(out, hidden, SS, SS), turns_of(rows)) > 1;
+    return 2 * padded((size_t)rows * hidden * gs::dtype_bytes(type)) + (parts ? PART_BYTES : 256);
 }
 
 extern "C" int gs_feed_forward(int type, int activation, int64_t rows, int width, int hidden, int out, const void* x,
@@ -538,6 +903,9 @@ extern "C" int gs_feed_forward(int type, int activation, int64_t rows, int width
     P.old = out;
     P.out[0] = y;
     direct = whole(h, hidden, hidden, type) && whole(down, hidden, hidden, type);
+    split(A, turns_of(hidden), workspace);
+    GS_REQUIRE(A.splits == 1 || (workspace != nullptr && (uintptr_t)workspace % 256 == 0),
+               "feed forward: these sizes need the workspace, 256-byte aligned");
     return launch<PLAIN, false, false>(type, A, direct, stream);
 }
 
@@ -554,7 +922,7 @@ extern "C" int gs_feed_forward_backward(int type, int activation, int64_t rows, 
     if (rows > 0) {
         GS_REQUIRE(x && gate && up && down && a && b && h && dy,
                    "feed forward: x, the weights, a, b, h and dy must be non-null");
-        GS_REQUIRE(!inner || (workspace != nullptr && (uintptr_t)workspace % 256 == 0),
+        GS_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 256 == 0,
                    "feed forward: the backward needs its workspace, 256-byte aligned");
     }
     char* da = (char*)workspace;
@@ -563,6 +931,7 @@ extern "C" int gs_feed_forward_backward(int type, int activation, int64_t rows, 
     A.act = activation;
     A.splits = 1;
     A.count = 1;
+    void* part = db + padded((size_t)rows * hidden * gs::dtype_bytes(type));
     if (inner && rows > 0) {
         Product& P = A.p[0];
         P.l[0] = dy;
@@ -596,6 +965,7 @@ extern "C" int gs_feed_forward_backward(int type, int activation, int64_t rows, 
         P.out[0] = dx;
         const bool direct = whole(da, hidden, hidden, type) && whole(gate, width, width, type) &&
                             whole(up, width, width, type);
+        split(A, 2 * turns_of(hidden), part);
         if (int rc = launch<SUM, false, true>(type, A, direct, stream)) return rc;
     }
     // the weights' gradients, one after the other in one launch
@@ -620,5 +990,6 @@ extern "C" int gs_feed_forward_backward(int type, int activation, int64_t rows, 
     add(db, hidden, hidden, x, x_stride, width, dup);
     add(dy, dy_stride, out, h, hidden, hidden, ddown);
     if (A.count == 0) return GS_OK;
+    split(A, turns_of(rows), part);
     return launch<PLAIN, true, true>(type, A, direct, stream);
 }
