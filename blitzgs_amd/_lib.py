@@ -121,8 +121,8 @@ _SIGS = {
     "gs_momentum_update": (_i, [_i, _i, _i64, C.POINTER(_c), C.POINTER(_c), _f, _i, _c, _c]),
     "gs_momentum_apply": (_i, [_i, _i, _i64, C.POINTER(_c), _f, _f, _c, _c]),
     "gs_feed_forward_workspace_bytes": (_sz, [_i, _i64, _i, _i, _i, _i]),
-    "gs_feed_forward": (_i, [_i, _i, _i64, _i, _i, _i, _c, _i64] + [_c] * 9),
-    "gs_feed_forward_backward": (_i, [_i, _i, _i64, _i, _i, _i, _c, _i64] + [_c] * 7 + [_i64] + [_c] * 6),
+    "gs_feed_forward": (_i, [_i, _i, _i64, _i, _i, _i, _c, _i64] + [_c] * 10),
+    "gs_feed_forward_backward": (_i, [_i, _i, _i64, _i, _i, _i, _c, _i64] + [_c] * 8 + [_i64] + [_c] * 6),
     "gs_adamw_update": (_i, [_i, _i, _i, C.POINTER(_i64)] + [C.POINTER(_c)] * 6 + [C.POINTER(AdamWSettings), _c]),
     "gs_adamw_values": (_i, [_i, _i64] + [_c] * 7),
     "gs_diag_math": (_i, [_i, _i, _c, _c, _c]),

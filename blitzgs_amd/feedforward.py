@@ -8,9 +8,10 @@ or 'gelu', a (1 + erf(a / sqrt(2))) / 2.  One call is two kernels: both projecti
 the activation and the product, and the projection down.
 
 Sums are fp32.  Besides y, what lies between two products is rounded to the tensors'
-type: act(a) * b, and for the backward a, b and their gradients, so float16's range (up
-to 65504, from 6e-5 at full precision) holds for those too.  A call that needs gradients
-keeps x, the weights, a, b and act(a) * b.  The weights' gradients are added up in a
+type: act(a) * b, and the gradients of a = x gate^T and b = x up^T, so float16's range (up
+to 65504, from 6e-5 at full precision) holds for those too, and for a and b.  A call that
+needs gradients keeps x, the weights, a, b (in the 16-bit types with four more bits each)
+and act(a) * b.  The weights' gradients are added up in a
 fixed order: equal inputs give equal bits.
 """
 import torch
@@ -34,7 +35,7 @@ def _rows(t, width):
 
 
 def _forward(x, gate, up, down, activation, grads):
-    """y and, for a backward, a, b, h and what it is called with."""
+    """y and, for a backward, a, b, their rests, h and what it is called with."""
     (hidden, width), out = gate.shape, down.shape[0]
     n = x.numel() // width
     rows, apart = _rows(x, width)
@@ -42,19 +43,20 @@ def _forward(x, gate, up, down, activation, grads):
     lib, new = _t.load(), lambda *shape: torch.empty(shape, device=x.device, dtype=x.dtype)
     y, h = new(*x.shape[:-1], out), new(n, hidden)
     a, b = (new(n, hidden), new(n, hidden)) if grads else (None, None)
+    rest = torch.empty((n, hidden), device=x.device, dtype=torch.uint8) if grads and x.dtype != torch.float32 else None
     ws = _t.workspace(lib.gs_feed_forward_workspace_bytes(sizes[0], *sizes[2:], 0), x.device)
     with _t.on_device(x.device):
         _t.check(lib.gs_feed_forward(*sizes, rows.data_ptr(), apart, gate.data_ptr(), up.data_ptr(), down.data_ptr(),
-                                     _t.ptr(a), _t.ptr(b), h.data_ptr(), y.data_ptr(), _t.ptr(ws),
+                                     _t.ptr(a), _t.ptr(b), _t.ptr(rest), h.data_ptr(), y.data_ptr(), _t.ptr(ws),
                                      _t.stream(x.device)), "gs_feed_forward")
-    return y, a, b, h, sizes
+    return y, a, b, rest, h, sizes
 
 
 class _FeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, up, down, activation):
-        y, a, b, h, ctx.how = _forward(x.detach(), gate, up, down, activation, True)
-        ctx.save_for_backward(x, gate, up, down, a, b, h)
+        y, a, b, rest, h, ctx.how = _forward(x.detach(), gate, up, down, activation, True)
+        ctx.save_for_backward(x, gate, up, down, a, b, rest, h)
         ctx.ws_bytes = _t.load().gs_feed_forward_workspace_bytes(ctx.how[0], *ctx.how[2:], 1)
         return y
 
@@ -65,7 +67,7 @@ class _FeedForward(torch.autograd.Function):
     def backward(ctx, dy):
         # hooks on saved tensors give them back with the same values, not in the same places
         x, *saved = ctx.saved_tensors
-        gate, up, down, a, b, h = (t.contiguous() for t in saved)
+        gate, up, down, a, b, rest, h = (t if t is None else t.contiguous() for t in saved)
         _, _, n, width, hidden, out = ctx.how
         rows, apart = _rows(x, width)
         drows, dapart = _rows(dy, out)
@@ -75,7 +77,7 @@ class _FeedForward(torch.autograd.Function):
         ws = _t.workspace(ctx.ws_bytes, x.device)
         _t.check(_t.load().gs_feed_forward_backward(
             *ctx.how, rows.data_ptr(), apart, gate.data_ptr(), up.data_ptr(), down.data_ptr(), a.data_ptr(), b.data_ptr(),
-            h.data_ptr(), drows.data_ptr(), dapart, _t.ptr(dx), _t.ptr(dgate), _t.ptr(dup), _t.ptr(ddown), _t.ptr(ws),
+            _t.ptr(rest), h.data_ptr(), drows.data_ptr(), dapart, _t.ptr(dx), _t.ptr(dgate), _t.ptr(dup), _t.ptr(ddown), _t.ptr(ws),
             _t.stream(x.device)), "gs_feed_forward_backward")
         return dx, dgate, dup, ddown, None
 

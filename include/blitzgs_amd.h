@@ -747,8 +747,11 @@ int gs_rotary_backward(int type, int param_type, int B, int Hq, int Hk, int T, i
  * GS_SILU, a / (1 + exp(-a)), or GS_GELU, a (1 + erf(a / sqrt(2))) / 2.  x's (and
  * dy's) rows are x_stride elements apart and contiguous inside, all else is
  * contiguous.  h (rows, hidden) is written: act(a) * b of a = x gate^T, b = x up^T,
- * rounded to `type`; a and b (rows, hidden) too, for the backward, or both NULL.
- *   Backward, from a, b and h: dx, dgate, dup, ddown, each unless NULL.
+ * rounded to `type`; a and b (rows, hidden) too, for the backward, or both NULL, and
+ * rest (rows, hidden), a byte each, may be NULL: with the 16-bit types four bits of
+ * what rounding a left and, above them, four of b.
+ *   Backward, from a, b, rest (NULL if the forward had none) and h: dx, dgate, dup,
+ * ddown, each unless NULL.
  *   workspace: 256-byte aligned, of gs_feed_forward_workspace_bytes (0: none is
  * needed, or the arguments are invalid). */
 #define GS_SILU 0
@@ -757,12 +760,12 @@ size_t gs_feed_forward_workspace_bytes(int type, int64_t rows, int width, int hi
                                        int backward);
 int gs_feed_forward(int type, int activation, int64_t rows, int width, int hidden, int out,
                     const void* x, int64_t x_stride, const void* gate, const void* up,
-                    const void* down, void* a, void* b, void* h, void* y, void* workspace,
-                    gs_stream_t stream);
+                    const void* down, void* a, void* b, void* rest, void* h, void* y,
+                    void* workspace, gs_stream_t stream);
 int gs_feed_forward_backward(int type, int activation, int64_t rows, int width, int hidden, int out,
                              const void* x, int64_t x_stride, const void* gate, const void* up,
-                             const void* down, const void* a, const void* b, const void* h,
-                             const void* dy, int64_t dy_stride, void* dx, void* dgate, void* dup,
+                             const void* down, const void* a, const void* b, const void* rest,
+                             const void* h, const void* dy, int64_t dy_stride, void* dx, void* dgate, void* dup,
                              void* ddown, void* workspace, gs_stream_t stream);
 
 /* The orthogonalised update of `count` matrices (m, n), contiguous: `steps` (1

@@ -118,8 +118,9 @@ def feed_forward_64(x, gate, up, down, activation, dy=None):
     if dy is None:
         return out
     dy = dy.double().cpu()
-    # the backward's a and b are rounded
-    e_a, e_b = e_a + u * a.abs() + step, e_b + u * b.abs() + step
+    # the backward's a and b are rounded, to a sixteenth of the last bit
+    near_u = u if t == torch.float32 else u / 8          # a half of the last bit is held as 7 sixteenths
+    e_a, e_b = e_a + near_u * a.abs() + step, e_b + near_u * b.abs() + step
     e_act, _ = hidden(e_a, e_b)
     dh = dy @ down
     e_dh = s(O) * (dy.abs() @ down.abs())

@@ -62,8 +62,8 @@ def test_rotary(lib):
 
 
 def test_feed_forward(lib):
-    def fwd(type=BF16, act=0, rows=4, W=8, H=16, O=8, x=NZ, a=None, b=None, h=NZ):
-        return lib.gs_feed_forward(type, act, rows, W, H, O, x, W, NZ, NZ, NZ, a, b, h, NZ, NZ, None)
+    def fwd(type=BF16, act=0, rows=4, W=8, H=16, O=8, x=NZ, a=None, b=None, rest=None, h=NZ):
+        return lib.gs_feed_forward(type, act, rows, W, H, O, x, W, NZ, NZ, NZ, a, b, rest, h, NZ, NZ, None)
     _refused(lib, fwd(type=3), b"element type")
     _refused(lib, fwd(act=2), b"activation")
     _refused(lib, fwd(rows=-1), b"rows")
@@ -71,13 +71,14 @@ def test_feed_forward(lib):
     for bad in (dict(W=0), dict(H=0), dict(O=0), dict(H=2 ** 24 + 1)):
         _refused(lib, fwd(**bad), b"width, hidden and out")
     _refused(lib, fwd(a=NZ), b"together")
+    _refused(lib, fwd(rest=NZ), b"together")
     _refused(lib, fwd(x=None), b"non-null")
     _refused(lib, fwd(h=None), b"non-null")
     assert fwd(rows=0) == 0
 
     def bwd(x=NZ, dx=NZ, dd=NZ, ws=NZ, rows=4):
-        return lib.gs_feed_forward_backward(BF16, 0, rows, 8, 16, 8, x, 8, NZ, NZ, NZ, NZ, NZ, NZ, NZ, 8, dx, None, None, dd,
-                                            ws, None)
+        return lib.gs_feed_forward_backward(BF16, 0, rows, 8, 16, 8, x, 8, NZ, NZ, NZ, NZ, NZ, NZ, NZ, NZ, 8, dx, None, None,
+                                            dd, ws, None)
     _refused(lib, bwd(x=None), b"non-null")
     _refused(lib, bwd(ws=None), b"workspace")
     _refused(lib, bwd(ws=C.c_void_p(264)), b"aligned")
