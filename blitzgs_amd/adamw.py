@@ -39,14 +39,19 @@ def new_moments(param, bits=32):
             zeros(2, -(-param.numel() // BLOCK), dtype=torch.uint8))
 
 
-def _checked(ts, name, dtype, params):
-    """Contiguous tensors like the parameters, of a type."""
-    if len(ts) != len(params):
-        raise RuntimeError(f"{name} must hold a tensor for each of {len(params)} parameters, got {len(ts)}")
-    for t, p in zip(ts, params):
-        if (not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != p.shape or t.device != p.device
-                or not t.is_contiguous()):
-            raise RuntimeError(f"{name} must hold contiguous {dtype} tensors of the parameters' shapes on {p.device}")
+def _checked(ts, name, dtype, shapes, device):
+    """Contiguous tensors of a type and of the parameters' shapes."""
+    if len(ts) != len(shapes):
+        raise RuntimeError(f"{name} must hold a tensor for each of {len(shapes)} parameters, got {len(ts)}")
+    # attribute by attribute: a call over many tensors is bound by this otherwise
+    index = device.index
+    try:
+        fit = (all([t.dtype is dtype for t in ts]) and all([t.get_device() == index for t in ts])
+               and [t.shape for t in ts] == shapes and all([t.is_contiguous() for t in ts]))
+    except AttributeError:        # no tensor
+        fit = False
+    if not fit:
+        raise RuntimeError(f"{name} must hold contiguous {dtype} tensors of the parameters' shapes on {device}")
 
 
 def _settings(lr, betas, eps, weight_decay):
@@ -76,34 +81,32 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
         return
     first = params[0]
     _t.require_tensor(first, "params")
-    _checked(params, "params", first.dtype, params)
-    device = first.device
-    for p in params:
-        if p.device != device:
-            raise RuntimeError(f"params must be on one device, got {device} and {p.device}")
-    for g in grads:
-        if isinstance(g, torch.Tensor) and g.is_sparse:
-            raise RuntimeError("gradients must be dense")
-    grads = [g.contiguous() if isinstance(g, torch.Tensor) else g for g in grads]
-    _checked(grads, "grads", first.dtype, params)
+    device, shapes = first.device, [p.shape if isinstance(p, torch.Tensor) else None for p in params]
+    _checked(params, "params", first.dtype, shapes, device)
+    if not all([isinstance(g, torch.Tensor) and g.layout is torch.strided for g in grads]):
+        raise RuntimeError("grads must hold dense tensors")
+    grads = [g.contiguous() for g in grads]
+    _checked(grads, "grads", first.dtype, shapes, device)
     moment = torch.float32 if scales is None else torch.uint8
-    _checked(exp_avgs, "exp_avgs", moment, params)
-    _checked(exp_avg_sqs, "exp_avg_sqs", moment, params)
-    n = len(params)
+    _checked(exp_avgs, "exp_avgs", moment, shapes, device)
+    _checked(exp_avg_sqs, "exp_avg_sqs", moment, shapes, device)
+    n, sizes = len(params), [p.numel() for p in params]
     pointers = lambda addresses: (C.c_void_p * n)(*addresses)  # noqa: E731
     written = [[t.data_ptr() for t in ts] for ts in (params, exp_avgs, exp_avg_sqs)]
     low = high = None
     if scales is not None:
         if len(scales) != n:
             raise RuntimeError(f"scales must hold a tensor for each of {n} parameters, got {len(scales)}")
-        for s, p in zip(scales, params):
-            if (not isinstance(s, torch.Tensor) or s.dtype != torch.uint8 or s.device != device
-                    or s.shape != (2, -(-p.numel() // BLOCK)) or (s.shape[1] > 1 and s.stride(1) != 1)):
-                raise RuntimeError(f"scales must hold uint8 tensors of shape (2, ceil(n / {BLOCK})) with contiguous rows "
-                                   f"on {device}")
+        blocks = [-(-size // BLOCK) for size in sizes]
+        if not (all([isinstance(s, torch.Tensor) and s.dtype is torch.uint8 for s in scales])
+                and all([s.get_device() == device.index for s in scales])
+                and [s.shape for s in scales] == [(2, b) for b in blocks]
+                and all([s.is_contiguous() or s.stride() >= (b, 1) and s.stride(1) == 1
+                         for s, b in zip(scales, blocks)])):
+            raise RuntimeError(f"scales must hold uint8 tensors of shape (2, ceil(n / {BLOCK})) with contiguous rows on "
+                               f"{device}")
         written += [[s.data_ptr() for s in scales], [s.data_ptr() + s.stride(0) for s in scales]]
         low, high = (pointers(a) for a in written[3:])
-    sizes = [p.numel() for p in params]
     addresses = [a for column in written for a, size in zip(column, sizes) if size]
     if len(set(addresses)) != len(addresses):
         raise RuntimeError("a tensor may not come twice in a call")

@@ -97,6 +97,17 @@ __device__ __forceinline__ uint32_t encoded(float x, float over, uint32_t draw)
     return SIGN ? c | (c > 0 && x < 0.0f ? 128u : 0u) : c;
 }
 
+// The hardware's square root, and its reciprocal in the step, are off by one last bit, of
+// an update that is a small part of its parameter; with 8-bit moments the step is bound by
+// its instructions, and with the exact ones 183M bfloat16 elements took 472 us for 417.
+// The hardware's takes no subnormals.
+__device__ __forceinline__ float root_of(float v)
+{
+    const bool tiny = v < 0x1p-96f;
+    const float r = __builtin_amdgcn_sqrtf(tiny ? v * 0x1p96f : v);
+    return tiny ? r * 0x1p-48f : r;
+}
+
 template <typename T, int BITS, bool WHOLE>
 __device__ __forceinline__ void step(const AdamArgs& A, const Tensor& t, int64_t at)
 {
@@ -145,8 +156,8 @@ __device__ __forceinline__ void step(const AdamArgs& A, const Tensor& t, int64_t
         const float gi = (float)tg[i];
         m[i] = __builtin_fmaf(A.b1, m[i], A.c1 * gi);
         v[i] = __builtin_fmaf(A.b2, v[i], A.c2 * gi * gi);
-        const float by = __builtin_fmaf(__builtin_sqrtf(v[i]), A.root, A.eps);
-        tp[i] = (T)__builtin_fmaf((float)tp[i], A.keep, -(A.rate * (m[i] / by)));
+        const float by = __builtin_fmaf(root_of(v[i]), A.root, A.eps);
+        tp[i] = (T)__builtin_fmaf((float)tp[i], A.keep, -(A.rate * (m[i] * __builtin_amdgcn_rcpf(by))));
     }
     put(p, tp);
     if constexpr (BITS == 32) {

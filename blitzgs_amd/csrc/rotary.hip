@@ -124,13 +124,29 @@ __device__ __forceinline__ Item item_of(int i, int N, int D)
     return t;
 }
 
-template <typename T, int V>
+// Where pairs are neighbours an item is one piece of 2 V elements.
+template <typename T, int V, bool IL>
 __device__ __forceinline__ void load_item(const T* row, const Item& t, float (&v)[2 * V])
 {
 #pragma unroll
     for (int i = 0; i < 2 * V; i++) v[i] = 0.0f;
+    if (IL && t.has_hi) {
+        load<T, 2 * V>(row + t.lo, v);
+        return;
+    }
     if (t.has_lo) load<T, V>(row + t.lo, v);
-    if (t.has_hi) load<T, V>(row + t.hi, v + V);
+    if (!IL && t.has_hi) load<T, V>(row + t.hi, v + V);
+}
+
+template <typename T, int V, bool IL>
+__device__ __forceinline__ void store_item(T* row, const Item& t, const float (&v)[2 * V])
+{
+    if (IL && t.has_hi) {
+        store<T, 2 * V>(row + t.lo, v);
+        return;
+    }
+    if (t.has_lo) store<T, V>(row + t.lo, v);
+    if (!IL && t.has_hi) store<T, V>(row + t.hi, v + V);
 }
 
 // The rotation by the table's angles, or back.
@@ -154,9 +170,9 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
     extern __shared__ uint64_t lds[];
     const Side& S = A.side[blockIdx.y];
     if (blockIdx.x >= S.blocks) return;
-    // [tokens][3] offsets of x, dy, out; then [tokens][N] of cosine and sine
+    // [tokens][4] offsets of x, dy, out and the positions; then [tokens][N] of cosine and sine
     int64_t* offset = (int64_t*)lds;
-    float2* table = (float2*)(lds + 3 * S.tokens);
+    float2* table = (float2*)(lds + 4 * S.tokens);
     const int lpr = A.lpr, lane = threadIdx.x & (lpr - 1), group = threadIdx.x / lpr, groups = BLOCK / lpr;
     const int N = A.N, D = A.D;
 
@@ -172,45 +188,55 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
         }
         if (NORM && S.w != nullptr) {
             if (A.w32)
-                load_item<float, V>((const float*)S.w, items[c], w[c]);
+                load_item<float, V, IL>((const float*)S.w, items[c], w[c]);
             else
-                load_item<T, V>((const T*)S.w, items[c], w[c]);
+                load_item<T, V, IL>((const T*)S.w, items[c], w[c]);
         }
     }
-    // a group's rows are `groups` apart
+    // a group's rows are `groups` apart, a thread's pairs BLOCK: no divisions in the loops
     const int step_token = groups / S.heads, step_head = groups % S.heads;
+    const int first_head = group % S.heads, first_token = group / S.heads;
+    const int table_token = threadIdx.x / N, table_pair = threadIdx.x - table_token * N;
+    const int table_tokens = BLOCK / N, table_pairs = BLOCK - table_tokens * N;
 
     for (int64_t first = (int64_t)blockIdx.x * S.tokens; first < A.n_tokens; first += (int64_t)S.blocks * S.tokens) {
         const int here = A.n_tokens - first < S.tokens ? (int)(A.n_tokens - first) : S.tokens;
-        for (int e = threadIdx.x; e < here * N; e += BLOCK) {
-            const int token = e / N, pair = e - token * N;
-            const int64_t b = (first + token) / A.T, t = (first + token) - b * A.T;
-            const int64_t at = b * A.ps[0] + t * A.ps[1] + pair / A.pairs * A.ps[2];
+        if (threadIdx.x < here) {
+            const int64_t b = (first + threadIdx.x) / A.T, t = (first + threadIdx.x) - b * A.T;
+            offset[4 * threadIdx.x] = b * S.xs[0] + t * S.xs[2];
+            offset[4 * threadIdx.x + 1] = b * S.dys[0] + t * S.dys[2];
+            offset[4 * threadIdx.x + 2] = b * S.outs[0] + t * S.outs[2];
+            offset[4 * threadIdx.x + 3] = b * A.ps[0] + t * A.ps[1];
+        }
+        __syncthreads();
+        for (int token = table_token, pair = table_pair; token < here;) {
+            int64_t at = offset[4 * token + 3];
+            if (A.pairs < N) at += pair / A.pairs * A.ps[2];
             const int64_t position = A.wide ? ((const int64_t*)A.positions)[at] : ((const int*)A.positions)[at];
             float c, s;
             cos_sin((uint64_t)position * A.frequencies[pair], c, s);
-            table[e] = make_float2(c * A.magnitude, s * A.magnitude);
-        }
-        if (threadIdx.x < here) {
-            const int64_t b = (first + threadIdx.x) / A.T, t = (first + threadIdx.x) - b * A.T;
-            offset[3 * threadIdx.x] = b * S.xs[0] + t * S.xs[2];
-            offset[3 * threadIdx.x + 1] = b * S.dys[0] + t * S.dys[2];
-            offset[3 * threadIdx.x + 2] = b * S.outs[0] + t * S.outs[2];
+            table[token * N + pair] = make_float2(c * A.magnitude, s * A.magnitude);
+            token += table_tokens;
+            pair += table_pairs;
+            if (pair >= N) {
+                pair -= N;
+                token++;
+            }
         }
         __syncthreads();
         // the lanes of a row leave the loop together
-        int token = group / S.heads, head = group - token * S.heads;
+        int token = first_token, head = first_head;
         while (token < here) {
-            const T* x = (const T*)S.x + offset[3 * token] + head * S.xs[1];
-            const T* dy = (const T*)S.dy + offset[3 * token + 1] + head * S.dys[1];
-            T* out = (T*)S.out + offset[3 * token + 2] + head * S.outs[1];
+            const T* x = (const T*)S.x + offset[4 * token] + head * S.xs[1];
+            const T* dy = (const T*)S.dy + offset[4 * token + 1] + head * S.dys[1];
+            T* out = (T*)S.out + offset[4 * token + 2] + head * S.outs[1];
             const float2* cs = table + token * N;
             float v[NC][2 * V], g[NC][2 * V];
             float r = 1.0f;
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-                if constexpr (!BWD || NORM) load_item<T, V>(x, items[c], v[c]);
-                if constexpr (BWD) load_item<T, V>(dy, items[c], g[c]);
+                if constexpr (!BWD || NORM) load_item<T, V, IL>(x, items[c], v[c]);
+                if constexpr (BWD) load_item<T, V, IL>(dy, items[c], g[c]);
             }
             if constexpr (NORM) {
                 float sum = 0.0f;
@@ -258,10 +284,7 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
                 }
             }
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                if (items[c].has_lo) store<T, V>(out + items[c].lo, v[c]);
-                if (items[c].has_hi) store<T, V>(out + items[c].hi, v[c] + V);
-            }
+            for (int c = 0; c < NC; c++) store_item<T, V, IL>(out, items[c], v[c]);
             head += step_head;
             token += step_token;
             if (head >= S.heads) {
@@ -345,9 +368,11 @@ Plan plan_of(int type, int64_t n_tokens, int heads, int D, int N, bool parts)
     const int items = (D + 2 * p.v - 1) / (2 * p.v);
     for (p.lpr = 1; p.lpr < 64 && p.lpr < items; p.lpr *= 2) {}
     p.nc = (items + p.lpr - 1) / p.lpr;
-    // eight rows a group, or fewer where that would leave CUs without work
+    // Four rows a group, or fewer where that would leave CUs without work: the angles of one
+    // workgroup are formed while others move rows (32768 tokens of 24 heads of 64, forward
+    // and backward: 103 us, with eight rows 111).
     const int64_t rows = BLOCK / p.lpr;
-    int64_t tokens = (8 * rows + heads - 1) / heads;
+    int64_t tokens = (4 * rows + heads - 1) / heads;
     while (tokens > 1 && (n_tokens + tokens - 1) / tokens < 1024) tokens = (tokens + 1) / 2;
     const int64_t fit = MAX_TABLE / N < BLOCK ? MAX_TABLE / N : BLOCK;
     p.tokens = (int)(tokens < fit ? tokens : fit);
@@ -428,7 +453,7 @@ size_t fill(RotaryArgs& A, Plan (&plan)[2], int type, int param_type, int B, con
         A.side[i].heads = heads[i];
         A.side[i].tokens = plan[i].tokens;
         A.side[i].blocks = heads[i] > 0 && A.side[i].out != nullptr ? plan[i].blocks : 0;
-        size_t n = (size_t)plan[i].tokens * (3 * sizeof(int64_t) + A.N * sizeof(float2));
+        size_t n = (size_t)plan[i].tokens * (4 * sizeof(int64_t) + A.N * sizeof(float2));
         if (parts && n < 2u * plan[i].v * BLOCK * sizeof(float)) n = 2u * plan[i].v * BLOCK * sizeof(float);
         if (A.side[i].blocks > 0 && n > lds) lds = n;
     }
