@@ -88,7 +88,7 @@ def test_moments_in_8_bits(gpu, t, step, seed):
             # the bounds are the same code but where the rest is at a border
             assert (low == high).double().mean() > 0.99
             if top == 14:
-                assert torch.equal((c >= 128), (x < 0) & (size > 0))
+                assert torch.equal((c >= 128)[size > 0], (x < 0)[size > 0])
         for dtype in (torch.float32, torch.bfloat16):
             a, b = moment_values(m[i], v[i], s[i], dtype=dtype)
             assert torch.equal(a.double().cpu(), values_8(m[i], s[i][0], 14))
@@ -131,6 +131,24 @@ def test_rounding_keeps_the_mean(gpu):
     noise = math.sqrt(k) * (1 / 16) / math.sqrt(n)
     assert abs(ratio - 0.999 ** k) <= 6 * noise and ratio < 0.9
     assert not torch.equal(v1, v0.float())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-12])
+def test_small_gradients_and_a_small_eps(gpu, bits, eps):
+    # second moments below fp32's normal range, which eps does not hide
+    from blitzgs_amd.adamw import adamw_update, new_moments
+    p = _rand((500,), torch.float32, 1)
+    g = _rand((500,), torch.float32, 2).sign() * torch.logspace(-20, -15, 500, device="cuda")
+    q = p.clone()
+    m, v, s = new_moments(q, bits)
+    how = dict(lr=0.1, betas=(0.9, 0.999), eps=eps, weight_decay=0.0)
+    adamw_update([q], [g], [m], [v], step=1, scales=None if bits == 32 else [s], **how)
+    g64 = g.double()
+    want = p.double() - 0.1 * g64 / (g64.abs() + eps)
+    # a subnormal v has a last bit of 2^-149: its root is off by that over twice the root; the update is at most 0.1
+    loose = 0.1 * torch.clamp(2.0 ** -149 / (0.001 * g64.square()), max=2.0) + 20 * 2.0 ** -24
+    assert ((q.double() - want).abs() <= loose + 2.0 ** -24 * p.abs().double()).all()
 
 
 def test_zero_nan_and_infinity(gpu):
