@@ -5,10 +5,11 @@ rasterizer, on synthetic images:
 
 A scene is one or two views; their patches are tokens of one sequence.  Two
 blocks of layer normalisation, attention (eight query heads on two key heads,
-scenes of unequal length in one padded batch) and a gated linear unit turn each
-token of the first view into four Gaussians, which are rendered and compared
-with that view by L1 and SSIM.  The weight matrices take orthogonalised updates,
-all other parameters Adam's."""
+normalised and rotated to their patch's row and column, scenes of unequal length
+in one padded batch) and a gated feed-forward turn each token of the first view
+into four Gaussians, which are rendered and compared with that view by L1 and
+SSIM.  The weight matrices take orthogonalised updates, all other parameters
+AdamW's, with moments in 8 bits."""
 import argparse
 import math
 
@@ -17,10 +18,13 @@ import torch
 from torch import nn
 
 from .. import synth
+from ..adamw import AdamW
 from ..attention import attention
+from ..feedforward import feed_forward
 from ..norm import layer_norm
 from ..orthogonal import OrthogonalMomentum
 from ..rasterizer import GaussianRasterizationSettings, GaussianRasterizer
+from ..rotary import norm_rotate, rotary_frequencies
 from ..ssim import fused_ssim
 
 SIDE, PATCH, PER_TOKEN = 128, 8, 4
@@ -41,19 +45,20 @@ class Block(nn.Module):
         super().__init__()
         self.heads, self.key_heads, self.head_dim = heads, key_heads, width // heads
         self.norm1, self.norm2 = nn.Parameter(torch.ones(width)), nn.Parameter(torch.ones(width))
+        self.norm_q, self.norm_k = (nn.Parameter(torch.ones(self.head_dim)) for _ in range(2))
         self.qkv = _matrix((heads + 2 * key_heads) * self.head_dim, width)
         self.proj = _matrix(width, width)
         self.gate, self.up, self.down = _matrix(2 * width, width), _matrix(2 * width, width), _matrix(width, 2 * width)
 
-    def forward(self, x, key_lengths):
+    def forward(self, x, key_lengths, places, frequencies):
         B, T, _ = x.shape
         mul = lambda a, w: a @ w.t().to(a.dtype)  # noqa: E731
         qkv = mul(layer_norm(x, self.norm1), self.qkv).view(B, T, -1, self.head_dim)
         q, k, v = qkv.split([self.heads, self.key_heads, self.key_heads], 2)
-        o = attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), key_lengths=key_lengths)
+        q, k = norm_rotate(q.transpose(1, 2), k.transpose(1, 2), self.norm_q, self.norm_k, places, frequencies)
+        o = attention(q, k, v.transpose(1, 2), key_lengths=key_lengths)
         x = x + mul(o.transpose(1, 2).reshape(B, T, -1), self.proj)
-        h = layer_norm(x, self.norm2)
-        return x + mul(nn.functional.silu(mul(h, self.gate)) * mul(h, self.up), self.down)
+        return x + feed_forward(layer_norm(x, self.norm2), *(w.to(x.dtype) for w in (self.gate, self.up, self.down)))
 
 
 class Predictor(nn.Module):
@@ -68,6 +73,10 @@ class Predictor(nn.Module):
         self.head = nn.Parameter(0.02 * torch.randn(PER_TOKEN * 14, width))
         at = (torch.arange(GRID) + 0.5) * 2 / GRID - 1
         y, x = torch.meshgrid(at, at, indexing="ij")
+        row, column = torch.meshgrid(torch.arange(GRID), torch.arange(GRID), indexing="ij")
+        self.register_buffer("places", torch.stack([row, column], -1).reshape(TOKENS, 2).repeat(views, 1))
+        # half of a head's pairs turn with the row, half with the column
+        self.register_buffer("frequencies", rotary_frequencies(width // heads // 4, base=100.0, axes=2, device="cpu"))
         self.register_buffer("centre", HALF * torch.stack([x, y, torch.zeros_like(x)], -1).reshape(TOKENS, 1, 3))
 
     def matrices(self):
@@ -80,7 +89,7 @@ class Predictor(nn.Module):
     def forward(self, patches, key_lengths):
         x = (patches @ self.embed.t() + self.position[:patches.shape[1]]).to(torch.bfloat16)
         for block in self.blocks:
-            x = block(x, key_lengths)
+            x = block(x, key_lengths, self.places[:x.shape[1]], self.frequencies)
         x = layer_norm(x[:, :TOKENS], self.norm_weight, self.norm_bias).float() @ self.head.t()
         move, scale, turn, opacity, colour = x.view(-1, TOKENS, PER_TOKEN, 14).split([3, 3, 4, 1, 3], -1)
         P = TOKENS * PER_TOKEN
@@ -131,7 +140,7 @@ def train(steps=60, seed=0, device="cuda", report=None):
     torch.manual_seed(seed)
     g = torch.Generator(device=device).manual_seed(seed)
     net, raster = Predictor().to(device), rasterizer(device)
-    opt = [OrthogonalMomentum(net.matrices(), lr=0.01), torch.optim.Adam(net.others(), lr=2e-3)]
+    opt = [OrthogonalMomentum(net.matrices(), lr=0.01), AdamW(net.others(), lr=2e-3, weight_decay=0.0, bits=8)]
     # two scenes: one of two views, one of a single view, whose second half is padding
     scenes = [images(2, g, device), images(1, g, device)]
     tokens = [patches_of(v) for v in scenes]
