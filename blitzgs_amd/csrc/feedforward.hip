@@ -699,7 +699,9 @@ __global__ __launch_bounds__(256, 1) void feed_small_kernel(FeedArgs A)
 #pragma unroll
         for (int w = 1; w < 4; w++) sum[u] += meet[((w * N + wave) * N + u) * 64 + lane];
     }
+    const bool none = m0 + 16 * wave >= P.rows;
     if (A.splits > 1) {
+        if (none) return;
         const int64_t tile_of = (int64_t)at.tm * P.tiles_n + at.tn + P.first / A.splits;
         f4* part = (f4*)A.part + (tile_of * A.splits + at.split) * (N * 256) + threadIdx.x;
 #pragma unroll
@@ -707,6 +709,7 @@ __global__ __launch_bounds__(256, 1) void feed_small_kernel(FeedArgs A)
         return;
     }
     arrived<0>();
+    if (none) return;
     using Out = Leave<T, K, SS>;
     const Out out(P, A.act, (float*)lds + wave * (16 * Out::LD), n0);
     typename Out::In in;
@@ -714,27 +717,30 @@ __global__ __launch_bounds__(256, 1) void feed_small_kernel(FeedArgs A)
     out.template give<false>(in, sum, m0 + 16 * wave);
 }
 
-// A tile's parts of the depth, added in order.
+// A tile's parts of the depth, added in order: 16 rows of it to a wave.
 template <typename T>
-__global__ __launch_bounds__(256) void feed_join_kernel(FeedArgs A)
+__global__ __launch_bounds__(64) void feed_join_kernel(FeedArgs A)
 {
     constexpr int N = SS / 16;
     using Out = Leave<T, PLAIN, SS>;
-    __shared__ float lds[4 * 16 * Out::LD];
+    __shared__ float lds[16 * Out::LD];
+    const int item = blockIdx.x / 4, wave = blockIdx.x % 4;
     int which = 0;
-    while (which + 1 < A.count && (int)blockIdx.x >= A.p[which + 1].first / A.splits) which++;
+    while (which + 1 < A.count && item >= A.p[which + 1].first / A.splits) which++;
     const Product& P = A.p[which];
-    const int tile = blockIdx.x - P.first / A.splits, tm = tile / P.tiles_n, tn = tile % P.tiles_n, wave = threadIdx.x >> 6;
-    const f4* part = (const f4*)A.part + (int64_t)blockIdx.x * A.splits * (N * 256) + threadIdx.x;
+    const int tile = item - P.first / A.splits, row0 = tile / P.tiles_n * SS + 16 * wave;
+    if (row0 >= P.rows) return;
+    const f4* part = (const f4*)A.part + (int64_t)item * A.splits * (N * 256) + 64 * wave + threadIdx.x;
     f4 sum[N];
 #pragma unroll
     for (int u = 0; u < N; u++) sum[u] = part[u * 256];
+#pragma unroll 4
     for (int s = 1; s < A.splits; s++)
 #pragma unroll
         for (int u = 0; u < N; u++) sum[u] += part[(int64_t)(s * N + u) * 256];
-    const Out out(P, A.act, lds + wave * (16 * Out::LD), tn * SS);
+    const Out out(P, A.act, lds, tile % P.tiles_n * SS);
     typename Out::In in;
-    out.template give<false>(in, sum, tm * SS + 16 * wave);
+    out.template give<false>(in, sum, row0);
 }
 
 // Lays the products' tiles of SM x SN out one after the other; the workgroups, or -1.
@@ -789,6 +795,7 @@ int launch_small(FeedArgs& A, hipStream_t stream)
     const int64_t blocks = lay_out<K>(A, SS, SS);
     GS_REQUIRE(blocks >= 0, "feed forward: too many tiles");
     constexpr size_t LDS = (size_t)(DIRECT && sizeof(T) == 2 ? 3 : 2) * 2 * SS * SKT * sizeof(T);
+    static_assert(LDS >= 4 * SS * SS * sizeof(float), "the waves' sums meet in it");
     auto kernel = feed_small_kernel<T, K, LDOWN, RDOWN, DIRECT>;
     static std::atomic<uint64_t> told{0};
     if (int rc = allow_lds(kernel, LDS, told)) return rc;
@@ -798,7 +805,7 @@ int launch_small(FeedArgs& A, hipStream_t stream)
     if constexpr (K == PLAIN || K == SUM) {
         if (A.splits > 1) {
             GS_TIMED("feed_join_kernel", stream,
-                     hipLaunchKernelGGL(feed_join_kernel<T>, dim3((unsigned)(blocks / A.splits)), dim3(256), 0, stream, A));
+                     hipLaunchKernelGGL(feed_join_kernel<T>, dim3((unsigned)(blocks / A.splits * 4)), dim3(64), 0, stream, A));
             GS_LAUNCH_CHECK("feed_join_kernel");
         }
     }
@@ -809,11 +816,12 @@ constexpr int CUS = 256;
 
 int64_t tiles_of(int64_t m, int64_t n, int sm, int sn) { return (m + sm - 1) / sm * ((n + sn - 1) / sn); }
 
-// Parts of the depth for `tiles` small tiles: while there are fewer than CUs, and three
-// turns or more in a part, of which one takes about what adding it up does.
-int splits_of(int64_t tiles, int64_t turns)
+// Parts of the depth for `tiles` small tiles: while there are fewer than places for them,
+// and three turns or more in a part, of which one takes about what adding it up does.  A
+// CU has LDS for one workgroup of whole chunks, for two without.
+int splits_of(int64_t tiles, int64_t turns, bool direct)
 {
-    int64_t n = tiles > 0 ? CUS / tiles : 1;
+    int64_t n = tiles > 0 ? (direct ? CUS : 2 * CUS) / tiles : 1;
     if (n > turns / 3) n = turns / 3;
     return (int)(n < 1 ? 1 : n);
 }
@@ -887,29 +895,29 @@ bool whole(const void* p, int64_t ld, int n, int type)
 size_t padded(size_t n) { return (n + 255) / 256 * 256; }
 
 // Sets A's parts of the depth.
-void split(FeedArgs& A, int64_t turns, void* part)
+void split(FeedArgs& A, int64_t turns, bool direct, void* part)
 {
     int64_t tiles = 0;
     for (int i = 0; i < A.count; i++) tiles += tiles_of(A.p[i].rows, A.p[i].cols, SS, SS);
-    A.splits = splits_of(tiles, turns);
+    A.splits = splits_of(tiles, turns, direct);
     A.part = (float*)part;
 }
 
 int64_t turns_of(int64_t depth) { return (depth + SKT - 1) / SKT; }
 
-// What the parts take: no more of them than CUs, of any products of a launch.
-constexpr size_t PART_BYTES = (size_t)CUS * SS * SS * sizeof(float);
+// What the parts take: no more of them than places, of any products of a launch.
+constexpr size_t PART_BYTES = (size_t)2 * CUS * SS * SS * sizeof(float);
 
 }  // namespace
 
 extern "C" size_t gs_feed_forward_workspace_bytes(int type, int64_t rows, int width, int hidden, int out, int backward)
 {
     if (check(type, GS_SILU, rows, width, hidden, out) != GS_OK) return 0;
-    if (!backward) return splits_of(tiles_of(rows, out, SS, SS), turns_of(hidden)) > 1 ? PART_BYTES : 0;
+    if (!backward) return splits_of(tiles_of(rows, out, SS, SS), turns_of(hidden), false) > 1 ? PART_BYTES : 0;
     // the weights' gradients are split alone or together, as many as are asked for
-    const bool parts = splits_of(tiles_of(rows, width, SS, SS), 2 * turns_of(hidden)) > 1 ||
-                       splits_of(tiles_of(hidden, width, SS, SS), turns_of(rows)) > 1 ||
-                       splits_of(tiles_of(out, hidden, SS, SS), turns_of(rows)) > 1;
+    const bool parts = splits_of(tiles_of(rows, width, SS, SS), 2 * turns_of(hidden), false) > 1 ||
+                       splits_of(tiles_of(hidden, width, SS, SS), turns_of(rows), false) > 1 ||
+                       splits_of(tiles_of(out, hidden, SS, SS), turns_of(rows), false) > 1;
     return 2 * padded((size_t)rows * hidden * gs::dtype_bytes(type)) + (parts ? PART_BYTES : 256);
 }
 
@@ -954,7 +962,7 @@ extern "C" int gs_feed_forward(int type, int activation, int64_t rows, int width
     P.old = out;
     P.out[0] = y;
     direct = whole(h, hidden, hidden, type) && whole(down, hidden, hidden, type);
-    split(A, turns_of(hidden), workspace);
+    split(A, turns_of(hidden), direct, workspace);
     GS_REQUIRE(A.splits == 1 || (workspace != nullptr && (uintptr_t)workspace % 256 == 0),
                "feed forward: these sizes need the workspace, 256-byte aligned");
     return launch<PLAIN, false, false>(type, A, direct, stream);
@@ -1018,7 +1026,7 @@ extern "C" int gs_feed_forward_backward(int type, int activation, int64_t rows, 
         P.out[0] = dx;
         const bool direct = whole(da, hidden, hidden, type) && whole(gate, width, width, type) &&
                             whole(up, width, width, type);
-        split(A, 2 * turns_of(hidden), part);
+        split(A, 2 * turns_of(hidden), direct, part);
         if (int rc = launch<SUM, false, true>(type, A, direct, stream)) return rc;
     }
     // the weights' gradients, one after the other in one launch
@@ -1043,6 +1051,6 @@ extern "C" int gs_feed_forward_backward(int type, int activation, int64_t rows, 
     add(db, hidden, hidden, x, x_stride, width, dup);
     add(dy, dy_stride, out, h, hidden, hidden, ddown);
     if (A.count == 0) return GS_OK;
-    split(A, turns_of(rows), part);
+    split(A, turns_of(rows), direct, part);
     return launch<PLAIN, true, true>(type, A, direct, stream);
 }

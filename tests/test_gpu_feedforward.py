@@ -94,6 +94,15 @@ def test_strides_and_dimensions(gpu, t):
     assert torch.equal(a, c) and torch.equal(b, c)
 
 
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_rows_far_apart_and_very_many(gpu, t):
+    # rows of 4 million elements each: a tile of them spans more than a 32-bit offset is used for
+    far = torch.empty((20, (1 << 22) + 8), device="cuda", dtype=t)[:, :64]
+    far.copy_(_rand((20, 64), t, 1))
+    _check(far, _weights(64, 72, 40, t))
+    _check(_rand((70001, 24), t, 2), _weights(24, 40, 16, t))
+
+
 @pytest.mark.parametrize("t", TYPES)
 def test_which_gradients_are_asked_for(gpu, t):
     from blitzgs_amd.feedforward import feed_forward
