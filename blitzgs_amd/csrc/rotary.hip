@@ -561,7 +561,6 @@ extern "C" int gs_rotary_backward(int type, int param_type, int B, int Hq, int H
             copy3(A.side[i].dys, gs_[i]);
             copy3(A.side[i].outs, os[i]);
         }
-        if (!any) return GS_OK;
         Plan plan[2];
         const size_t lds = fill(A, plan, type, param_type, B, heads, T, D, axes, pairs, magnitude, eps, positions,
                                 wide, position_strides, frequencies, parts);
@@ -576,9 +575,10 @@ extern "C" int gs_rotary_backward(int type, int param_type, int B, int Hq, int H
             if (parts) p += (size_t)plan[i].blocks * D;
         }
         const unsigned blocks = A.side[0].blocks > A.side[1].blocks ? A.side[0].blocks : A.side[1].blocks;
-        if (norm)
+        // without rows to write a weight of no heads has its gradient, zero, to come
+        if (any && norm)
             launch<true, true>(type, A, plan[0], interleaved != 0, dim3(blocks, 2), lds, stream);
-        else
+        else if (any)
             launch<false, true>(type, A, plan[0], interleaved != 0, dim3(blocks, 2), lds, stream);
         GS_LAUNCH_CHECK("rotary_bwd_kernel");
     }

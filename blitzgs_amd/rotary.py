@@ -161,6 +161,8 @@ def _call(q, k, qw, kw, positions, frequencies, interleaved, magnitude, norm, ep
         if k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (B, T, D):
             raise RuntimeError("k must have q's type, batch, tokens and head dimension; got q "
                                f"{tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}")
+    if max(*q.shape, 0 if k is None else k.shape[1]) >= 1 << 31:
+        raise RuntimeError(f"q and k must have sizes below 2^31, got {tuple(q.shape)}")
     if (not isinstance(frequencies, torch.Tensor) or frequencies.dtype != torch.int64 or frequencies.device != q.device
             or frequencies.dim() not in (1, 2) or frequencies.numel() == 0 or 2 * frequencies.numel() > D):
         raise RuntimeError(f"frequencies must be an int64 tensor of shape (pairs,) or (axes, pairs) on {q.device}, of at "

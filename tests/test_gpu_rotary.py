@@ -165,6 +165,18 @@ def test_nothing_and_nan(gpu):
     assert torch.equal(z, torch.zeros_like(z))
 
 
+def test_a_weight_of_no_heads(gpu):
+    # its gradient is zero, also where the other side asks for none
+    from blitzgs_amd.rotary import norm_rotate
+    at, f = torch.arange(5, device="cuda"), _frequencies(4)
+    for k in (None, torch.ones((2, 3, 5, 16), device="cuda")):
+        w = torch.ones(16, device="cuda", requires_grad=True)
+        y, _ = norm_rotate(torch.ones((2, 0, 5, 16), device="cuda"), k, w, None, at, f)
+        torch.full((16,), math.nan, device="cuda")      # what a gradient that is not written may hold
+        (g,) = torch.autograd.grad(y, w, torch.ones_like(y))
+        assert torch.equal(g, torch.zeros_like(w))
+
+
 def test_gradient_against_differences(gpu):
     # f = sum(y c): central differences along a random direction in fp32 with steps of 1e-2, as for layer norm
     from blitzgs_amd.rotary import norm_rotate
@@ -246,6 +258,8 @@ def test_refusals(gpu):
         args[i] = bad
         with pytest.raises(RuntimeError, match=words):
             norm_rotate(*args)
+    with pytest.raises(RuntimeError, match="below 2\\^31"):
+        rotate(q[:, :1].expand(2, 1 << 31, 3, 16), None, at, f)
     with pytest.raises(RuntimeError, match="k_weight needs k"):
         norm_rotate(q, None, None, w, at, f)
     with pytest.raises(RuntimeError, match="one type"):
