@@ -743,9 +743,10 @@ __global__ __launch_bounds__(64) void feed_join_kernel(FeedArgs A)
     out.template give<false>(in, sum, row0);
 }
 
-// Lays the products' tiles of SM x SN out one after the other; the workgroups, or -1.
+// Lays the products' tiles of SM x SN out one after the other; the workgroups, or -1 where
+// their threads would be 2^32 or more, which no launch takes.
 template <Kind K>
-int64_t lay_out(FeedArgs& A, int sm, int sn)
+int64_t lay_out(FeedArgs& A, int sm, int sn, int threads)
 {
     int64_t blocks = 0;
     for (int i = 0; i < A.count; i++) {
@@ -755,7 +756,7 @@ int64_t lay_out(FeedArgs& A, int sm, int sn)
         P.tiles_n = (P.cols + n - 1) / n;
         P.first = (int)blocks;
         blocks += (int64_t)P.tiles_m * P.tiles_n * A.splits;
-        if (blocks > 0x7fffffff) return -1;
+        if (blocks * threads > 0xffffffffll) return -1;
     }
     return blocks;
 }
@@ -777,7 +778,7 @@ int allow_lds(F kernel, size_t bytes, std::atomic<uint64_t>& told)
 template <typename T, Kind K, bool LDOWN, bool RDOWN, int SM, int SN, int WM, int WN, int BUFFERS>
 int launch_large(FeedArgs& A, hipStream_t stream)
 {
-    const int64_t blocks = lay_out<K>(A, SM, SN);
+    const int64_t blocks = lay_out<K>(A, SM, SN, 64 * WM * WN);
     GS_REQUIRE(blocks >= 0, "feed forward: too many tiles");
     constexpr size_t LDS = (size_t)BUFFERS * (SM + SN) * 128;
     auto kernel = feed_kernel<T, K, LDOWN, RDOWN, SM, SN, WM, WN, BUFFERS>;
@@ -792,7 +793,7 @@ int launch_large(FeedArgs& A, hipStream_t stream)
 template <typename T, Kind K, bool LDOWN, bool RDOWN, bool DIRECT>
 int launch_small(FeedArgs& A, hipStream_t stream)
 {
-    const int64_t blocks = lay_out<K>(A, SS, SS);
+    const int64_t blocks = lay_out<K>(A, SS, SS, 256);
     GS_REQUIRE(blocks >= 0, "feed forward: too many tiles");
     constexpr size_t LDS = (size_t)(DIRECT && sizeof(T) == 2 ? 3 : 2) * 2 * SS * SKT * sizeof(T);
     static_assert(LDS >= 4 * SS * SS * sizeof(float), "the waves' sums meet in it");
@@ -832,7 +833,7 @@ int splits_of(int64_t tiles, int64_t turns, bool direct)
 // 1024 x 4096, with 256 x 256, 256 x 128 (three buffers), 128 x 128 and 64 x 64:
 //   HIDDEN 155, 189, 184, 478   GRAD 141, 133, 124, 296   SUM 190, 123, 157, 277
 //   y 96, 65, 74, 143           weights' gradients 188, 237, 260, 427
-template <Kind K, bool LDOWN>
+template <Kind K>
 double estimate(const FeedArgs& A, int sm, int sn, double turn, double ends)
 {
     int64_t tiles = 0;
@@ -847,10 +848,10 @@ int launch_shape(FeedArgs& A, bool direct, hipStream_t stream)
 {
     if constexpr (sizeof(T) == 2) {
         if (direct) {
-            const double large = estimate<K, LDOWN>(A, 256, 256, 1.4, K == GRAD ? 48 : K == HIDDEN ? 15 : 7),
-                         wide = estimate<K, LDOWN>(A, 256, 128, 0.98, K == GRAD ? 18 : K == HIDDEN ? 9 : 5),
-                         middle = estimate<K, LDOWN>(A, 128, 128, LDOWN ? 0.68 : 0.58, K == GRAD ? 6 : 2) + 3,
-                         small = estimate<K, LDOWN>(A, 64, 64, 0.28, 1.5) / A.splits + (A.splits > 1 ? 7 : 3);
+            const double large = estimate<K>(A, 256, 256, 1.4, K == GRAD ? 48 : K == HIDDEN ? 15 : 7),
+                         wide = estimate<K>(A, 256, 128, 0.98, K == GRAD ? 18 : K == HIDDEN ? 9 : 5),
+                         middle = estimate<K>(A, 128, 128, LDOWN ? 0.68 : 0.58, K == GRAD ? 6 : 2) + 3,
+                         small = estimate<K>(A, 64, 64, 0.28, 1.5) / A.splits + (A.splits > 1 ? 7 : 3);
             const int splits = A.splits;
             A.splits = 1;
             if (large <= wide && large <= middle && large <= small)
@@ -930,6 +931,7 @@ extern "C" int gs_feed_forward(int type, int activation, int64_t rows, int width
     GS_REQUIRE((a == nullptr) == (b == nullptr) && (rest == nullptr || a != nullptr),
                "feed forward: a and b come together, rest with them");
     if (rows == 0) return GS_OK;
+    GS_REQUIRE(x_stride >= 0, "feed forward: a stride must not be negative");
     GS_REQUIRE(x && gate && up && down && h && y, "feed forward: x, the weights, h and y must be non-null");
     FeedArgs A{};
     A.act = activation;
@@ -980,6 +982,7 @@ extern "C" int gs_feed_forward_backward(int type, int activation, int64_t rows, 
     const bool inner = dx != nullptr || dgate != nullptr || dup != nullptr;
     if (!inner && ddown == nullptr) return GS_OK;
     if (rows > 0) {
+        GS_REQUIRE(x_stride >= 0 && dy_stride >= 0, "feed forward: a stride must not be negative");
         GS_REQUIRE(x && gate && up && down && a && b && h && dy,
                    "feed forward: x, the weights, a, b, h and dy must be non-null");
         GS_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 256 == 0,
