@@ -69,7 +69,8 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
     """Step number `step` (from 1 on), in place, over lists of tensors on one device.
 
     exp_avgs, exp_avg_sqs: float32, or uint8 with a list of scales, as new_moments makes
-    them.  A tensor may not come twice.  In a captured graph every replay is the step, with
+    them.  A tensor may not come twice, nor overlap another, nor a gradient one of them
+    (gradients may be one tensor).  In a captured graph every replay is the step, with
     the rates and the seed, that was captured."""
     params, grads = list(params), list(grads)
     how = _settings(lr, betas, eps, weight_decay)
@@ -107,9 +108,6 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
                                f"{device}")
         written += [[s.data_ptr() for s in scales], [s.data_ptr() + s.stride(0) for s in scales]]
         low, high = (pointers(a) for a in written[3:])
-    addresses = [a for column in written for a, size in zip(column, sizes) if size]
-    if len(set(addresses)) != len(addresses):
-        raise RuntimeError("a tensor may not come twice in a call")
     with _t.on_device(device):
         _t.check(_t.load().gs_adamw_update(
             _t.DTYPE_CODES[first.dtype], 32 if scales is None else 8, n, (C.c_int64 * n)(*sizes), pointers(written[0]),

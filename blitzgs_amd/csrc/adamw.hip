@@ -29,6 +29,10 @@
 // of an element were 87 and are about 50); their moments' values 177 us.
 #include <math.h>
 
+#include <algorithm>
+#include <memory>
+#include <new>
+
 #include "gs_host.h"
 #include "gs_types.h"
 #include "../../include/blitzgs_amd.h"
@@ -41,6 +45,7 @@ constexpr int V = 8;                       // elements of a lane
 constexpr int CHUNK = THREADS * V;
 constexpr int BLOCK_8 = 128;               // elements that share a power of two: 16 lanes
 constexpr int TOP_M = 14, TOP_V = 30;      // exponent codes of 1
+constexpr uint64_t MAX_GROUPS = (1u << 24) - 1;   // a launch has fewer than 2^32 threads
 
 struct Tensor {
     void* p;
@@ -322,6 +327,45 @@ void launch(int bits, const AdamArgs& A, unsigned blocks, hipStream_t stream)
     else launch<T, true>(bits, A, blocks, stream);
 }
 
+struct Range {
+    uintptr_t from, to;
+};
+
+// Tensors that are written lie apart from each other and from the gradients: of an overlap
+// the step would leave what its last workgroup wrote.
+int check_apart(int type, int bits, int count, const int64_t* sizes, void* const* params, const void* const* grads,
+                void* const* exp_avgs, void* const* exp_avg_sqs, uint8_t* const* exp_avg_scales,
+                uint8_t* const* exp_avg_sq_scales)
+{
+    const int64_t of_p = gs::dtype_bytes(type), of_m = bits / 8;
+    std::unique_ptr<Range[]> all(new (std::nothrow) Range[5 * (size_t)count]);
+    GS_REQUIRE(all != nullptr, "adamw: no memory for the addresses of %d tensors", count);
+    size_t n = 0;
+    auto add = [&](const void* p, int64_t bytes) { all[n++] = Range{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes}; };
+    for (int i = 0; i < count; i++) {
+        if (sizes[i] == 0) continue;
+        add(params[i], sizes[i] * of_p);
+        add(exp_avgs[i], sizes[i] * of_m);
+        add(exp_avg_sqs[i], sizes[i] * of_m);
+        if (bits == 32) continue;
+        const int64_t blocks = (sizes[i] + BLOCK_8 - 1) / BLOCK_8;
+        add(exp_avg_scales[i], blocks);
+        add(exp_avg_sq_scales[i], blocks);
+    }
+    Range* end = all.get() + n;
+    std::sort(all.get(), end, [](const Range& a, const Range& b) { return a.from < b.from; });
+    for (size_t i = 1; i < n; i++)
+        GS_REQUIRE(all[i - 1].to <= all[i].from, "adamw: a tensor may not come twice in a call or overlap another");
+    for (int i = 0; i < count; i++) {
+        if (sizes[i] == 0) continue;
+        const uintptr_t from = (uintptr_t)grads[i], to = from + (uintptr_t)(sizes[i] * of_p);
+        // the first that ends behind the gradient's begin
+        const Range* r = std::partition_point(all.get(), end, [&](const Range& a) { return a.to <= from; });
+        GS_REQUIRE(r == end || r->from >= to, "adamw: gradient %d overlaps a tensor that is written", i);
+    }
+    return GS_OK;
+}
+
 }  // namespace
 
 extern "C" int gs_adamw_update(int type, int bits, int count, const int64_t* sizes, void* const* params,
@@ -348,6 +392,9 @@ extern "C" int gs_adamw_update(int type, int bits, int count, const int64_t* siz
         GS_REQUIRE(params[i] && grads[i] && exp_avgs[i] && exp_avg_sqs[i], "adamw: tensor %d has a null pointer", i);
         GS_REQUIRE(bits == 32 || (exp_avg_scales[i] && exp_avg_sq_scales[i]), "adamw: tensor %d has no scales", i);
     }
+    if (int rc = check_apart(type, bits, count, sizes, params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales,
+                             exp_avg_sq_scales))
+        return rc;
     AdamArgs A;
     A.b1 = (float)beta1;
     A.c1 = (float)(1.0 - beta1);
@@ -358,14 +405,16 @@ extern "C" int gs_adamw_update(int type, int bits, int count, const int64_t* siz
     A.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)settings->step)));
     A.eps = (float)settings->eps;
     const uint32_t start = scrambled((uint32_t)settings->step * PHI + settings->seed);
-    A.chunks = 1;
+    int64_t largest = 0;
+    for (int i = 0; i < count; i++) largest = std::max(largest, sizes[i]);
+    A.chunks = 1 + (int)((uint64_t)largest / (MAX_GROUPS * CHUNK));
     for (int i = 0; i < count;) {
         uint64_t blocks = 0;
         A.count = 0;
         for (; i < count && A.count < MAX_TENSORS; i++) {
             if (sizes[i] == 0) continue;
             const uint64_t n = ((uint64_t)sizes[i] + (uint64_t)A.chunks * CHUNK - 1) / ((uint64_t)A.chunks * CHUNK);
-            if (A.count > 0 && blocks + n > 0x7fffffffu) break;
+            if (A.count > 0 && blocks + n > MAX_GROUPS) break;
             Tensor& t = A.t[A.count++];
             t.p = params[i];
             t.g = grads[i];

@@ -791,21 +791,23 @@ int gs_momentum_apply(int type, int count, int64_t size, void* const* params, fl
                       const float* update, gs_stream_t stream);
 
 /* One AdamW step, number `step` (from 1 on) of host-side `settings`, over `count`
- * tensors; the arrays are host arrays, of sizes in elements and of device pointers to contiguous tensors:
+ * tensors; the arrays are host arrays, of sizes in elements and of device pointers to
+ * contiguous tensors:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr weight_decay)
  *       - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
  * params and grads are of `type`, the moments of 32 bits (float32) or 8.  With 8
  * the elements of a tensor share in blocks of 128 a power of two 2^(scale - 127),
  * one byte each in exp_avg_scales and exp_avg_sq_scales (NULL with 32 bits), that of
- * the block's largest (scale 0: 2^-127 or less); a first moment's byte is a sign, four bits of exponent (1 is
- * 14) and three of mantissa, a second one's five (1 is 30) and three, both with
- * subnormals, and all ones (the sign apart) is NaN.  Bytes and scales of zero are a
+ * the block's largest (scale 0: 2^-127 or less); a first moment's byte is a sign, four
+ * bits of exponent (1 is 14) and three of mantissa, a second one's five (1 is 30) and
+ * three, both with subnormals, and all ones (the sign apart) is NaN.  Bytes and scales of zero are a
  * moment of zero.  They are rounded up with the probability of what is left, by
  * 16 bits each of s(s(i phi + s(step phi + seed)) + element phi), modulo 2^32,
  * where i is the tensor's place in the arrays, phi = 0x9E3779B9 and
  *   s(x): x ^= x >> 16; x *= 0x6A09E667; x ^= x >> 15; x *= 0xBB67AE85; x ^= x >> 16.
- * Tensors may not overlap.
+ * Tensors that are written may overlap neither each other nor a gradient; gradients may
+ * be one tensor.
  *   gs_adamw_values: the values of 8-bit moments, GS_F32 or GS_BF16. */
 typedef struct gs_adamw_settings {
     double lr;

@@ -74,6 +74,9 @@ def test_feed_forward(lib):
     _refused(lib, fwd(rest=NZ), b"together")
     _refused(lib, fwd(x=None), b"non-null")
     _refused(lib, fwd(h=None), b"non-null")
+    # tiles whose threads are more than a launch takes
+    _refused(lib, fwd(rows=2 ** 31 - 2 ** 17, type=F32), b"too many tiles")
+    _refused(lib, lib.gs_feed_forward(BF16, 0, 4, 8, 16, 8, NZ, -8, NZ, NZ, NZ, None, None, None, NZ, NZ, NZ, None), b"stride")
     assert fwd(rows=0) == 0
 
     def bwd(x=NZ, dx=NZ, dd=NZ, ws=NZ, rows=4):
@@ -111,6 +114,20 @@ def test_adamw(lib):
                        (dict(decay=-1.0), b"lr")):
         _refused(lib, call(how=_settings(**bad)), words)
     assert call(count=0) == 0 and call(size=0, params=none) == 0
+    # tensors of 4 floats (or codes, with a scale each) that lie on each other, or a gradient on one of them
+    def two(bits=32, **moved):
+        at = dict(p=(0, 16), g=(0x100, 0x100), m=(0x200, 0x210), v=(0x300, 0x310), ms=(0x400, 0x401), vs=(0x500, 0x501))
+        at = {k: (C.c_void_p * 2)(*(0x10000 + a for a in moved.get(k, places))) for k, places in at.items()}
+        scales = (at["ms"], at["vs"]) if bits == 8 else (None, None)
+        return lib.gs_adamw_update(F32, bits, 2, (C.c_int64 * 2)(4, 4), at["p"], at["g"], at["m"], at["v"], *scales,
+                                   _settings(), None)
+    for bits, moved in ((32, dict(p=(0, 0))), (32, dict(p=(0, 12))), (32, dict(m=(0x200, 0x1f8))), (32, dict(v=(0x20c, 0x310))),
+                        (8, dict(m=(0x200, 0x203))), (8, dict(ms=(0x400, 0x400))), (8, dict(vs=(0x202, 0x500)))):
+        _refused(lib, two(bits, **moved), b"twice in a call or overlap")
+    for bits, moved in ((32, dict(g=(0, 0x100))), (32, dict(g=(0x100, 0x1f4))), (32, dict(g=(0x21c, 0x100))),
+                        (8, dict(g=(0x100, 0x3f4))), (8, dict(g=(0x1f0, 0x1f1)))):
+        rc = two(bits, **moved)
+        _refused(lib, rc, b"overlaps")
     values = lambda type=F32, n=4, m=NZ: lib.gs_adamw_values(type, n, m, NZ, NZ, NZ, NZ, NZ, None)  # noqa: E731
     _refused(lib, values(type=F16), b"float32 or bfloat16")
     _refused(lib, values(n=-1), b"size")

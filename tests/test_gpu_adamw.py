@@ -275,6 +275,7 @@ def test_refusals(gpu):
             ((p, g, m, v, 1, 0.1), dict(scales=s8), "exp_avgs"), ((p, g, m8, v8, 1, 0.1), dict(scales=s8[:1]), "scales"),
             ((p, g, m8, v8, 1, 0.1), dict(scales=[s8[0][:, :0], s8[1]]), "scales"),
             (([p[0], p[0]], [g[0], g[0]], [m[0], m[0]], [v[0], v[0]], 1, 0.1), {}, "twice"),
+            (([p[0], p[0].view(-1)[7:]], [g[0], g[1]], m, v, 1, 0.1), {}, "overlap"), ((p, [p[0], g[1]], m, v, 1, 0.1), {}, "overlaps"),
             (([p[0].t(), p[1]], g, m, v, 1, 0.1), {}, "params"), (([p[0].cpu(), p[1]], g, m, v, 1, 0.1), {}, "HIP device"),
             ((p, g, [m[0].t(), m[1]], v, 1, 0.1), {}, "exp_avgs"), ((p, g, m, v, 1, 0.1), dict(seed=1.5), "seed")]:
         with pytest.raises(RuntimeError, match=words):
