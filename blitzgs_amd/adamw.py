@@ -47,7 +47,7 @@ def _checked(ts, name, dtype, shapes, device):
     index = device.index
     try:
         fit = (all([t.dtype is dtype for t in ts]) and all([t.get_device() == index for t in ts])
-               and [t.shape for t in ts] == shapes and all([t.is_contiguous() for t in ts]))
+               and all([t.is_contiguous() for t in ts]) and [t.shape for t in ts] == shapes)
     except AttributeError:        # no tensor
         fit = False
     if not fit:
@@ -99,14 +99,15 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
         if len(scales) != n:
             raise RuntimeError(f"scales must hold a tensor for each of {n} parameters, got {len(scales)}")
         blocks = [-(-size // BLOCK) for size in sizes]
-        if not (all([isinstance(s, torch.Tensor) and s.dtype is torch.uint8 for s in scales])
-                and all([s.get_device() == device.index for s in scales])
-                and [s.shape for s in scales] == [(2, b) for b in blocks]
-                and all([s.is_contiguous() or s.stride() >= (b, 1) and s.stride(1) == 1
-                         for s, b in zip(scales, blocks)])):
+        fit = (all([isinstance(s, torch.Tensor) and s.dtype is torch.uint8 for s in scales])
+               and all([s.get_device() == device.index for s in scales])
+               and [s.shape for s in scales] == [(2, b) for b in blocks])
+        strides = [s.stride() for s in scales] if fit else []
+        if not (fit and all([row >= b and (one == 1 or b < 2) for b, (row, one) in zip(blocks, strides)])):
             raise RuntimeError(f"scales must hold uint8 tensors of shape (2, ceil(n / {BLOCK})) with contiguous rows on "
                                f"{device}")
-        written += [[s.data_ptr() for s in scales], [s.data_ptr() + s.stride(0) for s in scales]]
+        first_rows = [s.data_ptr() for s in scales]
+        written += [first_rows, [a + row for a, (row, _) in zip(first_rows, strides)]]
         low, high = (pointers(a) for a in written[3:])
     with _t.on_device(device):
         _t.check(_t.load().gs_adamw_update(

@@ -34,30 +34,45 @@ def _rows(t, width):
     return t, apart if n > 1 else width
 
 
+def _padded(nbytes):
+    return -(-nbytes // 256) * 256
+
+
 def _forward(x, gate, up, down, activation, grads):
-    """y and, for a backward, a, b, their rests, h and what it is called with."""
+    """y, what the library is called with, and for a backward h, a, b and their rests, one after the other in bytes."""
     (hidden, width), out = gate.shape, down.shape[0]
-    n = x.numel() // width
+    n, dtype, device = x.numel() // width, x.dtype, x.device
     rows, apart = _rows(x, width)
-    sizes = _t.DTYPE_CODES[x.dtype], activation, n, width, hidden, out
-    lib, new = _t.load(), lambda *shape: torch.empty(shape, device=x.device, dtype=x.dtype)
-    y, h = new(*x.shape[:-1], out), new(n, hidden)
-    a, b = (new(n, hidden), new(n, hidden)) if grads else (None, None)
-    rest = torch.empty((n, hidden), device=x.device, dtype=torch.uint8) if grads and x.dtype != torch.float32 else None
-    ws = _t.workspace(lib.gs_feed_forward_workspace_bytes(sizes[0], *sizes[2:], 0), x.device)
-    with _t.on_device(x.device):
-        _t.check(lib.gs_feed_forward(*sizes, rows.data_ptr(), apart, gate.data_ptr(), up.data_ptr(), down.data_ptr(),
-                                     _t.ptr(a), _t.ptr(b), _t.ptr(rest), h.data_ptr(), y.data_ptr(), _t.ptr(ws),
-                                     _t.stream(x.device)), "gs_feed_forward")
-    return y, a, b, rest, h, sizes
+    code = _t.DTYPE_CODES[dtype]
+    sizes = code, activation, n, width, hidden, out
+    lib = _t.load()
+    y = torch.empty(x.shape[:-1] + (out,), device=device, dtype=dtype)
+    part, each = lib.gs_feed_forward_workspace_bytes(code, n, width, hidden, out, 0), _padded(n * hidden * x.element_size())
+    if grads:
+        kept = torch.empty(3 * each + (n * hidden if code else 0), device=device, dtype=torch.uint8)
+        ws = _t.workspace(part, device)
+        h, wsp = kept.data_ptr(), _t.ptr(ws)
+        a, b, rest = _places(h, each, code)
+    else:
+        kept = torch.empty(part + each, device=device, dtype=torch.uint8)
+        wsp = kept.data_ptr()
+        a, b, rest, h = None, None, None, wsp + part
+    with _t.on_device(device):
+        _t.check(lib.gs_feed_forward(*sizes, rows.data_ptr(), apart, gate.data_ptr(), up.data_ptr(), down.data_ptr(), a, b,
+                                     rest, h, y.data_ptr(), wsp, _t.stream(device)), "gs_feed_forward")
+    return y, sizes, kept
+
+
+def _places(h, each, code):
+    """a, b and, of the 16-bit types, their rests behind h."""
+    return h + each, h + 2 * each, h + 3 * each if code else None
 
 
 class _FeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, up, down, activation):
-        y, a, b, rest, h, ctx.how = _forward(x.detach(), gate, up, down, activation, True)
-        ctx.save_for_backward(x, gate, up, down, a, b, rest, h)
-        ctx.ws_bytes = _t.load().gs_feed_forward_workspace_bytes(ctx.how[0], *ctx.how[2:], 1)
+        y, ctx.how, kept = _forward(x, gate, up, down, activation, True)
+        ctx.save_for_backward(x, gate, up, down, kept)
         return y
 
     # The autograd engine calls this from a thread of its own, on the forward's
@@ -67,19 +82,22 @@ class _FeedForward(torch.autograd.Function):
     def backward(ctx, dy):
         # hooks on saved tensors give them back with the same values, not in the same places
         x, *saved = ctx.saved_tensors
-        gate, up, down, a, b, rest, h = (t if t is None else t.contiguous() for t in saved)
-        _, _, n, width, hidden, out = ctx.how
+        gate, up, down, kept = (t.contiguous() for t in saved)
+        code, _, n, width, hidden, out = ctx.how
+        device, dtype, lib = x.device, x.dtype, _t.load()
         rows, apart = _rows(x, width)
         drows, dapart = _rows(dy, out)
-        new = lambda i, like: (torch.empty(like.shape, device=x.device, dtype=x.dtype)  # noqa: E731
-                               if ctx.needs_input_grad[i] else None)
-        dx, dgate, dup, ddown = new(0, x), new(1, gate), new(2, up), new(3, down)
-        ws = _t.workspace(ctx.ws_bytes, x.device)
-        _t.check(_t.load().gs_feed_forward_backward(
-            *ctx.how, rows.data_ptr(), apart, gate.data_ptr(), up.data_ptr(), down.data_ptr(), a.data_ptr(), b.data_ptr(),
-            _t.ptr(rest), h.data_ptr(), drows.data_ptr(), dapart, _t.ptr(dx), _t.ptr(dgate), _t.ptr(dup), _t.ptr(ddown), _t.ptr(ws),
-            _t.stream(x.device)), "gs_feed_forward_backward")
-        return dx, dgate, dup, ddown, None
+        if kept.data_ptr() % 256:
+            kept = kept.clone()
+        h = kept.data_ptr()
+        a, b, rest = _places(h, _padded(n * hidden * x.element_size()), code)
+        grads = [torch.empty(t.shape, device=device, dtype=dtype) if need else None
+                 for need, t in zip(ctx.needs_input_grad, (x, gate, up, down))]
+        ws = _t.workspace(lib.gs_feed_forward_workspace_bytes(code, n, width, hidden, out, 1), device)
+        _t.check(lib.gs_feed_forward_backward(
+            *ctx.how, rows.data_ptr(), apart, gate.data_ptr(), up.data_ptr(), down.data_ptr(), a, b, rest, h,
+            drows.data_ptr(), dapart, *map(_t.ptr, grads), _t.ptr(ws), _t.stream(device)), "gs_feed_forward_backward")
+        return *grads, None
 
 
 def feed_forward(x, gate, up, down, activation="silu"):

@@ -32,7 +32,7 @@ from . import _tensors as _t
 
 MAX_HEAD_DIM = 256
 
-_Strides = C.c_int64 * 3
+_Strides = C.c_int64 * 4         # of which the library reads three
 
 
 def as_turns(radians, device=None):
@@ -72,58 +72,75 @@ def rotary_frequencies(pairs, base=10000.0, factor=1.0, trained=None, ramp=(1.0,
     return turns if axes == 1 else turns.expand(axes, pairs).contiguous()
 
 
-def _last_contiguous(t):
-    return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+def _rows(t):
+    """t with its last dimension contiguous, its address and its strides; None of them for no tensor."""
+    if t is None:
+        return None, None, None
+    strides = t.stride()
+    if strides[3] != 1 and t.shape[3] > 1:
+        t = t.contiguous()
+        strides = t.stride()
+    return t, t.data_ptr(), _Strides(*strides)
 
 
-def _strides(t):
-    return None if t is None else _Strides(*t.stride()[:3])
+class _Out:
+    """A result's layout: in memory (B, T, H, D)."""
 
+    def __init__(self, like):
+        B, H, T, D = like.shape
+        self.shape, self.strides = (B, H, T, D), (T * H * D, D, H * D, 1)
+        self.dtype, self.steps = like.dtype, _Strides(*self.strides)
 
-def _token_major(like):
-    B, H, T, D = like.shape
-    return torch.empty_strided((B, H, T, D), (T * H * D, D, H * D, 1), device=like.device, dtype=like.dtype)
+    def empty(self, device):
+        return torch.empty_strided(self.shape, self.strides, device=device, dtype=self.dtype)
 
 
 class _How:
     """What a call passes to the library beside its tensors."""
 
     def __init__(self, q, k, weight, frequencies, interleaved, magnitude, norm, eps):
-        B, Hq, T, D = q.shape
+        self.q, self.k = _Out(q), None if k is None else _Out(k)
+        B, Hq, T, D = self.q.shape
         code = _t.DTYPE_CODES[q.dtype]
         axes, pairs = (1, frequencies.shape[0]) if frequencies.dim() == 1 else frequencies.shape
-        self.sizes = code, B, Hq, 0 if k is None else k.shape[1], T, D, axes, pairs
+        self.sizes = code, B, Hq, 0 if k is None else self.k.shape[1], T, D, axes, pairs
         self.params = q.dtype if weight is None else weight.dtype
+        self.norm = norm
         self.first = code, _t.DTYPE_CODES[self.params], *self.sizes[1:], interleaved, magnitude, norm, eps
 
     def angles(self, positions, frequencies):
-        B, T, axes = self.sizes[1], self.sizes[4], self.sizes[6]
-        strides = list(positions.stride())
+        strides = positions.stride()
         if frequencies.dim() == 1:
-            strides.append(0)
+            strides += (0,)
         if len(strides) == 2:
-            strides.insert(0, 0)
-        return positions.data_ptr(), int(positions.dtype == torch.int64), _Strides(*strides), frequencies.data_ptr()
+            strides = (0, *strides)
+        return (positions.data_ptr(), 1 if positions.dtype is torch.int64 else 0, _Strides(*strides),
+                frequencies.data_ptr())
 
 
 def _forward(q, k, qw, kw, positions, frequencies, how):
-    qy, ky = _token_major(q), None if k is None else _token_major(k)
-    with _t.on_device(q.device):
+    """The results, and the rows as they were read."""
+    device = q.device
+    q, qp, qs = _rows(q)
+    k, kp, ks = _rows(k)
+    qy = how.q.empty(device)
+    ky, kyp, kys = (None, None, None) if k is None else ((ky := how.k.empty(device)), ky.data_ptr(), how.k.steps)
+    with _t.on_device(device):
         _t.check(_t.load().gs_rotary_forward(
-            *how.first, q.data_ptr(), _strides(q), _t.ptr(k), _strides(k), _t.ptr(qw), _t.ptr(kw),
-            *how.angles(positions, frequencies), qy.data_ptr(), _strides(qy), _t.ptr(ky), _strides(ky),
-            _t.stream(q.device)), "gs_rotary_forward")
-    return qy, ky
+            *how.first, qp, qs, kp, ks, _t.ptr(qw), _t.ptr(kw), *how.angles(positions, frequencies), qy.data_ptr(),
+            how.q.steps, kyp, kys, _t.stream(device)), "gs_rotary_forward")
+    return qy, ky, q, k
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, positions, frequencies, how):
-        q, k = _last_contiguous(q.detach()), None if k is None else _last_contiguous(k.detach())
-        ctx.how, ctx.like = how, (q.shape, None if k is None else k.shape, q.dtype)
-        norm = how.first[-2]
-        ctx.save_for_backward(*((q, k) if norm else (None, None)), qw, kw, positions, frequencies)
-        return _forward(q, k, qw, kw, positions, frequencies, how)
+        qy, ky, q, k = _forward(q, k, qw, kw, positions, frequencies, how)
+        ctx.how = how
+        if not how.norm:
+            q = k = None
+        ctx.save_for_backward(q, k, qw, kw, positions, frequencies)
+        return qy, ky
 
     # The autograd engine calls this from a thread of its own, on the forward's
     # device and stream.
@@ -132,22 +149,39 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, dqy, dky):
         # hooks on saved tensors give them back with the same values, not in the same places
         q, k, qw, kw, positions, frequencies = ctx.saved_tensors
-        q, k, dqy, dky = (_last_contiguous(t) for t in (q, k, dqy, dky))
-        qw, kw, frequencies = (t if t is None else t.contiguous() for t in (qw, kw, frequencies))
-        how, need = ctx.how, ctx.needs_input_grad
-        device, norm = frequencies.device, how.first[-2]
-        dq = _token_major(dqy) if need[0] or need[2] else None
-        dk = _token_major(dky) if dky is not None and (need[1] or need[3]) else None
-        dqw = torch.empty(qw.shape, device=device, dtype=how.params) if need[2] else None
-        dkw = torch.empty(kw.shape, device=device, dtype=how.params) if need[3] and dk is not None else None
-        lib = _t.load()
-        ws = _t.workspace(lib.gs_rotary_workspace_bytes(*how.sizes), device) if norm and (need[2] or need[3]) else None
+        how, (need_q, need_k, need_qw, need_kw, *_) = ctx.how, ctx.needs_input_grad
+        frequencies = frequencies.contiguous()
+        device, lib = frequencies.device, _t.load()
+        q, qp, qs = _rows(q)
+        k, kp, ks = _rows(k)
+        dqy, dqyp, dqys = _rows(dqy)
+        dky, dkyp, dkys = _rows(dky)
+        dq = dk = dqw = dkw = ws = dqp = dkp = dks = qwp = kwp = dqwp = dkwp = None
+        if need_q or need_qw:
+            dq = how.q.empty(device)
+            dqp = dq.data_ptr()
+        if dky is not None and (need_k or need_kw):
+            dk = how.k.empty(device)
+            dkp, dks = dk.data_ptr(), how.k.steps
+        if how.norm:
+            if qw is not None:
+                qw = qw.contiguous()
+                qwp = qw.data_ptr()
+            if kw is not None:
+                kw = kw.contiguous()
+                kwp = kw.data_ptr()
+            if need_qw:
+                dqw = torch.empty(qw.shape, device=device, dtype=how.params)
+                dqwp = dqw.data_ptr()
+            if need_kw and dk is not None:
+                dkw = torch.empty(kw.shape, device=device, dtype=how.params)
+                dkwp = dkw.data_ptr()
+            if need_qw or need_kw:
+                ws = _t.workspace(lib.gs_rotary_workspace_bytes(*how.sizes), device)
         _t.check(lib.gs_rotary_backward(
-            *how.first, _t.ptr(q), _strides(q), _t.ptr(k), _strides(k), _t.ptr(qw), _t.ptr(kw),
-            *how.angles(positions, frequencies), dqy.data_ptr(), _strides(dqy), _t.ptr(dky), _strides(dky),
-            _t.ptr(dq), _strides(dq), _t.ptr(dk), _strides(dk), _t.ptr(dqw), _t.ptr(dkw), _t.ptr(ws),
-            _t.stream(device)), "gs_rotary_backward")
-        return dq if need[0] else None, dk if need[1] else None, dqw, dkw, None, None, None
+            *how.first, qp, qs, kp, ks, qwp, kwp, *how.angles(positions, frequencies), dqyp, dqys, dkyp, dkys,
+            dqp, how.q.steps, dkp, dks, dqwp, dkwp, _t.ptr(ws), _t.stream(device)), "gs_rotary_backward")
+        return dq if need_q else None, dk if need_k else None, dqw, dkw, None, None, None
 
 
 def _call(q, k, qw, kw, positions, frequencies, interleaved, magnitude, norm, eps):
@@ -155,13 +189,13 @@ def _call(q, k, qw, kw, positions, frequencies, interleaved, magnitude, norm, ep
     if q.dim() != 4 or not 1 <= q.shape[3] <= MAX_HEAD_DIM:
         raise RuntimeError(f"q must have dimensions (B, H, T, D) with D of 1 to {MAX_HEAD_DIM}, got shape "
                            f"{tuple(q.shape)}")
-    B, _, T, D = q.shape
+    B, H, T, D = q.shape
     if k is not None:
         _t.require_tensor(k, "k", device=q.device)
         if k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (B, T, D):
             raise RuntimeError("k must have q's type, batch, tokens and head dimension; got q "
                                f"{tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}")
-    if max(*q.shape, 0 if k is None else k.shape[1]) >= 1 << 31:
+    if (B | H | T | (0 if k is None else k.shape[1])) >= 1 << 31:
         raise RuntimeError(f"q and k must have sizes below 2^31, got {tuple(q.shape)}")
     if (not isinstance(frequencies, torch.Tensor) or frequencies.dtype != torch.int64 or frequencies.device != q.device
             or frequencies.dim() not in (1, 2) or frequencies.numel() == 0 or 2 * frequencies.numel() > D):
@@ -191,7 +225,7 @@ def _call(q, k, qw, kw, positions, frequencies, interleaved, magnitude, norm, ep
     how = _How(q, k, kw if qw is None else qw, frequencies, int(bool(interleaved)), float(magnitude), norm, float(eps))
     if _t.wants_grad(q, k, qw, kw):
         return _Rotary.apply(q, k, qw, kw, positions, frequencies, how)
-    return _forward(_last_contiguous(q), _last_contiguous(k), qw, kw, positions, frequencies, how)
+    return _forward(q, k, qw, kw, positions, frequencies, how)[:2]
 
 
 def rotate(q, k, positions, frequencies, interleaved=False, magnitude=1.0):

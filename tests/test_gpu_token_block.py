@@ -235,8 +235,13 @@ def _spread(t):
     return torch.empty((*t.shape, 2), device=t.device, dtype=t.dtype)[..., 0].copy_(t)
 
 
+def _off(t):
+    # bytes from an odd address on
+    return torch.empty(t.numel() + 1, device=t.device, dtype=t.dtype)[1:].copy_(t) if t.dtype == torch.uint8 else t
+
+
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("kind", ["cpu", "packed", "turned", "spread"])
+@pytest.mark.parametrize("kind", ["cpu", "packed", "turned", "spread", "off"])
 def test_saved_tensors_in_other_places(gpu, kind, t):
     from blitzgs_amd.feedforward import feed_forward
     from blitzgs_amd.rotary import norm_rotate, rotary_frequencies
@@ -257,7 +262,7 @@ def test_saved_tensors_in_other_places(gpu, kind, t):
 
     want = grads()
     through = torch.autograd.graph.save_on_cpu() if kind == "cpu" else torch.autograd.graph.saved_tensors_hooks(
-        dict(packed=_packed, turned=_turned, spread=_spread)[kind], lambda t: t)
+        dict(packed=_packed, turned=_turned, spread=_spread, off=_off)[kind], lambda t: t)
     with through:
         got = grads()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
