@@ -743,6 +743,81 @@ __global__ __launch_bounds__(64) void feed_join_kernel(FeedArgs A)
     out.template give<false>(in, sum, row0);
 }
 
+// HIDDEN or PLAIN of C rows or fewer, whole chunks: C columns of the result to a workgroup,
+// operands straight to registers.  A matrix instruction takes 16 / C pieces of the depth at
+// once, one to each C of its rows and columns; what it makes of one piece's rows and
+// another's columns is left.  Eight waves take steps of the depth in turn, and their sums
+// meet in LDS, in order.
+template <typename T, Kind K, int C>
+__global__ __launch_bounds__(512) void feed_few_kernel(FeedArgs A)
+{
+    constexpr int WAVES = 8, AHEAD = sizeof(T) == 2 ? 8 : 4, STEP = 32 * (16 / C), N = K == HIDDEN ? 2 : 1;
+    __shared__ f4 meet[N][WAVES][64];
+    const Product& P = A.p[0];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * C, depth = P.depth, rows = P.rows, cols = P.cols;
+    // beyond the last row or column the last one comes again
+    const T* l = (const T*)P.l[0] + min(i % C, rows - 1) * P.lld;
+    const T* r[N];
+    f4 acc[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        r[n] = (const T*)P.r[n] + min(n0 + i % C, cols - 1) * P.rld;
+        acc[n] = f4{0, 0, 0, 0};
+    }
+    for (int first = wave * STEP; first < depth; first += WAVES * AHEAD * STEP) {
+        Raw<T, 8> lv[AHEAD], rv[AHEAD][N];
+        bool there[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int k = first + a * WAVES * STEP + i / C * 32 + 8 * g;
+            there[a] = k < depth;
+            const int at = there[a] ? k : 0;
+#pragma unroll
+            for (int n = 0; n < N; n++) __builtin_memcpy(&rv[a][n], r[n] + at, sizeof(rv[a][n]));
+            __builtin_memcpy(&lv[a], l + at, sizeof(lv[a]));
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            if (!there[a]) lv[a] = Raw<T, 8>{};
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                if (!there[a]) rv[a][n] = Raw<T, 8>{};
+                acc[n] = gs::mma(__builtin_bit_cast(Frag<T>, rv[a][n]), __builtin_bit_cast(Frag<T>, lv[a]), acc[n]);
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++) meet[n][wave][lane] = acc[n];
+    __syncthreads();
+    if (threadIdx.x >= C * C) return;
+    const int row = threadIdx.x / C, col = threadIdx.x % C;
+    if (row >= rows || n0 + col >= cols) return;
+    float sum[N] = {};
+#pragma unroll
+    for (int w = 0; w < WAVES; w++)
+#pragma unroll
+        for (int piece = 0; piece < 16 / C; piece++) {
+            const int j = piece * C + col;
+#pragma unroll
+            for (int n = 0; n < N; n++) sum[n] += meet[n][w][j / 4 * 16 + piece * C + row][j % 4];
+        }
+    const int64_t at = row * P.old + n0 + col;
+    if constexpr (K == HIDDEN) {
+        float value, slope;
+        activation<T>(A.act, sum[0], value, slope);
+        ((T*)P.out[0])[at] = (T)(value * sum[1]);
+        if (P.out[1] != nullptr) {
+            ((T*)P.out[1])[at] = (T)sum[0];
+            ((T*)P.out[2])[at] = (T)sum[1];
+            if constexpr (sizeof(T) == 2)
+                if (P.rest != nullptr) P.rest[at] = (uint8_t)(rest_of<T>(sum[0]) | rest_of<T>(sum[1]) << 4);
+        }
+    } else {
+        ((T*)P.out[0])[at] = (T)sum[0];
+    }
+}
+
 // Lays the products' tiles of SM x SN out one after the other; the workgroups, or -1 where
 // their threads would be 2^32 or more, which no launch takes.
 template <Kind K>
@@ -813,6 +888,16 @@ int launch_small(FeedArgs& A, hipStream_t stream)
     return GS_OK;
 }
 
+template <typename T, Kind K, int C>
+int launch_few(const FeedArgs& A, hipStream_t stream)
+{
+    GS_TIMED("feed_few_kernel", stream,
+             hipLaunchKernelGGL((feed_few_kernel<T, K, C>), dim3(gs_div_up((size_t)A.p[0].cols, C)), dim3(512), 0, stream,
+                                A));
+    GS_LAUNCH_CHECK("feed_few_kernel");
+    return GS_OK;
+}
+
 constexpr int CUS = 256;
 
 int64_t tiles_of(int64_t m, int64_t n, int sm, int sn) { return (m + sm - 1) / sm * ((n + sn - 1) / sn); }
@@ -843,9 +928,35 @@ double estimate(const FeedArgs& A, int sm, int sn, double turn, double ends)
     return (double)((tiles + CUS - 1) / CUS) * (turn * turns + ends);
 }
 
+// Columns of a workgroup of feed_few_kernel, or 0 where the tiles of 64 are as fast.  The
+// widest that leave every CU rows of weights to read, as many as there are rows of the
+// result at least.  Both products of rows x width x hidden x out, us with tiles and so:
+//   bfloat16  1 x 2048 x 8192 x 2048   26.0, 20.9    8 rows  26.2, 22.9    16 rows  26.3, 29.2
+//             1 x 4096 x 1024 x 16384  26.1, 14.3 with tiles for the second product still; 28.8 for
+//             the first still
+//   float32   1 x 2048 x 8192 x 2048   73.6, 37.6    16 rows 73.1, 55.6
+//   8 x 64 x 16384 x 64, whose second product would have 8 workgroups: bfloat16 18.7, 21.9
+template <Kind K>
+int few_columns(const Product& P, bool half)
+{
+    if (P.rows > (half ? 8 : 16)) return 0;
+    if (half && K == PLAIN && P.cols >= SS * CUS) return 0;
+    const int64_t matrix_rows = (int64_t)(K == HIDDEN ? 2 : 1) * P.cols;
+    int c = 16;
+    while (c > 4 && c / 2 >= P.rows && matrix_rows < (int64_t)c * CUS) c /= 2;
+    return matrix_rows >= 16 * c ? c : 0;
+}
+
 template <typename T, Kind K, bool LDOWN, bool RDOWN>
 int launch_shape(FeedArgs& A, bool direct, hipStream_t stream)
 {
+    if constexpr (!LDOWN && !RDOWN) {
+        switch (direct ? few_columns<K>(A.p[0], sizeof(T) == 2) : 0) {
+        case 4: return launch_few<T, K, 4>(A, stream);
+        case 8: return launch_few<T, K, 8>(A, stream);
+        case 16: return launch_few<T, K, 16>(A, stream);
+        }
+    }
     if constexpr (sizeof(T) == 2) {
         if (direct) {
             const double large = estimate<K>(A, 256, 256, 1.4, K == GRAD ? 48 : K == HIDDEN ? 15 : 7),

@@ -63,6 +63,15 @@ def test_few_rows_of_wide_blocks(gpu, t, M, W, H, O):
     _check(_rand((M, W), t, M), _weights(W, H, O, t))
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("M", [1, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("W,H,O", [(8, 256, 64), (264, 1000, 520), (2064, 2056, 72), (72, 4104, 2056), (4200, 40, 4104)])
+def test_few_rows_and_columns_of_a_workgroup(gpu, t, activation, M, W, H, O):
+    # 4, 8 and 16 columns to a workgroup, ends inside them and inside a step of the depth
+    _check(_rand((M, W), t, M), _weights(W, H, O, t), activation)
+
+
 @pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M,W,H,O", [(2100, 320, 768, 320), (5000, 64, 64, 64), (600, 1024, 1000, 1032)])
 def test_many_rows(gpu, t, M, W, H, O):
@@ -139,6 +148,20 @@ def test_the_ends_of_the_activations(gpu, activation):
     want = feed_forward_64(x[None], eye, eye, eye, activation, torch.ones((1, 12)))
     within(y, *want["y"], "y")
     within(g, *want["dx"], "dx")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M", [3, 8, 13])
+def test_nan_stays_in_its_row_of_few(gpu, t, M):
+    from blitzgs_amd.feedforward import feed_forward
+    x, weights = _rand((M, 200), t, 1), _weights(200, 520, 264, t)
+    clean = feed_forward(x, *weights)
+    for bad in (math.nan, math.inf):
+        y = x.clone()
+        y[1, 0] = y[1, 199] = bad
+        got = feed_forward(y, *weights)
+        others = [i for i in range(M) if i != 1]
+        assert got[1].isnan().any() and torch.equal(got[others], clean[others])
 
 
 def test_nan_stays_in_its_row(gpu):
