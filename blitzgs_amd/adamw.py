@@ -19,6 +19,7 @@ infinite or NaN is NaN in 8 bits.
 """
 import ctypes as C
 import math
+import operator
 
 import torch
 
@@ -39,18 +40,26 @@ def new_moments(param, bits=32):
             zeros(2, -(-param.numel() // BLOCK), dtype=torch.uint8))
 
 
+# over whole lists, without a line of Python for each tensor: a call over many is bound by these
+_SHAPE, _DTYPE, _LAYOUT = (operator.attrgetter(name) for name in ("shape", "dtype", "layout"))
+_CONTIGUOUS, _DEVICE, _NUMEL = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.numel
+_ADDRESS, _STRIDE = torch.Tensor.data_ptr, torch.Tensor.stride
+
+
+def _are(ts, dtype, shapes, device):
+    """Whether ts are tensors of a type, shapes and a device."""
+    try:
+        return (set(map(_DTYPE, ts)) == {dtype} and set(map(_DEVICE, ts)) == {device.index}
+                and list(map(_SHAPE, ts)) == shapes)
+    except (AttributeError, TypeError):        # no tensor
+        return False
+
+
 def _checked(ts, name, dtype, shapes, device):
     """Contiguous tensors of a type and of the parameters' shapes."""
     if len(ts) != len(shapes):
         raise RuntimeError(f"{name} must hold a tensor for each of {len(shapes)} parameters, got {len(ts)}")
-    # attribute by attribute: a call over many tensors is bound by this otherwise
-    index = device.index
-    try:
-        fit = (all([t.dtype is dtype for t in ts]) and all([t.get_device() == index for t in ts])
-               and all([t.is_contiguous() for t in ts]) and [t.shape for t in ts] == shapes)
-    except AttributeError:        # no tensor
-        fit = False
-    if not fit:
+    if not (_are(ts, dtype, shapes, device) and all(map(_CONTIGUOUS, ts))):
         raise RuntimeError(f"{name} must hold contiguous {dtype} tensors of the parameters' shapes on {device}")
 
 
@@ -82,37 +91,38 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
         return
     first = params[0]
     _t.require_tensor(first, "params")
-    device, shapes = first.device, [p.shape if isinstance(p, torch.Tensor) else None for p in params]
+    device, shapes = first.device, [getattr(p, "shape", None) for p in params]
     _checked(params, "params", first.dtype, shapes, device)
-    if not all([isinstance(g, torch.Tensor) and g.layout is torch.strided for g in grads]):
-        raise RuntimeError("grads must hold dense tensors")
-    grads = [g.contiguous() for g in grads]
+    try:
+        if set(map(_LAYOUT, grads)) - {torch.strided}:
+            raise TypeError
+        if not all(map(_CONTIGUOUS, grads)):
+            grads = [g.contiguous() for g in grads]
+    except (AttributeError, TypeError):
+        raise RuntimeError("grads must hold dense tensors") from None
     _checked(grads, "grads", first.dtype, shapes, device)
     moment = torch.float32 if scales is None else torch.uint8
     _checked(exp_avgs, "exp_avgs", moment, shapes, device)
     _checked(exp_avg_sqs, "exp_avg_sqs", moment, shapes, device)
-    n, sizes = len(params), [p.numel() for p in params]
+    n, sizes = len(params), list(map(_NUMEL, params))
     pointers = lambda addresses: (C.c_void_p * n)(*addresses)  # noqa: E731
-    written = [[t.data_ptr() for t in ts] for ts in (params, exp_avgs, exp_avg_sqs)]
+    written = [list(map(_ADDRESS, ts)) for ts in (params, exp_avgs, exp_avg_sqs)]
     low = high = None
     if scales is not None:
         if len(scales) != n:
             raise RuntimeError(f"scales must hold a tensor for each of {n} parameters, got {len(scales)}")
         blocks = [-(-size // BLOCK) for size in sizes]
-        fit = (all([isinstance(s, torch.Tensor) and s.dtype is torch.uint8 for s in scales])
-               and all([s.get_device() == device.index for s in scales])
-               and [s.shape for s in scales] == [(2, b) for b in blocks])
-        strides = [s.stride() for s in scales] if fit else []
-        if not (fit and all([row >= b and (one == 1 or b < 2) for b, (row, one) in zip(blocks, strides)])):
+        strides = list(map(_STRIDE, scales)) if _are(scales, torch.uint8, [(2, b) for b in blocks], device) else []
+        if not strides or not all([row >= b and (one == 1 or b < 2) for b, (row, one) in zip(blocks, strides)]):
             raise RuntimeError(f"scales must hold uint8 tensors of shape (2, ceil(n / {BLOCK})) with contiguous rows on "
                                f"{device}")
-        first_rows = [s.data_ptr() for s in scales]
+        first_rows = list(map(_ADDRESS, scales))
         written += [first_rows, [a + row for a, (row, _) in zip(first_rows, strides)]]
         low, high = (pointers(a) for a in written[3:])
     with _t.on_device(device):
         _t.check(_t.load().gs_adamw_update(
             _t.DTYPE_CODES[first.dtype], 32 if scales is None else 8, n, (C.c_int64 * n)(*sizes), pointers(written[0]),
-            pointers([g.data_ptr() for g in grads]), pointers(written[1]), pointers(written[2]), low, high,
+            pointers(list(map(_ADDRESS, grads))), pointers(written[1]), pointers(written[2]), low, high,
             C.byref(AdamWSettings(*how, step, seed & 0xFFFFFFFF)), _t.stream(device)), "gs_adamw_update")
     # written through their addresses: graphs that saved them are told
     torch.autograd.graph.increment_version(params)
