@@ -41,12 +41,12 @@ def _padded(nbytes):
 def _forward(x, gate, up, down, activation, grads):
     """y, what the library is called with, and for a backward h, a, b and their rests, one after the other in bytes."""
     (hidden, width), out = gate.shape, down.shape[0]
-    n, dtype, device = x.numel() // width, x.dtype, x.device
+    n, device = x.numel() // width, x.device
     rows, apart = _rows(x, width)
-    code = _t.DTYPE_CODES[dtype]
+    code = _t.DTYPE_CODES[x.dtype]
     sizes = code, activation, n, width, hidden, out
     lib = _t.load()
-    y = torch.empty(x.shape[:-1] + (out,), device=device, dtype=dtype)
+    y = x.new_empty(x.shape[:-1] + (out,))
     part, each = lib.gs_feed_forward_workspace_bytes(code, n, width, hidden, out, 0), _padded(n * hidden * x.element_size())
     if grads:
         kept = torch.empty(3 * each + (n * hidden if code else 0), device=device, dtype=torch.uint8)
@@ -84,15 +84,17 @@ class _FeedForward(torch.autograd.Function):
         x, *saved = ctx.saved_tensors
         gate, up, down, kept = (t.contiguous() for t in saved)
         code, _, n, width, hidden, out = ctx.how
-        device, dtype, lib = x.device, x.dtype, _t.load()
+        device, lib = x.device, _t.load()
         rows, apart = _rows(x, width)
         drows, dapart = _rows(dy, out)
         if kept.data_ptr() % 256:
             kept = kept.clone()
         h = kept.data_ptr()
         a, b, rest = _places(h, _padded(n * hidden * x.element_size()), code)
-        grads = [torch.empty(t.shape, device=device, dtype=dtype) if need else None
-                 for need, t in zip(ctx.needs_input_grad, (x, gate, up, down))]
+        need = ctx.needs_input_grad
+        grads = (torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None,
+                 torch.empty_like(gate) if need[1] else None, torch.empty_like(up) if need[2] else None,
+                 torch.empty_like(down) if need[3] else None)
         ws = _t.workspace(lib.gs_feed_forward_workspace_bytes(code, n, width, hidden, out, 1), device)
         _t.check(lib.gs_feed_forward_backward(
             *ctx.how, rows.data_ptr(), apart, gate.data_ptr(), up.data_ptr(), down.data_ptr(), a, b, rest, h,

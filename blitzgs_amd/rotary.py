@@ -89,10 +89,11 @@ class _Out:
     def __init__(self, like):
         B, H, T, D = like.shape
         self.shape, self.strides = (B, H, T, D), (T * H * D, D, H * D, 1)
-        self.dtype, self.steps = like.dtype, _Strides(*self.strides)
+        self.steps = _Strides(*self.strides)
 
-    def empty(self, device):
-        return torch.empty_strided(self.shape, self.strides, device=device, dtype=self.dtype)
+    def beside(self, t):
+        """A new one of t's type and device."""
+        return t.new_empty_strided(self.shape, self.strides)
 
 
 class _How:
@@ -104,9 +105,9 @@ class _How:
         code = _t.DTYPE_CODES[q.dtype]
         axes, pairs = (1, frequencies.shape[0]) if frequencies.dim() == 1 else frequencies.shape
         self.sizes = code, B, Hq, 0 if k is None else self.k.shape[1], T, D, axes, pairs
-        self.params = q.dtype if weight is None else weight.dtype
+        params = _t.DTYPE_CODES[q.dtype if weight is None else weight.dtype]
         self.norm = norm
-        self.first = code, _t.DTYPE_CODES[self.params], *self.sizes[1:], interleaved, magnitude, norm, eps
+        self.first = code, params, *self.sizes[1:], interleaved, magnitude, norm, eps
 
     def angles(self, positions, frequencies):
         strides = positions.stride()
@@ -123,8 +124,8 @@ def _forward(q, k, qw, kw, positions, frequencies, how):
     device = q.device
     q, qp, qs = _rows(q)
     k, kp, ks = _rows(k)
-    qy = how.q.empty(device)
-    ky, kyp, kys = (None, None, None) if k is None else ((ky := how.k.empty(device)), ky.data_ptr(), how.k.steps)
+    qy = how.q.beside(q)
+    ky, kyp, kys = (None, None, None) if k is None else ((ky := how.k.beside(k)), ky.data_ptr(), how.k.steps)
     with _t.on_device(device):
         _t.check(_t.load().gs_rotary_forward(
             *how.first, qp, qs, kp, ks, _t.ptr(qw), _t.ptr(kw), *how.angles(positions, frequencies), qy.data_ptr(),
@@ -158,10 +159,10 @@ class _Rotary(torch.autograd.Function):
         dky, dkyp, dkys = _rows(dky)
         dq = dk = dqw = dkw = ws = dqp = dkp = dks = qwp = kwp = dqwp = dkwp = None
         if need_q or need_qw:
-            dq = how.q.empty(device)
+            dq = how.q.beside(dqy)
             dqp = dq.data_ptr()
         if dky is not None and (need_k or need_kw):
-            dk = how.k.empty(device)
+            dk = how.k.beside(dky)
             dkp, dks = dk.data_ptr(), how.k.steps
         if how.norm:
             if qw is not None:
@@ -171,10 +172,10 @@ class _Rotary(torch.autograd.Function):
                 kw = kw.contiguous()
                 kwp = kw.data_ptr()
             if need_qw:
-                dqw = torch.empty(qw.shape, device=device, dtype=how.params)
+                dqw = torch.empty_like(qw)
                 dqwp = dqw.data_ptr()
             if need_kw and dk is not None:
-                dkw = torch.empty(kw.shape, device=device, dtype=how.params)
+                dkw = torch.empty_like(kw)
                 dkwp = dkw.data_ptr()
             if need_qw or need_kw:
                 ws = _t.workspace(lib.gs_rotary_workspace_bytes(*how.sizes), device)
