@@ -20,6 +20,7 @@ infinite or NaN is NaN in 8 bits.
 import ctypes as C
 import math
 import operator
+from array import array
 
 import torch
 
@@ -41,25 +42,33 @@ def new_moments(param, bits=32):
 
 
 # over whole lists, without a line of Python for each tensor: a call over many is bound by these
-_SHAPE, _DTYPE, _LAYOUT = (operator.attrgetter(name) for name in ("shape", "dtype", "layout"))
+_SHAPE, _DTYPE = operator.attrgetter("shape"), operator.attrgetter("dtype")
 _CONTIGUOUS, _DEVICE, _NUMEL = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.numel
 _ADDRESS, _STRIDE = torch.Tensor.data_ptr, torch.Tensor.stride
 
 
-def _are(ts, dtype, shapes, device):
-    """Whether ts are tensors of a type, shapes and a device."""
+def _are(ts, dtype, device, shapes=None):
+    """Whether ts are tensors of a type, on a device and of these shapes."""
     try:
         return (set(map(_DTYPE, ts)) == {dtype} and set(map(_DEVICE, ts)) == {device.index}
-                and list(map(_SHAPE, ts)) == shapes)
+                and (shapes is None or list(map(_SHAPE, ts)) == shapes))
     except (AttributeError, TypeError):        # no tensor
         return False
 
 
-def _checked(ts, name, dtype, shapes, device):
+def _contiguous(ts):
+    """Whether all are; what is no dense tensor is not."""
+    try:
+        return all(map(_CONTIGUOUS, ts))
+    except (TypeError, RuntimeError):
+        return False
+
+
+def _checked(ts, name, dtype, device, shapes):
     """Contiguous tensors of a type and of the parameters' shapes."""
     if len(ts) != len(shapes):
         raise RuntimeError(f"{name} must hold a tensor for each of {len(shapes)} parameters, got {len(ts)}")
-    if not (_are(ts, dtype, shapes, device) and all(map(_CONTIGUOUS, ts))):
+    if not (_are(ts, dtype, device, shapes) and _contiguous(ts)):
         raise RuntimeError(f"{name} must hold contiguous {dtype} tensors of the parameters' shapes on {device}")
 
 
@@ -91,28 +100,28 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
         return
     first = params[0]
     _t.require_tensor(first, "params")
-    device, shapes = first.device, [getattr(p, "shape", None) for p in params]
-    _checked(params, "params", first.dtype, shapes, device)
-    try:
-        if set(map(_LAYOUT, grads)) - {torch.strided}:
-            raise TypeError
-        if not all(map(_CONTIGUOUS, grads)):
-            grads = [g.contiguous() for g in grads]
-    except (AttributeError, TypeError):
-        raise RuntimeError("grads must hold dense tensors") from None
-    _checked(grads, "grads", first.dtype, shapes, device)
+    dtype, device = first.dtype, first.device
+    if not (_are(params, dtype, device) and _contiguous(params)):
+        raise RuntimeError(f"params must hold contiguous {dtype} tensors on {device}")
+    shapes = list(map(_SHAPE, params))
+    if not _contiguous(grads):
+        if not all([isinstance(g, torch.Tensor) and g.layout is torch.strided for g in grads]):
+            raise RuntimeError("grads must hold dense tensors")
+        grads = [g.contiguous() for g in grads]
+    if not _are(grads, dtype, device, shapes):
+        raise RuntimeError(f"grads must hold a {dtype} tensor of each parameter's shape on {device}")
     moment = torch.float32 if scales is None else torch.uint8
-    _checked(exp_avgs, "exp_avgs", moment, shapes, device)
-    _checked(exp_avg_sqs, "exp_avg_sqs", moment, shapes, device)
+    _checked(exp_avgs, "exp_avgs", moment, device, shapes)
+    _checked(exp_avg_sqs, "exp_avg_sqs", moment, device, shapes)
     n, sizes = len(params), list(map(_NUMEL, params))
-    pointers = lambda addresses: (C.c_void_p * n)(*addresses)  # noqa: E731
+    pointers = lambda addresses: (C.c_void_p * n).from_buffer(array("Q", addresses))  # noqa: E731
     written = [list(map(_ADDRESS, ts)) for ts in (params, exp_avgs, exp_avg_sqs)]
     low = high = None
     if scales is not None:
         if len(scales) != n:
             raise RuntimeError(f"scales must hold a tensor for each of {n} parameters, got {len(scales)}")
         blocks = [-(-size // BLOCK) for size in sizes]
-        strides = list(map(_STRIDE, scales)) if _are(scales, torch.uint8, [(2, b) for b in blocks], device) else []
+        strides = list(map(_STRIDE, scales)) if _are(scales, torch.uint8, device, [(2, b) for b in blocks]) else []
         if not strides or not all([row >= b and (one == 1 or b < 2) for b, (row, one) in zip(blocks, strides)]):
             raise RuntimeError(f"scales must hold uint8 tensors of shape (2, ceil(n / {BLOCK})) with contiguous rows on "
                                f"{device}")
@@ -121,8 +130,8 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
         low, high = (pointers(a) for a in written[3:])
     with _t.on_device(device):
         _t.check(_t.load().gs_adamw_update(
-            _t.DTYPE_CODES[first.dtype], 32 if scales is None else 8, n, (C.c_int64 * n)(*sizes), pointers(written[0]),
-            pointers(list(map(_ADDRESS, grads))), pointers(written[1]), pointers(written[2]), low, high,
+            _t.DTYPE_CODES[dtype], 32 if scales is None else 8, n, (C.c_int64 * n).from_buffer(array("q", sizes)),
+            pointers(written[0]), pointers(list(map(_ADDRESS, grads))), pointers(written[1]), pointers(written[2]), low, high,
             C.byref(AdamWSettings(*how, step, seed & 0xFFFFFFFF)), _t.stream(device)), "gs_adamw_update")
     # written through their addresses: graphs that saved them are told
     torch.autograd.graph.increment_version(params)
