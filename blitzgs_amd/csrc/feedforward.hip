@@ -49,6 +49,7 @@ struct Product {
     void* out[3];                 // HIDDEN: h, a, b; GRAD: da, db; else the result
     const void* in[2];            // GRAD: a, b
     uint8_t* rest;                // of a and b, or null
+    bool pad;                     // the result's rows end with zeros up to a whole piece of 8
     int first;                    // workgroup
 };
 
@@ -94,9 +95,10 @@ __device__ __forceinline__ void activation(int act, float a, float& value, float
 // An operand's tiles of S rows of the result by KT of the depth, as tiles of rows of W
 // elements, 128 bytes.  Along: KT / W tiles of S rows.  DOWN: S / W tiles of KT rows, which
 // lie in the order in which Tile::cols takes them as k = 8 g + j.
-//   DIRECT: straight to LDS, 16 bytes at a time; chunks are whole and aligned.  What
-//           lies beyond the depth comes from `zeros`; beyond the last row or column
-//           the last one comes again, whose results nobody keeps.
+//   DIRECT: straight to LDS, 16 bytes at a time; chunks are aligned and whole, with zeros
+//           behind the last element of an operand's row where its length is no whole
+//           number of them.  What lies beyond the depth comes from `zeros`; beyond the
+//           last row or column the last one comes again, whose results nobody keeps.
 //   else:   through registers, from any address; what lies beyond is zero
 template <typename T, int S, int KT, bool DOWN, int THREADS, bool DIRECT>
 struct Operand {
@@ -132,7 +134,7 @@ struct Operand {
                 int row, k;
                 place(threadIdx.x + THREADS * c, row, k);
                 row = map(row);
-                if constexpr (DOWN) at[c] = (uint32_t)(((int64_t)k * ld + min(row, limit - V)) * (int)sizeof(T));
+                if constexpr (DOWN) at[c] = (uint32_t)(((int64_t)k * ld + min(row, (limit - 1) / V * V)) * (int)sizeof(T));
                 else at[c] = (uint32_t)(((int64_t)min(row, limit - 1) * ld + k) * (int)sizeof(T));
             }
         }
@@ -268,10 +270,10 @@ struct Leave {
     T *out0, *out1, *out2;
     const T *in0, *in1;
     uint8_t* rest;
-    bool also;
+    bool also, pad;
 
     __device__ __forceinline__ Leave(const Product& P, int act, float* own, int first)
-        : own(own), lane(threadIdx.x & 63), act(act), rows(P.rows), old(P.old), also(P.out[1] != nullptr)
+        : own(own), lane(threadIdx.x & 63), act(act), rows(P.rows), old(P.old), also(P.out[1] != nullptr), pad(P.pad)
     {
         const int col = first + lane % C * 8;
         n = P.cols - col;
@@ -316,7 +318,8 @@ struct Leave {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int p = 0; p < PASSES; p++) {
-            const int r = p * RP + lane / C, row = row0 + r, count = here<WHOLE>(row);
+            const int r = p * RP + lane / C, row = row0 + r, real = here<WHOLE>(row);
+            const int count = !WHOLE && pad && real > 0 ? 8 : real;
             const float* from = own + r * LD;
             const int64_t at = row * old;
             float o[8], d[8];
@@ -326,6 +329,11 @@ struct Leave {
                 float a[8], b[8];
                 __builtin_memcpy(a, f, 32);
                 __builtin_memcpy(b, f + 16, 32);
+                if (!WHOLE && pad) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (e >= real) a[e] = b[e] = 0.0f;
+                }
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     float value, slope;
@@ -364,6 +372,7 @@ struct Leave {
                     activation<T>(act, a, value, slope);
                     o[e] = d[e] * b * slope;
                     d[e] = d[e] * value;
+                    if (!WHOLE && pad && e >= real) o[e] = d[e] = 0.0f;
                 }
                 put<T, 8, WHOLE>(out0 + at, o, count);
                 put<T, 8, WHOLE>(out1 + at, d, count);
@@ -796,7 +805,7 @@ __global__ __launch_bounds__(512) void feed_few_kernel(FeedArgs A)
     __syncthreads();
     if (threadIdx.x >= C * C) return;
     const int row = threadIdx.x / C, col = threadIdx.x % C;
-    if (row >= rows || n0 + col >= cols) return;
+    if (row >= rows || n0 + col >= (P.pad ? (cols + 7) / 8 * 8 : cols)) return;
     float sum[N] = {};
 #pragma unroll
     for (int w = 0; w < WAVES; w++)
@@ -807,6 +816,9 @@ __global__ __launch_bounds__(512) void feed_few_kernel(FeedArgs A)
             for (int n = 0; n < N; n++) sum[n] += meet[n][w][j / 4 * 16 + piece * C + row][j % 4];
         }
     const int64_t at = row * P.old + n0 + col;
+    if (n0 + col >= cols)
+#pragma unroll
+        for (int n = 0; n < N; n++) sum[n] = 0.0f;
     if constexpr (K == HIDDEN) {
         float value, slope;
         activation<T>(A.act, sum[0], value, slope);
@@ -819,6 +831,33 @@ __global__ __launch_bounds__(512) void feed_few_kernel(FeedArgs A)
         }
     } else {
         ((T*)P.out[0])[at] = (T)sum[0];
+    }
+}
+
+// Matrices of a 16-bit type copied to rows of whole 16-byte pieces, zeros behind their ends.
+struct PadArgs {
+    struct {
+        const uint16_t* from;
+        uint4* to;
+        int64_t ld;
+        int rows, cols, pieces;
+        unsigned first, blocks;
+    } m[5];
+    int count;
+    unsigned blocks;
+};
+
+__global__ __launch_bounds__(256) void feed_pad_kernel(PadArgs A)
+{
+    int which = 0;
+    while (which + 1 < A.count && blockIdx.x >= A.m[which + 1].first) which++;
+    const auto& M = A.m[which];
+    const int64_t all = (int64_t)M.rows * M.pieces;
+    for (int64_t i = (int64_t)(blockIdx.x - M.first) * 256 + threadIdx.x; i < all; i += (int64_t)M.blocks * 256) {
+        const int64_t row = i / M.pieces;
+        const int col = (int)(i - row * M.pieces) * 8;
+        const Raw<uint16_t, 8> v = get<uint16_t, 8, false>(M.from + row * M.ld + col, M.cols - col);
+        M.to[i] = __builtin_bit_cast(uint4, v);
     }
 }
 
@@ -896,8 +935,8 @@ template <typename T, Kind K, int C>
 int launch_few(const FeedArgs& A, hipStream_t stream)
 {
     GS_TIMED("feed_few_kernel", stream,
-             hipLaunchKernelGGL((feed_few_kernel<T, K, C>), dim3(gs_div_up((size_t)A.p[0].cols, C)), dim3(512), 0, stream,
-                                A));
+             hipLaunchKernelGGL((feed_few_kernel<T, K, C>), dim3(gs_div_up((size_t)A.p[0].cols + (A.p[0].pad ? 7 : 0), C)),
+                                dim3(512), 0, stream, A));
     GS_LAUNCH_CHECK("feed_few_kernel");
     return GS_OK;
 }
@@ -1008,6 +1047,9 @@ bool whole(const void* p, int64_t ld, int n, int type)
     return (uintptr_t)p % 16 == 0 && ld % v == 0 && n % v == 0 && ld < 1 << 21;
 }
 
+// n up to whole pieces of 8: what rows of h, a, b, their rests, da and db take
+int up8(int n) { return (n + 7) / 8 * 8; }
+
 size_t padded(size_t n) { return (n + 255) / 256 * 256; }
 
 // Sets A's parts of the depth.
@@ -1024,17 +1066,91 @@ int64_t turns_of(int64_t depth) { return (depth + SKT - 1) / SKT; }
 // What the parts take: no more of them than places, of any products of a launch.
 constexpr size_t PART_BYTES = (size_t)2 * CUS * SS * SS * sizeof(float);
 
+// Whether operands of a 16-bit type whose rows are no whole 16-byte pieces are copied to such rows:
+// then the large tiles, straight to LDS, do for them too.  It costs a launch each way and the
+// operands' bytes twice.  Forward and backward, bfloat16, us without and with: 8192 x 1023 x
+// 3000 2361, 677 (1024 x 3000: 639); 4096 x 511 x 1535 593, 182; 2048 x 255 x 1023 170, 141.
+// Smaller blocks take as long as the host does, which pays for the launches, and for fewer
+// rows the weights' copies take longer than their products.
+bool worth_copies(int type, int64_t rows, int width, int hidden, int out)
+{
+    return gs::dtype_bytes(type) == 2 && rows >= 256 && rows * hidden * (2.0 * width + out) >= 1 << 30;
+}
+
+size_t copy_bytes(int64_t rows, int n) { return padded((size_t)rows * up8(n) * 2); }
+
+// What the copies take: x, the gate and up; down; in the backward dy
+size_t copies_bytes(int type, int64_t rows, int width, int hidden, int out, bool backward)
+{
+    if (!worth_copies(type, rows, width, hidden, out)) return 0;
+    return (width % 8 ? copy_bytes(rows, width) + 2 * copy_bytes(hidden, width) : 0) +
+           (hidden % 8 ? copy_bytes(out, hidden) : 0) + (backward && out % 8 ? copy_bytes(rows, out) : 0);
+}
+
+bool forward_parts(int64_t rows, int hidden, int out)
+{
+    return splits_of(tiles_of(rows, out, SS, SS), turns_of(hidden), false) > 1;
+}
+
+// the weights' gradients are split alone or together, as many as are asked for
+bool backward_parts(int64_t rows, int width, int hidden, int out)
+{
+    return splits_of(tiles_of(rows, width, SS, SS), 2 * turns_of(hidden), false) > 1 ||
+           splits_of(tiles_of(hidden, width, SS, SS), turns_of(rows), false) > 1 ||
+           splits_of(tiles_of(out, hidden, SS, SS), turns_of(rows), false) > 1;
+}
+
+// An operand as the products read it.
+struct Matrix {
+    const void* p;
+    int64_t ld;
+    bool direct;
+};
+
+struct Copies {
+    PadArgs args{};
+    int type;
+    bool worth;
+    char* at;
+
+    Matrix operator()(const void* p, int64_t ld, int64_t rows, int n)
+    {
+        if (whole(p, ld, n, type)) return {p, ld, true};
+        if (!worth || n % 8 == 0 || up8(n) >= 1 << 21) return {p, ld, false};
+        auto& m = args.m[args.count++];
+        m.from = (const uint16_t*)p;
+        m.to = (uint4*)at;
+        m.ld = ld;
+        m.rows = (int)rows;
+        m.cols = n;
+        m.pieces = up8(n) / 8;
+        m.first = args.blocks;
+        const int64_t blocks = (rows * m.pieces + 255) / 256;
+        m.blocks = (unsigned)(blocks < 16384 ? blocks : 16384);
+        args.blocks += m.blocks;
+        const Matrix to{at, up8(n), true};
+        at += copy_bytes(rows, n);
+        return to;
+    }
+    int launch(hipStream_t stream)
+    {
+        if (args.count == 0) return GS_OK;
+        GS_TIMED("feed_pad_kernel", stream,
+                 hipLaunchKernelGGL(feed_pad_kernel, dim3(args.blocks), dim3(256), 0, stream, args));
+        GS_LAUNCH_CHECK("feed_pad_kernel");
+        return GS_OK;
+    }
+};
+
 }  // namespace
 
 extern "C" size_t gs_feed_forward_workspace_bytes(int type, int64_t rows, int width, int hidden, int out, int backward)
 {
     if (check(type, GS_SILU, rows, width, hidden, out) != GS_OK) return 0;
-    if (!backward) return splits_of(tiles_of(rows, out, SS, SS), turns_of(hidden), false) > 1 ? PART_BYTES : 0;
-    // the weights' gradients are split alone or together, as many as are asked for
-    const bool parts = splits_of(tiles_of(rows, width, SS, SS), 2 * turns_of(hidden), false) > 1 ||
-                       splits_of(tiles_of(hidden, width, SS, SS), turns_of(rows), false) > 1 ||
-                       splits_of(tiles_of(out, hidden, SS, SS), turns_of(rows), false) > 1;
-    return 2 * padded((size_t)rows * hidden * gs::dtype_bytes(type)) + (parts ? PART_BYTES : 256);
+    const size_t copies = copies_bytes(type, rows, width, hidden, out, backward != 0);
+    if (!backward) return (forward_parts(rows, hidden, out) ? PART_BYTES : 0) + copies;
+    return 2 * padded((size_t)rows * up8(hidden) * gs::dtype_bytes(type)) +
+           (backward_parts(rows, width, hidden, out) ? PART_BYTES : 256) + copies;
 }
 
 extern "C" int gs_feed_forward(int type, int activation, int64_t rows, int width, int hidden, int out, const void* x,
@@ -1048,40 +1164,49 @@ extern "C" int gs_feed_forward(int type, int activation, int64_t rows, int width
     if (rows == 0) return GS_OK;
     GS_REQUIRE(x_stride >= 0, "feed forward: a stride must not be negative");
     GS_REQUIRE(x && gate && up && down && h && y, "feed forward: x, the weights, h and y must be non-null");
+    const bool parts = forward_parts(rows, hidden, out);
+    const size_t copied = copies_bytes(type, rows, width, hidden, out, false);
+    GS_REQUIRE((!parts && copied == 0) || (workspace != nullptr && (uintptr_t)workspace % 256 == 0),
+               "feed forward: these sizes need the workspace, 256-byte aligned");
+    Copies copies;
+    copies.type = type;
+    copies.worth = copied > 0;
+    copies.at = (char*)workspace + (parts ? PART_BYTES : 0);
+    const Matrix X = copies(x, x_stride, rows, width), G = copies(gate, width, hidden, width),
+                 U = copies(up, width, hidden, width), D = copies(down, hidden, out, hidden);
+    if (int rc = copies.launch(stream)) return rc;
     FeedArgs A{};
     A.act = activation;
     A.splits = 1;
     A.count = 1;
     Product& P = A.p[0];
-    P.l[0] = x;
-    P.lld = x_stride;
-    P.r[0] = gate;
-    P.r[1] = up;
-    P.rld = width;
+    P.l[0] = X.p;
+    P.lld = X.ld;
+    P.r[0] = G.p;
+    P.r[1] = U.p;
+    P.rld = G.ld;
     P.rows = (int)rows;
     P.cols = hidden;
     P.depth = width;
-    P.old = hidden;
+    P.old = up8(hidden);
+    P.pad = true;
     P.out[0] = h;
     P.out[1] = a;
     P.out[2] = b;
     P.rest = (uint8_t*)rest;
-    bool direct = whole(x, x_stride, width, type) && whole(gate, width, width, type) && whole(up, width, width, type);
-    if (int rc = launch<HIDDEN, false, false>(type, A, direct, stream)) return rc;
+    if (int rc = launch<HIDDEN, false, false>(type, A, X.direct && G.direct && U.direct, stream)) return rc;
     P = Product{};
     P.l[0] = h;
-    P.lld = hidden;
-    P.r[0] = down;
-    P.rld = hidden;
+    P.lld = up8(hidden);
+    P.r[0] = D.p;
+    P.rld = D.ld;
     P.rows = (int)rows;
     P.cols = out;
     P.depth = hidden;
     P.old = out;
     P.out[0] = y;
-    direct = whole(h, hidden, hidden, type) && whole(down, hidden, hidden, type);
+    const bool direct = D.direct && whole(h, up8(hidden), up8(hidden), type);
     split(A, turns_of(hidden), direct, workspace);
-    GS_REQUIRE(A.splits == 1 || (workspace != nullptr && (uintptr_t)workspace % 256 == 0),
-               "feed forward: these sizes need the workspace, 256-byte aligned");
     return launch<PLAIN, false, false>(type, A, direct, stream);
 }
 
@@ -1103,71 +1228,79 @@ extern "C" int gs_feed_forward_backward(int type, int activation, int64_t rows, 
         GS_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 256 == 0,
                    "feed forward: the backward needs its workspace, 256-byte aligned");
     }
-    char* da = (char*)workspace;
-    char* db = da + padded((size_t)rows * hidden * gs::dtype_bytes(type));
+    const size_t inner_bytes = padded((size_t)rows * up8(hidden) * gs::dtype_bytes(type));
+    char *da = (char*)workspace, *db = da + inner_bytes, *part = db + inner_bytes;
     FeedArgs A{};
     A.act = activation;
     A.splits = 1;
     A.count = 1;
-    void* part = db + padded((size_t)rows * hidden * gs::dtype_bytes(type));
+    Copies copies;
+    copies.type = type;
+    copies.worth = copies_bytes(type, rows, width, hidden, out, true) > 0;
+    copies.at = part + (backward_parts(rows, width, hidden, out) ? PART_BYTES : 256);
+    const Matrix X = copies(x, x_stride, rows, width), Y = copies(dy, dy_stride, rows, out),
+                 G = copies(gate, width, hidden, width), U = copies(up, width, hidden, width),
+                 D = copies(down, hidden, out, hidden);
+    if (int rc = copies.launch(stream)) return rc;
+    const int ld = up8(hidden);
     if (inner && rows > 0) {
         Product& P = A.p[0];
-        P.l[0] = dy;
-        P.lld = dy_stride;
-        P.r[0] = down;
-        P.rld = hidden;
+        P.l[0] = Y.p;
+        P.lld = Y.ld;
+        P.r[0] = D.p;
+        P.rld = D.ld;
         P.rows = (int)rows;
         P.cols = hidden;
         P.depth = out;
-        P.old = hidden;
+        P.old = ld;
+        P.pad = true;
         P.out[0] = da;
         P.out[1] = db;
         P.in[0] = a;
         P.in[1] = b;
         P.rest = (uint8_t*)const_cast<void*>(rest);
-        const bool direct = whole(dy, dy_stride, out, type) && whole(down, hidden, hidden, type);
-        if (int rc = launch<GRAD, false, true>(type, A, direct, stream)) return rc;
+        if (int rc = launch<GRAD, false, true>(type, A, Y.direct && D.direct, stream)) return rc;
     }
     if (dx != nullptr && rows > 0) {
         Product& P = A.p[0];
         P = Product{};
         P.l[0] = da;
         P.l[1] = db;
-        P.lld = hidden;
-        P.r[0] = gate;
-        P.r[1] = up;
-        P.rld = width;
+        P.lld = ld;
+        P.r[0] = G.p;
+        P.r[1] = U.p;
+        P.rld = G.ld;
         P.rows = (int)rows;
         P.cols = width;
         P.depth = hidden;
         P.old = width;
         P.out[0] = dx;
-        const bool direct = whole(da, hidden, hidden, type) && whole(gate, width, width, type) &&
-                            whole(up, width, width, type);
+        const bool direct = G.direct && U.direct && whole(da, ld, ld, type);
         split(A, 2 * turns_of(hidden), direct, part);
         if (int rc = launch<SUM, false, true>(type, A, direct, stream)) return rc;
     }
     // the weights' gradients, one after the other in one launch
     A.count = 0;
     bool direct = true;
-    auto add = [&](const void* l, int64_t lld, int m, const void* r, int64_t rld, int n, void* to) {
+    auto add = [&](const Matrix& l, int m, const Matrix& r, int n, void* to) {
         if (to == nullptr) return;
         Product& P = A.p[A.count++];
         P = Product{};
-        P.l[0] = l;
-        P.lld = lld;
-        P.r[0] = r;
-        P.rld = rld;
+        P.l[0] = l.p;
+        P.lld = l.ld;
+        P.r[0] = r.p;
+        P.rld = r.ld;
         P.rows = m;
         P.cols = n;
         P.depth = (int)rows;
         P.old = n;
         P.out[0] = to;
-        direct = direct && whole(l, lld, m, type) && whole(r, rld, n, type);
+        direct = direct && l.direct && r.direct;
     };
-    add(da, hidden, hidden, x, x_stride, width, dgate);
-    add(db, hidden, hidden, x, x_stride, width, dup);
-    add(dy, dy_stride, out, h, hidden, hidden, ddown);
+    const bool inner_direct = whole(da, ld, ld, type), h_direct = whole(h, ld, ld, type);
+    add(Matrix{da, ld, inner_direct}, hidden, X, width, dgate);
+    add(Matrix{db, ld, inner_direct}, hidden, X, width, dup);
+    add(Y, out, Matrix{h, ld, h_direct}, hidden, ddown);
     if (A.count == 0) return GS_OK;
     split(A, turns_of(rows), direct, part);
     return launch<PLAIN, true, true>(type, A, direct, stream);

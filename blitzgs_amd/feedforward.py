@@ -34,8 +34,10 @@ def _rows(t, width):
     return t, apart if n > 1 else width
 
 
-def _padded(nbytes):
-    return -(-nbytes // 256) * 256
+def _inner(n, hidden, x):
+    """Elements and bytes of n rows of a, b or h, as the library lays them: whole pieces of 8."""
+    elements = n * (-(-hidden // 8) * 8)
+    return elements, -(-elements * x.element_size() // 256) * 256
 
 
 def _forward(x, gate, up, down, activation, grads):
@@ -47,9 +49,9 @@ def _forward(x, gate, up, down, activation, grads):
     sizes = code, activation, n, width, hidden, out
     lib = _t.load()
     y = x.new_empty(x.shape[:-1] + (out,))
-    part, each = lib.gs_feed_forward_workspace_bytes(code, n, width, hidden, out, 0), _padded(n * hidden * x.element_size())
+    part, (elements, each) = lib.gs_feed_forward_workspace_bytes(code, n, width, hidden, out, 0), _inner(n, hidden, x)
     if grads:
-        kept = torch.empty(3 * each + (n * hidden if code else 0), device=device, dtype=torch.uint8)
+        kept = torch.empty(3 * each + (elements if code else 0), device=device, dtype=torch.uint8)
         ws = _t.workspace(part, device)
         h, wsp = kept.data_ptr(), _t.ptr(ws)
         a, b, rest = _places(h, each, code)
@@ -90,7 +92,7 @@ class _FeedForward(torch.autograd.Function):
         if kept.data_ptr() % 256:
             kept = kept.clone()
         h = kept.data_ptr()
-        a, b, rest = _places(h, _padded(n * hidden * x.element_size()), code)
+        a, b, rest = _places(h, _inner(n, hidden, x)[1], code)
         need = ctx.needs_input_grad
         grads = (torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None,
                  torch.empty_like(gate) if need[1] else None, torch.empty_like(up) if need[2] else None,

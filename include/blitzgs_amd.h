@@ -746,10 +746,11 @@ int gs_rotary_backward(int type, int param_type, int B, int Hq, int Hk, int T, i
  * width), gate and up (hidden, width), down (out, hidden), y (rows, out); act is
  * GS_SILU, a / (1 + exp(-a)), or GS_GELU, a (1 + erf(a / sqrt(2))) / 2.  x's (and
  * dy's) rows are x_stride elements apart and contiguous inside, all else is
- * contiguous.  h (rows, hidden) is written: act(a) * b of a = x gate^T, b = x up^T,
- * rounded to `type`; a and b (rows, hidden) too, for the backward, or both NULL, and
- * rest (rows, hidden), a byte each, may be NULL: with the 16-bit types four bits of
- * what rounding a left and, above them, four of b.
+ * contiguous.  h (rows, hidden), whose rows (as a's, b's and rest's) are hidden rounded
+ * up to a multiple of 8 elements apart, is written: act(a) * b of a = x gate^T, b = x
+ * up^T, rounded to `type`, and zeros behind each row; a and b too, for the backward, or
+ * both NULL, and rest, a byte each, may be NULL: with the 16-bit types four bits of what
+ * rounding a left and, above them, four of b.
  *   Backward, from a, b, rest (NULL if the forward had none) and h: dx, dgate, dup,
  * ddown, each unless NULL.
  *   workspace: 256-byte aligned, of gs_feed_forward_workspace_bytes (0: none is

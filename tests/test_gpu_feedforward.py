@@ -79,6 +79,26 @@ def test_many_rows(gpu, t, M, W, H, O):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,W,H,O", [(600, 1023, 1001, 1030), (2100, 320, 771, 320), (700, 1020, 1024, 1023), (260, 1601, 1608, 800)])
+def test_large_odd_sizes(gpu, t, M, W, H, O):
+    # rows that are no whole 16 bytes: of x, gate and up; of down and what lies between; of dy; of all
+    wide = _rand((M, W + 5), t, 3)
+    _check(wide[:, 2:W + 2], _weights(W, H, O, t))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,W,H,O", [(9, 24, 13, 24), (40, 24, 200, 24), (700, 1023, 1001, 1030)])
+def test_infinite_gradients_stay_in_their_rows(gpu, t, M, W, H, O):
+    from blitzgs_amd.feedforward import feed_forward
+    x, weights, dy = _rand((M, W), t, 1).requires_grad_(True), _weights(W, H, O, t), _rand((M, O), t, 2)
+    (clean,) = torch.autograd.grad(feed_forward(x, *weights), x, dy)
+    dy[3, 0] = dy[5, O - 1] = math.inf
+    (g,) = torch.autograd.grad(feed_forward(x, *weights), x, dy)
+    rows = [r for r in range(M) if r not in (3, 5)]
+    assert torch.equal(g[rows], clean[rows]) and not torch.isfinite(g[[3, 5]]).any()
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_strides_and_dimensions(gpu, t):
     from blitzgs_amd.feedforward import feed_forward
     W, H, O = 64, 96, 64
