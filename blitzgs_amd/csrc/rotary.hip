@@ -24,7 +24,8 @@
 //
 // Forward and backward, bfloat16: 16384 tokens of 20 heads of 128, rotation alone, 75 us, 4.5
 // TB/s; 32768 tokens of 24 heads of 64 with norm and weights, 107 us, 4.7 TB/s (a large copy:
-// 5.15).  Rows of 75 float elements, read one by one: 37 us for 27567 of them.
+// 5.15).  27567 rows of 75 float elements, 41 MB: 38 us, a chain of loads, exchanges and stores
+// at few rows a CU.
 #include "gs_host.h"
 #include "gs_types.h"
 #include "../../include/blitzgs_amd.h"
@@ -102,63 +103,100 @@ __device__ __forceinline__ void store(T* p, const float* from)
     __builtin_memcpy(p, t, sizeof(t));
 }
 
-// An item of a row: elements lo .. lo + V - 1 and hi .. hi + V - 1, of the pairs
-// from `pair` on, or of none (pair < 0).
+// An item of a row: n_lo elements from lo on and n_hi from hi on, of the pairs from `pair`
+// on, or of none (pair < 0).  All are V or none but where the row is RAGGED: a last item of
+// the pairs and a last one of what is not rotated have fewer.
 struct Item {
     int lo, hi, pair;
-    bool has_lo, has_hi;
+    int n_lo, n_hi;
 };
 
 template <int V, bool IL>
 __device__ __forceinline__ Item item_of(int i, int N, int D)
 {
     Item t;
-    const int pair = i * V;
-    if (pair < N) {
+    const int pair = i * V, last = (N + V - 1) / V;
+    if (i < last) {
         t.lo = IL ? 2 * pair : pair;
         t.hi = IL ? 2 * pair + V : pair + N;
         t.pair = pair;
+        t.n_lo = t.n_hi = min(V, N - pair);
     } else {
-        t.lo = 2 * pair;
-        t.hi = 2 * pair + V;
+        t.lo = 2 * N + (i - last) * 2 * V;
+        t.hi = t.lo + V;
         t.pair = -1;
+        t.n_lo = max(0, min(V, D - t.lo));
+        t.n_hi = max(0, min(V, D - t.hi));
     }
-    t.has_lo = t.lo < D;
-    t.has_hi = t.hi < D;
     return t;
 }
 
-// Where pairs are neighbours an item is one piece of 2 V elements.
-template <typename T, int V, bool IL>
+// Whether the item's register i holds an element
+template <int V, bool IL>
+__device__ __forceinline__ bool holds(const Item& t, int i)
+{
+    return IL ? i < t.n_lo + t.n_hi : i < V ? i < t.n_lo : i - V < t.n_hi;
+}
+
+template <typename T, int V, bool RAGGED>
+__device__ __forceinline__ void load_part(const T* p, int n, float* to)
+{
+    if (n == V) {
+        load<T, V>(p, to);
+    } else if (RAGGED && n > 0) {
+        // without branches, so that all are under way together
+        T t[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) t[i] = p[min(i, n - 1)];
+#pragma unroll
+        for (int i = 0; i < V; i++) to[i] = i < n ? (float)t[i] : 0.0f;
+    }
+}
+
+template <typename T, int V, bool RAGGED>
+__device__ __forceinline__ void store_part(T* p, int n, const float* from)
+{
+    if (n == V) {
+        store<T, V>(p, from);
+    } else if (RAGGED) {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < n) p[i] = (T)from[i];
+    }
+}
+
+// Where pairs are neighbours an item is one piece of 2 V elements, of which the rest of a row may be half.
+template <typename T, int V, bool IL, bool RAGGED>
 __device__ __forceinline__ void load_item(const T* row, const Item& t, float (&v)[2 * V])
 {
 #pragma unroll
     for (int i = 0; i < 2 * V; i++) v[i] = 0.0f;
-    if (IL && t.has_hi) {
-        load<T, 2 * V>(row + t.lo, v);
-        return;
+    if constexpr (IL) {
+        load_part<T, 2 * V, RAGGED>(row + t.lo, t.n_lo + t.n_hi, v);
+    } else {
+        load_part<T, V, RAGGED>(row + t.lo, t.n_lo, v);
+        load_part<T, V, RAGGED>(row + t.hi, t.n_hi, v + V);
     }
-    if (t.has_lo) load<T, V>(row + t.lo, v);
-    if (!IL && t.has_hi) load<T, V>(row + t.hi, v + V);
 }
 
-template <typename T, int V, bool IL>
+template <typename T, int V, bool IL, bool RAGGED>
 __device__ __forceinline__ void store_item(T* row, const Item& t, const float (&v)[2 * V])
 {
-    if (IL && t.has_hi) {
-        store<T, 2 * V>(row + t.lo, v);
-        return;
+    if constexpr (IL) {
+        store_part<T, 2 * V, RAGGED>(row + t.lo, t.n_lo + t.n_hi, v);
+    } else {
+        store_part<T, V, RAGGED>(row + t.lo, t.n_lo, v);
+        store_part<T, V, RAGGED>(row + t.hi, t.n_hi, v + V);
     }
-    if (t.has_lo) store<T, V>(row + t.lo, v);
-    if (!IL && t.has_hi) store<T, V>(row + t.hi, v + V);
 }
 
 // The rotation by the table's angles, or back.
-template <int V, bool IL, bool BACK>
-__device__ __forceinline__ void turn(float (&v)[2 * V], const float2* cs)
+template <int V, bool IL, bool BACK, bool RAGGED>
+__device__ __forceinline__ void turn(float (&v)[2 * V], const float2* cs, int n)
 {
 #pragma unroll
     for (int j = 0; j < V; j++) {
+        if (RAGGED && j >= n) break;
         float& a = v[IL ? 2 * j : j];
         float& b = v[IL ? 2 * j + 1 : V + j];
         const float c = cs[j].x, s = BACK ? -cs[j].y : cs[j].y;
@@ -168,7 +206,7 @@ __device__ __forceinline__ void turn(float (&v)[2 * V], const float2* cs)
     }
 }
 
-template <typename T, int V, int NC, bool IL, bool NORM, bool BWD>
+template <typename T, int V, int NC, bool IL, bool RAGGED, bool NORM, bool BWD>
 __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
 {
     extern __shared__ uint64_t lds[];
@@ -192,9 +230,9 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
         }
         if (NORM && S.w != nullptr) {
             if (A.w32)
-                load_item<float, V, IL>((const float*)S.w, items[c], w[c]);
+                load_item<float, V, IL, RAGGED>((const float*)S.w, items[c], w[c]);
             else
-                load_item<T, V, IL>((const T*)S.w, items[c], w[c]);
+                load_item<T, V, IL, RAGGED>((const T*)S.w, items[c], w[c]);
         }
     }
     // a group's rows are `groups` apart, a thread's pairs BLOCK: no divisions in the loops
@@ -239,8 +277,8 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
             float r = 1.0f;
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-                if constexpr (!BWD || NORM) load_item<T, V, IL>(x, items[c], v[c]);
-                if constexpr (BWD) load_item<T, V, IL>(dy, items[c], g[c]);
+                if constexpr (!BWD || NORM) load_item<T, V, IL, RAGGED>(x, items[c], v[c]);
+                if constexpr (BWD) load_item<T, V, IL, RAGGED>(dy, items[c], g[c]);
             }
             if constexpr (NORM) {
                 float sum = 0.0f;
@@ -258,13 +296,13 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
 #pragma unroll
                         for (int i = 0; i < 2 * V; i++) v[c][i] = v[c][i] * r * w[c][i];
                     }
-                    if (items[c].pair >= 0) turn<V, IL, false>(v[c], cs + items[c].pair);
+                    if (items[c].pair >= 0) turn<V, IL, false, RAGGED>(v[c], cs + items[c].pair, items[c].n_lo);
                 }
             } else {
                 float sum = 0.0f;
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
-                    if (items[c].pair >= 0) turn<V, IL, true>(g[c], cs + items[c].pair);
+                    if (items[c].pair >= 0) turn<V, IL, true, RAGGED>(g[c], cs + items[c].pair, items[c].n_lo);
                     if constexpr (NORM) {
 #pragma unroll
                         for (int i = 0; i < 2 * V; i++) {
@@ -288,7 +326,7 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
                 }
             }
 #pragma unroll
-            for (int c = 0; c < NC; c++) store_item<T, V, IL>(out, items[c], v[c]);
+            for (int c = 0; c < NC; c++) store_item<T, V, IL, RAGGED>(out, items[c], v[c]);
             head += step_head;
             token += step_token;
             if (head >= S.heads) {
@@ -312,8 +350,7 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
                 float s = 0.0f;
                 for (int k = 0; k < groups; k++) s += sums[i * BLOCK + k * lpr + l];
                 const Item t = item_of<V, IL>(c * lpr + l, N, D);
-                const int at = i < V ? t.lo + i : t.hi + i - V;
-                if (i < V ? t.has_lo : t.has_hi) part[at] = s;
+                if (holds<V, IL>(t, i)) part[i < V ? t.lo + i : t.hi + i - V] = s;
             }
             __syncthreads();
         }
@@ -350,28 +387,46 @@ __global__ __launch_bounds__(1024) void rotary_columns_kernel(ColumnArgs A)
     dw[col] = (W)s;
 }
 
-// Elements per access: 16 bytes, 8, or one, where pairs and the rest are a whole
-// number of them.
-int vec_of(int type, int N, int D)
-{
-    const int full = 16 / gs::dtype_bytes(type);
-    for (int v : {full, full / 2})
-        if (N % v == 0 && (D - 2 * N) % (2 * v) == 0) return v;
-    return 1;
-}
-
 struct Plan {
     int v, lpr, nc, tokens;
+    bool ragged;
     unsigned blocks;
 };
+
+constexpr int RAGGED_V = 4;
+
+// Elements per access: 16 bytes, or 8, where pairs and the rest of a row are a whole number
+// of them.  Else four from any element on, with last items of fewer, or one by one where those
+// leave half of the lanes idle.  196608 rows of queries and 98304 of keys, forward with norm,
+// us with four and with one:
+//   75 of 37 pairs, interleaved   float 46, 73    bfloat16 45, 78
+//   33 of 16 pairs                float 29, 41    bfloat16 26, 40
+//   129 of 64 pairs (17 of 32 lanes)   float 119, 96    255 of 127 (33 of 64)   float 256, 124
+void lanes_of(Plan& p, int type, int N, int D)
+{
+    const int full = 16 / gs::dtype_bytes(type);
+    auto lanes = [&](int v) {
+        const int items = (N + v - 1) / v + (D - 2 * N + 2 * v - 1) / (2 * v);
+        for (p.lpr = 1; p.lpr < 64 && p.lpr < items; p.lpr *= 2) {}
+        p.nc = (items + p.lpr - 1) / p.lpr;
+        p.v = v;
+        return items;
+    };
+    p.ragged = false;
+    for (int v : {full, full / 2})
+        if (N % v == 0 && (D - 2 * N) % (2 * v) == 0) {
+            lanes(v);
+            return;
+        }
+    p.ragged = true;
+    const int items = lanes(RAGGED_V);
+    if (items * 16 < p.lpr * 9) lanes(1);
+}
 
 Plan plan_of(int type, int64_t n_tokens, int heads, int D, int N, bool parts)
 {
     Plan p;
-    p.v = vec_of(type, N, D);
-    const int items = (D + 2 * p.v - 1) / (2 * p.v);
-    for (p.lpr = 1; p.lpr < 64 && p.lpr < items; p.lpr *= 2) {}
-    p.nc = (items + p.lpr - 1) / p.lpr;
+    lanes_of(p, type, N, D);
     // Four rows a group, or fewer where that would leave CUs without work: the angles of one
     // workgroup are formed while others move rows (32768 tokens of 24 heads of 64, forward
     // and backward: 103 us, with eight rows 111).
@@ -386,25 +441,30 @@ Plan plan_of(int type, int64_t n_tokens, int heads, int D, int N, bool parts)
     return p;
 }
 
-template <typename T, int V, int NC, bool NORM, bool BWD>
+template <typename T, int V, int NC, bool RAGGED, bool NORM, bool BWD>
 void launch_layout(const RotaryArgs& A, bool interleaved, dim3 grid, size_t lds, hipStream_t stream)
 {
     if (interleaved)
         GS_TIMED(BWD ? "rotary_bwd_kernel" : "rotary_fwd_kernel", stream,
-                 hipLaunchKernelGGL((rotary_kernel<T, V, NC, true, NORM, BWD>), grid, dim3(BLOCK), lds, stream, A));
+                 hipLaunchKernelGGL((rotary_kernel<T, V, NC, true, RAGGED, NORM, BWD>), grid, dim3(BLOCK), lds, stream,
+                                    A));
     else
         GS_TIMED(BWD ? "rotary_bwd_kernel" : "rotary_fwd_kernel", stream,
-                 hipLaunchKernelGGL((rotary_kernel<T, V, NC, false, NORM, BWD>), grid, dim3(BLOCK), lds, stream, A));
+                 hipLaunchKernelGGL((rotary_kernel<T, V, NC, false, RAGGED, NORM, BWD>), grid, dim3(BLOCK), lds, stream,
+                                    A));
 }
 
 template <typename T, bool NORM, bool BWD>
 void launch_vec(const RotaryArgs& A, const Plan& p, bool interleaved, dim3 grid, size_t lds, hipStream_t stream)
 {
     constexpr int V = gs::Vec<T>::N;
-    if (p.v == V) return launch_layout<T, V, 1, NORM, BWD>(A, interleaved, grid, lds, stream);
-    if (p.v == V / 2) return launch_layout<T, V / 2, 1, NORM, BWD>(A, interleaved, grid, lds, stream);
-    if (p.nc == 1) return launch_layout<T, 1, 1, NORM, BWD>(A, interleaved, grid, lds, stream);
-    return launch_layout<T, 1, 2, NORM, BWD>(A, interleaved, grid, lds, stream);
+    if (!p.ragged) {
+        if (p.v == V) return launch_layout<T, V, 1, false, NORM, BWD>(A, interleaved, grid, lds, stream);
+        return launch_layout<T, V / 2, 1, false, NORM, BWD>(A, interleaved, grid, lds, stream);
+    }
+    if (p.v == RAGGED_V) return launch_layout<T, RAGGED_V, 1, true, NORM, BWD>(A, interleaved, grid, lds, stream);
+    if (p.nc == 1) return launch_layout<T, 1, 1, true, NORM, BWD>(A, interleaved, grid, lds, stream);
+    return launch_layout<T, 1, 2, true, NORM, BWD>(A, interleaved, grid, lds, stream);
 }
 
 template <bool NORM, bool BWD>

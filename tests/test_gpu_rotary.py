@@ -61,10 +61,10 @@ def _frequencies(pairs, axes=1, base=10000.0):
     (1, 1, 1, 1, 2, 1),            # the least there is
     (2, 4, 2, 9, 64, 32),          # whole accesses
     (3, 5, 1, 33, 128, 32),        # half of the head
-    (2, 3, 3, 17, 75, 35),         # odd heads, element by element
+    (2, 3, 3, 17, 75, 35),         # odd heads: items of fewer
     (1, 2, 1, 5, 40, 20),          # accesses of 8 bytes
     (1, 2, 2, 3, 256, 128),        # the widest
-    (1, 3, 2, 4, 255, 127),        # two items a lane
+    (1, 3, 2, 4, 255, 127),        # the widest odd ones
     (2, 6, 2, 700, 32, 16),        # many tokens
     (5, 1, 1, 3, 96, 16),
     (1, 300, 1, 2, 16, 8),         # more heads than groups of lanes
@@ -74,6 +74,19 @@ def test_sizes(gpu, t, norm, interleaved, B, Hq, Hk, T, D, pairs):
     w = [_rand((D,), t, 3 + i, 0.2, 1.0) for i in range(2)] if norm else [None, None]
     positions = torch.arange(T, device="cuda")[None] + 1000 * torch.arange(B, device="cuda")[:, None]
     _check(q, k, *w, positions.int(), _frequencies(pairs), interleaved, norm=norm)
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D", [2, 3, 5, 8, 9, 15, 17, 24, 31, 33, 47, 63, 75, 100, 129, 253])
+def test_every_end_of_a_row(gpu, t, interleaved, D):
+    # pairs and what is not rotated end anywhere inside an item
+    at, w = torch.arange(3, device="cuda"), _rand((D,), t, 3)
+    for pairs in sorted({1, 2, 3, 4, 5, 8, 9, D // 4, D // 2 - 1, D // 2}):
+        if 1 <= pairs <= D // 2:
+            q, k = _rand((1, 3, 3, D), t, pairs), _rand((1, 1, 3, D), t, 2)
+            _check(q, k, w, w, at, _frequencies(pairs), interleaved)
+            _check(q, k, None, None, at, _frequencies(pairs), interleaved, norm=False)
 
 
 @pytest.mark.parametrize("t", TYPES)
