@@ -24,9 +24,9 @@
 // exponent, without cases.  NaN and infinities, which would need some, have a path that a
 // wave takes only where it meets one.
 //
-// 122M elements in fp32: 645 us, 3.4 GB at 5.3 TB/s (a large copy: 5.15).  183M bfloat16
+// 122M elements in fp32: 651 us, 3.42 GB at 5.25 TB/s (a large copy: 5.15).  183M bfloat16
 // elements with 8-bit moments: 358 us, 1.83 GB at 5.1 TB/s (472 us before the instructions
-// of an element were 87 and are about 50); their moments' values 177 us.
+// of an element were 87 and are about 50); their moments' values 181 us.
 #include <math.h>
 
 #include <algorithm>
@@ -93,7 +93,8 @@ struct Codes {
     {
         uint32_t found = 0;
 #pragma unroll
-        for (int k = 0; k < 2; k++) found |= ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & (SIGN ? 0x80808080u : w[k] & 0x80808080u);
+        for (int k = 0; k < 2; k++)
+            found |= ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & (SIGN ? 0x80808080u : w[k] & 0x80808080u);
         return found != 0;
     }
 };
@@ -122,7 +123,8 @@ __device__ __forceinline__ uint32_t encoded(float x, int biased, uint32_t draw)
 
 // The hardware's square root, and its reciprocal in the step, are off by one last bit, of
 // an update that is a small part of its parameter; with 8-bit moments there is little room for
-// instructions: with the exact ones 183M bfloat16 elements took 55 us more.  The hardware's takes no subnormals, which matter only beside an eps that is one, or none.
+// instructions: with the exact ones 183M bfloat16 elements took 55 us more.  The hardware's
+// root takes no subnormals, which matter only beside an eps that is one, or none.
 template <bool TINY>
 __device__ __forceinline__ float root_of(float v)
 {

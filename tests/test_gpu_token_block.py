@@ -161,9 +161,10 @@ def test_rotation_in_a_graph(gpu, norm):
     _replays(make, change)
 
 
-# large, split, odd and single-row shapes
+# large, split, odd, single-row and large odd shapes
 @pytest.mark.parametrize("M,W,H,t", [(2100, 264, 520, torch.bfloat16), (700, 64, 128, torch.float32),
-                                     (90, 33, 65, torch.float16), (1, 512, 1024, torch.bfloat16)])
+                                     (90, 33, 65, torch.float16), (1, 512, 1024, torch.bfloat16),
+                                     (8, 512, 1030, torch.float32), (800, 515, 1001, torch.bfloat16)])
 def test_feed_forward_in_a_graph(gpu, M, W, H, t):
     from blitzgs_amd.feedforward import feed_forward
     leaves = [_rand(s, i, t, s[-1] ** -0.5 if i else 1.0).requires_grad_(True)
