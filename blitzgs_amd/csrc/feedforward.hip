@@ -982,7 +982,7 @@ double estimate(const FeedArgs& A, int sm, int sn, double turn, double ends)
 template <Kind K>
 int few_columns(const Product& P, bool half)
 {
-    if (P.rows > (half ? 8 : 16)) return 0;
+    if (P.rows > (half ? 8 : 16) || P.depth % 8) return 0;   // a lane takes eight of the depth
     if (half && K == PLAIN && P.cols >= SS * CUS) return 0;
     const int64_t matrix_rows = (int64_t)(K == HIDDEN ? 2 : 1) * P.cols;
     int c = 16;

@@ -170,6 +170,16 @@ def test_the_ends_of_the_activations(gpu, activation):
     within(g, *want["dx"], "dx")
 
 
+@pytest.mark.parametrize("M", [1, 4, 7, 16])
+@pytest.mark.parametrize("W,H,O", [(12, 20, 28), (1028, 516, 132), (2044, 1024, 260), (4, 4, 4), (8, 1028, 64), (64, 65, 64)])
+def test_few_rows_of_whole_pieces_of_four(gpu, M, W, H, O):
+    # float: 16 bytes are four elements, of which a depth may end half way in a lane's eight; what lies behind x is
+    # not a number
+    wide = torch.full((M, W + 4), math.nan, device="cuda")
+    wide[:, :W] = _rand((M, W), torch.float32, M)
+    _check(wide[:, :W], _weights(W, H, O, torch.float32))
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("M", [3, 8, 13])
 def test_nan_stays_in_its_row_of_few(gpu, t, M):
