@@ -19,6 +19,12 @@
 // (bar the sign) is NaN, which infinities become too; they leave their block's
 // power of two alone.  The step itself uses m and v before they are rounded.
 //
+// A v that is not zero never becomes zero: its root's smallest step is 2^-16 of the block's,
+// as m's is, and an m that was rounded up beside a v that was rounded away is divided by next
+// to nothing a step later (a block's elements of 1e-5 of its largest took updates of up to 1500
+// lr).  So elements whose root of v is below 2^-16 of their block's largest are stepped as if it
+// were that: by less than AdamW does, and never by more.
+//
 // A code shifted to fp32's exponent is the number up to a power of two, below the
 // smallest exponent too, where both are subnormal: decoding and encoding change an
 // exponent, without cases.  NaN and infinities, which would need some, have a path that a
@@ -109,14 +115,15 @@ __device__ __forceinline__ float decoded(uint32_t code, int biased)
     return SPECIAL && c == ONES ? __builtin_nanf("") : x;
 }
 
-// x over its block's power of two, rounded up where its rest and draw / 2^16 make a step; NaN and
-// infinities only with SPECIAL
+// x over its block's power of two, rounded up where its rest and draw / 2^16 make a step, and
+// without a sign at least the smallest code unless it is zero; NaN and infinities only with SPECIAL
 template <int TOP, bool SIGN, bool SPECIAL>
 __device__ __forceinline__ uint32_t encoded(float x, int biased, uint32_t draw)
 {
     constexpr uint32_t ONES = SIGN ? 127u : 255u;
     const float size = __builtin_ldexpf(__builtin_fabsf(x), TOP - biased);
     uint32_t c = (__float_as_uint(size) + (draw << 4)) >> 20;
+    if (!SIGN) c = max(c, min(__float_as_uint(x), 1u));   // v > 0: not zero
     if (SPECIAL && !(__builtin_fabsf(x) < __builtin_inff())) c = ONES;
     return SIGN ? c | (__float_as_uint(x) >> 24 & 128u) : c;
 }
