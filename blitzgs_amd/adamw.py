@@ -189,6 +189,9 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        # before anything is made: a capture records new moments' zeros, it does not write them
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW counts its steps on the host and cannot be captured; adamw_update can")
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -209,8 +212,6 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError(f"a parameter's state has not the {group['bits']} bits of its group")
                 alike.setdefault((p.device, p.dtype, state["step"]), []).append((p, state))
             calls += [(group, *key, pairs) for key, pairs in alike.items()]
-        if calls and calls[0][1].type == "cuda" and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW counts its steps on the host and cannot be captured; adamw_update can")
         for i, (group, _, _, step, pairs) in enumerate(calls):
             params, states = zip(*pairs)
             adamw_update(params, [p.grad for p in params], [s["exp_avg"] for s in states],
