@@ -57,12 +57,17 @@ def wants_grad(*tensors):
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
-def load_uncast(optimizer, load, state_dict, take):
+def load_uncast(optimizer, load, state_dict, take, fit=None):
     """load(state_dict) of an optimiser whose state keeps its own types: torch's loading
     casts a state to its parameter's type, so take(state, loaded, parameter) takes from
     what was loaded once more: after all hooks that may change that, and before any that
-    look at the result."""
+    look at the result.  fit(state_dict) may refuse what is loaded, or give it otherwise."""
     loaded = {}
+
+    def look(_, state):
+        state = state if fit is None else fit(state)
+        loaded.update(state)
+        return state
 
     def restore(_):
         ours = (p for group in optimizer.param_groups for p in group["params"])
@@ -70,7 +75,7 @@ def load_uncast(optimizer, load, state_dict, take):
             if key in loaded["state"]:
                 take(optimizer.state[p], loaded["state"][key], p)
 
-    hooks = [optimizer.register_load_state_dict_pre_hook(lambda _, state: loaded.update(state)),
+    hooks = [optimizer.register_load_state_dict_pre_hook(look),
              optimizer.register_load_state_dict_post_hook(restore, prepend=True)]
     try:
         load(state_dict)

@@ -178,14 +178,35 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits, seed=seed))
 
     def load_state_dict(self, state_dict):
+        """Takes a state of torch's AdamW and Adam too, moments of 16 bits as float32, unless its groups ask for
+        another step than this one."""
         def take(state, loaded, p):
             for name in ("exp_avg", "exp_avg_sq", "scales"):
-                if isinstance(loaded.get(name), torch.Tensor):
-                    state[name] = loaded[name].detach().to(p.device, copy=True).contiguous()
+                t = loaded.get(name)
+                if isinstance(t, torch.Tensor):
+                    dtype = torch.float32 if t.is_floating_point() else t.dtype
+                    state[name] = t.detach().to(p.device, dtype, copy=True).contiguous()
             if "step" in loaded:
                 state["step"] = int(loaded["step"])
 
-        _t.load_uncast(self, super().load_state_dict, state_dict, take)
+        def fit(saved):
+            groups = []
+            for group in saved["param_groups"]:
+                for name in ("lr", "betas", "eps", "weight_decay"):
+                    if name not in group:
+                        raise ValueError(f"a group of the loaded state has no {name}")
+                for name in ("amsgrad", "maximize"):
+                    if group.get(name):
+                        raise ValueError(f"AdamW has no {name}, which the loaded state asks for")
+                if group["weight_decay"] and not group.get("decoupled_weight_decay", True):
+                    raise ValueError("the loaded state's weight_decay is part of its gradients; AdamW's is not")
+                # what says nothing of bits has those of its moments
+                held = [saved["state"][k] for k in group["params"] if k in saved["state"]]
+                bits = 8 if any("scales" in s for s in held) else 32 if held else self.defaults["bits"]
+                groups.append({"bits": bits, "seed": self.defaults["seed"], **group})
+            return {**saved, "param_groups": groups}
+
+        _t.load_uncast(self, super().load_state_dict, state_dict, take, fit)
 
     @torch.no_grad()
     def step(self, closure=None):
