@@ -197,6 +197,30 @@ struct Raw {
     T v[N];
 };
 
+// float16 ends at 65504, where a or b may not: beside a small b or a h, y and the gradients are
+// within its range, and a slope of infinity is no number.  Such a number is kept, where it has a
+// rest, as its sign, an exponent of ones and 14 bits, ten behind the exponent and four in the
+// rest: float32's from 2^15 on, to seven of its mantissa.  What is no number is kept so too.
+constexpr uint32_t FAR_FROM = 0x477ff000u;   // 65520, the first that rounds to infinity
+template <typename T>
+__device__ __forceinline__ bool is_far(float x)
+{
+    return __is_same(T, gs::f16) && (__float_as_uint(x) & 0x7fffffffu) >= FAR_FROM;
+}
+__device__ __forceinline__ uint32_t far_code(float x)
+{
+    return ((x == x ? __float_as_uint(x) & 0x7fffffffu : 0x7fc00000u) - 0x47000000u + 0x8000u) >> 16;
+}
+// x as it is kept, with a rest
+template <typename T>
+__device__ __forceinline__ T kept_of(float x)
+{
+    if constexpr (__is_same(T, gs::f16))
+        if (is_far<T>(x))
+            return __builtin_bit_cast(T, (uint16_t)((__float_as_uint(x) >> 16 & 0x8000u) | 0x7c00u | far_code(x) >> 4));
+    return (T)x;
+}
+
 // Four bits of what rounding x to T left, in sixteenths of T's last bit, and x again.  As
 // integers: numbers of one sign follow one another as their bits do.
 template <typename T>
@@ -204,14 +228,20 @@ __device__ __forceinline__ uint32_t rest_of(float x)
 {
     constexpr int SHIFT = __is_same(T, gs::bf16) ? 12 : 9;
     const uint32_t kept = __float_as_uint((float)(T)x);
-    if ((kept & 0x7fffffffu) >= 0x7f800000u) return 0;
+    if ((kept & 0x7fffffffu) >= 0x7f800000u) return is_far<T>(x) ? far_code(x) & 15u : 0u;
     const int q = ((int)(__float_as_uint(x) - kept) + (1 << (SHIFT - 1))) >> SHIFT;
     return (uint32_t)(q > 7 ? 7 : q < -8 ? -8 : q) & 15u;
 }
+// `held`: x was kept with a rest
 template <typename T>
-__device__ __forceinline__ float with_rest(T x, uint32_t rest)
+__device__ __forceinline__ float with_rest(T x, uint32_t rest, bool held)
 {
     constexpr int SHIFT = __is_same(T, gs::bf16) ? 12 : 9;
+    if constexpr (__is_same(T, gs::f16)) {
+        const uint32_t h = __builtin_bit_cast(uint16_t, x);
+        if (held && (h & 0x7c00u) == 0x7c00u)
+            return __uint_as_float((h & 0x8000u) << 16 | (0x47000000u + (((h & 0x3ffu) << 4 | (rest & 15u)) << 16)));
+    }
     return __uint_as_float(__float_as_uint((float)x) + (uint32_t)(((int)(rest << 28) >> 28) * (1 << SHIFT)));
 }
 
@@ -306,6 +336,19 @@ struct Leave {
             }
         }
     }
+    // what float16 does not hold, over what was stored for it
+    __device__ __forceinline__ void keep_far(int64_t at, const float (&a)[8], const float (&b)[8], int count) const
+    {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 8; e++) any = any || is_far<T>(a[e]) || is_far<T>(b[e]);
+        if (!any) return;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (e < count && is_far<T>(a[e])) out1[at + e] = kept_of<T>(a[e]);
+            if (e < count && is_far<T>(b[e])) out2[at + e] = kept_of<T>(b[e]);
+        }
+    }
     template <bool WHOLE>
     __device__ __forceinline__ void give(const In& in, const f4 (&acc)[HN / 16], int row0) const
     {
@@ -356,6 +399,7 @@ struct Leave {
                                 for (int e = 0; e < 8; e++)
                                     if (e < count) rest[at + e] = q.v[e];
                             }
+                            keep_far(at, a, b, WHOLE ? 8 : count);
                         }
                     }
                 }
@@ -365,8 +409,8 @@ struct Leave {
                 for (int e = 0; e < 8; e++) {
                     float a = (float)in.v[p][0].v[e], b = (float)in.v[p][1].v[e];
                     if constexpr (sizeof(T) == 2) {
-                        a = with_rest(in.v[p][0].v[e], in.rest[p].v[e]);
-                        b = with_rest(in.v[p][1].v[e], in.rest[p].v[e] >> 4);
+                        a = with_rest(in.v[p][0].v[e], in.rest[p].v[e], rest != nullptr);
+                        b = with_rest(in.v[p][1].v[e], in.rest[p].v[e] >> 4, rest != nullptr);
                     }
                     float value, slope;
                     activation<T>(act, a, value, slope);
@@ -824,8 +868,8 @@ __global__ __launch_bounds__(512) void feed_few_kernel(FeedArgs A)
         activation<T>(A.act, sum[0], value, slope);
         ((T*)P.out[0])[at] = (T)(value * sum[1]);
         if (P.out[1] != nullptr) {
-            ((T*)P.out[1])[at] = (T)sum[0];
-            ((T*)P.out[2])[at] = (T)sum[1];
+            ((T*)P.out[1])[at] = P.rest != nullptr ? kept_of<T>(sum[0]) : (T)sum[0];
+            ((T*)P.out[2])[at] = P.rest != nullptr ? kept_of<T>(sum[1]) : (T)sum[1];
             if constexpr (sizeof(T) == 2)
                 if (P.rest != nullptr) P.rest[at] = (uint8_t)(rest_of<T>(sum[0]) | rest_of<T>(sum[1]) << 4);
         }

@@ -750,7 +750,9 @@ int gs_rotary_backward(int type, int param_type, int B, int Hq, int Hk, int T, i
  * up to a multiple of 8 elements apart, is written: act(a) * b of a = x gate^T, b = x
  * up^T, rounded to `type`, and zeros behind each row; a and b too, for the backward, or
  * both NULL, and rest, a byte each, may be NULL: with the 16-bit types four bits of what
- * rounding a left and, above them, four of b.
+ * rounding a left and, above them, four of b.  In float16 a and b that it does not hold
+ * are with a rest kept to seven bits of mantissa: a sign, an exponent of ones and, in the
+ * other ten bits and the rest's four, those of float32 less 0x4700 from its bit 16 on.
  *   Backward, from a, b, rest (NULL if the forward had none) and h: dx, dgate, dup,
  * ddown, each unless NULL.
  *   workspace: 256-byte aligned, of gs_feed_forward_workspace_bytes (0: none is
