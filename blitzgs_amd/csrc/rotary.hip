@@ -274,20 +274,40 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
             T* out = (T*)S.out + offset[4 * token + 2] + head * S.outs[1];
             const float2* cs = table + token * N;
             float v[NC][2 * V], g[NC][2 * V];
-            float r = 1.0f;
+            float r = 1.0f, up = 1.0f;
 #pragma unroll
             for (int c = 0; c < NC; c++) {
                 if constexpr (!BWD || NORM) load_item<T, V, IL, RAGGED>(x, items[c], v[c]);
                 if constexpr (BWD) load_item<T, V, IL, RAGGED>(dy, items[c], g[c]);
             }
             if constexpr (NORM) {
-                float sum = 0.0f;
+                // of what is multiplied by a power of two
+                auto mean_of_squares = [&](float by) __attribute__((always_inline)) {
+                    float sum = 0.0f;
 #pragma unroll
-                for (int c = 0; c < NC; c++)
+                    for (int c = 0; c < NC; c++)
 #pragma unroll
-                    for (int i = 0; i < 2 * V; i++) sum = __builtin_fmaf(v[c][i], v[c][i], sum);
-                for (int d = lpr / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
-                r = 1.0f / __builtin_sqrtf(__builtin_fmaf(sum, A.inv_d, A.eps));
+                        for (int i = 0; i < 2 * V; i++) {
+                            const float x = v[c][i] * by;
+                            sum = __builtin_fmaf(x, x, sum);
+                        }
+                    for (int d = lpr / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+                    return __builtin_fmaf(sum, A.inv_d, A.eps * by * by);
+                };
+                const float mean = mean_of_squares(1.0f);
+                r = 1.0f / __builtin_sqrtf(mean);
+                // Squares that fp32 does not hold, or not to its last bit: a row's lanes go together
+                if (mean > 0x1p100f) {
+                    r = 0x1p-96f / __builtin_sqrtf(mean_of_squares(0x1p-96f));
+                } else if (mean < 0x1p-100f) {
+                    // beside such a row 1 / r may pass fp32's range, so that the row itself grows
+                    up = 0x1p96f;
+                    r = 1.0f / __builtin_sqrtf(mean_of_squares(up));
+#pragma unroll
+                    for (int c = 0; c < NC; c++)
+#pragma unroll
+                        for (int i = 0; i < 2 * V; i++) v[c][i] *= up;
+                }
             }
             if constexpr (!BWD) {
 #pragma unroll
@@ -323,6 +343,12 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryArgs A)
                     for (int c = 0; c < NC; c++)
 #pragma unroll
                         for (int i = 0; i < 2 * V; i++) v[c][i] = r * __builtin_fmaf(-v[c][i], mean, g[c][i]);
+                    if (up != 1.0f) {
+#pragma unroll
+                        for (int c = 0; c < NC; c++)
+#pragma unroll
+                            for (int i = 0; i < 2 * V; i++) v[c][i] *= up;
+                    }
                 }
             }
 #pragma unroll

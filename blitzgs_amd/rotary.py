@@ -19,8 +19,8 @@ formed modulo a turn, without error however far the position, and its cosine and
 in float32.  rotary_frequencies makes the usual ones, also scaled for contexts longer
 than those of the training, as_turns makes them from any angles.
 
-Sums are fp32, each output is rounded to its type once.  A row whose squares pass
-fp32's range (elements of 1e18 and more) becomes zero under the norm.  The weights'
+Sums are fp32, each output is rounded to its type once.  A row whose squares are not
+within fp32's range is normed by those of the row times a power of two.  The weights'
 gradients are added up in a fixed order: equal inputs give equal bits.
 """
 import ctypes as C
