@@ -22,6 +22,16 @@ def require_tensor(t, name, device=None):
         raise RuntimeError(f"{name} must be on {device}, got {t.device}")
 
 
+_tracing = torch._C._get_tracing_state
+
+
+def not_traced():
+    """A trace would hold the results' memory and not the kernels, or the kernels without the checks of their
+    arguments, on tensors of other sizes."""
+    if _tracing() is not None:
+        raise RuntimeError("the operators of blitzgs_amd cannot be traced")
+
+
 def ptr(t):
     """A tensor's address; None (NULL) for no tensor."""
     return None if t is None else t.data_ptr()
@@ -49,12 +59,16 @@ def workspace(nbytes, device):
 
 def wants_grad(*tensors):
     """Whether a call has to go through its autograd function: a backward may follow, or
-    a tensor has a forward-mode tangent, which that function refuses."""
+    a tensor has a forward-mode tangent, which that function refuses.  A call that does not
+    is not traced."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         return True
     # -1 outside all dual levels, where no tensor has a tangent
-    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        return True
+    not_traced()
+    return False
 
 
 def load_uncast(optimizer, load, state_dict, take, fit=None):

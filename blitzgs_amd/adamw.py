@@ -92,6 +92,7 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
     them.  A tensor may not come twice, nor overlap another, nor a gradient one of them
     (gradients may be one tensor).  In a captured graph every replay is the step, with
     the rates and the seed, that was captured."""
+    _t.not_traced()
     params, grads = list(params), list(grads)
     how = _settings(lr, betas, eps, weight_decay)
     if not isinstance(step, int) or not 1 <= step < 2 ** 53:
@@ -142,6 +143,7 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
 @torch.no_grad()
 def moment_values(exp_avg, exp_avg_sq, scales, dtype=torch.float32):
     """The values that 8-bit moments stand for, float32 or (which holds them whole) bfloat16."""
+    _t.not_traced()
     for name, t in (("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq), ("scales", scales)):
         if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.device != exp_avg.device):
             raise RuntimeError(f"{name} must be a uint8 HIP device tensor (of exp_avg's device)")

@@ -106,6 +106,7 @@ class _FeedForward(torch.autograd.Function):
 
 def feed_forward(x, gate, up, down, activation="silu"):
     """The gated block of x over its last dimension; differentiable in x and the three weights."""
+    _t.not_traced()
     _t.require_tensor(x, "x")
     for name, w in (("gate", gate), ("up", up), ("down", down)):
         _t.require_tensor(w, name, device=x.device)

@@ -38,6 +38,7 @@ def orthogonalise(update, steps=5):
 
     All matrices of one call go through the device together.  Not
     differentiable.  steps: 1 to 32."""
+    _t.not_traced()
     _t.require_tensor(update, "update")
     if update.dim() < 2 or max(update.shape[-2:]) > 65536:
         raise RuntimeError(f"update must hold matrices with sides of up to 65536, got shape {tuple(update.shape)}")

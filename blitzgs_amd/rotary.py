@@ -186,6 +186,7 @@ class _Rotary(torch.autograd.Function):
 
 
 def _call(q, k, qw, kw, positions, frequencies, interleaved, magnitude, norm, eps):
+    _t.not_traced()
     _t.require_tensor(q, "q")
     if q.dim() != 4 or not 1 <= q.shape[3] <= MAX_HEAD_DIM:
         raise RuntimeError(f"q must have dimensions (B, H, T, D) with D of 1 to {MAX_HEAD_DIM}, got shape "
