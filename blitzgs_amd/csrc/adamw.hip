@@ -116,7 +116,8 @@ __device__ __forceinline__ float decoded(uint32_t code, int biased)
 }
 
 // x over its block's power of two, rounded up where its rest and draw / 2^16 make a step, and
-// without a sign at least the smallest code unless it is zero; NaN and infinities only with SPECIAL
+// without a sign at least the smallest code unless it is zero; NaN, infinities and what could be
+// rounded up to one only with SPECIAL
 template <int TOP, bool SIGN, bool SPECIAL>
 __device__ __forceinline__ uint32_t encoded(float x, int biased, uint32_t draw)
 {
@@ -124,6 +125,8 @@ __device__ __forceinline__ uint32_t encoded(float x, int biased, uint32_t draw)
     const float size = __builtin_ldexpf(__builtin_fabsf(x), TOP - biased);
     uint32_t c = (__float_as_uint(size) + (draw << 4)) >> 20;
     if (!SIGN) c = max(c, min(__float_as_uint(x), 1u));   // v > 0: not zero
+    // no number is above 2^128
+    if (SPECIAL && biased == 254) c = min(c, 8u * TOP + 7u);
     if (SPECIAL && !(__builtin_fabsf(x) < __builtin_inff())) c = ONES;
     return SIGN ? c | (__float_as_uint(x) >> 24 & 128u) : c;
 }
@@ -244,9 +247,9 @@ __device__ __forceinline__ void step(const AdamArgs& A, const Tensor& t, int64_t
     } else {
         Codes cm, cv;
         uint32_t em, ev;
-        // NaN and infinities have larger bits than any number
+        // NaN and infinities have larger bits than any number, and 1.875 2^127 is the last below a code of 2^128
         const int there = WHOLE ? V : n;
-        const bool special = max(largest_of<false>(m, there), largest_of<false>(v, there)) >= 0x7f800000u;
+        const bool special = max(largest_of<false>(m, there), largest_of<false>(v, there)) >= 0x7f700000u;
         if (__any(special)) keep<true>(t, at, there, m, v, cm, cv, em, ev);
         else keep<false>(t, at, there, m, v, cm, cv, em, ev);
         put((uint8_t*)t.m + at, __builtin_bit_cast(Bytes, cm).b);

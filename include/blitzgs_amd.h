@@ -807,7 +807,7 @@ int gs_momentum_apply(int type, int count, int64_t size, void* const* params, fl
  * three, both with subnormals, and all ones (the sign apart) is NaN.  Bytes and scales of zero are a
  * moment of zero.  A second moment that is not zero keeps a byte of at least 1: an element
  * far below its block's largest (2^-32 of it) is stepped by less than with 32 bits, not by
- * more.  Otherwise they are rounded up with the probability of what is left, by
+ * more.  No moment is rounded up to 2^128.  Otherwise they are rounded up with the probability of what is left, by
  * 16 bits each of s(s(i phi + s(step phi + seed)) + element phi), modulo 2^32,
  * where i is the tensor's place in the arrays, phi = 0x9E3779B9 and
  *   s(x): x ^= x >> 16; x *= 0x6A09E667; x ^= x >> 15; x *= 0xBB67AE85; x ^= x >> 16.

@@ -1,5 +1,5 @@
 """8-bit moments over many steps beside AdamW's own: blocks of elements whose gradients are
-of very different sizes."""
+of very different sizes; moments next to the largest number there is."""
 import math
 
 import pytest
@@ -48,3 +48,17 @@ def test_quiet_elements_of_a_loud_block(gpu, kind, constant):
     assert (square[quiet] / steps).mean().sqrt().item() <= 1 + 1.15 * math.sqrt(2)
     # a second moment that is not zero is not forgotten
     assert (v[size > 0] > 0).all()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_moments_next_to_the_largest_number(gpu, seed):
+    # 1.97 2^127 lies between the code of 1.875 2^127 and that of 2^128, which is no number: it is never rounded up
+    from blitzgs_amd.adamw import adamw_update, moment_values, new_moments
+    top = 1.97 * 2.0 ** 127
+    for moment, g, betas in ((0, top, (0.0, 0.999)), (0, -top, (0.0, 0.999)), (1, math.sqrt(top), (0.0, 0.0))):
+        p = torch.zeros(300, device="cuda")
+        m, v, s = new_moments(p, 8)
+        adamw_update([p], [torch.full_like(p, g)], [m], [v], step=1, lr=0.0, betas=betas, weight_decay=0.0, scales=[s],
+                     seed=seed)
+        got = moment_values(m, v, s)[moment]
+        assert torch.equal(got, torch.full_like(got, math.copysign(1.875 * 2.0 ** 127, g)))
