@@ -91,7 +91,8 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.9
     exp_avgs, exp_avg_sqs: float32, or uint8 with a list of scales, as new_moments makes
     them.  A tensor may not come twice, nor overlap another, nor a gradient one of them
     (gradients may be one tensor).  In a captured graph every replay is the step, with
-    the rates and the seed, that was captured."""
+    the rates and the seed, that was captured: its 8-bit moments are rounded by the same
+    bits each time."""
     _t.not_traced()
     params, grads = list(params), list(grads)
     how = _settings(lr, betas, eps, weight_decay)

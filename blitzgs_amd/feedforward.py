@@ -9,7 +9,8 @@ the activation and the product, and the projection down.
 
 Sums are fp32.  Besides y, what lies between two products is rounded to the tensors'
 type: act(a) * b, and the gradients of a = x gate^T and b = x up^T, so float16's range (up
-to 65504, from 6e-5 at full precision) holds for those too.  It does not for a and b.  A
+to 65504, from 6e-5 at full precision) holds for those too: gradients of y far below 1e-3
+want a loss that is scaled up.  a and b themselves may pass that range.  A
 call that needs gradients keeps x, the weights, a, b (in the 16-bit types with four more
 bits each; what is beyond float16's range to eight bits) and act(a) * b.  The weights'
 gradients are added up in a fixed order: equal inputs give equal bits.

@@ -750,9 +750,9 @@ int gs_rotary_backward(int type, int param_type, int B, int Hq, int Hk, int T, i
  * up to a multiple of 8 elements apart, is written: act(a) * b of a = x gate^T, b = x
  * up^T, rounded to `type`, and zeros behind each row; a and b too, for the backward, or
  * both NULL, and rest, a byte each, may be NULL: with the 16-bit types four bits of what
- * rounding a left and, above them, four of b.  In float16 a and b that it does not hold
- * are with a rest kept to seven bits of mantissa: a sign, an exponent of ones and, in the
- * other ten bits and the rest's four, those of float32 less 0x4700 from its bit 16 on.
+ * rounding a left and, above them, four of b.  Numbers of a and b beyond float16's range,
+ * and those that are none, are with a rest kept as a sign, an exponent of ones and 14 bits,
+ * ten behind it and four in the rest: float32's upper 16 bits without the sign, less 0x4700.
  *   Backward, from a, b, rest (NULL if the forward had none) and h: dx, dgate, dup,
  * ddown, each unless NULL.
  *   workspace: 256-byte aligned, of gs_feed_forward_workspace_bytes (0: none is
@@ -808,8 +808,8 @@ int gs_momentum_apply(int type, int count, int64_t size, void* const* params, fl
  * moment of zero.  A second moment that is not zero keeps a byte of at least 1: an element
  * far below its block's largest (2^-32 of it) is stepped by less than with 32 bits, not by
  * more.  No moment is rounded up to 2^128.  Otherwise they are rounded up with the probability of what is left, by
- * 16 bits each of s(s(i phi + s(step phi + seed)) + element phi), modulo 2^32,
- * where i is the tensor's place in the arrays, phi = 0x9E3779B9 and
+ * 16 bits each of s(s(i phi + s(step phi + seed)) + element phi + (element >> 32)
+ * 0x6A09E667), modulo 2^32, where i is the tensor's place in the arrays, phi = 0x9E3779B9 and
  *   s(x): x ^= x >> 16; x *= 0x6A09E667; x ^= x >> 15; x *= 0xBB67AE85; x ^= x >> 16.
  * Tensors that are written may overlap neither each other nor a gradient; gradients may
  * be one tensor.
