@@ -31,8 +31,8 @@
 // wave takes only where it meets one.
 //
 // 122M elements in fp32: 651 us, 3.42 GB at 5.25 TB/s (a large copy: 5.15).  183M bfloat16
-// elements with 8-bit moments: 358 us, 1.83 GB at 5.1 TB/s (472 us before the instructions
-// of an element were 87 and are about 50); their moments' values 181 us.
+// elements with 8-bit moments: 361 us, 1.83 GB at 5.1 TB/s (472 us before the instructions
+// of an element were 87 and are about 50); their moments' values 180 us.
 #include <math.h>
 
 #include <algorithm>
