@@ -17,7 +17,7 @@ follow from seed, step, the tensor's place in the call and the element's: equal 
 give equal bits.  A step uses the moments before they are rounded.  A moment that is
 infinite or NaN is NaN in 8 bits.  A second moment that is not zero is not rounded to
 zero: an element whose gradients are below 2^-16 of the largest of its 128 moves as if
-they were measured by that, which is less than with 32 bits and never more.
+they were measured by that, which is on average less than with 32 bits.
 """
 import ctypes as C
 import math

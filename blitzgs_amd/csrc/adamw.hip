@@ -23,7 +23,7 @@
 // as m's is, and an m that was rounded up beside a v that was rounded away is divided by next
 // to nothing a step later (a block's elements of 1e-5 of its largest took updates of up to 1500
 // lr).  So elements whose root of v is below 2^-16 of their block's largest are stepped as if it
-// were that: by less than AdamW does, and never by more.
+// were that: by less than AdamW does on average, in single steps by up to 2.4 lr.
 //
 // A code shifted to fp32's exponent is the number up to a power of two, below the
 // smallest exponent too, where both are subnormal: decoding and encoding change an

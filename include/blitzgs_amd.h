@@ -806,8 +806,8 @@ int gs_momentum_apply(int type, int count, int64_t size, void* const* params, fl
  * bits of exponent (1 is 14) and three of mantissa, a second one's five (1 is 30) and
  * three, both with subnormals, and all ones (the sign apart) is NaN.  Bytes and scales of zero are a
  * moment of zero.  A second moment that is not zero keeps a byte of at least 1: an element
- * far below its block's largest (2^-32 of it) is stepped by less than with 32 bits, not by
- * more.  No moment is rounded up to 2^128.  Otherwise they are rounded up with the probability of what is left, by
+ * far below its block's largest (2^-32 of it) is stepped on average by less than with 32
+ * bits.  No moment is rounded up to 2^128.  Otherwise they are rounded up with the probability of what is left, by
  * 16 bits each of s(s(i phi + s(step phi + seed)) + element phi + (element >> 32)
  * 0x6A09E667), modulo 2^32, where i is the tensor's place in the arrays, phi = 0x9E3779B9 and
  *   s(x): x ^= x >> 16; x *= 0x6A09E667; x ^= x >> 15; x *= 0xBB67AE85; x ^= x >> 16.
